@@ -7,7 +7,7 @@ holds; with `own` false the same results come from elementary torch operations.
 
 An edited logit is pen(cap(l) + bias): the model's final softcap, the request's bias, then the repetition and the
 frequency / presence penalties over the row's history, each step rounded to fp32 as ferro's sampler rounds its steps; a
-token whose mask bit is 0, or whose logit is NaN or -inf before the penalties, is no candidate.
+token whose mask bit is 0, or whose edited logit is NaN or -inf, is no candidate.
 """
 import ctypes
 import functools
@@ -346,15 +346,15 @@ def _edited(d, penalties=True):
         b = torch.zeros((c["B"], V), device="cuda")
         b[_row_of(d["b_off"], d["n_bias"]), d["b_ids"].long()] = d["b_val"]
         x = x + (b.repeat_interleave(M, 0) if M > 1 else b)
-    ok = x > -math.inf
-    if c["mask"] != "none":
-        ok = ok & _allowed(d)
     if penalties and c["H"] and (c["mixed"] or c["rep"] != 1.0 or c["freq"] or c["pres"]):
         n = _counts(d)
         rep, freq, pres = (p[k].repeat_interleave(M)[:, None] for k in ("rep", "freq", "pres"))
         y = torch.where(rep != 1.0, torch.where(x > 0, x / rep, x * rep), x)
         y = y - (n * freq + pres)
         x = torch.where(n > 0, y, x)
+    ok = x > -math.inf
+    if c["mask"] != "none":
+        ok = ok & _allowed(d)
     return x, ok
 
 
