@@ -24,6 +24,9 @@ FS_W_RECOVERED = 1          # success; an earlier call's give-up was cleared (FS
 FS_WAIT_GIVE_UP = 0xFFFFFFFF
 FS_DEVERR_COUNT_OVERFLOW = 1
 FS_DEVERR_INTERNAL = 2
+FS_DEVERR_MASK = 8
+FS_F32, FS_BF16, FS_F16 = 0, 1, 2
+FS_MAX_TOP = 64
 
 # fs_row_params (include/ferro_sampler.h); field order follows ferro's SamplerParams (src/sampler.h:12-21).
 PARAMS_DTYPE = np.dtype([
@@ -32,6 +35,14 @@ PARAMS_DTYPE = np.dtype([
     ("repeat_last_n", np.int32), ("penalty_from", np.int32), ("softcap", np.float32),
 ])
 assert PARAMS_DTYPE.itemsize == 40
+
+
+class FsEdits(ctypes.Structure):
+    """fs_edits (include/ferro_sampler.h): device pointers of a call's masks and biases."""
+    _fields_ = [("d_mask", ctypes.c_void_p), ("mask_ld", ctypes.c_int64), ("n_masks", ctypes.c_int32),
+                ("d_mask_of", ctypes.c_void_p), ("d_bias_ids", ctypes.c_void_p), ("d_bias", ctypes.c_void_p),
+                ("d_bias_off", ctypes.c_void_p)]
+
 
 # Every symbol include/ferro_sampler.h declares, with its ctypes signature.
 _P = ctypes.c_void_p
@@ -49,6 +60,11 @@ SIGNATURES = {
     "fs_argmax_batch": (ctypes.c_int, [_P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P]),
     "fs_verify": (ctypes.c_int, [_P, _P, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _P]),
     "fs_verify_hp": (ctypes.c_int, [_P, _P, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _P]),
+    "fs_sample_edited": (ctypes.c_int, [_P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _P, _P]),
+    "fs_verify_edited": (ctypes.c_int, [_P, _P, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _P]),
+    "fs_decode_step_edited": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "fs_edit_batch": (ctypes.c_int, [_P, _P, _I32, _I64, _I32, _I32, _P, _P, _P, _P, _P, _I64, _P]),
+    "fs_logprobs": (ctypes.c_int, [_P, _P, _I32, _I64, _I32, _I32, _P, _P, _P, _I32, _P, _P, _P, _P, _P]),
     "fs_penalize_batch": (ctypes.c_int, [_P, _P, _I64, _I32, _I32, _P, _P, _P, _P]),
     "fs_softcap_batch": (ctypes.c_int, [_P, _P, _I64, ctypes.c_float, _P]),
     "fs_device_error": (ctypes.c_int, [_P, _P, _P]),

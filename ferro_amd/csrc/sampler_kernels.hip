@@ -153,6 +153,16 @@ struct fs_context {
     size_t stream_cap = 0;
     int32_t* err = nullptr;        // [0]: error bits; [1]: dirty (a merge gave up; see fs_device_error); [2..3]: hflag_dev
     uint32_t merge_spins = fs::MERGE_SPINS;
+    float* ed_rows = nullptr;          // calls under edits: [ed_logits] edited logits,
+    fs_row_params* ed_params = nullptr;//   [ed_param_rows] their parameters,
+    uint32_t* ed_any = nullptr;        //   [ed_any_rows] whether a row has a candidate (left at 0),
+    double* ed_u = nullptr;            //   [ed_u_rows] a decode step's draws,
+    int64_t* ed_off = nullptr;         //   [ed_off_rows] zeros: the offsets of empty histories
+    size_t ed_logits = 0, ed_param_rows = 0, ed_any_rows = 0, ed_u_rows = 0, ed_off_rows = 0;
+    fs::LpPart* lp_part = nullptr;     // fs_logprobs: [lp_segs] segments' sums,
+    uint64_t* lp_lists = nullptr;      //   [lp_list_segs][LP_TOP] their largest logits,
+    uint32_t* lp_ticket = nullptr;     //   [lp_rows] segment tickets, left at 0
+    size_t lp_segs = 0, lp_list_segs = 0, lp_rows = 0;
     int static_dev = -1;       // device whose static workspace fs_sample_batch_static used with this context
     uint64_t* trace = nullptr; // FS_TRACE builds: phase timestamps, trace_cap entries (fs_trace_set)
     int64_t trace_cap = 0;
@@ -696,6 +706,136 @@ int launch(fs_context* ctx, fs::Args a, int64_t rows, int64_t streams, hipStream
     return rc != FS_OK ? rc : done;
 }
 
+// ---- calls under edits (fs_sample_edited, fs_verify_edited, fs_decode_step_edited)
+// The context on the current device, a workspace buffer for a call on st: under capture none may grow.
+int edited_ready(fs_context* c) {
+    const int rc = device_of(c);
+    if (rc != FS_OK) return rc;
+    int dev = -1;
+    if (hipGetDevice(&dev) != hipSuccess) return FS_E_HIP;
+    return dev == c->device ? FS_OK : FS_E_INVALID;
+}
+
+// Logits per thread and segments per row of the edit kernel: the larger segments where they fill the device.
+int edit_plan(int cus, int64_t B, int32_t V, int& nseg) {
+    int nl = 8;
+    if (B * (((int64_t)V + fs::SK_LT * 32 - 1) / (fs::SK_LT * 32)) < cus) nl = 4;
+    nseg = (int)(((int64_t)V + fs::SK_LT * nl * 4 - 1) / (fs::SK_LT * nl * 4));
+    return nl;
+}
+
+// The rows edited into the workspace, sampled there without penalties by whichever kernel takes them, and the call's end:
+// rows without a candidate, a window's accepted prefix. Right for every batch.
+int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params, const fs::EdArgs& ed, hipStream_t st) {
+    const bool verify = a.mode == fs::MODE_VERIFY, decode = a.dmt != nullptr;
+    const size_t B = (size_t)a.B, ld = ((size_t)a.V + 3) & ~(size_t)3;
+    int nseg = 0, nl = 0;
+    {
+        std::lock_guard<std::mutex> g(ctx->mu);
+        int rc = edited_ready(ctx);
+        if (rc != FS_OK) return rc;
+        nl = edit_plan(ctx->cus, a.B, a.V, nseg);
+        if ((int64_t)a.B * nseg > 0x7fffffff) return FS_E_INVALID;
+        const bool zeros = decode && !a.hist_off;
+        if (capturing(st)) {
+            if (B * ld > ctx->ed_logits || B > ctx->ed_param_rows || B > ctx->ed_any_rows ||
+                (decode && B > ctx->ed_u_rows) || (zeros && B + 1 > ctx->ed_off_rows) || !ctx->err)
+                return FS_E_NOMEM;
+            ctx->captured = true;
+        } else {
+            rc = grow(ctx, 0, 0, 0);
+            if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_rows, ctx->ed_logits, B * ld, 1, false);
+            if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_params, ctx->ed_param_rows, B, 1, false);
+            if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_any, ctx->ed_any_rows, B, 1, true);
+            if (rc == FS_OK && decode) rc = grow_buffer(ctx, ctx->ed_u, ctx->ed_u_rows, B, 1, false);
+            if (rc == FS_OK && zeros) rc = grow_buffer(ctx, ctx->ed_off, ctx->ed_off_rows, B + 1, 1, true);
+            if (rc != FS_OK) return rc;
+        }
+    }
+    fs::EditArgs e = {};
+    e.logits = a.logits; e.type = FS_F32; e.ld = a.ld; e.B = a.B; e.V = a.V; e.nseg = nseg;
+    e.hist = a.hist; e.hist_off = a.hist_off; e.params = a.params; e.ed = ed;
+    if (verify) { e.rows = a.rows; e.row_off = a.row_off; e.n_streams = a.n_streams; }
+    e.out = ctx->ed_rows; e.out_ld = (int64_t)ld; e.err = ctx->err; e.any = ctx->ed_any; e.rparams = ctx->ed_params;
+    if (fs::launch_edit(nl, e, st) != hipSuccess) return FS_E_HIP;
+
+    fs::Args s = {};
+    s.logits = ctx->ed_rows; s.ld = (int64_t)ld; s.B = a.B; s.V = a.V; s.params = ctx->ed_params; s.u = a.u; s.tok = a.tok;
+    s.kcap = a.kcap; s.cand_ids = a.cand_ids; s.cand_probs = a.cand_probs; s.keep = a.keep;
+    s.mode = fs::MODE_SAMPLE; s.eos = -1;
+    if (decode) {
+        hipLaunchKernelGGL(fs::drng_draw_kernel, dim3((unsigned)((B + 63) / 64)), dim3(64), 0, st, a.dmt, a.didx, a.B,
+                           (const int64_t*)nullptr, a.params, ctx->ed_u, 0, ctx->err);
+        if (hipGetLastError() != hipSuccess) return FS_E_HIP;
+        s.u = ctx->ed_u;
+    }
+    int rc = FS_OK;
+    bool used = false;
+    std::unique_ptr<fs_row_params[]> h;
+    if (h_params && !verify) {                     // (a window's rows have their streams' parameters, known on the device)
+        h.reset(new (std::nothrow) fs_row_params[B]);
+        if (!h) return FS_E_NOMEM;
+        for (size_t b = 0; b < B; ++b) {
+            h[b] = h_params[b];
+            h[b].repetition_penalty = 1.0f; h[b].frequency_penalty = 0.0f; h[b].presence_penalty = 0.0f;
+            h[b].repeat_last_n = 0; h[b].penalty_from = 0; h[b].softcap = 0.0f;
+        }
+        rc = launch_small(ctx, s, h.get(), st, used);
+        if (rc == FS_OK && !used) rc = launch_mid(ctx, s, h.get(), st, used, mixed_merges(h.get(), a.B, a.V) ? 4 : 2);
+        if (rc < 0) return rc;
+    }
+    if (!used) rc = launch(ctx, s, a.B, 0, st, h ? (mixed_merges(h.get(), a.B, a.V) ? 4 : 2) : 2);
+    if (rc < 0) return rc;
+
+    fs::EditEnd f = {};
+    f.B = a.B; f.any = ctx->ed_any; f.rparams = ctx->ed_params; f.tok = a.tok; f.keep = a.keep;
+    f.kcap = a.kcap; f.cand_ids = a.cand_ids; f.cand_probs = a.cand_probs;
+    if (verify) {
+        f.rows = a.rows; f.row_off = a.row_off; f.n_streams = a.n_streams; f.eos = a.eos; f.accepted = a.accepted;
+    }
+    if (fs::launch_edit_end(f, st) != hipSuccess) return FS_E_HIP;
+    if (decode) {
+        const int32_t* hist = a.hist ? a.hist : a.tok;         // (empty histories: never read)
+        const int64_t* off = a.hist_off ? a.hist_off : ctx->ed_off;
+        if (fs::launch_hist_append(a.B, hist, off, a.tok, nullptr, nullptr, a.out_hist, a.out_hist_off, a.out_cap, ctx->err,
+                                   st) != hipSuccess)
+            return FS_E_HIP;
+    }
+    return rc;
+}
+
+int launch_edited(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params, const fs::EdArgs& ed, hipStream_t st) {
+    return launch_composed(ctx, a, h_params, ed, st);
+}
+
+// The host's checks of a call's edits; `edits` NULL: none.
+int edit_args(const fs_edits* edits, int32_t rows, int32_t V, fs::EdArgs& ed) {
+    ed = {};
+    if (!edits) return FS_OK;
+    if (edits->d_mask) {
+        if (edits->mask_ld < ((int64_t)V + 31) / 32 || edits->n_masks < 0) return FS_E_INVALID;
+        if (!edits->d_mask_of && edits->n_masks < rows) return FS_E_INVALID;
+        if (((uintptr_t)edits->d_mask & 3u) != 0) return FS_E_INVALID;
+    } else if (edits->d_mask_of || edits->n_masks != 0) {
+        return FS_E_INVALID;
+    }
+    if (edits->d_bias_off ? (!edits->d_bias_ids || !edits->d_bias) : (edits->d_bias_ids || edits->d_bias)) return FS_E_INVALID;
+    ed.mask = edits->d_mask; ed.mask_ld = edits->mask_ld; ed.n_masks = edits->n_masks; ed.mask_of = edits->d_mask_of;
+    ed.bias_ids = edits->d_bias_ids; ed.bias = edits->d_bias; ed.bias_off = edits->d_bias_off;
+    return FS_OK;
+}
+
+size_t type_size(int32_t type) { return type == FS_F32 ? 4 : type == FS_BF16 || type == FS_F16 ? 2 : 0; }
+
+// Rows of logits of any type: check_rows for FS_F32, four logits' alignment for the others.
+int check_typed(const void* d_logits, int32_t type, int64_t ld, int32_t B, int32_t V) {
+    const size_t size = type_size(type);
+    if (size == 0 || !d_logits || B < 0 || V < 1 || V > FS_MAX_VOCAB || ld < V || (ld & 3) != 0 ||
+        ((uintptr_t)d_logits & (4 * size - 1)) != 0)
+        return FS_E_INVALID;
+    return FS_OK;
+}
+
 }  // namespace
 
 // ------------------------------------------------------------------------------------------------ static workspace
@@ -793,6 +933,14 @@ int fs_destroy(fs_context* c) {
     (void)hipFree(c->stream_cnt);
     (void)hipFree(c->err);
     (void)hipFree(c->greedy);
+    (void)hipFree(c->ed_rows);
+    (void)hipFree(c->ed_params);
+    (void)hipFree(c->ed_any);
+    (void)hipFree(c->ed_u);
+    (void)hipFree(c->ed_off);
+    (void)hipFree(c->lp_part);
+    (void)hipFree(c->lp_lists);
+    (void)hipFree(c->lp_ticket);
     for (void* p : c->retired) (void)hipFree(p);
     if (c->hflag) (void)hipHostFree(c->hflag);
     delete c;
@@ -995,6 +1143,115 @@ int fs_verify(fs_context* ctx, const float* d_logits, int64_t ld, int32_t n_stre
     return launch(ctx, a, total_rows, n_streams, (hipStream_t)stream);
 }
 
+int fs_sample_edited(fs_context* ctx, const float* d_logits, int64_t ld, int32_t B, int32_t V, const int32_t* d_hist,
+                     const int64_t* d_hist_off, const fs_row_params* d_params, const fs_row_params* h_params,
+                     const fs_edits* edits, const double* d_u, int32_t* d_tok, int32_t kcap, int32_t* d_cand_ids,
+                     double* d_cand_probs, int32_t* d_keep, void* stream) {
+    if (!ctx || !edits || !d_params || !d_tok || kcap < 0 || ((d_cand_ids || d_cand_probs) && kcap == 0))
+        return FS_E_INVALID;
+    int rc = check_rows(d_logits, ld, B, V);
+    if (rc != FS_OK) return rc;
+    fs::EdArgs ed;
+    rc = edit_args(edits, B, V, ed);
+    if (rc != FS_OK) return rc;
+    if (B == 0) return FS_OK;
+    fs::Args a = {};
+    a.logits = d_logits; a.ld = ld; a.B = B; a.V = V; a.hist = d_hist; a.hist_off = d_hist_off; a.params = d_params;
+    a.u = d_u; a.tok = d_tok; a.kcap = kcap; a.cand_ids = d_cand_ids; a.cand_probs = d_cand_probs; a.keep = d_keep;
+    a.mode = fs::MODE_SAMPLE; a.eos = -1;
+    return launch_edited(ctx, a, h_params, ed, (hipStream_t)stream);
+}
+
+int fs_verify_edited(fs_context* ctx, const float* d_logits, int64_t ld, int32_t n_streams, int32_t total_rows, int32_t V,
+                     const int32_t* d_rows, const int64_t* d_row_off, const int32_t* d_hist, const int64_t* d_hist_off,
+                     const fs_row_params* d_params, const fs_row_params* h_params, const fs_edits* edits,
+                     const double* d_u, int32_t eos_id, int32_t* d_tok, int32_t* d_accepted, void* stream) {
+    if (!ctx || !edits || !d_rows || !d_row_off || !d_params || !d_tok || !d_accepted || n_streams < 0 || total_rows < 0)
+        return FS_E_INVALID;
+    int rc = check_rows(d_logits, ld, total_rows, V);
+    if (rc != FS_OK) return rc;
+    fs::EdArgs ed;
+    rc = edit_args(edits, total_rows, V, ed);
+    if (rc != FS_OK) return rc;
+    if (total_rows == 0 || n_streams == 0) return FS_OK;
+    fs::Args a = {};
+    a.logits = d_logits; a.ld = ld; a.B = total_rows; a.V = V; a.hist = d_hist; a.hist_off = d_hist_off;
+    a.params = d_params; a.u = d_u; a.tok = d_tok; a.rows = d_rows; a.row_off = d_row_off; a.n_streams = n_streams;
+    a.eos = eos_id; a.accepted = d_accepted; a.mode = fs::MODE_VERIFY;
+    return launch_edited(ctx, a, h_params, ed, (hipStream_t)stream);
+}
+
+int fs_edit_batch(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld, int32_t B, int32_t V,
+                  const int32_t* d_hist, const int64_t* d_hist_off, const fs_row_params* d_params, const fs_edits* edits,
+                  float* d_out, int64_t out_ld, void* stream) {
+    if (!ctx || !d_out || out_ld < V || (out_ld & 3) != 0 || !aligned16(d_out)) return FS_E_INVALID;
+    int rc = check_typed(d_logits, type, ld, B, V);
+    if (rc != FS_OK) return rc;
+    fs::EditArgs e = {};
+    rc = edit_args(edits, B, V, e.ed);
+    if (rc != FS_OK) return rc;
+    if (B == 0) return FS_OK;
+    if (!(type == FS_F32 && d_out == d_logits && out_ld == ld)) {
+        const uintptr_t i0 = (uintptr_t)d_logits, i1 = i0 + ((size_t)(B - 1) * (size_t)ld + (size_t)V) * type_size(type);
+        const uintptr_t o0 = (uintptr_t)d_out, o1 = o0 + ((size_t)(B - 1) * (size_t)out_ld + (size_t)V) * sizeof(float);
+        if (i0 < o1 && o0 < i1) return FS_E_INVALID;
+    }
+    int nl = 0;
+    {
+        std::lock_guard<std::mutex> g(ctx->mu);
+        rc = edited_ready(ctx);
+        if (rc == FS_OK) rc = grow(ctx, 0, 0, 0);              // the error word
+        if (rc != FS_OK) return rc;
+        nl = edit_plan(ctx->cus, B, V, e.nseg);
+    }
+    if ((int64_t)B * e.nseg > 0x7fffffff) return FS_E_INVALID;
+    e.logits = d_logits; e.type = type; e.ld = ld; e.B = B; e.V = V;
+    e.hist = d_hist; e.hist_off = d_hist_off; e.params = d_params;
+    e.out = d_out; e.out_ld = out_ld; e.err = ctx->err;
+    return fs::launch_edit(nl, e, (hipStream_t)stream) == hipSuccess ? FS_OK : FS_E_HIP;
+}
+
+int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld, int32_t B, int32_t V,
+                const fs_row_params* d_params, const fs_edits* edits, const int32_t* d_tok, int32_t n, float* d_lp,
+                int32_t* d_rank, int32_t* d_top_ids, float* d_top_lp, void* stream) {
+    if (!ctx || n < 0 || n > FS_MAX_TOP || ((d_lp || d_rank) && !d_tok) || ((d_top_ids || d_top_lp) && n == 0))
+        return FS_E_INVALID;
+    int rc = check_typed(d_logits, type, ld, B, V);
+    if (rc != FS_OK) return rc;
+    fs::LpArgs a = {};
+    rc = edit_args(edits, B, V, a.ed);
+    if (rc != FS_OK) return rc;
+    if (B == 0) return FS_OK;
+    const hipStream_t st = (hipStream_t)stream;
+    const int top = d_top_ids || d_top_lp ? n : 0;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    rc = edited_ready(ctx);
+    if (rc != FS_OK) return rc;
+    int nl = 4;
+    for (const int l : {16, 8, 4}) {                           // the largest segments that give every CU four workgroups
+        nl = l;
+        a.nseg = (int)(((int64_t)V + fs::SK_LT * l * 4 - 1) / (fs::SK_LT * l * 4));
+        if ((int64_t)B * a.nseg >= 4 * (int64_t)ctx->cus) break;
+    }
+    if ((int64_t)B * a.nseg > 0x7fffffff) return FS_E_INVALID;
+    const size_t segs = (size_t)B * a.nseg;
+    if (capturing(st)) {
+        if (segs > ctx->lp_segs || (top > 0 && segs > ctx->lp_list_segs) || (size_t)B > ctx->lp_rows || !ctx->err)
+            return FS_E_NOMEM;
+        ctx->captured = true;
+    } else {
+        rc = grow(ctx, 0, 0, 0);
+        if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_part, ctx->lp_segs, segs, 1, false);
+        if (rc == FS_OK && top > 0) rc = grow_buffer(ctx, ctx->lp_lists, ctx->lp_list_segs, segs, fs::LP_TOP, false);
+        if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_ticket, ctx->lp_rows, (size_t)B, 1, true);
+        if (rc != FS_OK) return rc;
+    }
+    a.logits = d_logits; a.ld = ld; a.B = B; a.V = V; a.n = top; a.params = d_params; a.tok = d_tok;
+    a.lp = d_lp; a.rank = d_rank; a.ids = d_top_ids; a.top = d_top_lp;
+    a.part = ctx->lp_part; a.lists = ctx->lp_lists; a.ticket = ctx->lp_ticket; a.err = ctx->err;
+    return fs::launch_logprobs(nl, type, a, st) == hipSuccess ? FS_OK : FS_E_HIP;
+}
+
 int fs_penalize_batch(fs_context* ctx, float* d_logits, int64_t ld, int32_t B, int32_t V, const int32_t* d_hist,
                       const int64_t* d_hist_off, const fs_row_params* d_params, void* stream) {
     if (!ctx || !d_params) return FS_E_INVALID;
@@ -1192,6 +1449,30 @@ int fs_decode_step_hp(fs_context* ctx, fs_drng* r, const float* d_logits, int64_
         if (rc != FS_OK || used) return rc;
     }
     return launch(ctx, a, B, 0, (hipStream_t)stream);
+}
+
+int fs_decode_step_edited(fs_context* ctx, fs_drng* r, const float* d_logits, int64_t ld, int32_t B, int32_t V,
+                          const int32_t* d_hist, const int64_t* d_hist_off, const fs_row_params* d_params,
+                          const fs_row_params* h_params, const fs_edits* edits, int32_t* d_tok, int32_t* d_keep,
+                          int32_t* d_out_hist, int64_t* d_out_hist_off, int64_t out_cap, void* stream) {
+    if (!ctx || !r || !edits || !d_params || !d_tok || !d_out_hist_off || out_cap < 0 || (out_cap > 0 && !d_out_hist) ||
+        (d_hist == nullptr) != (d_hist_off == nullptr) || B > r->n)
+        return FS_E_INVALID;
+    int rc = check_rows(d_logits, ld, B, V);
+    if (rc != FS_OK) return rc;
+    fs::EdArgs ed;
+    rc = edit_args(edits, B, V, ed);
+    if (rc != FS_OK) return rc;
+    int dev = -1;
+    if (hipGetDevice(&dev) != hipSuccess) return FS_E_HIP;
+    if (dev != r->device) return FS_E_INVALID;
+    if (B == 0) return FS_OK;
+    fs::Args a = {};
+    a.logits = d_logits; a.ld = ld; a.B = B; a.V = V; a.hist = d_hist; a.hist_off = d_hist_off; a.params = d_params;
+    a.u = nullptr; a.tok = d_tok; a.kcap = 0; a.keep = d_keep;
+    a.mode = fs::MODE_SAMPLE; a.eos = -1;
+    a.dmt = r->mt; a.didx = r->idx; a.out_hist = d_out_hist; a.out_hist_off = d_out_hist_off; a.out_cap = out_cap;
+    return launch_edited(ctx, a, h_params, ed, (hipStream_t)stream);
 }
 
 int fs_decode_step(fs_context* ctx, fs_drng* r, const float* d_logits, int64_t ld, int32_t B, int32_t V,

@@ -14,6 +14,17 @@ struct Args;
 hipError_t launch_segments(const Args& a, unsigned grid, hipStream_t st);
 hipError_t launch_merges(const Args& a, unsigned rows, int nseg, int alone, hipStream_t st);
 
+// The edits of a call's logits (fs_edits) beside the penalties: masks of allowed tokens and biases.
+struct EdArgs {
+    const uint32_t* mask;                  // [n_masks][mask_ld] words (NULL: no masks)
+    int64_t mask_ld;
+    int n_masks;
+    const int32_t* mask_of;                // [rows] (NULL: row r takes mask r)
+    const int32_t* bias_ids;               // CSR, ids ascending (bias_off NULL: no biases)
+    const float* bias;
+    const int64_t* bias_off;
+};
+
 constexpr int SK_LT = 256;                 // threads per segment workgroup
 constexpr int SK_NW = SK_LT / 64;
 constexpr int SK_K = 64;                   // largest k (one candidate per lane of the finishing wave)
@@ -81,6 +92,69 @@ struct MkArgs {
 };
 // all: some row samples with every token a candidate
 hipError_t launch_mid_k(int nl, bool capped, bool all, unsigned grid, int flags, const MkArgs& m, hipStream_t st);
+
+// Edited logits written out (edit_kernels.hip). nl: groups of four logits per thread (4 or 8).
+struct EditArgs {
+    const void* logits;
+    int type;                              // FS_F32, FS_BF16, FS_F16
+    int64_t ld;
+    int B, V, nseg;
+    const int32_t* hist;
+    const int64_t* hist_off;
+    const fs_row_params* params;           // NULL: no softcap, no penalties
+    EdArgs ed;
+    const int32_t* rows;                   // verification windows (n_streams > 0): params, histories and biases by stream
+    const int64_t* row_off;
+    int n_streams;
+    float* out;
+    int64_t out_ld;
+    int32_t* err;
+    uint32_t* any;                         // rows for the sampling kernels: [B], nonzero where a row has a candidate (else NULL)
+    fs_row_params* rparams;                //   and their parameters, the penalties and the softcap off
+};
+hipError_t launch_edit(int nl, const EditArgs& e, hipStream_t st);
+
+// The end of a sampling call on such rows: rows without a candidate get token -1, then a window's accepted prefixes.
+struct EditEnd {
+    int B;
+    uint32_t* any;                         // left at 0
+    const fs_row_params* rparams;
+    int32_t* tok;
+    int32_t* keep;
+    int kcap;
+    int32_t* cand_ids;
+    double* cand_probs;
+    const int32_t* rows;
+    const int64_t* row_off;
+    int n_streams, eos;
+    int32_t* accepted;
+};
+hipError_t launch_edit_end(const EditEnd& e, hipStream_t st);
+
+// Log-probabilities (logprob_kernel.hip).
+constexpr int LP_TOP = 64;                 // largest n: one entry per lane of the finishing wave
+struct LpPart {                            // a segment's share of its row
+    double sum;                            // of exp((x - max) / T)
+    float max;
+    uint32_t above;                        // logits above the chosen token's
+};
+struct LpArgs {
+    const void* logits;
+    int64_t ld;
+    int B, V, nseg, n;
+    const fs_row_params* params;           // NULL: no softcap, temperature 1
+    EdArgs ed;
+    const int32_t* tok;
+    float* lp;
+    int32_t* rank;
+    int32_t* ids;                          // [B][n]
+    float* top;
+    LpPart* part;                          // [B][nseg]
+    uint64_t* lists;                       // [B][nseg][LP_TOP]
+    uint32_t* ticket;                      // [B], left at 0
+    int32_t* err;
+};
+hipError_t launch_logprobs(int nl, int type, const LpArgs& a, hipStream_t st);
 
 hipError_t launch_lookup_draft(int n_streams, const int32_t* hist, const int64_t* hist_off, const int32_t* kmax,
                                const int32_t* min_n, int eos, int32_t* draft, int draft_ld, int32_t* ndraft,

@@ -6,6 +6,8 @@
   stream (one draw per non-greedy call, none for greedy: sampler.cpp:19-23, 45-46).
 - `sample_batch`, `argmax_batch`, `verify` are the batched device entry points (fs_sample_batch, fs_argmax_batch,
   fs_verify) on torch CUDA tensors, launched on torch's current stream.
+- `Edits` holds masks of allowed tokens and biases (fs_edits) for those calls and `decode_step`; `edit_batch` writes
+  edited logits out, `logprobs` gives log-probabilities.
 
 PyTorch only supplies device memory and streams; all sampling arithmetic runs in libferro_sampler.so.
 """
@@ -18,10 +20,12 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from ._lib import PARAMS_DTYPE, FS_OK, SamplerError, check, lib
+from ._lib import FS_BF16, FS_F16, FS_F32, FS_MAX_TOP, PARAMS_DTYPE, FS_OK, FsEdits, SamplerError, check, lib
 
-__all__ = ["SamplerParams", "Sampler", "Context", "Rng", "params_array", "sample_batch", "argmax_batch", "verify",
-           "device_error", "PARAMS_DTYPE", "SamplerError"]
+__all__ = ["SamplerParams", "Sampler", "Context", "Rng", "Edits", "params_array", "sample_batch", "argmax_batch", "verify",
+           "edit_batch", "logprobs", "device_error", "PARAMS_DTYPE", "SamplerError"]
+
+F32, BF16, F16 = FS_F32, FS_BF16, FS_F16          # types of logits (edit_batch, logprobs)
 
 
 @dataclass
@@ -86,6 +90,11 @@ def _dev(x, dtype, device):
 def _stream(stream=None):
     s = stream if stream is not None else torch.cuda.current_stream()
     return ctypes.c_void_p(s.cuda_stream)
+
+
+def _hptr(a):
+    """Host pointer of a numpy array (None: NULL)."""
+    return None if a is None else a.ctypes.data_as(ctypes.c_void_p)
 
 
 def _dev_params(params, device) -> torch.Tensor:
@@ -245,10 +254,129 @@ def _hist_tensors(hist, hist_off, B, device):
 ROUTE = "host"
 
 
-def sample_batch(logits, params, u, hist=None, hist_off=None, V=None, kcap=0, ctx=None, stream=None, route=None):
+class Edits:
+    """Masks of allowed tokens and biases (fs_edits): what a program keeps from step to step for edits= of sample_batch,
+    argmax_batch, verify, decode_step, edit_batch and logprobs.
+
+    mask: int32 or uint32 words [n, W] (or [W]: one mask), W >= ceil(V / 32); token t is allowed where bit t % 32 of word
+    t // 32 is set (as grammar engines write them; `pack` makes them from truth values). mask_of: each logits row's mask,
+    negative: every token is allowed (default: row r takes mask r). bias: one {token: bias} per record, or CSR (ids,
+    values, offsets) with ids ascending within a record; a record per row, per stream in verify. Arrays go to `device`
+    here; device tensors are used in place, so a program may write the next step's masks into them."""
+
+    def __init__(self, mask=None, mask_of=None, bias=None, device=None):
+        dev = torch.device("cuda" if device is None else device)
+        if device is None:
+            given = [mask, mask_of] + (list(bias) if isinstance(bias, tuple) else [])
+            dev = next((t.device for t in given if isinstance(t, torch.Tensor) and t.is_cuda), dev)
+        if dev.type == "cuda" and dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        self.mask = self.mask_of = self.bias_ids = self.bias = self.bias_off = None
+        if mask is not None:
+            if isinstance(mask, np.ndarray) and mask.dtype == np.uint32:
+                mask = mask.view(np.int32)
+            mask = torch.as_tensor(mask)
+            if mask.dtype == torch.uint32:
+                mask = mask.view(torch.int32)
+            if mask.dtype != torch.int32 or mask.dim() not in (1, 2):
+                raise SamplerError("masks must be int32 or uint32 words [n, W]")
+            mask = (mask.unsqueeze(0) if mask.dim() == 1 else mask).to(dev)
+            if mask.shape[1] > 1 and mask.stride(1) != 1 or (mask.shape[0] > 1 and mask.stride(0) < mask.shape[1]):
+                mask = mask.contiguous()
+            self.mask = mask
+        if mask_of is not None:
+            if mask is None:
+                raise SamplerError("mask_of needs masks")
+            self.mask_of = _dev(mask_of, torch.int32, dev)
+        if bias is not None:
+            if not isinstance(bias, tuple):
+                bias = self._csr(bias)
+            ids, val, off = bias
+            if not any(isinstance(t, torch.Tensor) and t.is_cuda for t in bias):
+                self._check(np.asarray(ids, np.int64), np.asarray(val), np.asarray(off, np.int64))
+            self.bias_ids, self.bias = _dev(ids, torch.int32, dev), _dev(val, torch.float32, dev)
+            self.bias_off = _dev(off, torch.int64, dev)
+            if self.bias_ids.numel() != self.bias.numel() or self.bias_off.numel() < 1:
+                raise SamplerError("biases are CSR lists (ids, values, offsets)")
+            if self.bias_ids.numel() == 0:                    # no bias at all: valid pointers, never read
+                self.bias_ids = torch.zeros(1, dtype=torch.int32, device=dev)
+                self.bias = torch.zeros(1, dtype=torch.float32, device=dev)
+        self.device = dev
+        self.c = FsEdits()
+        if self.mask is not None:
+            self.c.d_mask = self.mask.data_ptr()
+            self.c.mask_ld = self.mask.stride(0) if self.mask.shape[0] > 1 else self.mask.shape[1]
+            self.c.n_masks = self.mask.shape[0]
+            self.c.d_mask_of = self.mask_of.data_ptr() if self.mask_of is not None else None
+        if self.bias_off is not None:
+            self.c.d_bias_ids, self.c.d_bias = self.bias_ids.data_ptr(), self.bias.data_ptr()
+            self.c.d_bias_off = self.bias_off.data_ptr()
+
+    @staticmethod
+    def _csr(dicts):
+        rows = [sorted((int(t), float(b)) for t, b in (d or {}).items()) for d in dicts]
+        off = np.zeros(len(rows) + 1, np.int64)
+        off[1:] = np.cumsum([len(r) for r in rows])
+        flat = [e for r in rows for e in r]
+        return (np.array([t for t, _ in flat], np.int32), np.array([b for _, b in flat], np.float32), off)
+
+    @staticmethod
+    def _check(ids, val, off):
+        if ids.ndim != 1 or val.shape != ids.shape or off.ndim != 1 or off.size < 1 or off[0] < 0 or off[-1] > ids.size \
+                or np.any(np.diff(off) < 0):
+            raise SamplerError("biases are CSR lists (ids, values, offsets)")
+        step = np.diff(ids) < 0                               # descents are only allowed where a record begins
+        step[[o - 1 for o in off if 0 < o < ids.size]] = False
+        if np.any(step[off[0]:max(off[-1] - 1, off[0])]):
+            raise SamplerError("the ids of a record's biases must ascend")
+
+    @staticmethod
+    def pack(allowed):
+        """Mask words from truth values [n, V] (or [V]): int32 [n, ceil(V / 32)]."""
+        if isinstance(allowed, torch.Tensor):
+            a = allowed.bool()
+            a = a.unsqueeze(0) if a.dim() == 1 else a
+            a = torch.nn.functional.pad(a, (0, (-a.shape[1]) % 32)).view(a.shape[0], -1, 32)
+            bit = 1 << torch.arange(32, dtype=torch.int64, device=a.device)
+            return (a * bit).sum(2).to(torch.int32)
+        a = np.atleast_2d(np.asarray(allowed, bool))
+        a = np.pad(a, ((0, 0), (0, (-a.shape[1]) % 32)))
+        return np.packbits(a, axis=1, bitorder="little").view(np.int32)
+
+    def _ref(self, rows: int, records: int, V: int, dev):
+        """The checked fs_edits for a call of `rows` logits rows and `records` records."""
+        if dev != self.device:
+            raise SamplerError(f"edits on {self.device}, logits on {dev}")
+        if self.mask is not None:
+            if self.mask.shape[1] * 32 < V:
+                raise SamplerError(f"masks of {self.mask.shape[1]} words for {V} tokens")
+            if (self.mask_of.numel() != rows) if self.mask_of is not None else (self.mask.shape[0] < rows):
+                raise SamplerError("one mask index per row" if self.mask_of is not None else "one mask per row")
+        if self.bias_off is not None and self.bias_off.numel() != records + 1:
+            raise SamplerError("one bias list per record")
+        return ctypes.byref(self.c)
+
+
+def _on(stream, dev, *tensors):
+    """The stream of a call on device `dev`, as the C ABI takes it. A stream other than the current one first waits for
+    the current one, on which the wrapper's tensors are made, and is known to their allocator as a user."""
+    cur = torch.cuda.current_stream(dev)
+    if stream is not None and stream.cuda_stream != cur.cuda_stream:
+        stream.wait_stream(cur)
+        for t in tensors:
+            if t is not None and t.is_cuda:
+                t.record_stream(stream)
+        return ctypes.c_void_p(stream.cuda_stream)
+    return ctypes.c_void_p(cur.cuda_stream)
+
+
+def sample_batch(logits, params, u, hist=None, hist_off=None, V=None, kcap=0, ctx=None, stream=None, route=None,
+                 edits=None):
     """fs_sample_batch(_hp) on device tensors: logits [B, ld] fp32 (rows 16-byte aligned), params (B records),
     u [B] float64 draws, hist/hist_off CSR histories. Returns dict(tok, keep, cand_ids, cand_probs) (device).
-    route: "host" / "device" (default: the module's ROUTE); params given as a device tensor always go "device"."""
+    route: "host" / "device" (default: the module's ROUTE); params given as a device tensor always go "device".
+    edits: an Edits, the masks and biases the rows are sampled under (fs_sample_edited); a row without a candidate has
+    token -1."""
     logits, ld, n = _check_logits(logits, V)
     B = logits.shape[0]
     dev = logits.device
@@ -265,6 +393,13 @@ def sample_batch(logits, params, u, hist=None, hist_off=None, V=None, kcap=0, ct
     hp = None                                             # the host copy of the parameters picks the kernel
     if (route or ROUTE) == "host" and not isinstance(params, torch.Tensor):
         hp = params_array(params)
+    if edits is not None:
+        with torch.cuda.device(dev), ctx.lock:
+            check(lib().fs_sample_edited(ctx.h, _lptr(logits), ld, B, n, _ptr(hist), _ptr(hist_off), _ptr(p), _hptr(hp),
+                                         edits._ref(B, B, n, dev), _ptr(u), _ptr(tok), kcap, _ptr(ids), _ptr(probs),
+                                         _ptr(keep), _on(stream, dev, logits, p, u, hist, hist_off, tok, keep, ids, probs)),
+                  "fs_sample_edited")
+        return dict(tok=tok, keep=keep, cand_ids=ids, cand_probs=probs, _keepalive=(p, u, hist, hist_off))
     with ctx.lock:
         if hp is not None:
             check(lib().fs_sample_batch_hp(ctx.h, _lptr(logits), ld, B, n, _ptr(hist), _ptr(hist_off), _ptr(p),
@@ -277,8 +412,22 @@ def sample_batch(logits, params, u, hist=None, hist_off=None, V=None, kcap=0, ct
     return dict(tok=tok, keep=keep, cand_ids=ids, cand_probs=probs, _keepalive=(p, u, hist, hist_off))
 
 
-def argmax_batch(logits, hist=None, hist_off=None, params=None, V=None, ctx=None, stream=None):
-    """fs_argmax_batch: greedy token per row after the penalties of `params` (None = no penalty)."""
+def argmax_batch(logits, hist=None, hist_off=None, params=None, V=None, ctx=None, stream=None, edits=None):
+    """fs_argmax_batch: greedy token per row after the penalties of `params` (None = no penalty). edits: the masks and
+    biases of the rows (fs_sample_edited with greedy records); a row without a candidate has token -1."""
+    if edits is not None:
+        B = logits.shape[0] if logits.dim() == 2 else 1
+        if isinstance(params, torch.Tensor):
+            params = params.clone()
+            params.view(torch.float32).view(-1, PARAMS_DTYPE.itemsize // 4)[:, 0] = 0.0
+        else:
+            g = np.zeros(B, PARAMS_DTYPE) if params is None else params_array(params).copy()
+            g["temperature"] = 0.0
+            if params is None:
+                g["repetition_penalty"], g["top_p"], hist = 1.0, 1.0, None
+            params = g
+        return sample_batch(logits, params, np.zeros(B), hist=hist, hist_off=hist_off, V=V, ctx=ctx, stream=stream,
+                            edits=edits)["tok"]
     logits, ld, n = _check_logits(logits, V)
     B = logits.shape[0]
     dev = logits.device
@@ -293,9 +442,10 @@ def argmax_batch(logits, hist=None, hist_off=None, params=None, V=None, ctx=None
 
 
 def verify(logits, rows, row_off, params, u=None, hist=None, hist_off=None, eos_id=-1, V=None, ctx=None,
-           stream=None, route=None):
+           stream=None, route=None, edits=None):
     """fs_verify(_hp): per-row tokens and per-stream accepted prefix lengths of a speculative window. route as for
-    sample_batch ("host": the host copy of the stream parameters goes along, fs_verify_hp)."""
+    sample_batch ("host": the host copy of the stream parameters goes along, fs_verify_hp). edits: masks by row and
+    biases by stream (fs_verify_edited); a row without a candidate has token -1 and ends its window."""
     logits, ld, n = _check_logits(logits, V)
     R = logits.shape[0]
     dev = logits.device
@@ -313,6 +463,14 @@ def verify(logits, rows, row_off, params, u=None, hist=None, hist_off=None, eos_
     hp = None
     if (route or ROUTE) == "host" and not isinstance(params, torch.Tensor):
         hp = params_array(params)
+    if edits is not None:
+        with torch.cuda.device(dev), ctx.lock:
+            check(lib().fs_verify_edited(ctx.h, _lptr(logits), ld, S, R, n, _ptr(rows), _ptr(row_off), _ptr(hist),
+                                         _ptr(hist_off), _ptr(p), _hptr(hp), edits._ref(R, S, n, dev), _ptr(u), int(eos_id),
+                                         _ptr(tok), _ptr(acc),
+                                         _on(stream, dev, logits, rows, row_off, p, u, hist, hist_off, tok, acc)),
+                  "fs_verify_edited")
+        return tok, acc
     with ctx.lock:
         if hp is not None:
             check(lib().fs_verify_hp(ctx.h, _lptr(logits), ld, S, R, n, _ptr(rows), _ptr(row_off), _ptr(hist),
@@ -395,12 +553,13 @@ def hist_append(hist, hist_off, tok, row_off=None, count=None, out_cap=None, ctx
 
 
 def decode_step(logits, params, rng, hist=None, hist_off=None, out_cap=None, V=None, ctx=None, stream=None,
-                route=None):
+                route=None, edits=None):
     """fs_decode_step(_hp): one decode step in one launch - each row's draw from its DeviceRng stream (row s = stream
     s), fs_sample_batch's token, and the token appended to the stream's history (server.cpp:603-606, then :342).
     Returns (tok, keep, out_hist, out_off); out_hist holds out_cap ids (default: room for one more per stream), of
     which out_off[-1] are used. Stays on the device. route as for sample_batch ("host": the host copy of the
-    parameters goes along, fs_decode_step_hp)."""
+    parameters goes along, fs_decode_step_hp). edits: the rows' masks and biases (fs_decode_step_edited); a row without a
+    candidate appends token -1."""
     logits, ld, n = _check_logits(logits, V)
     B = logits.shape[0]
     dev = logits.device
@@ -418,6 +577,14 @@ def decode_step(logits, params, rng, hist=None, hist_off=None, out_cap=None, V=N
     out_off = torch.empty(B + 1, dtype=torch.int64, device=dev)
     ctx = ctx or Context.default(dev)
     hp = params_array(params) if (route or ROUTE) == "host" and not isinstance(params, torch.Tensor) else None
+    if edits is not None:
+        with torch.cuda.device(dev), ctx.lock:
+            check(lib().fs_decode_step_edited(ctx.h, rng.h, _lptr(logits), ld, B, n, _ptr(hist), _ptr(hist_off), _ptr(p),
+                                              _hptr(hp), edits._ref(B, B, n, dev), _ptr(tok), _ptr(keep), _ptr(out),
+                                              _ptr(out_off), int(out_cap),
+                                              _on(stream, dev, logits, p, hist, hist_off, tok, keep, out, out_off)),
+                  "fs_decode_step_edited")
+        return tok, keep, out, out_off
     with ctx.lock:
         if hp is not None:
             check(lib().fs_decode_step_hp(ctx.h, rng.h, _lptr(logits), ld, B, n, _ptr(hist), _ptr(hist_off), _ptr(p),
@@ -428,6 +595,90 @@ def decode_step(logits, params, rng, hist=None, hist_off=None, out_cap=None, V=N
                                        _ptr(tok), _ptr(keep), _ptr(out), _ptr(out_off), int(out_cap),
                                        _stream(stream)), "fs_decode_step")
     return tok, keep, out, out_off
+
+
+_TYPES = {torch.float32: FS_F32, torch.bfloat16: FS_BF16, torch.float16: FS_F16}
+
+
+def _typed_logits(logits, V):
+    """(logits, ld, V, type) of a [B, ld] or [ld] device tensor of any type; other layouts are repacked."""
+    if not (isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dtype in _TYPES):
+        raise SamplerError("logits must be a float32, bfloat16 or float16 CUDA tensor")
+    if logits.dim() == 1:
+        logits = logits.unsqueeze(0)
+    if logits.dim() != 2:
+        raise SamplerError("logits must be [B, V]")
+    n = logits.shape[1] if V is None else V
+    if n > logits.shape[1]:
+        raise SamplerError("V exceeds the row length")
+    ld = logits.stride(0) if logits.shape[0] > 1 else n + (-n) % 4
+    if (n > 1 and logits.stride(1) != 1) or ld % 4 or ld < n or logits.data_ptr() % (4 * logits.element_size()) \
+            or (logits.shape[0] == 1 and n % 4):              # (a lone row's last four must lie inside its buffer)
+        padded = torch.zeros((logits.shape[0], n + (-n) % 4), dtype=logits.dtype, device=logits.device)
+        padded[:, :n] = logits[:, :n]
+        logits, ld = padded, padded.stride(0)
+    return logits, ld, n, _TYPES[logits.dtype]
+
+
+def edit_batch(logits, params=None, hist=None, hist_off=None, edits=None, V=None, out=None, ctx=None, stream=None):
+    """fs_edit_batch: the edited logits in float32 [B, V] - softcap, biases, penalties, -inf where the row's mask does not
+    allow a token. logits [B, ld] float32, bfloat16 or float16; params (B records; None: no softcap, no penalties).
+    out: a float32 [B, >= V] tensor with 16-byte aligned rows, logits itself included (default: a new one); returned."""
+    logits, ld, n, kind = _typed_logits(logits, V)
+    B, dev = logits.shape[0], logits.device
+    p = None
+    if params is not None:
+        p = _dev_params(params, dev)
+        if p.numel() != B * PARAMS_DTYPE.itemsize:
+            raise SamplerError("one params record per row")
+    hist, hist_off = _hist_tensors(hist, hist_off, B, dev)
+    if out is None:
+        out = torch.empty((B, n + (-n) % 4), dtype=torch.float32, device=dev)[:, :n]
+    o2 = out.unsqueeze(0) if out.dim() == 1 else out
+    out_ld = o2.stride(0) if B > 1 else n + (-n) % 4
+    if o2.dtype != torch.float32 or o2.device != dev or o2.dim() != 2 or o2.shape[0] != B or o2.shape[1] < n \
+            or (o2.shape[1] > 1 and o2.stride(1) != 1):
+        raise SamplerError("out must be a float32 [B, V] tensor on the logits' device with packed rows")
+    if B == 1 and o2.data_ptr() == logits.data_ptr():
+        out_ld = ld
+    ctx = ctx or Context.default(dev)
+    with torch.cuda.device(dev), ctx.lock:
+        check(lib().fs_edit_batch(ctx.h, _lptr(logits), kind, ld, B, n, _ptr(hist), _ptr(hist_off), _ptr(p),
+                                  None if edits is None else edits._ref(B, B, n, dev), ctypes.c_void_p(o2.data_ptr()),
+                                  out_ld, _on(stream, dev, logits, p, hist, hist_off, out)), "fs_edit_batch")
+    return out
+
+
+def logprobs(logits, tok=None, n=0, params=None, edits=None, V=None, ctx=None, stream=None):
+    """fs_logprobs: log-probabilities under softmax((softcap(l) + bias) / T) over the allowed tokens. logits [B, ld]
+    float32, bfloat16 or float16; params (B records, their softcap and temperature; None: the logits' own distribution).
+    Returns dict(lp [B], rank [B]) of the tokens `tok` [B] and dict entries ids, top [B, n] of the n largest (None where
+    not asked for)."""
+    logits, ld, v, kind = _typed_logits(logits, V)
+    B, dev = logits.shape[0], logits.device
+    if not 0 <= n <= FS_MAX_TOP:
+        raise SamplerError(f"n must lie in [0, {FS_MAX_TOP}]")
+    p = None
+    if params is not None:
+        p = _dev_params(params, dev)
+        if p.numel() != B * PARAMS_DTYPE.itemsize:
+            raise SamplerError("one params record per row")
+    t = lp = rank = ids = top = None
+    if tok is not None:
+        t = _dev(tok, torch.int32, dev)
+        if t.numel() != B:
+            raise SamplerError("one token per row")
+        lp = torch.empty(B, dtype=torch.float32, device=dev)
+        rank = torch.empty(B, dtype=torch.int32, device=dev)
+    if n:
+        ids = torch.empty((B, n), dtype=torch.int32, device=dev)
+        top = torch.empty((B, n), dtype=torch.float32, device=dev)
+    ctx = ctx or Context.default(dev)
+    with torch.cuda.device(dev), ctx.lock:
+        check(lib().fs_logprobs(ctx.h, _lptr(logits), kind, ld, B, v, _ptr(p),
+                                None if edits is None else edits._ref(B, B, v, dev), _ptr(t), n, _ptr(lp), _ptr(rank),
+                                _ptr(ids), _ptr(top), _on(stream, dev, logits, p, t, lp, rank, ids, top)), "fs_logprobs")
+    return dict(lp=lp, rank=rank, ids=ids, top=top)
 
 
 def device_error(ctx=None, stream=None) -> int:

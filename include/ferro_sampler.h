@@ -46,6 +46,13 @@ extern "C" {
 #define FS_DEVERR_HIST_APPEND 4      /* fs_hist_append: the new histories exceed out_cap (ids past it are not
                                         written), or a count lies outside [0, its stream's rows] (clamped) */
 
+#define FS_DEVERR_MASK 8             /* a row's mask index lies past the last mask: no token of the row is allowed */
+
+/* Types of logits (fs_edit_batch, fs_logprobs; the sampling calls read FS_F32). */
+#define FS_F32 0
+#define FS_BF16 1
+#define FS_F16 2
+
 /* Limits. A row is read through one buffer resource (32-bit byte range): V * 4 < 2^31. */
 #define FS_MAX_VOCAB (1 << 28)
 
@@ -250,6 +257,65 @@ int fs_decode_step_hp(fs_context* ctx, fs_drng* r, const float* d_logits, int64_
  * left untouched. Same row layout rules as fs_sample_batch. */
 int fs_penalize_batch(fs_context* ctx, float* d_logits, int64_t ld, int32_t B, int32_t V, const int32_t* d_hist,
                       const int64_t* d_hist_off, const fs_row_params* d_params, void* stream);
+
+/* What a call edits in its logits beside the penalties: masks of allowed tokens (a grammar's or a tool schema's, as the
+ * engines that compile them write them) and biases (a request's logit_bias). The edited logit of token t in row r is
+ *     pen(cap(l) + bias(t)),   -inf where the row's mask does not allow t:
+ * the softcap first, then the biases, then the repetition and the frequency / presence penalties, each step rounded to
+ * fp32. The struct is read before the call returns; its pointers are device memory. No counterpart in the reference
+ * (ferro has no grammars and no logit_bias). */
+typedef struct fs_edits {
+    const uint32_t* d_mask;     /* [n_masks][mask_ld] words: token t is allowed where bit t % 32 of word t / 32 is set; bits
+                                   past the vocabulary do not matter. NULL: no masks */
+    int64_t mask_ld;            /* words from a mask to the next, >= ceil(V / 32) */
+    int32_t n_masks;
+    const int32_t* d_mask_of;   /* [rows] each logits row's mask; negative: every token is allowed; >= n_masks: none is, and
+                                   FS_DEVERR_MASK is set. NULL: row r takes mask r */
+    const int32_t* d_bias_ids;  /* biases of record s: [d_bias_off[s], d_bias_off[s+1]), ids ascending within a record; equal */
+    const float* d_bias;        /* ids add up one after another; ids outside [0, V) are ignored. A bias of -inf bans its token */
+    const int64_t* d_bias_off;  /* [records + 1]: a record per row, per stream in fs_verify_edited. NULL: no biases */
+} fs_edits;
+
+/* Sampling under edits: fs_sample_batch_hp, fs_verify_hp and fs_decode_step_hp on the edited logits, with the same
+ * arguments and outputs beside `edits` (h_params may be NULL here too; edits may not). A row's candidates are its allowed
+ * tokens whose edited logit is above -inf: k, min-p and top-p count those alone. A row without a candidate has token -1
+ * and 0 kept (a greedy row's candidate outputs are -1 and 0); -1 ends a verification window at its row, and fs_decode_step_
+ * edited appends it to the history, where the penalties ignore it. The rows are edited into a workspace of V * 4 bytes a
+ * row first, which grows as a context's other buffers do (a call under graph capture that would need a larger one
+ * returns FS_E_NOMEM). */
+int fs_sample_edited(fs_context* ctx, const float* d_logits, int64_t ld, int32_t B, int32_t V, const int32_t* d_hist,
+                     const int64_t* d_hist_off, const fs_row_params* d_params, const fs_row_params* h_params,
+                     const fs_edits* edits, const double* d_u, int32_t* d_tok, int32_t kcap, int32_t* d_cand_ids,
+                     double* d_cand_probs, int32_t* d_keep, void* stream);
+int fs_verify_edited(fs_context* ctx, const float* d_logits, int64_t ld, int32_t n_streams, int32_t total_rows, int32_t V,
+                     const int32_t* d_rows, const int64_t* d_row_off, const int32_t* d_hist, const int64_t* d_hist_off,
+                     const fs_row_params* d_params, const fs_row_params* h_params, const fs_edits* edits,
+                     const double* d_u, int32_t eos_id, int32_t* d_tok, int32_t* d_accepted, void* stream);
+int fs_decode_step_edited(fs_context* ctx, fs_drng* r, const float* d_logits, int64_t ld, int32_t B, int32_t V,
+                          const int32_t* d_hist, const int64_t* d_hist_off, const fs_row_params* d_params,
+                          const fs_row_params* h_params, const fs_edits* edits, int32_t* d_tok, int32_t* d_keep,
+                          int32_t* d_out_hist, int64_t* d_out_hist_off, int64_t out_cap, void* stream);
+
+/* The edited logits themselves, in fp32: row b of d_logits (type FS_F32, FS_BF16 or FS_F16; d_logits aligned to four
+ * logits, ld % 4 == 0) to row b of d_out (16-byte aligned, out_ld % 4 == 0, out_ld >= V; elements past V are left as they
+ * were). Tokens that are not allowed become -inf. d_params NULL: no softcap and no penalties; edits NULL: no masks and no
+ * biases. In place when FS_F32, d_out == d_logits and out_ld == ld; other overlaps are refused. */
+int fs_edit_batch(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld, int32_t B, int32_t V,
+                  const int32_t* d_hist, const int64_t* d_hist_off, const fs_row_params* d_params, const fs_edits* edits,
+                  float* d_out, int64_t out_ld, void* stream);
+
+/* Log-probabilities over a row's tokens: of d_tok[b] (d_lp[b]) with its rank (d_rank[b]: 1 + the number of tokens with a
+ * larger logit), and of the n largest (d_top_ids / d_top_lp [B][n], the lower id first among equal logits). The
+ * distribution is softmax((cap(l) + bias) / T) over the allowed tokens (cap and T of d_params[b], T = 1 where it is <= 0;
+ * d_params NULL: the logits' own), without penalties (fs_edit_batch writes penalised rows). A token that is not allowed,
+ * whose logit is NaN or -inf, or that is outside [0, V) has -inf and rank 0; places past a row's tokens have id -1 and
+ * -inf. Where the largest logit is +inf, its tokens share the probability. n <= FS_MAX_TOP; each output may be NULL
+ * (d_lp and d_rank need d_tok). Rows and types as in fs_edit_batch. The sum of exponentials is taken in fp32 over 64 terms
+ * and in fp64 over those. */
+#define FS_MAX_TOP 64
+int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld, int32_t B, int32_t V,
+                const fs_row_params* d_params, const fs_edits* edits, const int32_t* d_tok, int32_t n, float* d_lp,
+                int32_t* d_rank, int32_t* d_top_ids, float* d_top_lp, void* stream);
 
 /* Gemma 4's final-logit softcap as the sampler applies it (fs_row_params.softcap): d_out[i] = cap * tanhf(d_in[i] /
  * cap), the host loop of model_gemma4_gpu.cpp:282-283, bit-identical to it on a glibc host (its float tanh is
