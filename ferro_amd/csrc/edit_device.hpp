@@ -18,22 +18,42 @@ struct EdRow {
     const float* val;
     int64_t nb;
 };
-// row: the logits row (its mask); rec: its record (its biases)
+// row: the logits row
+__device__ __forceinline__ void ed_mask(EdRow& r, const EdArgs& ed, int row, int32_t* err) {
+    r.words = nullptr;
+    r.closed = false;
+    if (!ed.mask) return;
+    const int m = ed.mask_of ? ld_const(ed.mask_of + row) : row;
+    r.closed = m >= ed.n_masks;
+    if (r.closed && threadIdx.x == 0) atomicOr(err, FS_DEVERR_MASK);
+    if (m >= 0 && !r.closed) r.words = ed.mask + (int64_t)m * ed.mask_ld;
+}
+// rec: its record
+__device__ __forceinline__ void ed_bias(EdRow& r, const EdArgs& ed, int rec) {
+    r.nb = 0;
+    if (!ed.bias_off) return;
+    const int64_t b = ld_const(ed.bias_off + rec);
+    r.nb = ld_const(ed.bias_off + rec + 1) - b;
+    r.ids = ed.bias_ids + b;
+    r.val = ed.bias + b;
+}
 __device__ __forceinline__ EdRow ed_row(const EdArgs& ed, int row, int rec, int32_t* err) {
     EdRow r = {nullptr, false, nullptr, nullptr, 0};
-    if (ed.mask) {
-        const int m = ed.mask_of ? ld_const(ed.mask_of + row) : row;
-        r.closed = m >= ed.n_masks;
-        if (r.closed && threadIdx.x == 0) atomicOr(err, FS_DEVERR_MASK);
-        if (m >= 0 && !r.closed) r.words = ed.mask + (int64_t)m * ed.mask_ld;
-    }
-    if (ed.bias_off) {
-        const int64_t b = ld_const(ed.bias_off + rec);
-        r.nb = ld_const(ed.bias_off + rec + 1) - b;
-        r.ids = ed.bias_ids + b;
-        r.val = ed.bias + b;
-    }
+    ed_mask(r, ed, row, err);
+    ed_bias(r, ed, rec);
     return r;
+}
+// One logit, by one lane: a bit of the mask, a bisection of the biases. For the paths that read a row again.
+__device__ __forceinline__ float ed_lane(const EdRow& r, float l, int id) {
+    if (r.nb > 0) {
+        int64_t lo = 0, hi = r.nb;                             // the first bias whose id is at least id
+        while (lo < hi) {
+            const int64_t m = (lo + hi) >> 1;
+            if (r.ids[m] < id) lo = m + 1; else hi = m;
+        }
+        for (; lo < r.nb && r.ids[lo] == id; ++lo) l = __fadd_rn(l, r.val[lo]);
+    }
+    return r.closed || (r.words && ((r.words[id >> 5] >> (id & 31)) & 1u) == 0u) ? __builtin_nanf("") : l;
 }
 
 // A wave's share of the segment's mask: 32 NL words, word q * 8 + j of which covers lanes 8 j .. 8 j + 7 of group q. Lane l
@@ -89,19 +109,21 @@ __device__ __forceinline__ void ed_add(const EdRow& r, int seg_lo, int n_in, X x
         const int id = in ? r.ids[i + lane] : 0x7fffffff;
         const uint32_t rel = (uint32_t)id - (uint32_t)seg_lo;
         const float val = in ? r.val[i + lane] : 0.0f;
-        for (uint64_t m = __ballot(rel < (uint32_t)n_in && ((rel >> 2) & (SK_LT - 1)) / WAVE == (uint32_t)w); m; m &= m - 1) {
-            const int from = __ffsll((unsigned long long)m) - 1;
-            const uint32_t at = (uint32_t)read_lane((int)rel, from);
-            const float d = read_lane(val, from);
-            const int q = (int)(at >> 2) / SK_LT, c = (int)(at & 3u);
-            const bool mine = (int)((at >> 2) & (WAVE - 1)) == lane;
+        const bool here = rel < (uint32_t)n_in && ((rel >> 2) & (SK_LT - 1)) / WAVE == (uint32_t)w;
+        if (__ballot(here) != 0ull) {                          // (most waves hold none of the 64)
 #pragma unroll
-            for (int qq = 0; qq < NL; ++qq)
-                if (q == qq) {                                 // uniform
+            for (int q = 0; q < NL; ++q) {
+                for (uint64_t m = __ballot(here && (int)(rel >> 2) / SK_LT == q); m; m &= m - 1) {
+                    const int from = __ffsll((unsigned long long)m) - 1;
+                    const uint32_t at = (uint32_t)read_lane((int)rel, from);
+                    const float d = read_lane(val, from);
+                    if ((int)((at >> 2) & (WAVE - 1)) == lane) {
 #pragma unroll
-                    for (int cc = 0; cc < 4; ++cc)
-                        if (c == cc) x(qq, cc) = mine ? __fadd_rn(x(qq, cc), d) : x(qq, cc);
+                        for (int c = 0; c < 4; ++c)
+                            if ((int)(at & 3u) == c) x(q, c) = __fadd_rn(x(q, c), d);
+                    }
                 }
+            }
         }
         if (r.nb > 4 * WAVE && __ballot(id < seg_lo + n_in) != ~0ull) break;   // ascending: the rest lies behind
     }

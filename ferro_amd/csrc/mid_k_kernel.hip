@@ -23,6 +23,7 @@
 // Rows with every token a candidate (ak_segment, ak_finish) stay in registers through all their passes; the fused kernel
 // reads such a row again for each, and gave flat ones to one workgroup: 32 rows of 65536 N(0, 2) logits at temperature 1
 // 51.5 us -> 24.2, 3 rows of 178740 698 -> 28.6, 64 rows of 262144 heavy-tailed logits with top-p 0.95 37.5 -> 37.1.
+#include "edit_device.hpp"
 #include "exp_table.hpp"
 #include "row_device.hpp"
 
@@ -273,8 +274,9 @@ struct MkPen {
 };
 
 // f(logit, place) for a chunk of n logits of a row that one workgroup selects alone: eight loads in flight per thread.
-template <class F>
-__device__ __forceinline__ void slow_each(const float* p, int n, F f) {
+// ED: under the row's masks and biases (first: the chunk's first token).
+template <bool ED, class F>
+__device__ __forceinline__ void slow_each(const float* p, int n, const EdRow& er, int first, F f) {
 #pragma unroll 1
     for (int i0 = threadIdx.x; i0 < n; i0 += 8 * SK_LT) {
         float x[8];
@@ -285,6 +287,7 @@ __device__ __forceinline__ void slow_each(const float* p, int n, F f) {
             float l = x[0];
 #pragma unroll
             for (int t = 1; t < 8; ++t) l = q == t ? x[t] : l;
+            if (ED) l = ed_lane(er, l, first + i0 + q * SK_LT);
             f(l, i0 + q * SK_LT);
         }
     }
@@ -294,9 +297,9 @@ __device__ __forceinline__ void slow_each(const float* p, int n, F f) {
 // time (it stops where a digit's bin is wholly inside), then the composites at or above the k-th to the row's list.
 // The penalties are counted again chunk by chunk. Returns the list's length. For rows with thousands of equal logits at
 // the bound, and rows whose segments gave up waiting.
-template <bool CAP>
+template <bool CAP, bool ED>
 __device__ __forceinline__ uint32_t mk_slow(const float* rowp, int V, int k, bool pen, const MkWin& win, const MkPen& pn,
-                                            uint64_t* list, MkShared& s) {
+                                            const EdRow& er, uint64_t* list, MkShared& s) {
     constexpr int CH = SK_LT * 16 * 4;                         // logits per chunk
     const int tid = threadIdx.x;
     uint64_t prefix = 0ull, mask = 0ull;
@@ -330,13 +333,13 @@ __device__ __forceinline__ uint32_t mk_slow(const float* rowp, int V, int k, boo
                 }
                 __syncthreads();
             }
-            slow_each(rowp + lo, n, [&](float l, int i) {
+            slow_each<ED>(rowp + lo, n, er, lo, [&](float l, int i) {
                 if (CAP && pn.cap > 0.0f) l = softcap_one(l, pn.cap);
                 if (pen && ((s.b.bmp[i >> 5] >> (i & 31)) & 1u))
                     l = pn.apply(l, pn.fp_on ? (s.u.cnt[i >> 1] >> ((i & 1) * 16)) & 0xFFFFu : 0u);
                 const uint32_t key = key_of(l);
                 const uint64_t c = comp_of(key, (uint32_t)(lo + i));
-                if (key == 0u) return;
+                if (ED ? !(l > -__builtin_huge_valf()) : key == 0u) return;
                 if (gather) {
                     if ((c & mask) >= prefix) {
                         const uint32_t pos = atomicAdd(&s.misc[2], 1u);
@@ -742,9 +745,10 @@ __device__ __forceinline__ int ak_walk(int n, double above, double target, float
 // A row with every token a candidate from its logits alone, by one workgroup: extremes and the mass total in one pass,
 // then for top-p's crossing and for the draw a radix select by mass over the composites, ten bits at a time. Exact, and
 // slow (about 20 passes): rows whose mass no single bin narrows down (all logits equal), infinite maxima, give-ups.
-template <bool CAP>
+template <bool CAP, bool ED>
 __device__ __forceinline__ void ak_slow(const float* rowp, int V, bool pen, const MkWin& win, const MkPen& pn,
-                                        const fs_row_params& p, double u, MkShared& s, int& tok, int& keep) {
+                                        const EdRow& er, const fs_row_params& p, double u, MkShared& s, int& tok,
+                                        int& keep) {
     constexpr int CH = SK_LT * 8 * 4;                          // logits per chunk
     const int tid = threadIdx.x;
     const double Td = (double)p.temperature;
@@ -782,12 +786,12 @@ __device__ __forceinline__ void ak_slow(const float* rowp, int V, bool pen, cons
                 }
                 __syncthreads();
             }
-            slow_each(rowp + lo, n, [&](float l, int i) {
+            slow_each<ED>(rowp + lo, n, er, lo, [&](float l, int i) {
                 if (CAP && pn.cap > 0.0f) l = softcap_one(l, pn.cap);
                 if (pen && ((s.b.bmp[i >> 5] >> (i & 31)) & 1u))
                     l = pn.apply(l, pn.fp_on ? (s.u.z.cnt[i >> 1] >> ((i & 1) * 16)) & 0xFFFFu : 0u);
                 const uint32_t key = key_of(l);
-                if (key == 0u) return;
+                if (ED ? !(l > -__builtin_huge_valf()) : key == 0u) return;
                 const uint64_t c = comp_of(key, (uint32_t)(lo + i));
                 if (phase == 0) {
                     mxc = c > mxc ? c : mxc;
@@ -1319,9 +1323,9 @@ __device__ __forceinline__ bool ak_finish(const uint64_t* list, uint32_t n0, uin
 // 160 on the fused kernel, whose histogram is of keys). Returns false when a part holds too many, too, or a target lies
 // outside. One workgroup, two passes (four with the parts): 32 rows of 262144 logits rounded to halves 10140 us with ak_slow,
 // now 830 (2460 on the fused kernel).
-template <bool CAP>
-__device__ __forceinline__ bool ak_values(const float* rowp, int V, bool pen, const MkWin& win, const MkPen& pn, uint64_t* list,
-                                          uint32_t above, const AkRow& r, const fs_row_params& p, MkShared& s, int& tok,
+template <bool CAP, bool ED>
+__device__ __forceinline__ bool ak_values(const float* rowp, int V, bool pen, const MkWin& win, const MkPen& pn,
+                                          const EdRow& er, uint64_t* list, uint32_t above, const AkRow& r, const fs_row_params& p, MkShared& s, int& tok,
                                           int& keep) {
     constexpr int PT = 32, CH = SK_LT * PT;                    // logits of a thread, of a chunk
     const int tid = threadIdx.x, lane = lane_id();
@@ -1363,9 +1367,11 @@ __device__ __forceinline__ bool ak_values(const float* rowp, int V, bool pen, co
         }
         __syncthreads();
     };
-    auto value = [&](float l, int i) {                         // i: in the chunk
+    auto value = [&](float l, int lo, int i) {                 // i: in the chunk from lo on
+        if (ED && lo + i < V) l = ed_lane(er, l, lo + i);
         if (CAP && pn.cap > 0.0f) l = softcap_one(l, pn.cap);
         if (pen && ((s.b.bmp[i >> 5] >> (i & 31)) & 1u)) l = pn.apply(l, (s.u.z.cnt[i >> 1] >> ((i & 1) * 16)) & 0xFFFFu);
+        if (ED && !(l > -__builtin_huge_valf())) l = __builtin_nanf("");
         return l;
     };
     auto put = [&](int l, uint32_t key, uint32_t n) {          // open addressing
@@ -1396,7 +1402,7 @@ __device__ __forceinline__ bool ak_values(const float* rowp, int V, bool pen, co
                 float y = x[0];
 #pragma unroll
                 for (int t = 1; t < 8; ++t) y = q == t ? x[t] : y;
-                f(value(y, (q0 + q) * SK_LT + tid));
+                f(value(y, lo, (q0 + q) * SK_LT + tid));
             }
         }
     };
@@ -1568,7 +1574,7 @@ __device__ __forceinline__ bool ak_values(const float* rowp, int V, bool pen, co
 #pragma unroll 4
     for (int q = 0; q < PT; ++q) {
         const int i = tid * PT + q;
-        const float y = value(i < n ? rowp[lo + i] : __builtin_nanf(""), i);
+        const float y = value(i < n ? rowp[lo + i] : __builtin_nanf(""), lo, i);
         eq |= (key_of(y) == comp_key(c) ? 1u : 0u) << q;
     }
     uint32_t all;
@@ -1596,7 +1602,8 @@ constexpr size_t MK_ARGS_OFF = offsetof(MkKernargs, m);
 // CAP: some row of the batch has a softcap. It never decreases, so the bound is taken over raw logits and the merge caps
 // the list (an entry whose value is final already, a penalised one, has its id word's top bit cleared).
 // ALL: some row samples with every token a candidate.
-template <int NL, bool CAP, bool ALL>
+// ED: the rows have masks and biases, as in the small-k kernel; logits that are not allowed are NaN from the registers on.
+template <int NL, bool CAP, bool ALL, bool ED>
 __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, int64_t ld, int B, int V, int nseg,
                                                          int flags, const fs_row_params* params,
                                                          const int64_t* hist_off, const int32_t* hist, MkArgs m_) {
@@ -1619,8 +1626,20 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<float*>(rowp + seg_lo), (short)0, ((n_in + 3) & ~3) * 4, 0x00020000);
     float v[NL][4];
+    EdBits eb = {~0u, ~0u};
+    bool masked = false;
+    if constexpr (ED) {                                        // the row's mask first: it decides which loads are made
+        const MkArgs& em = *(const MkArgs*)((const __attribute__((address_space(4))) char*)
+                                            __builtin_amdgcn_kernarg_segment_ptr() + MK_ARGS_OFF);
+        EdRow er;
+        ed_mask(er, em.a.ed, row, em.a.err);
+        eb = ed_bits<NL>(er, seg_lo, V);
+        masked = er.words || er.closed;
+    }
     auto load = [&](int q) {
-        const f32x4 t = raw_buffer_load_f32x4(rs, (q * SK_LT + tid) * 16, 0, 2);    // nontemporal: read once
+        int at = (q * SK_LT + tid) * 16;
+        if (ED && masked) at = ed_nibble(eb, q) != 0u ? at : 0x7ffffff0;           // (past the buffer: no read, zeros)
+        const f32x4 t = raw_buffer_load_f32x4(rs, at, 0, 2);       // nontemporal: read once
         v[q][0] = t.x; v[q][1] = t.y; v[q][2] = t.z; v[q][3] = t.w;
     };
     // the first half, then the window's ids, then the rest: a wave's loads return in order, and so the bitmap is built
@@ -1704,11 +1723,76 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
     uint32_t* ctr = mk.ctr + (int64_t)row * MK_CTR;            // [0] barrier; [32] ticket, [33] list length, [34] slow, [35] spill
     uint64_t* list = mk.list + (int64_t)row * MK_LCAP;
     uint64_t* spill = mk.spill + (int64_t)row * MK_SPILL;
+    // the logits under the mask and the biases (-inf, too, is no candidate; with a softcap it is: the cap makes it a number)
+    auto edit = [&]() {
+        if constexpr (ED) {
+            if (!CAP) {
+                EdRow er;
+                ed_bias(er, a.ed, pidx);
+                if (er.nb > 0) ed_add<NL>(er, seg_lo, n_in, [&](int q, int c) -> float& { return v[q][c]; });
+            }
+            if (masked) {
+                asm volatile("" : "+v"(eb.a), "+v"(eb.b));         // (the nibbles again: kept from the loads they spill)
+#pragma unroll
+                for (int q = 0; q < NL; ++q) {
+                    const uint32_t nib = ed_nibble(eb, q);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[q][c] = ed_keep(v[q][c], nib, c, 0x7FC00000u);
+                }
+            }
+            if (ALL && !(CAP && pn.cap > 0.0f)) {
+#pragma unroll
+                for (int q = 0; q < NL; ++q)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        v[q][c] = v[q][c] > -__builtin_huge_valf() ? v[q][c] : __builtin_nanf("");
+            }
+        }
+    };
     // this wave's flagged logits: nf of them, in LDS from place pb on, or in the row's spill list (far; over: it is full)
     uint32_t nf = 0u, pb = 0u;
     bool far = false, over = false;
+    // the flagged logits to the wave's list, and out of the registers (NaN: no comparison takes it)
+    auto extract = [&]() {
+        const uint32_t m0 = s.b.bmp[2 * tid], m1 = NL > 8 ? s.b.bmp[2 * tid + 1] : 0u;
+        const uint32_t mine = (uint32_t)(__popc(m0) + __popc(m1));
+        const uint32_t incl = wave_incl_scan_u32(mine);
+        nf = (uint32_t)__builtin_amdgcn_readlane((int)incl, WAVE - 1);
+        __syncthreads();                                       // every thread has read its bits
+        if (nf != 0u) {
+            if (lane == 0) pb = atomicAdd(&s.np, nf);
+            pb = (uint32_t)__builtin_amdgcn_readfirstlane((int)pb);
+            far = pb + nf > (uint32_t)MK_PC;
+            if (far) {
+                if (lane == 0) pb = __hip_atomic_fetch_add(ctr + 35, nf, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                pb = (uint32_t)__builtin_amdgcn_readfirstlane((int)pb);
+                over = pb + nf > (uint32_t)MK_SPILL;
+                if (over) nf = 0u;
+            }
+            uint32_t at = pb + incl - mine;
+#pragma unroll
+            for (int q = 0; q < NL; ++q) {
+                const uint32_t nib = ((q < 8 ? m0 : m1) >> (4 * (q & 7))) & 15u;
+                if (__ballot(nib != 0u) != 0ull) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if ((nib >> c) & 1u) {
+                            const uint32_t rel = (uint32_t)((q * SK_LT + tid) * 4 + c);
+                            if (!far) {
+                                s.b.pv[at] = v[q][c];
+                                s.prel[at] = (uint16_t)rel;
+                            } else if (!over) {
+                                spill[at] = ((uint64_t)rel << 32) | __float_as_uint(v[q][c]);
+                            }
+                            ++at;
+                            v[q][c] = __builtin_nanf("");
+                        }
+                    }
+                }
+            }
+        }
+    };
     if (pen) {
-        uint32_t m0 = 0u, m1 = 0u;
         bool ovf = false;
         for (int i = tid; i < SK_LT * 2; i += SK_LT) s.b.bmp[i] = 0u;
         if (tid == 0) s.np = 0u;
@@ -1787,45 +1871,11 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
         }
         if (ovf) atomicOr(a.err, FS_DEVERR_COUNT_OVERFLOW);
         __syncthreads();
-        m0 = s.b.bmp[2 * tid];
-        m1 = NL > 8 ? s.b.bmp[2 * tid + 1] : 0u;
-        // the flagged logits to the wave's list, and out of the registers (NaN: no comparison takes it)
-        const uint32_t mine = (uint32_t)(__popc(m0) + __popc(m1));
-        const uint32_t incl = wave_incl_scan_u32(mine);
-        nf = (uint32_t)__builtin_amdgcn_readlane((int)incl, WAVE - 1);
-        __syncthreads();                                       // every thread has read its bits
-        if (nf != 0u) {
-            if (lane == 0) pb = atomicAdd(&s.np, nf);
-            pb = (uint32_t)__builtin_amdgcn_readfirstlane((int)pb);
-            far = pb + nf > (uint32_t)MK_PC;
-            if (far) {
-                if (lane == 0) pb = __hip_atomic_fetch_add(ctr + 35, nf, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                pb = (uint32_t)__builtin_amdgcn_readfirstlane((int)pb);
-                over = pb + nf > (uint32_t)MK_SPILL;
-                if (over) nf = 0u;
-            }
-            uint32_t at = pb + incl - mine;
-#pragma unroll
-            for (int q = 0; q < NL; ++q) {
-                const uint32_t nib = ((q < 8 ? m0 : m1) >> (4 * (q & 7))) & 15u;
-                if (__ballot(nib != 0u) != 0ull) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        if ((nib >> c) & 1u) {
-                            const uint32_t rel = (uint32_t)((q * SK_LT + tid) * 4 + c);
-                            if (!far) {
-                                s.b.pv[at] = v[q][c];
-                                s.prel[at] = (uint16_t)rel;
-                            } else if (!over) {
-                                spill[at] = ((uint64_t)rel << 32) | __float_as_uint(v[q][c]);
-                            }
-                            ++at;
-                            v[q][c] = __builtin_nanf("");
-                        }
-                    }
-                }
-            }
-        }
+        if (!ED) extract();
+    }
+    if constexpr (ED) {
+        edit();
+        if (pen) extract();
     }
     if (n_in < SEG) {                                          // past the row's end: NaN, no comparison takes it
 #pragma unroll
@@ -1848,6 +1898,7 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
             float l = far ? __uint_as_float((uint32_t)e) : s.b.pv[pb + i];
             if (CAP && pn.cap > 0.0f) l = softcap_one(l, pn.cap);
             l = pn.apply(l, pn.fp_on ? (s.u.cnt[rel >> 1] >> ((rel & 1u) * 16u)) & 0xFFFFu : 0u);
+            if (ED && !(l > -__builtin_huge_valf())) l = __builtin_nanf("");
             if (far) st_agent(&spill[pb + i], (e & 0xFFFFFFFF00000000ull) | __float_as_uint(l));
             else s.b.pv[pb + i] = l;
         }
@@ -1907,7 +1958,7 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
             tied = sum > (uint32_t)(k + k / 8 + 48) && sum > many;
             if (tied) T = mk_bound_exact(qk, nseg, T, need, s);
             SK_MARK(4);
-            tc = T > 0x007FFFFFu ? val_of(T) : -__builtin_huge_valf();
+            tc = T > 0x007FFFFFu ? val_of(T) : ED ? -3.402823466e+38f : -__builtin_huge_valf();
             tr = tb = tc;
             if (CAP && pn.cap > 0.0f) {
                 // tc: the capped bound; tr: a raw value that every logit whose capped value reaches tc reaches. Lane
@@ -1938,7 +1989,7 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
     if (scan) {
         // the segment's first maximum (ferro's scan, sampler.cpp:19-23)
         uint64_t best = 0ull;
-        if (lm == lm) {
+        if (ED ? lm > -__builtin_huge_valf() : lm == lm) {
             uint32_t first = 0u;
 #pragma unroll
             for (int q = NL - 1; q >= 0; --q)
@@ -2092,11 +2143,20 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
     int tok = 0, keep = 1;
     // a greedy row's token (ferro keeps index 0 when its logit is NaN)
     auto greedy_end = [&](uint64_t top) {
-        tok = (rowp[0] != rowp[0] || top == 0ull) ? 0 : (int)comp_id(top);
+        if constexpr (ED) {
+            keep = top != 0ull ? 1 : 0;
+            tok = top != 0ull ? (int)comp_id(top) : -1;
+        } else {
+            tok = (rowp[0] != rowp[0] || top == 0ull) ? 0 : (int)comp_id(top);
+        }
         if (lane == 0 && a.mode != MODE_VERIFY && a.kcap > 0) {
             if (a.cand_ids) a.cand_ids[(int64_t)row * a.kcap] = tok;
-            if (a.cand_probs) a.cand_probs[(int64_t)row * a.kcap] = 1.0;
+            if (a.cand_probs) a.cand_probs[(int64_t)row * a.kcap] = (double)keep;
         }
+    };
+    auto again_row = [&]() {                                   // for the paths that read the row again
+        if constexpr (ED) return ed_row(a.ed, row, pidx, a.err);
+        else return EdRow{nullptr, false, nullptr, nullptr, 0};
     };
     const uint32_t slow = ld_agent(ctr + 34);                  // uniform
     uint32_t n0 = 0u, n1 = 0u, above = 0u;
@@ -2128,8 +2188,9 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
         bool done = false;
         if (slow == 0u && !ak.plain && fits) done = ak_finish(list, n0, n1, c0, c1, above, ak, p, s, tok, keep);
         else if ((slow & ~1u) == 0u && (!ak.plain || (ak.nv != 0u && ak.scale == 0.0f)))
-            done = ak_values<CAP>(rowp, V, pen, win, pn, list, above, ak, p, s, tok, keep);
-        if (!done) ak_slow<CAP>(rowp, V, pen, win, pn, p, dr.u, s, tok, keep);
+            done = ak_values<CAP, ED>(rowp, V, pen, win, pn, again_row(), list, above, ak, p, s, tok, keep);
+        if (!done) ak_slow<CAP, ED>(rowp, V, pen, win, pn, again_row(), p, dr.u, s, tok, keep);
+        if (ED && keep == 0) tok = -1;
         if (w != 0) return;
     } else {
         uint32_t C = ld_agent(ctr + 33);
@@ -2146,11 +2207,12 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
         }
         do {
             if (again) {
-                C = mk_slow<CAP>(rowp, V, k, pen, win, pn, list, s);
+                C = mk_slow<CAP, ED>(rowp, V, k, pen, win, pn, again_row(), list, s);
                 capped_list = false;
             }
             if (C == 0u) {                                     // every logit NaN: token 0, nothing kept
                 keep = greedy ? 1 : 0;
+                if (ED) tok = -1;
                 if (greedy && w == 0) greedy_end(0ull);
                 break;
             }
@@ -2241,25 +2303,30 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
     SK_FLUSH();
 }
 
-hipError_t launch_mid_k(int nl, bool capped, bool all, unsigned grid, int flags, const MkArgs& m, hipStream_t st) {
+hipError_t launch_mid_k(int nl, bool capped, bool all, bool edited, unsigned grid, int flags, const MkArgs& m,
+                        hipStream_t st) {
     auto go = [&](auto kern) {
         hipLaunchKernelGGL(kern, dim3(grid), dim3(SK_LT), 0, st, m.a.logits, m.a.ld, m.a.B, m.a.V, m.a.nseg, flags,
                            m.a.params, m.a.hist_off, m.a.hist, m);
     };
-    auto by_nl = [&](auto cap, auto every) {
-        constexpr bool C = decltype(cap)::value, A = decltype(every)::value;
-        if (nl == 16) go(mid_k_kernel<16, C, A>);
-        else if (nl == 8) go(mid_k_kernel<8, C, A>);
-        else go(mid_k_kernel<4, C, A>);
+    auto by_nl = [&](auto cap, auto every, auto ed) {
+        constexpr bool C = decltype(cap)::value, A = decltype(every)::value, E = decltype(ed)::value;
+        if (nl == 16) go(mid_k_kernel<16, C, A, E>);
+        else if (nl == 8) go(mid_k_kernel<8, C, A, E>);
+        else go(mid_k_kernel<4, C, A, E>);
     };
     const std::true_type yes;
     const std::false_type no;
-    if (capped) {
-        if (all) by_nl(yes, yes);
-        else by_nl(yes, no);
+    auto by_rows = [&](auto cap, auto ed) {
+        if (all) by_nl(cap, yes, ed);
+        else by_nl(cap, no, ed);
+    };
+    if (edited) {
+        if (capped) by_rows(yes, yes);
+        else by_rows(no, yes);
     } else {
-        if (all) by_nl(no, yes);
-        else by_nl(no, no);
+        if (capped) by_rows(yes, no);
+        else by_rows(no, no);
     }
     return hipGetLastError();
 }

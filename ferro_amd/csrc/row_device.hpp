@@ -190,13 +190,13 @@ __device__ __forceinline__ void sk_finish(const SkArgs& a, int row, int pidx, bo
         const int m = (int)(ld_const(a.row_off + pidx + 1) - r0);
         if (m <= 32) {
             // Streams of up to 32 rows: one 64-bit atomic per row carries everything - the count of rows done in its
-            // high word, in its low word a bit for each row that ends the walk (an eos token, the last row, or a
-            // token other than the next row's draft). The last row's fetched value holds every other row's bit, so
+            // high word, in its low word a bit for each row that ends the walk (an eos token, no token, the last row,
+            // or a token other than the next row's draft). The last row's fetched value holds every other row's bit, so
             // its accepted prefix is the lowest set bit + 1, with no token exchanged and no wait for stores.
             if (lane == 0) {
                 a.tok[row] = tok;
                 const int rr = row - (int)r0;
-                const bool stop = (a.eos >= 0 && tok == a.eos) || rr + 1 >= m || tok != ld_const(a.rows + row + 1);
+                const bool stop = (a.eos >= 0 && tok == a.eos) || tok < 0 || rr + 1 >= m || tok != ld_const(a.rows + row + 1);
                 const uint64_t mine = stop ? (1ull << rr) : 0ull;
                 uint64_t* cnt = reinterpret_cast<uint64_t*>(a.stream_cnt) + pidx;
                 const uint64_t old = __hip_atomic_fetch_add(cnt, (1ull << 32) | mine, __ATOMIC_RELAXED,

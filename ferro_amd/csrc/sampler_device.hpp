@@ -265,7 +265,7 @@ __device__ __forceinline__ int accepted_prefix(const int32_t* tok, const int32_t
         bool stop = false;
         if (r < m) {
             const int t = ld_agent(&tok[r0 + r]);
-            stop = (eos >= 0 && t == eos) || r + 1 >= m || t != rows[r0 + r + 1];
+            stop = (eos >= 0 && t == eos) || t < 0 || r + 1 >= m || t != rows[r0 + r + 1];
         }
         const uint64_t b = __ballot(stop);
         if (b) return c0 + __ffsll((unsigned long long)b);    // 1-based: the row that ends the walk, plus one

@@ -130,6 +130,7 @@ struct fs_context {
     bool seg_layout = true;    // the segment grid's hand-off holds on this device (XCDS % xccs == 0)
     int32_t* hflag = nullptr;  // host-mapped: a merge of an earlier call gave up (set by the kernel, read here)
     int32_t* hflag_dev = nullptr;
+    bool frozen = false;       // a call under edits is being recorded into a graph: nothing may be allocated
     bool captured = false;     // a call was recorded into a graph: workspaces are retired, never freed, on growth
     std::vector<void*> retired;
     uint64_t* sk_lists = nullptr;   // small-k kernel: [slots][SK_K] sorted segment lists
@@ -205,6 +206,8 @@ void release(fs_context* c, void* p) {
 }
 
 int grow(fs_context* c, size_t slots, size_t rows, size_t streams) {
+    if (c->frozen && (slots > c->cand_slots || rows > c->row_cap || streams > c->stream_cap || !c->hflag || !c->err))
+        return FS_E_NOMEM;
     if (slots > c->cand_slots) {
         release(c, c->cand);
         release(c, c->meta);
@@ -395,6 +398,7 @@ int small_k_plan(int cus, int64_t B, int32_t V, int& nl, int& nseg) {
 }
 
 int grow_small(fs_context* c, size_t slots, size_t rows) {
+    if (c->frozen && (slots > c->sk_slots || rows > c->sk_rows)) return FS_E_NOMEM;
     if (slots > c->sk_slots) {
         release(c, c->sk_lists);
         c->sk_lists = nullptr; c->sk_slots = 0;
@@ -479,8 +483,9 @@ fs::SkArgs row_args(const fs_context* ctx, const fs::Args& a, int nseg) {
 // Launches the small-k kernel when the batch fits it; *used = false (nothing launched) otherwise. a.mode selects
 // sampling (h_params: B records) or verification windows (h_params: n_streams records).
 // h_params NULL: every row greedy without penalties (fs_argmax_batch without parameters): the context's greedy
-// records stand for the parameters, on the device and the host.
-int launch_small(fs_context* ctx, const fs::Args& a_in, const fs_row_params* h_params, hipStream_t st, bool& used) {
+// records stand for the parameters, on the device and the host. ed: the rows' masks and biases.
+int launch_small(fs_context* ctx, const fs::Args& a_in, const fs_row_params* h_params, hipStream_t st, bool& used,
+                 const fs::EdArgs* ed = nullptr) {
     used = false;
     std::lock_guard<std::mutex> g(ctx->mu);
     int rc = device_of(ctx);
@@ -497,6 +502,7 @@ int launch_small(fs_context* ctx, const fs::Args& a_in, const fs_row_params* h_p
     SmallKChoice ch;
     if (!small_k_choice(ctx->cus, h_params, verify ? (int64_t)a.n_streams : (int64_t)a.B, a.B, a.V, verify, ch))
         return FS_OK;
+    if (ed && ed->bias_off && ch.capped) return FS_OK;     // (the softcap, late in this kernel, comes before the biases)
     const int nl = ch.nl, nseg = ch.nseg;
     const int64_t per_x = ((int64_t)a.B + fs::XCDS - 1) / fs::XCDS;
     const int64_t grid = (int64_t)fs::XCDS * nseg * per_x;
@@ -509,6 +515,7 @@ int launch_small(fs_context* ctx, const fs::Args& a_in, const fs_row_params* h_p
     if (capturing(st)) ctx->captured = true;
     fs::SkArgs k = row_args(ctx, a, nseg);
     k.lists = ctx->sk_lists; k.ticket = ctx->sk_ticket;
+    if (ed) k.ed = *ed;
     k.trace = nullptr;
 #ifdef FS_TRACE
     if (ctx->trace && grid * fs::TRACE_W <= ctx->trace_cap) k.trace = ctx->trace;
@@ -518,7 +525,7 @@ int launch_small(fs_context* ctx, const fs::Args& a_in, const fs_row_params* h_p
     // a verification window reaches this kernel only without an active penalty (small_k_windows)
     may_pen = may_pen && !verify && a.hist && a.hist_off;
     const int flags = (may_pen ? fs::SK_MAY_PEN : 0) | (a.out_hist_off ? fs::SK_COPY : 0);
-    if (fs::launch_small_k(nl, capped, all_greedy, (unsigned)grid, flags, k, st) != hipSuccess) return FS_E_HIP;
+    if (fs::launch_small_k(nl, capped, all_greedy, ed != nullptr, (unsigned)grid, flags, k, st) != hipSuccess) return FS_E_HIP;
     used = true;
     return FS_OK;
 }
@@ -573,6 +580,7 @@ bool mid_k_choice(int cus, const fs_row_params* h, int64_t n, int64_t rows, int3
 template <class T>
 int grow_buffer(fs_context* c, T*& p, size_t& cap, size_t n, size_t per, bool zero) {
     if (n <= cap) return FS_OK;
+    if (c->frozen) return FS_E_NOMEM;
     T* q = nullptr;
     size_t m = std::max(n, cap + cap / 2);
     if (hipMalloc(&q, m * per * sizeof(T)) != hipSuccess) {
@@ -629,7 +637,8 @@ int grow_fused(fs_context* ctx, fs::Args& a, int64_t rows, int64_t streams, int 
 // without one), and so does one that the device has no room for.
 // per_cu: as launch's; the fused kernel's workspace grows as launch would grow it, so that a context warmed up with any
 // parameters of a shape allocates nothing when a call of that shape with others is recorded.
-int launch_mid(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params, hipStream_t st, bool& used, int per_cu = 2) {
+int launch_mid(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params, hipStream_t st, bool& used, int per_cu = 2,
+               const fs::EdArgs* ed = nullptr) {
     used = false;
     std::lock_guard<std::mutex> g(ctx->mu);
     int rc = device_of(ctx);
@@ -640,6 +649,7 @@ int launch_mid(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params
     if (!mid_k_choice(ctx->cus, h_params, verify ? (int64_t)a.n_streams : (int64_t)a.B, a.B, a.V,
                       a.cand_ids || a.cand_probs, ch))
         return FS_OK;
+    if (ed && ed->bias_off && ch.capped) return FS_OK;     // (the softcap, late in this kernel, comes before the biases)
     const size_t streams = verify ? 3 * (size_t)a.n_streams : 0;
     const bool cap = capturing(st);
     if (cap && (mid_grows(ctx, ch, (size_t)a.B) || streams > ctx->stream_cap || !ctx->err)) return FS_OK;
@@ -661,13 +671,14 @@ int launch_mid(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params
     m.a = row_args(ctx, a, ch.nseg);
     m.ctr = ctx->mk_ctr; m.qk = ctx->mk_qk; m.list = ctx->mk_list; m.spill = ctx->mk_spill;
     m.mass = ctx->mk_mass; m.spins = ctx->merge_spins;
+    if (ed) m.a.ed = *ed;
     const int64_t grid = (int64_t)fs::XCDS * ch.nseg * (((int64_t)a.B + fs::XCDS - 1) / fs::XCDS);
 #ifdef FS_TRACE
     if (ctx->trace && grid * fs::TRACE_W <= ctx->trace_cap) m.a.trace = ctx->trace;
 #endif
     const int flags = (ch.may_pen ? fs::SK_MAY_PEN : 0) | (a.out_hist_off ? fs::SK_COPY : 0) |
                       (verify ? fs::MK_VERIFY : 0);
-    if (fs::launch_mid_k(ch.nl, ch.capped, ch.all, (unsigned)grid, flags, m, st) != hipSuccess) return FS_E_HIP;
+    if (fs::launch_mid_k(ch.nl, ch.capped, ch.all, ed != nullptr, (unsigned)grid, flags, m, st) != hipSuccess) return FS_E_HIP;
     used = true;
     return FS_OK;
 }
@@ -707,14 +718,21 @@ int launch(fs_context* ctx, fs::Args a, int64_t rows, int64_t streams, hipStream
 }
 
 // ---- calls under edits (fs_sample_edited, fs_verify_edited, fs_decode_step_edited)
-// The context on the current device, a workspace buffer for a call on st: under capture none may grow.
-int edited_ready(fs_context* c) {
-    const int rc = device_of(c);
-    if (rc != FS_OK) return rc;
-    int dev = -1;
-    if (hipGetDevice(&dev) != hipSuccess) return FS_E_HIP;
-    return dev == c->device ? FS_OK : FS_E_INVALID;
-}
+// For such a call's time: the context is on the current device, and no workspace grows where the call is being recorded (an
+// allocation would end the capture).
+struct Edited {
+    fs_context* c;
+    int rc = FS_OK;
+    Edited(fs_context* ctx, hipStream_t st) : c(ctx) {
+        std::lock_guard<std::mutex> g(c->mu);
+        rc = device_of(c);
+        int dev = -1;
+        if (rc == FS_OK && hipGetDevice(&dev) != hipSuccess) rc = FS_E_HIP;
+        if (rc == FS_OK && dev != c->device) rc = FS_E_INVALID;
+        if (rc == FS_OK && capturing(st)) c->frozen = c->captured = true;
+    }
+    ~Edited() { c->frozen = false; }
+};
 
 // Logits per thread and segments per row of the edit kernel: the larger segments where they fill the device.
 int edit_plan(int cus, int64_t B, int32_t V, int& nseg) {
@@ -732,25 +750,15 @@ int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_p
     int nseg = 0, nl = 0;
     {
         std::lock_guard<std::mutex> g(ctx->mu);
-        int rc = edited_ready(ctx);
-        if (rc != FS_OK) return rc;
         nl = edit_plan(ctx->cus, a.B, a.V, nseg);
         if ((int64_t)a.B * nseg > 0x7fffffff) return FS_E_INVALID;
-        const bool zeros = decode && !a.hist_off;
-        if (capturing(st)) {
-            if (B * ld > ctx->ed_logits || B > ctx->ed_param_rows || B > ctx->ed_any_rows ||
-                (decode && B > ctx->ed_u_rows) || (zeros && B + 1 > ctx->ed_off_rows) || !ctx->err)
-                return FS_E_NOMEM;
-            ctx->captured = true;
-        } else {
-            rc = grow(ctx, 0, 0, 0);
-            if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_rows, ctx->ed_logits, B * ld, 1, false);
-            if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_params, ctx->ed_param_rows, B, 1, false);
-            if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_any, ctx->ed_any_rows, B, 1, true);
-            if (rc == FS_OK && decode) rc = grow_buffer(ctx, ctx->ed_u, ctx->ed_u_rows, B, 1, false);
-            if (rc == FS_OK && zeros) rc = grow_buffer(ctx, ctx->ed_off, ctx->ed_off_rows, B + 1, 1, true);
-            if (rc != FS_OK) return rc;
-        }
+        int rc = grow(ctx, 0, 0, 0);
+        if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_rows, ctx->ed_logits, B * ld, 1, false);
+        if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_params, ctx->ed_param_rows, B, 1, false);
+        if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_any, ctx->ed_any_rows, B, 1, true);
+        if (rc == FS_OK && decode) rc = grow_buffer(ctx, ctx->ed_u, ctx->ed_u_rows, B, 1, false);
+        if (rc == FS_OK && decode && !a.hist_off) rc = grow_buffer(ctx, ctx->ed_off, ctx->ed_off_rows, B + 1, 1, true);
+        if (rc != FS_OK) return rc;
     }
     fs::EditArgs e = {};
     e.logits = a.logits; e.type = FS_F32; e.ld = a.ld; e.B = a.B; e.V = a.V; e.nseg = nseg;
@@ -804,7 +812,17 @@ int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_p
     return rc;
 }
 
+// The kernels that read masks and biases themselves where one takes the batch, else the edited rows.
 int launch_edited(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params, const fs::EdArgs& ed, hipStream_t st) {
+    const Edited call(ctx, st);
+    if (call.rc != FS_OK) return call.rc;
+    if (h_params) {
+        bool used = false;
+        int rc = launch_small(ctx, a, h_params, st, used, &ed);
+        if (rc != FS_OK || used) return rc;
+        rc = launch_mid(ctx, a, h_params, st, used, 2, &ed);
+        if (rc != FS_OK || used) return rc;
+    }
     return launch_composed(ctx, a, h_params, ed, st);
 }
 
@@ -1197,10 +1215,11 @@ int fs_edit_batch(fs_context* ctx, const void* d_logits, int32_t type, int64_t l
         if (i0 < o1 && o0 < i1) return FS_E_INVALID;
     }
     int nl = 0;
+    const Edited call(ctx, (hipStream_t)stream);
+    if (call.rc != FS_OK) return call.rc;
     {
         std::lock_guard<std::mutex> g(ctx->mu);
-        rc = edited_ready(ctx);
-        if (rc == FS_OK) rc = grow(ctx, 0, 0, 0);              // the error word
+        rc = grow(ctx, 0, 0, 0);                               // the error word
         if (rc != FS_OK) return rc;
         nl = edit_plan(ctx->cus, B, V, e.nseg);
     }
@@ -1224,9 +1243,9 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
     if (B == 0) return FS_OK;
     const hipStream_t st = (hipStream_t)stream;
     const int top = d_top_ids || d_top_lp ? n : 0;
+    const Edited call(ctx, st);
+    if (call.rc != FS_OK) return call.rc;
     std::lock_guard<std::mutex> g(ctx->mu);
-    rc = edited_ready(ctx);
-    if (rc != FS_OK) return rc;
     int nl = 4;
     for (const int l : {16, 8, 4}) {                           // the largest segments that give every CU four workgroups
         nl = l;
@@ -1235,17 +1254,11 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
     }
     if ((int64_t)B * a.nseg > 0x7fffffff) return FS_E_INVALID;
     const size_t segs = (size_t)B * a.nseg;
-    if (capturing(st)) {
-        if (segs > ctx->lp_segs || (top > 0 && segs > ctx->lp_list_segs) || (size_t)B > ctx->lp_rows || !ctx->err)
-            return FS_E_NOMEM;
-        ctx->captured = true;
-    } else {
-        rc = grow(ctx, 0, 0, 0);
-        if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_part, ctx->lp_segs, segs, 1, false);
-        if (rc == FS_OK && top > 0) rc = grow_buffer(ctx, ctx->lp_lists, ctx->lp_list_segs, segs, fs::LP_TOP, false);
-        if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_ticket, ctx->lp_rows, (size_t)B, 1, true);
-        if (rc != FS_OK) return rc;
-    }
+    rc = grow(ctx, 0, 0, 0);
+    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_part, ctx->lp_segs, segs, 1, false);
+    if (rc == FS_OK && top > 0) rc = grow_buffer(ctx, ctx->lp_lists, ctx->lp_list_segs, segs, fs::LP_TOP, false);
+    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_ticket, ctx->lp_rows, (size_t)B, 1, true);
+    if (rc != FS_OK) return rc;
     a.logits = d_logits; a.ld = ld; a.B = B; a.V = V; a.n = top; a.params = d_params; a.tok = d_tok;
     a.lp = d_lp; a.rank = d_rank; a.ids = d_top_ids; a.top = d_top_lp;
     a.part = ctx->lp_part; a.lists = ctx->lp_lists; a.ticket = ctx->lp_ticket; a.err = ctx->err;

@@ -62,13 +62,14 @@ struct SkArgs {
     int32_t* out_hist;
     int64_t* out_hist_off;
     int64_t out_cap;
+    EdArgs ed;                             // the edited instantiations: masks and biases
 };
 
 // flags of a launch: some row has an active penalty window; a decode step (the histories are copied); a verification
 // window (mid-k kernel)
 constexpr int SK_MAY_PEN = 1, SK_COPY = 2, MK_VERIFY = 4;
-// nl: float4 loads per thread (4, 8 or 16); the grid and k's layout come from the small-k plan.
-hipError_t launch_small_k(int nl, bool capped, bool all_greedy, unsigned grid, int flags, const SkArgs& k,
+// nl: float4 loads per thread (4, 8 or 16); the grid and k's layout come from the small-k plan. edited: under k.ed.
+hipError_t launch_small_k(int nl, bool capped, bool all_greedy, bool edited, unsigned grid, int flags, const SkArgs& k,
                           hipStream_t st);
 
 // The mid-k kernel: the small-k kernel's arguments (lists and ticket unused) and its own workspace.
@@ -90,8 +91,9 @@ struct MkArgs {
     uint64_t* mass;                        // [B][2048] mass bins of rows with every token a candidate, left at 0
     uint32_t spins;                        // bounded wait for a row's segments (polls)
 };
-// all: some row samples with every token a candidate
-hipError_t launch_mid_k(int nl, bool capped, bool all, unsigned grid, int flags, const MkArgs& m, hipStream_t st);
+// all: some row samples with every token a candidate; edited: under m.a.ed
+hipError_t launch_mid_k(int nl, bool capped, bool all, bool edited, unsigned grid, int flags, const MkArgs& m,
+                        hipStream_t st);
 
 // Edited logits written out (edit_kernels.hip). nl: groups of four logits per thread (4 or 8).
 struct EditArgs {

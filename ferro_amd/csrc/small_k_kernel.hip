@@ -1,4 +1,5 @@
 // small_k_kernel.hip - the kernel of batches whose every row is greedy or samples from at most 64 candidates.
+#include "edit_device.hpp"
 #include "row_device.hpp"
 
 #include <type_traits>
@@ -49,9 +50,9 @@ static_assert(offsetof(SkShared, cand) % 16 == 0, "the rank loops read the candi
 // logits are re-read from memory (the L2 holds them by then) in batches of SK_EB per thread, sixteen loads in flight,
 // and transformed again (softcap, then the repetition penalty from the segment's bitmap; past n: NaN).
 constexpr int SK_EB = 16;
-template <bool CAP, class F>
-__device__ __forceinline__ void sk_each(const float* segp, int n, int nseg_elems, float cap, bool pen, float rep,
-                                        const uint32_t* bmp, F f) {
+template <bool CAP, bool ED, class F>
+__device__ __forceinline__ void sk_each(const float* segp, int seg_lo, int n, int nseg_elems, float cap, bool pen,
+                                        float rep, const uint32_t* bmp, const EdRow& er, F f) {
     const int tid = threadIdx.x;
 #pragma unroll 1
     for (int i0 = 0; i0 < nseg_elems; i0 += SK_LT * SK_EB) {
@@ -60,6 +61,7 @@ __device__ __forceinline__ void sk_each(const float* segp, int n, int nseg_elems
         for (int j = 0; j < SK_EB; ++j) {
             const int i = i0 + j * SK_LT + tid;
             x[j] = i < n ? segp[i] : 0.0f;
+            if (ED && i < n) x[j] = ed_lane(er, x[j], seg_lo + i);
         }
         if (CAP && cap > 0.0f) softcap_vals(x, cap);
 #pragma unroll
@@ -67,15 +69,15 @@ __device__ __forceinline__ void sk_each(const float* segp, int n, int nseg_elems
             const int i = i0 + j * SK_LT + tid;
             float l = x[j];
             if (pen && i < n && ((bmp[i >> 5] >> (i & 31)) & 1u)) l = l > 0.0f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);
-            f(i, i < n ? key_of(l) : 0u);
+            f(i, i < n && !(ED && !(l > -__builtin_huge_valf())) ? key_of(l) : 0u);
         }
     }
 }
 // The exact k-th largest composite of the segment (every composite is distinct: the id is part of it), by a radix
 // select over 4-bit digits. Slow, and rare.
-template <bool CAP>
+template <bool CAP, bool ED>
 __device__ __forceinline__ uint64_t sk_kth_exact(const float* segp, int seg_lo, int n, int nseg_elems, float cap,
-                                                 bool pen, float rep, int k, SkShared& s) {
+                                                 bool pen, float rep, const EdRow& er, int k, SkShared& s) {
     const int tid = threadIdx.x;
     uint64_t prefix = 0ull;
     int need = k;
@@ -84,7 +86,7 @@ __device__ __forceinline__ uint64_t sk_kth_exact(const float* segp, int seg_lo, 
         if (tid < 16) s.hist[tid] = 0u;
         __syncthreads();
         const uint64_t hi_mask = sh + 4 >= 64 ? 0ull : (~0ull << (sh + 4));
-        sk_each<CAP>(segp, n, nseg_elems, cap, pen, rep, s.bmp, [&](int i, uint32_t key) {
+        sk_each<CAP, ED>(segp, seg_lo, n, nseg_elems, cap, pen, rep, s.bmp, er, [&](int i, uint32_t key) {
             const uint64_t cm = comp_of(key, (uint32_t)(seg_lo + i));
             if (key != 0u && (cm & hi_mask) == prefix) atomicAdd(&s.hist[(uint32_t)(cm >> sh) & 15u], 1u);
         });
@@ -185,7 +187,11 @@ constexpr unsigned SK_PAD_LDS = 16384;
 
 // MANY: more than 4 * SK_NW lists per row (sk_merge_many; left out of the others, which it cost 0.2 us of 8.4).
 // GREEDY: every row of the batch is greedy (the selection code is left out: fewer registers, more workgroups per CU).
-template <int NL, bool CAP, bool GREEDY, bool MANY>
+// ED: the rows have masks and biases (fs_edits; no biases with a softcap, which comes before them but is applied to the
+// candidates alone). A row's mask is read first and the logits' loads then skip the groups of four without an allowed
+// token. A logit that is not allowed becomes NaN, which nothing below takes; candidates are above -inf; a row without one
+// has token -1.
+template <int NL, bool CAP, bool GREEDY, bool MANY, bool ED>
 __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, int64_t ld, int B, int V, int nseg,
                                                         int flags, const fs_row_params* params,
                                                         const int64_t* hist_off, const int32_t* hist, SkArgs a_) {
@@ -217,9 +223,21 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
     const __amdgpu_buffer_rsrc_t rs =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(rowp + seg_lo), (short)0, nrec, 0x00020000);
     float4 v[NL];
+    EdBits eb = {~0u, ~0u};
+    bool masked = false;
+    if constexpr (ED) {
+        const SkArgs& ea = *(const SkArgs*)((const __attribute__((address_space(4))) char*)
+                                            __builtin_amdgcn_kernarg_segment_ptr() + SK_ARGS_OFF);
+        EdRow er;
+        ed_mask(er, ea.ed, row, ea.err);
+        eb = ed_bits<NL>(er, seg_lo, V);
+        masked = er.words || er.closed;
+    }
 #pragma unroll
     for (int q = 0; q < NL; ++q) {
-        const f32x4 t = raw_buffer_load_f32x4(rs, (q * SK_LT + tid) * 16, 0, 2);    // nontemporal: read once
+        int at = (q * SK_LT + tid) * 16;
+        if (ED && masked) at = ed_nibble(eb, q) != 0u ? at : 0x7ffffff0;           // (past the buffer: no read, zeros)
+        const f32x4 t = raw_buffer_load_f32x4(rs, at, 0, 2);       // nontemporal: read once
         v[q] = make_float4(t.x, t.y, t.z, t.w);
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -389,6 +407,25 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
     }
     const bool wpen = __ballot(pm != 0ull) != 0ull;
     const bool tail = n_in < SEG;
+    if constexpr (ED) {
+        if (!CAP) {
+            EdRow er;
+            ed_bias(er, a.ed, pidx);
+            if (er.nb > 0)
+                ed_add<NL>(er, seg_lo, n_in, [&](int q, int c) -> float& {
+                    return c == 0 ? v[q].x : c == 1 ? v[q].y : c == 2 ? v[q].z : v[q].w;
+                });
+        }
+        if (masked) {
+            asm volatile("" : "+v"(eb.a), "+v"(eb.b));         // (the nibbles again: kept from the loads they spill)
+#pragma unroll
+            for (int q = 0; q < NL; ++q) {
+                const uint32_t nib = ed_nibble(eb, q);
+                v[q] = make_float4(ed_keep(v[q].x, nib, 0, 0x7FC00000u), ed_keep(v[q].y, nib, 1, 0x7FC00000u),
+                                   ed_keep(v[q].z, nib, 2, 0x7FC00000u), ed_keep(v[q].w, nib, 3, 0x7FC00000u));
+            }
+        }
+    }
 
     // the logits as ferro's sampler sees them (softcap; rep < 1: the penalty; past the row's end: NaN, never a
     // candidate) and the lane maximum (NaN-free: fmaxf drops NaN; NaN when every logit of the lane is NaN)
@@ -431,7 +468,7 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
     const bool gfast = greedy;
     if (gfast) {
         uint64_t best = 0ull;
-        if (lm == lm) {                                        // NaN: every logit of the lane is NaN
+        if (ED ? lm > -__builtin_huge_valf() : lm == lm) {     // NaN: every logit of the lane is NaN
             uint32_t first = 0u;
 #pragma unroll
             for (int q = NL - 1; q >= 0; --q) {
@@ -468,7 +505,8 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
 #pragma unroll
         for (int q = 1; q < SK_NW; ++q) tau = s.wb[q] < tau ? s.wb[q] : tau;
         if (tau == 0u) tau = 1u;                                   // NaN (key 0) is never a candidate
-        const float tf = tau > 0x007FFFFFu ? val_of(tau) : -__builtin_huge_valf();
+        constexpr float LOWEST = ED ? -3.402823466e+38f : -__builtin_huge_valf();   // of a candidate
+        const float tf = tau > 0x007FFFFFu ? val_of(tau) : LOWEST;
         // cap_late: the candidates are the logits whose capped value reaches the capped bound tc; tr is a raw value that
         // every one of them reaches: lane j < 32 caps the value 2^j keys below the bound (lane 32 the bound itself), and the first that falls
         // below tc (the cap is flat where it saturates) ends the range.
@@ -580,7 +618,7 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
         // With the penalty applied after the bound, fewer than k logits may stay at or above it: the segment's top k
         // may then hold a logit below the bound, which was not handed over (never expected with the spare lane per
         // wave)
-        const bool short_k = pen_late && ntot < (uint32_t)k && tf > -__builtin_huge_valf();
+        const bool short_k = pen_late && ntot < (uint32_t)k && tau > 0x007FFFFFu;
         const bool exact = gover || short_k || ntot > (uint32_t)SK_CAP;   // uniform
         if (!exact) {
             uint32_t pos = cbase + cincl - nc;
@@ -592,10 +630,12 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
             // ties at the bound: the exact k-th composite of the segment, then the (exactly k) composites at or above
             // it
             const float* segp = rowp + seg_lo;
-            const uint64_t kth = sk_kth_exact<CAP>(segp, seg_lo, n_in, SEG, cap, pen, rep, k, s);
+            EdRow er = {nullptr, false, nullptr, nullptr, 0};
+            if constexpr (ED) er = ed_row(a.ed, row, pidx, a.err);
+            const uint64_t kth = sk_kth_exact<CAP, ED>(segp, seg_lo, n_in, SEG, cap, pen, rep, er, k, s);
             if (tid == 0) s.misc[0] = 0u;
             __syncthreads();
-            sk_each<CAP>(segp, n_in, SEG, cap, pen, rep, s.bmp, [&](int i, uint32_t key) {
+            sk_each<CAP, ED>(segp, seg_lo, n_in, SEG, cap, pen, rep, s.bmp, er, [&](int i, uint32_t key) {
                 const uint64_t c64 = comp_of(key, (uint32_t)(seg_lo + i));
                 if (key != 0u && c64 >= kth) {
                     const uint32_t p = atomicAdd(&s.misc[0], 1u);
@@ -708,15 +748,20 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
     int tok = 0, keep = 1;
     if (greedy) {
         // ferro's scan (sampler.cpp:19-23) keeps index 0 when its logit is NaN; otherwise the first maximum
-        float l0 = ld_const(rowp);
-        if (CAP && cap > 0.0f) l0 = softcap_one(l0, cap);
-        tok = (l0 != l0 || kk == 0) ? 0 : (int)comp_id(read_lane(acc, 0));
+        if constexpr (ED) {
+            tok = kk == 0 ? -1 : (int)comp_id(read_lane(acc, 0));
+            keep = kk;
+        } else {
+            float l0 = ld_const(rowp);
+            if (CAP && cap > 0.0f) l0 = softcap_one(l0, cap);
+            tok = (l0 != l0 || kk == 0) ? 0 : (int)comp_id(read_lane(acc, 0));
+        }
         if (lane == 0 && a.kcap > 0) {
             if (a.cand_ids) a.cand_ids[(int64_t)row * a.kcap] = tok;
-            if (a.cand_probs) a.cand_probs[(int64_t)row * a.kcap] = 1.0;
+            if (a.cand_probs) a.cand_probs[(int64_t)row * a.kcap] = (double)keep;
         }
     } else if (kk == 0) {
-        tok = 0; keep = 0;                                     // every logit NaN: token 0, nothing kept
+        tok = ED ? -1 : 0; keep = 0;                           // no candidate (every logit NaN: token 0), nothing kept
     } else {
         if (!a.dmt) dr = sk_draw(a, row);
         wave_softmax(fa, rc, lane < kk ? acc : 0ull, kk, dr.u, tok, keep);
@@ -726,7 +771,7 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
     SK_FLUSH();
 }
 
-hipError_t launch_small_k(int nl, bool capped, bool all_greedy, unsigned grid, int flags, const SkArgs& k,
+hipError_t launch_small_k(int nl, bool capped, bool all_greedy, bool edited, unsigned grid, int flags, const SkArgs& k,
                           hipStream_t st) {
     const dim3 gd(grid), bd(SK_LT);
     // all-greedy batches: the greedy-only kernel, without the LDS pad (its registers allow more workgroups per CU)
@@ -734,24 +779,27 @@ hipError_t launch_small_k(int nl, bool capped, bool all_greedy, unsigned grid, i
         hipLaunchKernelGGL(kern, gd, bd, pad, st, k.logits, k.ld, k.B, k.V, k.nseg, flags, k.params, k.hist_off,
                            k.hist, k);
     };
-    auto by_nl = [&](auto cap, auto greedy, auto many) {
+    auto by_nl = [&](auto cap, auto greedy, auto many, auto ed) {
         constexpr bool C = decltype(cap)::value, G = decltype(greedy)::value, M = decltype(many)::value;
+        constexpr bool E = decltype(ed)::value;
         const unsigned pad = G ? 0u : SK_PAD_LDS;
-        if (nl == 16) go(small_k_kernel<16, C, G, M>, pad);
-        else if (nl == 8) go(small_k_kernel<8, C, G, M>, pad);
-        else go(small_k_kernel<4, C, G, M>, pad);
+        if (nl == 16) go(small_k_kernel<16, C, G, M, E>, pad);
+        else if (nl == 8) go(small_k_kernel<8, C, G, M, E>, pad);
+        else go(small_k_kernel<4, C, G, M, E>, pad);
     };
     const std::true_type yes;
     const std::false_type no;
-    if (all_greedy) {
-        if (capped) by_nl(yes, yes, no);
-        else by_nl(no, yes, no);
-    } else if (k.nseg > 4 * SK_NW) {
-        if (capped) by_nl(yes, no, yes);
-        else by_nl(no, no, yes);
+    auto by_rows = [&](auto cap, auto ed) {
+        if (all_greedy) by_nl(cap, yes, no, ed);
+        else if (k.nseg > 4 * SK_NW) by_nl(cap, no, yes, ed);
+        else by_nl(cap, no, no, ed);
+    };
+    if (edited) {
+        if (capped) by_rows(yes, yes);
+        else by_rows(no, yes);
     } else {
-        if (capped) by_nl(yes, no, no);
-        else by_nl(no, no, no);
+        if (capped) by_rows(yes, no);
+        else by_rows(no, no);
     }
     return hipGetLastError();
 }

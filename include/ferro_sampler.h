@@ -280,9 +280,11 @@ typedef struct fs_edits {
  * arguments and outputs beside `edits` (h_params may be NULL here too; edits may not). A row's candidates are its allowed
  * tokens whose edited logit is above -inf: k, min-p and top-p count those alone. A row without a candidate has token -1
  * and 0 kept (a greedy row's candidate outputs are -1 and 0); -1 ends a verification window at its row, and fs_decode_step_
- * edited appends it to the history, where the penalties ignore it. The rows are edited into a workspace of V * 4 bytes a
- * row first, which grows as a context's other buffers do (a call under graph capture that would need a larger one
- * returns FS_E_NOMEM). */
+ * edited appends it to the history, where the penalties ignore it. With h_params, batches that the small-k or the mid-k
+ * kernel takes (fs_route_plan, fs_mid_k_plan) and that have no biases beside a softcap read their logits once, where they
+ * are, and of masked rows only the groups of four with an allowed token; others are edited into a workspace of V * 4 bytes
+ * a row first, which grows as a context's other buffers do. A call under graph capture whose workspace would have to grow
+ * returns FS_E_NOMEM and leaves the capture as it was. */
 int fs_sample_edited(fs_context* ctx, const float* d_logits, int64_t ld, int32_t B, int32_t V, const int32_t* d_hist,
                      const int64_t* d_hist_off, const fs_row_params* d_params, const fs_row_params* h_params,
                      const fs_edits* edits, const double* d_u, int32_t* d_tok, int32_t kcap, int32_t* d_cand_ids,
