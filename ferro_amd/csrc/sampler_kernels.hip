@@ -843,6 +843,13 @@ int edit_args(const fs_edits* edits, int32_t rows, int32_t V, fs::EdArgs& ed) {
     return FS_OK;
 }
 
+// Parts per row of fs_logprobs: as many as fill the device once with four workgroups per CU, and no more than the row has
+// chunks.
+int logprob_parts(int cus, int64_t B, int32_t V, int32_t type) {
+    const int64_t chunk = (int64_t)fs::SK_LT * 4 * fs::LP_NL(type), n = ((int64_t)V + chunk - 1) / chunk;
+    return (int)std::min<int64_t>(n, std::max<int64_t>(1, 4 * (int64_t)cus / B));
+}
+
 size_t type_size(int32_t type) { return type == FS_F32 ? 4 : type == FS_BF16 || type == FS_F16 ? 2 : 0; }
 
 // Rows of logits of any type: check_rows for FS_F32, four logits' alignment for the others.
@@ -1246,23 +1253,18 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
     const Edited call(ctx, st);
     if (call.rc != FS_OK) return call.rc;
     std::lock_guard<std::mutex> g(ctx->mu);
-    int nl = 4;
-    for (const int l : {16, 8, 4}) {                           // the largest segments that give every CU four workgroups
-        nl = l;
-        a.nseg = (int)(((int64_t)V + fs::SK_LT * l * 4 - 1) / (fs::SK_LT * l * 4));
-        if ((int64_t)B * a.nseg >= 4 * (int64_t)ctx->cus) break;
-    }
+    a.nseg = logprob_parts(ctx->cus, B, V, type);
     if ((int64_t)B * a.nseg > 0x7fffffff) return FS_E_INVALID;
-    const size_t segs = (size_t)B * a.nseg;
+    const size_t segs = a.nseg > 1 ? (size_t)B * a.nseg : 0;   // (a row of one part needs no workspace)
     rc = grow(ctx, 0, 0, 0);
     if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_part, ctx->lp_segs, segs, 1, false);
     if (rc == FS_OK && top > 0) rc = grow_buffer(ctx, ctx->lp_lists, ctx->lp_list_segs, segs, fs::LP_TOP, false);
-    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_ticket, ctx->lp_rows, (size_t)B, 1, true);
+    if (rc == FS_OK && segs > 0) rc = grow_buffer(ctx, ctx->lp_ticket, ctx->lp_rows, (size_t)B, 1, true);
     if (rc != FS_OK) return rc;
     a.logits = d_logits; a.ld = ld; a.B = B; a.V = V; a.n = top; a.params = d_params; a.tok = d_tok;
     a.lp = d_lp; a.rank = d_rank; a.ids = d_top_ids; a.top = d_top_lp;
     a.part = ctx->lp_part; a.lists = ctx->lp_lists; a.ticket = ctx->lp_ticket; a.err = ctx->err;
-    return fs::launch_logprobs(nl, type, a, st) == hipSuccess ? FS_OK : FS_E_HIP;
+    return fs::launch_logprobs(type, a, st) == hipSuccess ? FS_OK : FS_E_HIP;
 }
 
 int fs_penalize_batch(fs_context* ctx, float* d_logits, int64_t ld, int32_t B, int32_t V, const int32_t* d_hist,

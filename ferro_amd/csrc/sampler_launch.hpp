@@ -135,15 +135,16 @@ hipError_t launch_edit_end(const EditEnd& e, hipStream_t st);
 
 // Log-probabilities (logprob_kernel.hip).
 constexpr int LP_TOP = 64;                 // largest n: one entry per lane of the finishing wave
-struct LpPart {                            // a segment's share of its row
+constexpr int LP_NL(int type) { return type == FS_F32 ? 4 : 8; }   // groups of four per thread in a chunk of 16 KB
+struct LpPart {                            // a part's share of its row
     double sum;                            // of exp((x - max) / T)
-    float max;
     uint32_t above;                        // logits above the chosen token's
+    float max;
 };
 struct LpArgs {
     const void* logits;
     int64_t ld;
-    int B, V, nseg, n;
+    int B, V, nseg, n;                     // nseg: parts per row
     const fs_row_params* params;           // NULL: no softcap, temperature 1
     EdArgs ed;
     const int32_t* tok;
@@ -156,7 +157,7 @@ struct LpArgs {
     uint32_t* ticket;                      // [B], left at 0
     int32_t* err;
 };
-hipError_t launch_logprobs(int nl, int type, const LpArgs& a, hipStream_t st);
+hipError_t launch_logprobs(int type, const LpArgs& a, hipStream_t st);
 
 hipError_t launch_lookup_draft(int n_streams, const int32_t* hist, const int64_t* hist_off, const int32_t* kmax,
                                const int32_t* min_n, int eos, int32_t* draft, int draft_ld, int32_t* ndraft,
