@@ -99,16 +99,33 @@ __device__ __forceinline__ int64_t ed_lower(const EdRow& r, int id) {
     }
     return lo + __popcll(__ballot(lo + lane_id() < hi && r.ids[lo + lane_id()] < id));
 }
+// A row's biases in registers, one per lane, where it has no more of them (held by kernels that pass over several chunks).
+struct EdList {
+    int id;
+    float val;
+};
+__device__ __forceinline__ EdList ed_list(const EdRow& r) {
+    EdList l = {0x7fffffff, 0.0f};
+    if (lane_id() < r.nb && r.nb <= WAVE) l = {r.ids[lane_id()], r.val[lane_id()]};
+    return l;
+}
 // Adds the row's biases to the wave's logits of the segment, one after another in list order (equal ids add up): each is
 // read by one lane, and the wave gives it to the lane whose logit it is. x(q, c): the lane's logits.
 template <int NL, class X>
-__device__ __forceinline__ void ed_add(const EdRow& r, int seg_lo, int n_in, X x) {
+__device__ __forceinline__ void ed_add(const EdRow& r, const EdList* held, int seg_lo, int n_in, X x) {
     const int lane = lane_id(), w = (int)threadIdx.x / WAVE;
+#pragma unroll 1
     for (int64_t i = r.nb > 4 * WAVE ? ed_lower(r, seg_lo) : 0; i < r.nb; i += WAVE) {
-        const bool in = i + lane < r.nb;
-        const int id = in ? r.ids[i + lane] : 0x7fffffff;
+        int id = 0x7fffffff;
+        float val = 0.0f;
+        if (held && r.nb <= WAVE) {
+            id = held->id;
+            val = held->val;
+        } else if (i + lane < r.nb) {
+            id = r.ids[i + lane];
+            val = r.val[i + lane];
+        }
         const uint32_t rel = (uint32_t)id - (uint32_t)seg_lo;
-        const float val = in ? r.val[i + lane] : 0.0f;
         const bool here = rel < (uint32_t)n_in && ((rel >> 2) & (SK_LT - 1)) / WAVE == (uint32_t)w;
         if (__ballot(here) != 0ull) {                          // (most waves hold none of the 64)
 #pragma unroll
@@ -130,12 +147,13 @@ __device__ __forceinline__ void ed_add(const EdRow& r, int seg_lo, int n_in, X x
 }
 
 // Token id's logit l with its mask and biases, on every lane (whole wave): NaN where it is not allowed.
-__device__ __forceinline__ float ed_one(const EdRow& r, float l, int id) {
-    for (int64_t i = ed_lower(r, id); i < r.nb; i += WAVE) {
-        const int at = i + lane_id() < r.nb ? r.ids[i + lane_id()] : 0x7fffffff;
+__device__ __forceinline__ float ed_one(const EdRow& r, const EdList& list, float l, int id) {
+    for (int64_t i = r.nb <= WAVE ? 0 : ed_lower(r, id); i < r.nb; i += WAVE) {
+        const bool held = r.nb <= WAVE, in = i + lane_id() < r.nb;
+        const int at = held ? list.id : in ? r.ids[i + lane_id()] : 0x7fffffff;
+        const float val = held ? list.val : in ? r.val[i + lane_id()] : 0.0f;
         uint64_t m = __ballot(at == id);
         const bool more = m == ~0ull;
-        const float val = at == id ? r.val[i + lane_id()] : 0.0f;
         for (; m; m &= m - 1) l = __fadd_rn(l, read_lane(val, __ffsll((unsigned long long)m) - 1));
         if (!more) break;
     }

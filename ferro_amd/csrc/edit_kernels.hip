@@ -88,7 +88,7 @@ __global__ __launch_bounds__(SK_LT) void edit_kernel(EditArgs e) {
         L::floats(raw[q], x[q]);
         if (p.softcap > 0.0f) softcap_vals(x[q], p.softcap);
     }
-    if (r.nb > 0) ed_add<NL>(r, seg_lo, n_in, [&](int q, int c) -> float& { return x[q][c]; });
+    if (r.nb > 0) ed_add<NL>(r, nullptr, seg_lo, n_in, [&](int q, int c) -> float& { return x[q][c]; });
     const bool greedy = p.temperature <= 0.0f || p.top_k == 1;
     const uint32_t none = e.any ? 0x7FC00000u : 0xFF800000u;   // the sampling kernels' rows: NaN, never a candidate
     float* out = e.out + (int64_t)row * e.out_ld + seg_lo;

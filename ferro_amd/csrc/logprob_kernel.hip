@@ -11,10 +11,13 @@
 //     subtraction, a product, an exponential and an addition a logit;
 //   - a chunk whose sum is NaN (NaN or infinite logits) is added again with those left out; where the row's largest logit
 //     is infinite its tokens are counted instead;
-//   - the n largest: a bound, first the n-th of the wave's 64 lane maxima, passes over chunks without a candidate by one
-//     compare a lane; the others go to a list in LDS, cut to the 64 largest by register sorts whenever it may overflow, which
-//     raises the bound.
-// The waves' lists and sums are joined, then the parts' by the row's last one (a ticket).
+//   - the n largest: a bound, the n-th of the wave's 64 lane maxima so far, passes over chunks without a candidate by one
+//     compare a lane; the others go to a list in LDS, which is cut to the n largest by register sorts whenever it may
+//     overflow. The lane maxima are sorted again when the list has grown by LP_GROWN entries.
+// At the end of a part the entries of its lists at or above the waves' best bound (about 2.5 n) are ranked; the row's last part (a ticket; a row's parts share an XCD and its L2)
+// joins the parts' sums and lists.
+// A chunk's mask is read a chunk ahead of its logits, whose groups of four without an allowed token are not read (the
+// part's first chunk is requested whole, at once).
 // Bound: HBM; the arithmetic (about 10 instructions a logit) takes about half of the time of reading 16-bit logits.
 #include "edit_device.hpp"
 #include "row_device.hpp"
@@ -22,9 +25,16 @@
 namespace fs {
 
 constexpr int LP_LIST = LP_TOP + 4 * WAVE; // entries of a wave's list: the largest so far and one group of four per lane
+constexpr int LP_JOIN = 512;               // entries that are ranked at once
+constexpr int LP_GROWN = 16;
 
 struct LpShared {
     uint64_t list[SK_NW][LP_LIST];
+    uint64_t join[LP_JOIN];
+    uint64_t top[LP_TOP];
+    uint32_t rank[SK_LT];
+    float bound[SK_NW];
+    uint32_t n;
     double sum[SK_NW];
     float max[SK_NW];
     uint32_t above[SK_NW];
@@ -48,12 +58,32 @@ __device__ __forceinline__ uint64_t lp_cut(uint64_t* list, int& cnt, int n) {
     const int lane = lane_id();
     lp_wave_sync();
     uint64_t acc = 0ull;
-    for (int i = 0; i < cnt; i += WAVE) acc = merge_top64(acc, sort64<false>(i + lane < cnt ? list[i + lane] : 0ull));
+    for (int i = 0; i < cnt; i += WAVE) {
+        const uint64_t e = i + lane < cnt ? list[i + lane] : 0ull;
+        acc = i == 0 ? sort64<true>(e) : merge_top64(acc, sort64<false>(e));
+    }
     acc = lane < n ? acc : 0ull;
     lp_wave_sync();
     list[lane] = acc;
     cnt = __popcll(__ballot(acc != 0ull));
     return acc;
+}
+
+// The n largest of the s.n <= LP_JOIN distinct entries of s.join, sorted to s.top, which is zero before. Whole workgroup,
+// after a barrier; ends with one.
+__device__ __forceinline__ void lp_rank(LpShared& s, int n) {
+    const int cnt = (int)s.n;
+    if (cnt <= SK_LT) {
+        sk_rank(s.join, s.rank, cnt, [&](uint32_t r, uint64_t c) { if (r < (uint32_t)n) s.top[r] = c; });
+    } else {
+        for (int c = threadIdx.x; c < cnt; c += SK_LT) {
+            const uint64_t me = s.join[c];
+            uint32_t r = 0u;
+            for (int j = 0; j < cnt; ++j) r += s.join[j] > me ? 1u : 0u;
+            if (r < (uint32_t)n) s.top[r] = me;
+        }
+    }
+    __syncthreads();
 }
 
 // The tokens at +inf of a row whose largest logit that is, by one workgroup.
@@ -71,33 +101,60 @@ __device__ __forceinline__ double lp_infinite(const LpArgs& a, const EdRow& r, i
     return s.sum[0] + s.sum[1] + s.sum[2] + s.sum[3];
 }
 
+// The kernel's argument list as a struct: the argument segment follows the same layout rules
+struct LpKernargs {
+    const void* logits;
+    int64_t ld;
+    int B, V, nseg, n;
+    LpArgs a;
+};
+
 // NL: groups of four per thread and chunk. TOP: the n largest are asked for.
 template <int TYPE, int NL, bool TOP>
-__global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(LpArgs a) {
+__global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, int64_t ld, int B, int V, int nseg, int n,
+                                                           LpArgs a_) {
     constexpr int CHUNK = SK_LT * NL * 4;
     __shared__ __align__(16) LpShared s;
     const int tid = threadIdx.x, lane = lane_id(), w = tid / WAVE;
-    const int row = (int)blockIdx.x / a.nseg, part = (int)blockIdx.x - row * a.nseg;
-    const int V = a.V;
+    // a row's parts are consecutive workgroups of one index class mod XCDS, as in the small-k kernel
+    const int j = (int)(blockIdx.x / (unsigned)XCDS);
+    const int q_row = __builtin_amdgcn_readfirstlane(j / nseg);
+    const int part = j - q_row * nseg;
+    const int row = (int)(blockIdx.x % (unsigned)XCDS) + XCDS * q_row;
+    if (row >= B) return;
     using L = Logits4<TYPE>;
     // the part's chunks [c0, c1): the row's, dealt evenly
     const int nchunk = (V + CHUNK - 1) / CHUNK;
-    const int c0 = (int)((int64_t)nchunk * part / a.nseg), c1 = (int)((int64_t)nchunk * (part + 1) / a.nseg);
+    const int c0 = (int)((int64_t)nchunk * part / nseg), c1 = (int)((int64_t)nchunk * (part + 1) / nseg);
+    typename L::raw raw[NL];
+    auto load = [&](int c, bool skip, const EdBits& bits) {
+        const int lo = c * CHUNK, n_in = V - lo < CHUNK ? V - lo : CHUNK;
+        const __amdgpu_buffer_rsrc_t rs = L::rsrc(logits, (int64_t)row * ld + lo, n_in);
+#pragma unroll
+        for (int q = 0; q < NL; ++q) {
+            int at = q * SK_LT + tid;
+            if (skip) at = ed_nibble(bits, q) != 0u ? at : 0x07ffffff;       // (past the buffer: no read, zeros)
+            raw[q] = L::load(rs, at);
+        }
+    };
+    EdBits bits = {~0u, ~0u}, next = bits;                     // of the chunk in raw; of the one after it
+    load(c0, false, bits);
+    __builtin_amdgcn_sched_barrier(0);
+    const __attribute__((address_space(4))) char* kseg =       // (as in the small-k kernel: no argument is read earlier)
+        (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(kseg) : : "memory");
+    const LpArgs& a = *(const LpArgs*)(kseg + offsetof(LpKernargs, a));
+    (void)a_;
     EdRow r = {nullptr, false, nullptr, nullptr, 0};
     ed_mask(r, a.ed, row, a.err);
     const bool masked = r.words || r.closed;
-    typename L::raw raw[NL];
-    EdBits bits = {~0u, ~0u};
-    auto load = [&](int c) {
-        const int lo = c * CHUNK, n_in = V - lo < CHUNK ? V - lo : CHUNK;
-        const __amdgpu_buffer_rsrc_t rs = L::rsrc(a.logits, (int64_t)row * a.ld + lo, n_in);
-#pragma unroll
-        for (int q = 0; q < NL; ++q) raw[q] = L::load(rs, q * SK_LT + tid);
-        if (masked) bits = ed_bits<NL>(r, lo, V);
-    };
-    load(c0);
-    __builtin_amdgcn_sched_barrier(0);
+    if (masked) {
+        bits = ed_bits<NL>(r, c0 * CHUNK, V);
+        if (c0 + 1 < c1) next = ed_bits<NL>(r, (c0 + 1) * CHUNK, V);
+    }
     ed_bias(r, a.ed, row);
+    const EdList few = ed_list(r);
+    const int t = a.tok ? ld_const(a.tok + row) : -1;
     float cap = 0.0f, T = 1.0f;
     if (a.params) {
         cap = ld_const(&a.params[row].softcap);
@@ -106,23 +163,26 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(LpArgs a) {
     }
     auto fmx = [](float u, float v) { return fmaxf(u, v); };
     const float c2 = (float)(1.4426950408889634 / (double)T);
-    // the chosen token's logit
-    const int t = a.tok ? ld_const(a.tok + row) : -1;
-    float xt = __builtin_huge_valf();
+    // the chosen token's logit (NaN: it takes no part), and what the others are compared with
+    float xv = __builtin_nanf("");
     if (t >= 0 && t < V) {
-        float l = L::one(a.logits, (int64_t)row * a.ld + t);
-        if (cap > 0.0f) l = softcap_one(l, cap);
-        xt = ed_one(r, l, t);
-        if (!(xt > LP_NONE)) xt = __builtin_huge_valf();       // takes no part: nothing to count
+        xv = L::one(logits, (int64_t)row * ld + t);
+        if (cap > 0.0f) xv = softcap_one(xv, cap);
+        xv = ed_one(r, few, xv, t);
+        xv = xv > LP_NONE ? xv : __builtin_nanf("");
     }
-    const bool has = xt < __builtin_huge_valf();
+    const bool has = xv < __builtin_huge_valf();               // (none is larger than +inf)
 
     float mx = LP_LOWEST;                                      // the wave's largest logit: its sums' reference
     double sum = 0.0;
     uint32_t above = 0u;                                       // the wave's count
-    float bound = 0.0f;                                        // TOP: of the wave's candidates
-    bool bounded = false;
-    int cnt = 0;
+    // TOP: the bound of new candidates; what n logits of the wave reach; the lane's largest logit
+    float bound = LP_LOWEST, reach = LP_LOWEST, lm = LP_NONE;
+    int cnt = 0, sorted_at = -LP_GROWN;                        // the list's length, when the bound was taken
+    if (TOP) {
+        if (tid == 0) s.n = 0u;
+        if (tid < LP_TOP) s.top[tid] = 0ull;
+    }
 #pragma unroll 1
     for (int c = c0; c < c1; ++c) {
         const int lo = c * CHUNK, n_in = V - lo < CHUNK ? V - lo : CHUNK;
@@ -130,13 +190,15 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(LpArgs a) {
 #pragma unroll
         for (int q = 0; q < NL; ++q) L::floats(raw[q], x[q]);
         const EdBits now = bits;
-        if (c + 1 < c1) load(c + 1);
+        bits = next;
+        if (c + 1 < c1) load(c + 1, masked, bits);
+        if (masked && c + 2 < c1) next = ed_bits<NL>(r, (c + 2) * CHUNK, V);
         __builtin_amdgcn_sched_barrier(0);
         if (cap > 0.0f) {
 #pragma unroll
             for (int q = 0; q < NL; ++q) softcap_vals(x[q], cap);
         }
-        if (r.nb > 0) ed_add<NL>(r, lo, n_in, [&](int q, int c_) -> float& { return x[q][c_]; });
+        if (r.nb > 0) ed_add<NL>(r, &few, lo, n_in, [&](int q, int c_) -> float& { return x[q][c_]; });
         if (masked) {
 #pragma unroll
             for (int q = 0; q < NL; ++q) {
@@ -165,9 +227,11 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(LpArgs a) {
             }
             float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int q = 0; q < NL; ++q)
+            for (int q = 0; q < NL; ++q) {
 #pragma unroll
                 for (int c_ = 0; c_ < 4; ++c_) e[c_] += __builtin_amdgcn_exp2f((x[q][c_] - mx) * c2);
+                __builtin_amdgcn_sched_barrier(0);             // (all exponentials at once need more registers)
+            }
             return (e[0] + e[1]) + (e[2] + e[3]);
         };
         lane_max();
@@ -181,31 +245,38 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(LpArgs a) {
             e = fminf(add(), 1e30f);                           // (the tokens at +inf are counted by themselves)
         }
         sum += (double)e;
-        if (has && __ballot(cm > xt) != 0ull) {
+        if (has && __ballot(cm > xv) != 0ull) {
 #pragma unroll
             for (int q = 0; q < NL; ++q)
 #pragma unroll
-                for (int c_ = 0; c_ < 4; ++c_) above += (uint32_t)__popcll(__ballot(x[q][c_] > xt));
+                for (int c_ = 0; c_ < 4; ++c_) above += (uint32_t)__popcll(__ballot(x[q][c_] > xv));
         }
         if (TOP) {
-            if (!bounded) {                                    // n lanes reach the n-th of their maxima
-                const uint32_t srt = sort64_desc_u32(cm > LP_NONE ? key_of(cm) : 0u);
-                const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)srt, a.n - 1);
-                bounded = key != 0u;
-                bound = bounded ? val_of(key) : -3.402823466e+38f;
+            lm = fmaxf(lm, cm);
+            if (cnt - sorted_at >= LP_GROWN && __ballot(cm > bound) != 0ull) {
+                float b;
+                if (n == 1) {
+                    b = mx;
+                } else {
+                    const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)sort64_desc_u32(key_of(lm)), n - 1);
+                    b = key > 0x007FFFFFu ? val_of(key) : LP_LOWEST;
+                }
+                bound = fmaxf(bound, b);
+                reach = fmaxf(reach, b);
+                sorted_at = b > LP_LOWEST ? cnt : sorted_at;
             }
             if (__ballot(cm >= bound) != 0ull) {
 #pragma unroll
                 for (int q = 0; q < NL; ++q) {
                     if (__ballot(lp_max3(lp_max3(LP_NONE, x[q][0], x[q][1]), x[q][2], x[q][3]) >= bound) != 0ull) {
                         if (cnt > LP_LIST - 4 * WAVE) {
-                            const uint64_t acc = lp_cut(s.list[w], cnt, a.n);
-                            const uint32_t key = comp_key(read_lane(acc, a.n - 1));
-                            // later ids lose to equal values: the next value up
+                            const uint64_t acc = lp_cut(s.list[w], cnt, n);
+                            const uint32_t key = comp_key(read_lane(acc, n - 1));
                             if (key != 0u) {
-                                bounded = true;
-                                bound = val_of(key + 1u);
+                                reach = val_of(key);
+                                bound = val_of(key + 1u);      // later ids lose to equal values: the next value up
                             }
+                            sorted_at = cnt;
                         }
 #pragma unroll
                         for (int c_ = 0; c_ < 4; ++c_) {
@@ -224,10 +295,12 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(LpArgs a) {
     auto addu = [](uint32_t u, uint32_t v) { return u + v; };
     auto addf = [](double u, double v) { return u + v; };
     sum = wave_allreduce(sum, addf);
-    uint64_t acc = 0ull;
-    if (TOP) acc = lp_cut(s.list[w], cnt, a.n);                // (and keeps it in the list)
+    if (TOP && cnt > LP_JOIN / SK_NW) {
+        const uint32_t key = comp_key(read_lane(lp_cut(s.list[w], cnt, n), n - 1));
+        if (key != 0u) reach = val_of(key);
+    }
     if (lane == 0) {
-        s.sum[w] = sum; s.max[w] = mx; s.above[w] = above;
+        s.sum[w] = sum; s.max[w] = mx; s.above[w] = above; s.bound[w] = reach;
     }
     __syncthreads();
     // a sum S relative to m, relative to M >= m instead
@@ -237,59 +310,88 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(LpArgs a) {
     float M = fmaxf(fmaxf(s.max[0], s.max[1]), fmaxf(s.max[2], s.max[3]));
     double S = wave_allreduce(lane < SK_NW ? to(s.sum[lane & (SK_NW - 1)], s.max[lane & (SK_NW - 1)], M) : 0.0, addf);
     uint32_t ab = s.above[0] + s.above[1] + s.above[2] + s.above[3];
-    if (TOP && w == 0) {
-#pragma unroll 1
-        for (int i = 1; i < SK_NW; ++i) acc = merge_top64(acc, s.list[i][WAVE - 1 - lane]);
+    if (TOP) {                                                 // the waves' entries that reach the best of their bounds
+        const float best = fmaxf(fmaxf(s.bound[0], s.bound[1]), fmaxf(s.bound[2], s.bound[3]));
+        const uint32_t key = key_of(best);
+        for (int i = 0; i < cnt; i += WAVE) {
+            const uint64_t e = i + lane < cnt ? s.list[w][i + lane] : 0ull;
+            const uint64_t m = __ballot(comp_key(e) >= key);
+            if (m == 0ull) continue;
+            uint32_t base = 0u;
+            if (lane == 0) base = atomicAdd(&s.n, (uint32_t)__popcll(m));
+            base = (uint32_t)__builtin_amdgcn_readfirstlane((int)base);
+            if (comp_key(e) >= key) s.join[base + mbcnt(m)] = e;
+        }
+        __syncthreads();
+        lp_rank(s, n);
     }
-    if (a.nseg > 1) {                                          // uniform
-        LpPart* pr = a.part + (int64_t)row * a.nseg;
-        uint64_t* rl = a.lists + (int64_t)row * a.nseg * LP_TOP;
+    if (nseg > 1) {                                            // uniform
+        LpPart* pr = a.part + (int64_t)row * nseg;
+        uint64_t* rl = a.lists + (int64_t)row * nseg * LP_TOP;
+        if (TOP && tid < n) rl[part * LP_TOP + tid] = s.top[tid];
+        if (tid == 0) {
+            pr[part].sum = S;
+            pr[part].above = ab;
+            pr[part].max = M;
+        }
         if (w == 0) {
-            if (TOP) st_agent(&rl[(int64_t)part * LP_TOP + lane], acc);
-            if (lane == 0) {
-                uint64_t* o = reinterpret_cast<uint64_t*>(pr + part);
-                st_agent(o, (uint64_t)__double_as_longlong(S));
-                st_agent(o + 1, ((uint64_t)__float_as_uint(M) << 32) | ab);
-            }
-            vm_drain();                                        // the part's results are out
+            vm_drain();                                        // the part's results are in the L2
             if (lane == 0)
-                s.last = __hip_atomic_fetch_add(a.ticket + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                         (uint32_t)a.nseg - 1u ? 1u : 0u;
+                s.last = __hip_atomic_fetch_add(a.ticket + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) ==
+                         (uint32_t)nseg - 1u ? 1u : 0u;
         }
         __syncthreads();
         if (s.last == 0u) return;
         // ---- the row's end, by its last part
-        if (tid == 0) __hip_atomic_store(a.ticket + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (TOP) {                                             // wave w folds lists w, w + SK_NW, ..., then wave 0 the waves'
-            acc = 0ull;
-            for (int i = w; i < a.nseg; i += SK_NW)
-                acc = merge_top64(acc, ld_agent(&rl[(int64_t)i * LP_TOP + WAVE - 1 - lane]));      // ascending
-            s.list[w][lane] = acc;
+        if (tid == 0) {
+            a.ticket[row] = 0u;
+            s.n = 0u;
         }
-        M = LP_LOWEST;
-        S = 0.0;
-        ab = 0u;
-        for (int i = lane; i < a.nseg; i += WAVE) {            // (a lane's parts, one after another)
-            const uint64_t* o = reinterpret_cast<const uint64_t*>(pr + i);
-            const uint64_t e = ld_agent(o + 1);
-            const double Si = __longlong_as_double((long long)ld_agent(o));
-            const float m = __uint_as_float((uint32_t)(e >> 32)), both = fmaxf(m, M);
-            S = to(S, M, both) + to(Si, m, both);
-            M = both;
-            ab += (uint32_t)e;
-        }
-        const float all = wave_allreduce(M, fmx);
-        S = to(S, M, all);
-        M = all;
-        S = wave_allreduce(S, addf);
-        ab = wave_allreduce(ab, addu);
+        if (TOP && tid < LP_TOP) s.top[tid] = 0ull;
+        const LpPart mine = lane < nseg ? pr[lane] : LpPart{0.0, 0u, LP_LOWEST};
         if (TOP) {
+            // Every list's q-th entry, q = ceil(2 n / nseg): ceil(n / q) of them at or above a value make n entries that
+            // reach it. Those (about 1.5 n) are ranked.
+            const int q = (2 * n + nseg - 1) / nseg < n ? (2 * n + nseg - 1) / nseg : n, m = (n + q - 1) / q;
+            const uint64_t at = lane < nseg ? rl[lane * LP_TOP + q - 1] : 0ull;
+            constexpr int U = 4;                               // entries in flight per thread
+            const int total = nseg * n;
+            uint64_t e[U];
+            auto fetch = [&](int i0) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int i = i0 + u * SK_LT + tid;
+                    e[u] = i < total ? rl[i / n * LP_TOP + i % n] : 0ull;
+                }
+            };
+            fetch(0);
+            uint32_t least = m == 1 ? wave_max(comp_key(at))
+                                    : (uint32_t)__builtin_amdgcn_readlane((int)sort64_desc_u32(comp_key(at)), m - 1);
+            if (least == 0u) least = 1u;                       // fewer lists hold q entries: every entry
             __syncthreads();
-            if (w == 0) {
-#pragma unroll 1
-                for (int i = 1; i < SK_NW; ++i) acc = merge_top64(acc, s.list[i][WAVE - 1 - lane]);
+            for (int i0 = 0; i0 < total; i0 += U * SK_LT) {
+                if (i0 > 0) fetch(i0);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (comp_key(e[u]) >= least) {
+                        const uint32_t p = atomicAdd(&s.n, 1u);
+                        if (p < (uint32_t)LP_JOIN) s.join[p] = e[u];
+                    }
+            }
+            __syncthreads();
+            if (s.n <= (uint32_t)LP_JOIN) {
+                lp_rank(s, n);
+            } else if (w == 0) {                               // one wave merges the lists
+                uint64_t acc = 0ull;
+                for (int i = 0; i < nseg; ++i)
+                    acc = merge_top64(acc, WAVE - 1 - lane < n ? rl[i * LP_TOP + WAVE - 1 - lane] : 0ull);   // ascending
+                s.top[lane] = acc;
+                lp_wave_sync();
             }
         }
+        M = wave_allreduce(mine.max, fmx);
+        S = wave_allreduce(to(mine.sum, mine.max, M), addf);
+        ab = wave_allreduce(mine.above, addu);
     }
     if (!(M < __builtin_huge_valf())) {                        // uniform
         __syncthreads();
@@ -301,28 +403,22 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(LpArgs a) {
         return v > LP_NONE ? (float)((v == M ? 0.0 : ((double)v - (double)M) / (double)T) - z) : LP_NONE;
     };
     if (lane == 0) {
-        bool part_of = t >= 0 && t < V;
-        float v = LP_NONE;
-        if (part_of) {                                         // (+inf counts too: xt stands for "nothing to count" above)
-            v = L::one(a.logits, (int64_t)row * a.ld + t);
-            if (cap > 0.0f) v = softcap_one(v, cap);
-            v = ed_lane(r, v, t);
-            part_of = v > LP_NONE;
-        }
-        if (a.lp) a.lp[row] = part_of ? lp_of(v) : LP_NONE;
-        if (a.rank) a.rank[row] = part_of ? (has ? (int)ab + 1 : 1) : 0;
+        if (a.lp) a.lp[row] = lp_of(xv);
+        if (a.rank) a.rank[row] = xv > LP_NONE ? (has ? (int)ab + 1 : 1) : 0;
     }
-    if (TOP && lane < a.n) {
-        if (a.ids) a.ids[(int64_t)row * a.n + lane] = acc != 0ull ? (int)comp_id(acc) : -1;
-        if (a.top) a.top[(int64_t)row * a.n + lane] = acc != 0ull ? lp_of(val_of(comp_key(acc))) : LP_NONE;
+    if (TOP && lane < n) {
+        const uint64_t acc = s.top[lane];
+        if (a.ids) a.ids[(int64_t)row * n + lane] = acc != 0ull ? (int)comp_id(acc) : -1;
+        if (a.top) a.top[(int64_t)row * n + lane] = acc != 0ull ? lp_of(val_of(comp_key(acc))) : LP_NONE;
     }
 }
 
 hipError_t launch_logprobs(int type, const LpArgs& a, hipStream_t st) {
-    const dim3 grid((unsigned)((int64_t)a.B * a.nseg)), block(SK_LT);
+    const dim3 grid((unsigned)((int64_t)XCDS * a.nseg * (((int64_t)a.B + XCDS - 1) / XCDS))), block(SK_LT);
     auto go = [&](auto t, auto top) {
         constexpr int T = decltype(t)::value;
-        hipLaunchKernelGGL((logprob_kernel<T, LP_NL(T), decltype(top)::value>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((logprob_kernel<T, LP_NL(T), decltype(top)::value>), grid, block, 0, st, a.logits, a.ld, a.B,
+                           a.V, a.nseg, a.n, a);
     };
     auto by_top = [&](auto t) {
         if (a.n > 0) go(t, std::true_type{});

@@ -1729,7 +1729,7 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
             if (!CAP) {
                 EdRow er;
                 ed_bias(er, a.ed, pidx);
-                if (er.nb > 0) ed_add<NL>(er, seg_lo, n_in, [&](int q, int c) -> float& { return v[q][c]; });
+                if (er.nb > 0) ed_add<NL>(er, nullptr, seg_lo, n_in, [&](int q, int c) -> float& { return v[q][c]; });
             }
             if (masked) {
                 asm volatile("" : "+v"(eb.a), "+v"(eb.b));         // (the nibbles again: kept from the loads they spill)

@@ -844,10 +844,11 @@ int edit_args(const fs_edits* edits, int32_t rows, int32_t V, fs::EdArgs& ed) {
 }
 
 // Parts per row of fs_logprobs: as many as fill the device once with four workgroups per CU, and no more than the row has
-// chunks.
-int logprob_parts(int cus, int64_t B, int32_t V, int32_t type) {
+// chunks or the join takes lists (one per lane).
+int logprob_parts(const fs_context* c, int64_t B, int32_t V, int32_t type) {
     const int64_t chunk = (int64_t)fs::SK_LT * 4 * fs::LP_NL(type), n = ((int64_t)V + chunk - 1) / chunk;
-    return (int)std::min<int64_t>(n, std::max<int64_t>(1, 4 * (int64_t)cus / B));
+    if (!c->seg_layout) return 1;                  // (a row's parts would not share an L2)
+    return (int)std::min<int64_t>(std::min<int64_t>(n, fs::LP_PARTS), std::max<int64_t>(1, 4 * (int64_t)c->cus / B));
 }
 
 size_t type_size(int32_t type) { return type == FS_F32 ? 4 : type == FS_BF16 || type == FS_F16 ? 2 : 0; }
@@ -1253,8 +1254,8 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
     const Edited call(ctx, st);
     if (call.rc != FS_OK) return call.rc;
     std::lock_guard<std::mutex> g(ctx->mu);
-    a.nseg = logprob_parts(ctx->cus, B, V, type);
-    if ((int64_t)B * a.nseg > 0x7fffffff) return FS_E_INVALID;
+    a.nseg = logprob_parts(ctx, B, V, type);
+    if (((int64_t)B + fs::XCDS) * a.nseg > 0x7fffffff) return FS_E_INVALID;
     const size_t segs = a.nseg > 1 ? (size_t)B * a.nseg : 0;   // (a row of one part needs no workspace)
     rc = grow(ctx, 0, 0, 0);
     if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_part, ctx->lp_segs, segs, 1, false);

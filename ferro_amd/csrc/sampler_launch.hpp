@@ -135,6 +135,7 @@ hipError_t launch_edit_end(const EditEnd& e, hipStream_t st);
 
 // Log-probabilities (logprob_kernel.hip).
 constexpr int LP_TOP = 64;                 // largest n: one entry per lane of the finishing wave
+constexpr int LP_PARTS = 64;               // parts per row: the join holds one per lane
 constexpr int LP_NL(int type) { return type == FS_F32 ? 4 : 8; }   // groups of four per thread in a chunk of 16 KB
 struct LpPart {                            // a part's share of its row
     double sum;                            // of exp((x - max) / T)

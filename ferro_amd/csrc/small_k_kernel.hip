@@ -412,7 +412,7 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
             EdRow er;
             ed_bias(er, a.ed, pidx);
             if (er.nb > 0)
-                ed_add<NL>(er, seg_lo, n_in, [&](int q, int c) -> float& {
+                ed_add<NL>(er, nullptr, seg_lo, n_in, [&](int q, int c) -> float& {
                     return c == 0 ? v[q].x : c == 1 ? v[q].y : c == 2 ? v[q].z : v[q].w;
                 });
         }
