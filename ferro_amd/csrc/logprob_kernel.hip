@@ -11,11 +11,13 @@
 //     subtraction, a product, an exponential and an addition a logit;
 //   - a chunk whose sum is NaN (NaN or infinite logits) is added again with those left out; where the row's largest logit
 //     is infinite its tokens are counted instead;
-//   - the n largest: a bound, the n-th of the wave's 64 lane maxima so far, passes over chunks without a candidate by one
-//     compare a lane; the others go to a list in LDS, which is cut to the n largest by register sorts whenever it may
-//     overflow. The lane maxima are sorted again when the list has grown by LP_GROWN entries.
-// At the end of a part the entries of its lists at or above the waves' best bound (about 2.5 n) are ranked; the row's last part (a ticket; a row's parts share an XCD and its L2)
-// joins the parts' sums and lists.
+//   - the n largest: a bound that n of the wave's 64 lane maxima so far reach (bisected with a compare a step; sorting them
+//     takes six times the instructions) passes over chunks without a candidate by one compare a lane; of the others the
+//     groups of four with a candidate go to a list in LDS as they are. The list is cut to the n largest tokens by register
+//     sorts where it may overflow.
+// At the end of a part its waves write out their tokens at or above the best of their bounds (about 2.5 n in a part). The
+// row's last part (a ticket; a row's parts share an XCD and its L2) joins the parts' sums, takes a bound from 256 maxima
+// of groups of lanes that the parts publish, and ranks the tokens that reach it (about 1.2 n).
 // A chunk's mask is read a chunk ahead of its logits, whose groups of four without an allowed token are not read (the
 // part's first chunk is requested whole, at once).
 // Bound: HBM; the arithmetic (about 10 instructions a logit) takes about half of the time of reading 16-bit logits.
@@ -24,21 +26,23 @@
 
 namespace fs {
 
-constexpr int LP_LIST = LP_TOP + 4 * WAVE; // entries of a wave's list: the largest so far and one group of four per lane
-constexpr int LP_JOIN = 512;               // entries that are ranked at once
-constexpr int LP_GROWN = 16;
+constexpr int LP_GROUPS = 256;             // groups of four in a wave's list
+constexpr int LP_JOIN = 1024;              // entries that are ranked at once
+constexpr int LP_GROWN = 16;               // groups in a list since its bound was taken, after which it is taken again
 
 struct LpShared {
-    uint64_t list[SK_NW][LP_LIST];
+    float4 gval[SK_NW][LP_GROUPS];
+    int gid[SK_NW][LP_GROUPS];             // the id of a group's first token
+    uint64_t kept[SK_NW][LP_TOP];          // what a cut left: sorted, 0 past the entries
     uint64_t join[LP_JOIN];
     uint64_t top[LP_TOP];
     uint32_t rank[SK_LT];
-    float bound[SK_NW];
-    uint32_t n;
     double sum[SK_NW];
     float max[SK_NW];
+    float bound[SK_NW];
     uint32_t above[SK_NW];
-    uint32_t last;
+    int cnt[SK_NW];
+    uint32_t n, last;
 };
 
 constexpr float LP_NONE = -__builtin_huge_valf(), LP_LOWEST = -3.402823466e+38f;
@@ -53,33 +57,68 @@ __device__ __forceinline__ float lp_max3(float a, float b, float c) {   // (fmax
     return a;
 }
 
-// The n largest of the cnt entries (whole wave): sorted, one per lane, 0 past them; the list keeps them.
-__device__ __forceinline__ uint64_t lp_cut(uint64_t* list, int& cnt, int n) {
-    const int lane = lane_id();
+// A key that n of the wave's 64 K keys reach, and about a quarter more at most where they differ; n reach `lo` already.
+// Bisected: K compares a step.
+template <int K>
+__device__ __forceinline__ uint32_t lp_nth(const uint32_t (&key)[K], uint32_t lo, int n) {
+    uint32_t hi = key[0];
+#pragma unroll
+    for (int u = 1; u < K; ++u) hi = key[u] > hi ? key[u] : hi;
+    hi = wave_max(hi);
+    if (n == 1) return hi > lo ? hi : lo;
+    uint32_t step = hi > lo ? hi - lo : 0u;                    // the n-th largest lies in [lo, lo + step]
+#pragma unroll 1
+    while (step > 0u) {
+        const uint32_t up = (step >> 1) + (step & 1u);
+        int c = 0;
+#pragma unroll
+        for (int u = 0; u < K; ++u) c += __popcll(__ballot(key[u] >= lo + up));
+        if (c >= n) {
+            lo += up;
+            step -= up;
+            if (c <= n + n / 4) break;
+        } else {
+            step = up - 1u;
+        }
+    }
+    return lo;
+}
+
+// What the wave keeps of its list of g groups and an earlier cut: its n largest tokens at or above the bound, sorted, one
+// per lane, 0 past them (also in s.kept).
+__device__ __forceinline__ uint64_t lp_cut(LpShared& s, int& g, bool& cut, float bound, int n) {
+    const int lane = lane_id(), w = (int)threadIdx.x / WAVE;
     lp_wave_sync();
-    uint64_t acc = 0ull;
-    for (int i = 0; i < cnt; i += WAVE) {
-        const uint64_t e = i + lane < cnt ? list[i + lane] : 0ull;
-        acc = i == 0 ? sort64<true>(e) : merge_top64(acc, sort64<false>(e));
+    uint64_t acc = cut ? s.kept[w][lane] : 0ull;
+#pragma unroll 1
+    for (int i = 0; i < 4 * g; i += WAVE) {                    // sixteen groups at a time
+        const int at = (i + lane) >> 2;
+        const float x = at < g ? reinterpret_cast<const float*>(&s.gval[w][at])[lane & 3] : LP_NONE;
+        acc = merge_top64(acc, sort64<false>(x >= bound ? comp_of(key_of(x), (uint32_t)(s.gid[w][at] + (lane & 3))) : 0ull));
     }
     acc = lane < n ? acc : 0ull;
     lp_wave_sync();
-    list[lane] = acc;
-    cnt = __popcll(__ballot(acc != 0ull));
+    s.kept[w][lane] = acc;
+    g = 0;
+    cut = true;
     return acc;
 }
 
-// The n largest of the s.n <= LP_JOIN distinct entries of s.join, sorted to s.top, which is zero before. Whole workgroup,
-// after a barrier; ends with one.
-__device__ __forceinline__ void lp_rank(LpShared& s, int n) {
-    const int cnt = (int)s.n;
+// Lanes whose logits a part publishes the largest of.
+__device__ __forceinline__ int lp_group(int nseg) {
+    return nseg <= 4 ? 4 : nseg <= 8 ? 8 : nseg <= 16 ? 16 : nseg <= 32 ? 32 : 64;
+}
+
+// The n largest of the cnt distinct entries in[0, cnt), sorted to s.top, which is zero before. Whole workgroup, after a
+// barrier; ends with one.
+__device__ __forceinline__ void lp_rank(const uint64_t* in, int cnt, LpShared& s, int n) {
     if (cnt <= SK_LT) {
-        sk_rank(s.join, s.rank, cnt, [&](uint32_t r, uint64_t c) { if (r < (uint32_t)n) s.top[r] = c; });
+        sk_rank(in, s.rank, cnt, [&](uint32_t r, uint64_t c) { if (r < (uint32_t)n) s.top[r] = c; });
     } else {
         for (int c = threadIdx.x; c < cnt; c += SK_LT) {
-            const uint64_t me = s.join[c];
+            const uint64_t me = in[c];
             uint32_t r = 0u;
-            for (int j = 0; j < cnt; ++j) r += s.join[j] > me ? 1u : 0u;
+            for (int j = 0; j < cnt; ++j) r += in[j] > me ? 1u : 0u;
             if (r < (uint32_t)n) s.top[r] = me;
         }
     }
@@ -178,7 +217,8 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
     uint32_t above = 0u;                                       // the wave's count
     // TOP: the bound of new candidates; what n logits of the wave reach; the lane's largest logit
     float bound = LP_LOWEST, reach = LP_LOWEST, lm = LP_NONE;
-    int cnt = 0, sorted_at = -LP_GROWN;                        // the list's length, when the bound was taken
+    int g = 0, bound_at = -LP_GROWN;                           // groups in the list, and when the bound was taken
+    bool cut = false;
     if (TOP) {
         if (tid == 0) s.n = 0u;
         if (tid < LP_TOP) s.top[tid] = 0ull;
@@ -253,38 +293,36 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
         }
         if (TOP) {
             lm = fmaxf(lm, cm);
-            if (cnt - sorted_at >= LP_GROWN && __ballot(cm > bound) != 0ull) {
-                float b;
-                if (n == 1) {
-                    b = mx;
-                } else {
-                    const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)sort64_desc_u32(key_of(lm)), n - 1);
-                    b = key > 0x007FFFFFu ? val_of(key) : LP_LOWEST;
-                }
+            const bool any = __ballot(cm >= bound) != 0ull;
+            if (any && g - bound_at >= LP_GROWN) {
+                const uint32_t key[1] = {key_of(lm)};
+                uint32_t from = wave_min(key[0]);              // (every lane reaches it)
+                from = reach > LP_LOWEST && from < key_of(reach) ? key_of(reach) : from;
+                const uint32_t nth = lp_nth(key, from, n);
+                const float b = nth > 0x007FFFFFu ? val_of(nth) : LP_LOWEST;
                 bound = fmaxf(bound, b);
                 reach = fmaxf(reach, b);
-                sorted_at = b > LP_LOWEST ? cnt : sorted_at;
+                bound_at = b > LP_LOWEST ? g : bound_at;
             }
-            if (__ballot(cm >= bound) != 0ull) {
+            if (any) {
 #pragma unroll
                 for (int q = 0; q < NL; ++q) {
-                    if (__ballot(lp_max3(lp_max3(LP_NONE, x[q][0], x[q][1]), x[q][2], x[q][3]) >= bound) != 0ull) {
-                        if (cnt > LP_LIST - 4 * WAVE) {
-                            const uint64_t acc = lp_cut(s.list[w], cnt, n);
-                            const uint32_t key = comp_key(read_lane(acc, n - 1));
+                    const bool mine = lp_max3(lp_max3(LP_NONE, x[q][0], x[q][1]), x[q][2], x[q][3]) >= bound;
+                    const uint64_t m = __ballot(mine);
+                    if (m != 0ull) {
+                        if (mine) {
+                            const int at = g + (int)mbcnt(m);
+                            s.gval[w][at] = make_float4(x[q][0], x[q][1], x[q][2], x[q][3]);
+                            s.gid[w][at] = lo + (q * SK_LT + tid) * 4;
+                        }
+                        g += __popcll(m);
+                        if (g > LP_GROUPS - WAVE) {
+                            const uint32_t key = comp_key(read_lane(lp_cut(s, g, cut, bound, n), n - 1));
                             if (key != 0u) {
                                 reach = val_of(key);
                                 bound = val_of(key + 1u);      // later ids lose to equal values: the next value up
                             }
-                            sorted_at = cnt;
-                        }
-#pragma unroll
-                        for (int c_ = 0; c_ < 4; ++c_) {
-                            const uint64_t m = __ballot(x[q][c_] >= bound);
-                            if (x[q][c_] >= bound)
-                                s.list[w][cnt + (int)mbcnt(m)] =
-                                    comp_of(key_of(x[q][c_]), (uint32_t)(lo + (q * SK_LT + tid) * 4 + c_));
-                            cnt += __popcll(m);
+                            bound_at = 0;
                         }
                     }
                 }
@@ -295,10 +333,6 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
     auto addu = [](uint32_t u, uint32_t v) { return u + v; };
     auto addf = [](double u, double v) { return u + v; };
     sum = wave_allreduce(sum, addf);
-    if (TOP && cnt > LP_JOIN / SK_NW) {
-        const uint32_t key = comp_key(read_lane(lp_cut(s.list[w], cnt, n), n - 1));
-        if (key != 0u) reach = val_of(key);
-    }
     if (lane == 0) {
         s.sum[w] = sum; s.max[w] = mx; s.above[w] = above; s.bound[w] = reach;
     }
@@ -310,88 +344,126 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
     float M = fmaxf(fmaxf(s.max[0], s.max[1]), fmaxf(s.max[2], s.max[3]));
     double S = wave_allreduce(lane < SK_NW ? to(s.sum[lane & (SK_NW - 1)], s.max[lane & (SK_NW - 1)], M) : 0.0, addf);
     uint32_t ab = s.above[0] + s.above[1] + s.above[2] + s.above[3];
-    if (TOP) {                                                 // the waves' entries that reach the best of their bounds
-        const float best = fmaxf(fmaxf(s.bound[0], s.bound[1]), fmaxf(s.bound[2], s.bound[3]));
-        const uint32_t key = key_of(best);
-        for (int i = 0; i < cnt; i += WAVE) {
-            const uint64_t e = i + lane < cnt ? s.list[w][i + lane] : 0ull;
-            const uint64_t m = __ballot(comp_key(e) >= key);
-            if (m == 0ull) continue;
-            uint32_t base = 0u;
-            if (lane == 0) base = atomicAdd(&s.n, (uint32_t)__popcll(m));
-            base = (uint32_t)__builtin_amdgcn_readfirstlane((int)base);
-            if (comp_key(e) >= key) s.join[base + mbcnt(m)] = e;
+    float best = LP_LOWEST;
+    if (TOP) {                                                 // the wave's tokens that reach the best of the bounds
+        best = fmaxf(fmaxf(s.bound[0], s.bound[1]), fmaxf(s.bound[2], s.bound[3]));
+        uint64_t* out = nseg > 1 ? a.lists + (((int64_t)row * nseg + part) * SK_NW + w) * LP_TOP : &s.join[w * LP_TOP];
+        int cnt = 0;
+        bool fits = !cut;
+        for (int i = lane; fits && i - lane < 4 * g; i += WAVE) {
+            const float x = i < 4 * g ? reinterpret_cast<const float*>(&s.gval[w][i >> 2])[i & 3] : LP_NONE;
+            const uint64_t m = __ballot(x >= best);
+            fits = cnt + __popcll(m) <= LP_TOP;
+            if (fits && x >= best) out[cnt + (int)mbcnt(m)] = comp_of(key_of(x), (uint32_t)(s.gid[w][i >> 2] + (i & 3)));
+            cnt += __popcll(m);
         }
-        __syncthreads();
-        lp_rank(s, n);
+        if (!fits) {                                           // a list that was cut, or equal logits at the bound
+            const uint64_t e = lp_cut(s, g, cut, best, n);
+            cnt = __popcll(__ballot(e != 0ull));
+            if (lane < cnt) out[lane] = e;
+        }
+        // the largest logits of the part's groups of `size` lanes: 256 in a row of up to 64 parts
+        if (nseg > 1) {
+            uint32_t top = lm > LP_NONE ? key_of(lm) : 0u;
+            auto both = [](uint32_t u, uint32_t v) { return u > v ? u : v; };
+            top = both(top, xor_lane32<1>(top));
+            top = both(top, xor_lane32<2>(top));
+            if (nseg > 4) top = both(top, xor_lane32<4>(top));
+            if (nseg > 8) top = both(top, xor_lane32<8>(top));
+            if (nseg > 16) top = both(top, xor_lane32<16>(top));
+            if (nseg > 32) top = both(top, xor_lane32<32>(top));
+            const int size = lp_group(nseg);
+            if (lane % size == 0) a.part[(int64_t)row * nseg + part].key[(w * WAVE + lane) / size] = top;
+        }
+        if (lane == 0) s.cnt[w] = cnt;
+        if (lane == 0 && nseg > 1) a.part[(int64_t)row * nseg + part].cnt[w] = cnt;
     }
     if (nseg > 1) {                                            // uniform
         LpPart* pr = a.part + (int64_t)row * nseg;
-        uint64_t* rl = a.lists + (int64_t)row * nseg * LP_TOP;
-        if (TOP && tid < n) rl[part * LP_TOP + tid] = s.top[tid];
         if (tid == 0) {
             pr[part].sum = S;
             pr[part].above = ab;
             pr[part].max = M;
+            pr[part].bound = best;
         }
-        if (w == 0) {
-            vm_drain();                                        // the part's results are in the L2
-            if (lane == 0)
-                s.last = __hip_atomic_fetch_add(a.ticket + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) ==
-                         (uint32_t)nseg - 1u ? 1u : 0u;
-        }
+        vm_drain();                                            // the wave's results are in the L2
+        if (TOP) __syncthreads();
+        if (tid == 0)
+            s.last = __hip_atomic_fetch_add(a.ticket + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) ==
+                     (uint32_t)nseg - 1u ? 1u : 0u;
         __syncthreads();
         if (s.last == 0u) return;
         // ---- the row's end, by its last part
-        if (tid == 0) {
-            a.ticket[row] = 0u;
-            s.n = 0u;
-        }
-        if (TOP && tid < LP_TOP) s.top[tid] = 0ull;
-        const LpPart mine = lane < nseg ? pr[lane] : LpPart{0.0, 0u, LP_LOWEST};
+        if (tid == 0) a.ticket[row] = 0u;
+        const bool is = lane < nseg;
+        const double si = is ? pr[lane].sum : 0.0;
+        const float mi = is ? pr[lane].max : LP_LOWEST, bi = is ? pr[lane].bound : LP_LOWEST;
+        const uint32_t ai = is ? pr[lane].above : 0u;
         if (TOP) {
-            // Every list's q-th entry, q = ceil(2 n / nseg): ceil(n / q) of them at or above a value make n entries that
-            // reach it. Those (about 1.5 n) are ranked.
-            const int q = (2 * n + nseg - 1) / nseg < n ? (2 * n + nseg - 1) / nseg : n, m = (n + q - 1) / q;
-            const uint64_t at = lane < nseg ? rl[lane * LP_TOP + q - 1] : 0ull;
-            constexpr int U = 4;                               // entries in flight per thread
-            const int total = nseg * n;
-            uint64_t e[U];
-            auto fetch = [&](int i0) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int i = i0 + u * SK_LT + tid;
-                    e[u] = i < total ? rl[i / n * LP_TOP + i % n] : 0ull;
-                }
-            };
-            fetch(0);
-            uint32_t least = m == 1 ? wave_max(comp_key(at))
-                                    : (uint32_t)__builtin_amdgcn_readlane((int)sort64_desc_u32(comp_key(at)), m - 1);
-            if (least == 0u) least = 1u;                       // fewer lists hold q entries: every entry
-            __syncthreads();
-            for (int i0 = 0; i0 < total; i0 += U * SK_LT) {
-                if (i0 > 0) fetch(i0);
+            // per = SK_LT / (waves' lists, rounded up) threads for each list; its first entries with its length
+            constexpr int U = 4;
+            const int lists = nseg * SK_NW;
+            int per = 1;
+            while (2 * per * lists <= SK_LT) per *= 2;
+            const int l = tid / per, k0 = tid % per;
+            const uint64_t* rl = a.lists + ((int64_t)row * lists + l) * LP_TOP;
+            uint64_t e[U] = {0ull, 0ull, 0ull, 0ull};
+            int len = 0;
+            if (l < lists) {
+                len = pr[l / SK_NW].cnt[l % SK_NW];
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    if (comp_key(e[u]) >= least) {
-                        const uint32_t p = atomicAdd(&s.n, 1u);
-                        if (p < (uint32_t)LP_JOIN) s.join[p] = e[u];
-                    }
+                    if (k0 + u * per < LP_TOP) e[u] = rl[k0 + u * per];
             }
+            const int kp = SK_LT / lp_group(nseg);             // keys of a part
+            uint32_t key[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = u * WAVE + lane;
+                key[u] = i < nseg * kp ? pr[i / kp].key[i % kp] : 0u;
+            }
+            best = wave_allreduce(bi, fmx);
+            const uint32_t least = lp_nth(key, key_of(best), n);
+            auto join = [&](uint64_t c, bool in) {
+                if (in && comp_key(c) >= least) {
+                    const uint32_t at = atomicAdd(&s.n, 1u);
+                    if (at < (uint32_t)LP_JOIN) s.join[at] = c;
+                }
+            };
+#pragma unroll
+            for (int u = 0; u < U; ++u) join(e[u], k0 + u * per < len);
+            for (int k = k0 + U * per; k < len; k += per) join(rl[k], true);
             __syncthreads();
-            if (s.n <= (uint32_t)LP_JOIN) {
-                lp_rank(s, n);
-            } else if (w == 0) {                               // one wave merges the lists
-                uint64_t acc = 0ull;
-                for (int i = 0; i < nseg; ++i)
-                    acc = merge_top64(acc, WAVE - 1 - lane < n ? rl[i * LP_TOP + WAVE - 1 - lane] : 0ull);   // ascending
-                s.top[lane] = acc;
-                lp_wave_sync();
+            if (s.n > (uint32_t)LP_JOIN) {                     // equal logits at the bound: one wave sorts the lists
+                if (w == 0) {
+                    uint64_t acc = 0ull;
+                    for (int i = 0; i < lists; ++i) {
+                        const int c = pr[i / SK_NW].cnt[i % SK_NW];
+                        acc = merge_top64(acc, sort64<false>(
+                            lane < c ? a.lists[((int64_t)row * lists + i) * LP_TOP + lane] : 0ull));
+                    }
+                    s.top[lane] = lane < n ? acc : 0ull;
+                }
+                __syncthreads();
+            } else {
+                lp_rank(s.join, (int)s.n, s, n);
             }
         }
-        M = wave_allreduce(mine.max, fmx);
-        S = wave_allreduce(to(mine.sum, mine.max, M), addf);
-        ab = wave_allreduce(mine.above, addu);
+        M = wave_allreduce(mi, fmx);
+        S = wave_allreduce(to(si, mi, M), addf);
+        ab = wave_allreduce(ai, addu);
+    } else if (TOP) {                                          // the waves' lists close up
+        __syncthreads();
+        int base = 0, all = 0;
+#pragma unroll
+        for (int q = 0; q < SK_NW; ++q) {
+            base += q < w ? s.cnt[q] : 0;
+            all += s.cnt[q];
+        }
+        uint64_t* list = s.join + SK_NW * LP_TOP;
+        if (lane < s.cnt[w]) list[base + lane] = s.join[w * LP_TOP + lane];
+        __syncthreads();
+        lp_rank(list, all, s, n);
     }
     if (!(M < __builtin_huge_valf())) {                        // uniform
         __syncthreads();

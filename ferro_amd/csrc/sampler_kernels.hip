@@ -161,7 +161,7 @@ struct fs_context {
     int64_t* ed_off = nullptr;         //   [ed_off_rows] zeros: the offsets of empty histories
     size_t ed_logits = 0, ed_param_rows = 0, ed_any_rows = 0, ed_u_rows = 0, ed_off_rows = 0;
     fs::LpPart* lp_part = nullptr;     // fs_logprobs: [lp_segs] segments' sums,
-    uint64_t* lp_lists = nullptr;      //   [lp_list_segs][LP_TOP] their largest logits,
+    uint64_t* lp_lists = nullptr;      //   [lp_list_segs][SK_NW][LP_TOP] their waves' lists,
     uint32_t* lp_ticket = nullptr;     //   [lp_rows] segment tickets, left at 0
     size_t lp_segs = 0, lp_list_segs = 0, lp_rows = 0;
     int static_dev = -1;       // device whose static workspace fs_sample_batch_static used with this context
@@ -1259,7 +1259,7 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
     const size_t segs = a.nseg > 1 ? (size_t)B * a.nseg : 0;   // (a row of one part needs no workspace)
     rc = grow(ctx, 0, 0, 0);
     if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_part, ctx->lp_segs, segs, 1, false);
-    if (rc == FS_OK && top > 0) rc = grow_buffer(ctx, ctx->lp_lists, ctx->lp_list_segs, segs, fs::LP_TOP, false);
+    if (rc == FS_OK && top > 0) rc = grow_buffer(ctx, ctx->lp_lists, ctx->lp_list_segs, segs, fs::SK_NW * fs::LP_TOP, false);
     if (rc == FS_OK && segs > 0) rc = grow_buffer(ctx, ctx->lp_ticket, ctx->lp_rows, (size_t)B, 1, true);
     if (rc != FS_OK) return rc;
     a.logits = d_logits; a.ld = ld; a.B = B; a.V = V; a.n = top; a.params = d_params; a.tok = d_tok;

@@ -141,6 +141,9 @@ struct LpPart {                            // a part's share of its row
     double sum;                            // of exp((x - max) / T)
     uint32_t above;                        // logits above the chosen token's
     float max;
+    float bound;                           // n of its logits reach it
+    int cnt[SK_NW];                        // tokens in its waves' lists
+    uint32_t key[64];                      // the largest logits (as keys) of groups of its lanes
 };
 struct LpArgs {
     const void* logits;
@@ -154,7 +157,7 @@ struct LpArgs {
     int32_t* ids;                          // [B][n]
     float* top;
     LpPart* part;                          // [B][nseg]
-    uint64_t* lists;                       // [B][nseg][LP_TOP]
+    uint64_t* lists;                       // [B][nseg][SK_NW][LP_TOP]
     uint32_t* ticket;                      // [B], left at 0
     int32_t* err;
 };
