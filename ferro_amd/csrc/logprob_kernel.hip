@@ -9,15 +9,16 @@
 //   - the sum: exponentials of c (x - m), c = log2 e / T and m the wave's largest x so far (the largest term is 1, exactly).
 //     A chunk's 16 or 32 terms of a lane are added in fp32, chunks in fp64, and a new m scales the lanes' sums in fp64; a
 //     subtraction, a product, an exponential and an addition a logit;
-//   - a chunk whose sum is NaN (NaN or infinite logits) is added again with those left out; where the row's largest logit
-//     is infinite its tokens are counted instead;
+//   - a chunk whose sum is NaN (NaN or infinite logits) is added again with NaN left out; once the largest logit is
+//     infinite its tokens are counted instead;
 //   - the n largest: a bound that n of the wave's 64 lane maxima so far reach (bisected with a compare a step; sorting them
 //     takes six times the instructions) passes over chunks without a candidate by one compare a lane; of the others the
 //     groups of four with a candidate go to a list in LDS as they are. The list is cut to the n largest tokens by register
 //     sorts where it may overflow.
-// At the end of a part its waves write out their tokens at or above the best of their bounds (about 2.5 n in a part). The
-// row's last part (a ticket; a row's parts share an XCD and its L2) joins the parts' sums, takes a bound from 256 maxima
-// of groups of lanes that the parts publish, and ranks the tokens that reach it (about 1.2 n).
+// At the end of a part its waves write out their sums and their tokens at or above the best of their bounds (about 2.5 n in
+// a part). One wave of the row's last part (a ticket per part; a row's parts share an XCD and its L2. With one per wave the
+// atomics on a line took longer than the reading: 64 rows of 262144 16.8 -> 33.8 us) joins the sums, takes a bound from 256
+// maxima of groups of lanes that the waves publish, and sorts the tokens that reach it (about 1.2 n) in registers.
 // A chunk's mask is read a chunk ahead of its logits, whose groups of four without an allowed token are not read (the
 // part's first chunk is requested whole, at once).
 // Bound: HBM; the arithmetic (about 10 instructions a logit) takes about half of the time of reading 16-bit logits.
@@ -27,22 +28,13 @@
 namespace fs {
 
 constexpr int LP_GROUPS = 256;             // groups of four in a wave's list
-constexpr int LP_JOIN = 1024;              // entries that are ranked at once
 constexpr int LP_GROWN = 16;               // groups in a list since its bound was taken, after which it is taken again
 
 struct LpShared {
-    float4 gval[SK_NW][LP_GROUPS];
+    float4 gval[SK_NW][LP_GROUPS];         // (the row's end gathers its tokens here)
     int gid[SK_NW][LP_GROUPS];             // the id of a group's first token
     uint64_t kept[SK_NW][LP_TOP];          // what a cut left: sorted, 0 past the entries
-    uint64_t join[LP_JOIN];
-    uint64_t top[LP_TOP];
-    uint32_t rank[SK_LT];
-    double sum[SK_NW];
-    float max[SK_NW];
     float bound[SK_NW];
-    uint32_t above[SK_NW];
-    int cnt[SK_NW];
-    uint32_t n, last;
 };
 
 constexpr float LP_NONE = -__builtin_huge_valf(), LP_LOWEST = -3.402823466e+38f;
@@ -104,40 +96,9 @@ __device__ __forceinline__ uint64_t lp_cut(LpShared& s, int& g, bool& cut, float
     return acc;
 }
 
-// Lanes whose logits a part publishes the largest of.
+// The lanes (a power of two, its logarithm) whose largest logit a wave publishes: 256 groups in a row of up to 64 parts.
 __device__ __forceinline__ int lp_group(int nseg) {
-    return nseg <= 4 ? 4 : nseg <= 8 ? 8 : nseg <= 16 ? 16 : nseg <= 32 ? 32 : 64;
-}
-
-// The n largest of the cnt distinct entries in[0, cnt), sorted to s.top, which is zero before. Whole workgroup, after a
-// barrier; ends with one.
-__device__ __forceinline__ void lp_rank(const uint64_t* in, int cnt, LpShared& s, int n) {
-    if (cnt <= SK_LT) {
-        sk_rank(in, s.rank, cnt, [&](uint32_t r, uint64_t c) { if (r < (uint32_t)n) s.top[r] = c; });
-    } else {
-        for (int c = threadIdx.x; c < cnt; c += SK_LT) {
-            const uint64_t me = in[c];
-            uint32_t r = 0u;
-            for (int j = 0; j < cnt; ++j) r += in[j] > me ? 1u : 0u;
-            if (r < (uint32_t)n) s.top[r] = me;
-        }
-    }
-    __syncthreads();
-}
-
-// The tokens at +inf of a row whose largest logit that is, by one workgroup.
-template <int TYPE>
-__device__ __forceinline__ double lp_infinite(const LpArgs& a, const EdRow& r, int row, float cap, LpShared& s) {
-    double e = 0.0;
-    for (int i = threadIdx.x; i < a.V; i += SK_LT) {
-        float x = Logits4<TYPE>::one(a.logits, (int64_t)row * a.ld + i);
-        if (cap > 0.0f) x = softcap_one(x, cap);
-        e += ed_lane(r, x, i) == __builtin_huge_valf() ? 1.0 : 0.0;
-    }
-    e = wave_allreduce(e, [](double u, double v) { return u + v; });
-    if (lane_id() == 0) s.sum[threadIdx.x / WAVE] = e;
-    __syncthreads();
-    return s.sum[0] + s.sum[1] + s.sum[2] + s.sum[3];
+    return nseg <= 4 ? 2 : nseg <= 8 ? 3 : nseg <= 16 ? 4 : nseg <= 32 ? 5 : 6;
 }
 
 // The kernel's argument list as a struct: the argument segment follows the same layout rules
@@ -219,10 +180,6 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
     float bound = LP_LOWEST, reach = LP_LOWEST, lm = LP_NONE;
     int g = 0, bound_at = -LP_GROWN;                           // groups in the list, and when the bound was taken
     bool cut = false;
-    if (TOP) {
-        if (tid == 0) s.n = 0u;
-        if (tid < LP_TOP) s.top[tid] = 0ull;
-    }
 #pragma unroll 1
     for (int c = c0; c < c1; ++c) {
         const int lo = c * CHUNK, n_in = V - lo < CHUNK ? V - lo : CHUNK;
@@ -282,7 +239,14 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
 #pragma unroll
                 for (int c_ = 0; c_ < 4; ++c_) x[q][c_] = x[q][c_] == x[q][c_] ? x[q][c_] : LP_NONE;
             lane_max();
-            e = fminf(add(), 1e30f);                           // (the tokens at +inf are counted by themselves)
+            e = add();
+            if (!(mx < __builtin_huge_valf())) {
+                e = 0.0f;
+#pragma unroll
+                for (int q = 0; q < NL; ++q)
+#pragma unroll
+                    for (int c_ = 0; c_ < 4; ++c_) e += x[q][c_] == mx ? 1.0f : 0.0f;
+            }
         }
         sum += (double)e;
         if (has && __ballot(cm > xv) != 0ull) {
@@ -329,147 +293,105 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
             }
         }
     }
-    // ---- the part's end
+    // ---- the wave's end
     auto addu = [](uint32_t u, uint32_t v) { return u + v; };
     auto addf = [](double u, double v) { return u + v; };
+    LpRow* rw = a.rows + row;
+    const int lists = nseg * SK_NW, me = part * SK_NW + w;
+    uint64_t* rl = a.lists + (int64_t)row * lists * LP_TOP;
     sum = wave_allreduce(sum, addf);
-    if (lane == 0) {
-        s.sum[w] = sum; s.max[w] = mx; s.above[w] = above; s.bound[w] = reach;
-    }
-    __syncthreads();
-    // a sum S relative to m, relative to M >= m instead
-    auto to = [&](double S, float m, float M) {
-        return m == M || !(M < __builtin_huge_valf()) ? S : S * exp(((double)m - (double)M) / (double)T);
-    };
-    float M = fmaxf(fmaxf(s.max[0], s.max[1]), fmaxf(s.max[2], s.max[3]));
-    double S = wave_allreduce(lane < SK_NW ? to(s.sum[lane & (SK_NW - 1)], s.max[lane & (SK_NW - 1)], M) : 0.0, addf);
-    uint32_t ab = s.above[0] + s.above[1] + s.above[2] + s.above[3];
-    float best = LP_LOWEST;
-    if (TOP) {                                                 // the wave's tokens that reach the best of the bounds
-        best = fmaxf(fmaxf(s.bound[0], s.bound[1]), fmaxf(s.bound[2], s.bound[3]));
-        uint64_t* out = nseg > 1 ? a.lists + (((int64_t)row * nseg + part) * SK_NW + w) * LP_TOP : &s.join[w * LP_TOP];
+    if (TOP) {                                                 // the wave's tokens that reach the best of the part's bounds
+        if (lane == 0) s.bound[w] = reach;
+        __syncthreads();
+        reach = fmaxf(fmaxf(s.bound[0], s.bound[1]), fmaxf(s.bound[2], s.bound[3]));
+        uint64_t* out = rl + me * LP_TOP;
         int cnt = 0;
         bool fits = !cut;
-        for (int i = lane; fits && i - lane < 4 * g; i += WAVE) {
-            const float x = i < 4 * g ? reinterpret_cast<const float*>(&s.gval[w][i >> 2])[i & 3] : LP_NONE;
-            const uint64_t m = __ballot(x >= best);
-            fits = cnt + __popcll(m) <= LP_TOP;
-            if (fits && x >= best) out[cnt + (int)mbcnt(m)] = comp_of(key_of(x), (uint32_t)(s.gid[w][i >> 2] + (i & 3)));
-            cnt += __popcll(m);
+#pragma unroll 1
+        for (int i = 0; fits && i < g; i += WAVE) {
+            const bool in = i + lane < g;
+            const float4 v = in ? s.gval[w][i + lane] : make_float4(LP_NONE, LP_NONE, LP_NONE, LP_NONE);
+            const uint32_t id = in ? (uint32_t)s.gid[w][i + lane] : 0u;
+            const float y[4] = {v.x, v.y, v.z, v.w};
+            uint64_t m[4];
+            int all = cnt;
+#pragma unroll
+            for (int c_ = 0; c_ < 4; ++c_) {
+                m[c_] = __ballot(y[c_] >= reach);
+                all += __popcll(m[c_]);
+            }
+            fits = all <= LP_TOP;
+            if (fits) {
+#pragma unroll
+                for (int c_ = 0; c_ < 4; ++c_) {
+                    if (y[c_] >= reach) out[cnt + (int)mbcnt(m[c_])] = comp_of(key_of(y[c_]), id + (uint32_t)c_);
+                    cnt += __popcll(m[c_]);
+                }
+            }
         }
         if (!fits) {                                           // a list that was cut, or equal logits at the bound
-            const uint64_t e = lp_cut(s, g, cut, best, n);
+            const uint64_t e = lp_cut(s, g, cut, reach, n);
             cnt = __popcll(__ballot(e != 0ull));
             if (lane < cnt) out[lane] = e;
         }
-        // the largest logits of the part's groups of `size` lanes: 256 in a row of up to 64 parts
-        if (nseg > 1) {
-            uint32_t top = lm > LP_NONE ? key_of(lm) : 0u;
-            auto both = [](uint32_t u, uint32_t v) { return u > v ? u : v; };
-            top = both(top, xor_lane32<1>(top));
-            top = both(top, xor_lane32<2>(top));
-            if (nseg > 4) top = both(top, xor_lane32<4>(top));
-            if (nseg > 8) top = both(top, xor_lane32<8>(top));
-            if (nseg > 16) top = both(top, xor_lane32<16>(top));
-            if (nseg > 32) top = both(top, xor_lane32<32>(top));
-            const int size = lp_group(nseg);
-            if (lane % size == 0) a.part[(int64_t)row * nseg + part].key[(w * WAVE + lane) / size] = top;
+        uint32_t top = lm > LP_NONE ? key_of(lm) : 0u;
+        auto both = [](uint32_t u, uint32_t v) { return u > v ? u : v; };
+        top = both(top, xor_lane32<1>(top));
+        top = both(top, xor_lane32<2>(top));
+        if (nseg > 4) top = both(top, xor_lane32<4>(top));
+        if (nseg > 8) top = both(top, xor_lane32<8>(top));
+        if (nseg > 16) top = both(top, xor_lane32<16>(top));
+        if (nseg > 32) top = both(top, xor_lane32<32>(top));
+        const int lg = lp_group(nseg);
+        if ((lane & ((1 << lg) - 1)) == 0) rw->key[((me << 6) + lane) >> lg] = top;
+        if (lane == 0) {
+            rw->cnt[me] = cnt;
+            rw->bound[me] = reach;
         }
-        if (lane == 0) s.cnt[w] = cnt;
-        if (lane == 0 && nseg > 1) a.part[(int64_t)row * nseg + part].cnt[w] = cnt;
     }
-    if (nseg > 1) {                                            // uniform
-        LpPart* pr = a.part + (int64_t)row * nseg;
-        if (tid == 0) {
-            pr[part].sum = S;
-            pr[part].above = ab;
-            pr[part].max = M;
-            pr[part].bound = best;
-        }
-        vm_drain();                                            // the wave's results are in the L2
-        if (TOP) __syncthreads();
-        if (tid == 0)
-            s.last = __hip_atomic_fetch_add(a.ticket + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) ==
-                     (uint32_t)nseg - 1u ? 1u : 0u;
-        __syncthreads();
-        if (s.last == 0u) return;
-        // ---- the row's end, by its last part
-        if (tid == 0) a.ticket[row] = 0u;
-        const bool is = lane < nseg;
-        const double si = is ? pr[lane].sum : 0.0;
-        const float mi = is ? pr[lane].max : LP_LOWEST, bi = is ? pr[lane].bound : LP_LOWEST;
-        const uint32_t ai = is ? pr[lane].above : 0u;
-        if (TOP) {
-            // per = SK_LT / (waves' lists, rounded up) threads for each list; its first entries with its length
-            constexpr int U = 4;
-            const int lists = nseg * SK_NW;
-            int per = 1;
-            while (2 * per * lists <= SK_LT) per *= 2;
-            const int l = tid / per, k0 = tid % per;
-            const uint64_t* rl = a.lists + ((int64_t)row * lists + l) * LP_TOP;
-            uint64_t e[U] = {0ull, 0ull, 0ull, 0ull};
-            int len = 0;
-            if (l < lists) {
-                len = pr[l / SK_NW].cnt[l % SK_NW];
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (k0 + u * per < LP_TOP) e[u] = rl[k0 + u * per];
-            }
-            const int kp = SK_LT / lp_group(nseg);             // keys of a part
-            uint32_t key[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int i = u * WAVE + lane;
-                key[u] = i < nseg * kp ? pr[i / kp].key[i % kp] : 0u;
-            }
-            best = wave_allreduce(bi, fmx);
-            const uint32_t least = lp_nth(key, key_of(best), n);
-            auto join = [&](uint64_t c, bool in) {
-                if (in && comp_key(c) >= least) {
-                    const uint32_t at = atomicAdd(&s.n, 1u);
-                    if (at < (uint32_t)LP_JOIN) s.join[at] = c;
-                }
-            };
-#pragma unroll
-            for (int u = 0; u < U; ++u) join(e[u], k0 + u * per < len);
-            for (int k = k0 + U * per; k < len; k += per) join(rl[k], true);
-            __syncthreads();
-            if (s.n > (uint32_t)LP_JOIN) {                     // equal logits at the bound: one wave sorts the lists
-                if (w == 0) {
-                    uint64_t acc = 0ull;
-                    for (int i = 0; i < lists; ++i) {
-                        const int c = pr[i / SK_NW].cnt[i % SK_NW];
-                        acc = merge_top64(acc, sort64<false>(
-                            lane < c ? a.lists[((int64_t)row * lists + i) * LP_TOP + lane] : 0ull));
-                    }
-                    s.top[lane] = lane < n ? acc : 0ull;
-                }
-                __syncthreads();
-            } else {
-                lp_rank(s.join, (int)s.n, s, n);
-            }
-        }
-        M = wave_allreduce(mi, fmx);
-        S = wave_allreduce(to(si, mi, M), addf);
-        ab = wave_allreduce(ai, addu);
-    } else if (TOP) {                                          // the waves' lists close up
-        __syncthreads();
-        int base = 0, all = 0;
-#pragma unroll
-        for (int q = 0; q < SK_NW; ++q) {
-            base += q < w ? s.cnt[q] : 0;
-            all += s.cnt[q];
-        }
-        uint64_t* list = s.join + SK_NW * LP_TOP;
-        if (lane < s.cnt[w]) list[base + lane] = s.join[w * LP_TOP + lane];
-        __syncthreads();
-        lp_rank(list, all, s, n);
+    uint32_t turn = 0u;
+    if (lane == 0) {
+        rw->sum[me] = sum;
+        rw->max[me] = mx;
+        rw->above[me] = above;
     }
-    if (!(M < __builtin_huge_valf())) {                        // uniform
-        __syncthreads();
-        S = lp_infinite<TYPE>(a, r, row, cap, s);
-    }
+    vm_drain();                                                // the wave's results are in the L2
+    __syncthreads();
     if (w != 0) return;
+    if (lane == 0) turn = __hip_atomic_fetch_add(&rw->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    if (read_lane(turn, 0) != (uint32_t)nseg - 1u) return;
+    // ---- the row's end, by its last part's first wave
+    if (lane == 0) rw->ticket = 0u;
+    constexpr int LL = LP_PARTS * SK_NW / WAVE;                // waves' results per lane
+    double si[LL];
+    float mi[LL], bi[LL];
+    uint32_t key[LL], ab = 0u;
+    int len[LL];
+#pragma unroll
+    for (int u = 0; u < LL; ++u) {
+        const int i = u * WAVE + lane;
+        const bool in = i < lists;
+        si[u] = in ? rw->sum[i] : 0.0;
+        mi[u] = in ? rw->max[i] : LP_LOWEST;
+        ab += in ? rw->above[i] : 0u;
+        if (TOP) {
+            bi[u] = in ? rw->bound[i] : LP_LOWEST;
+            len[u] = in ? rw->cnt[i] : 0;
+            key[u] = i < (lists << 6) >> lp_group(nseg) ? rw->key[i] : 0u;
+        }
+    }
+    float M = LP_LOWEST;
+#pragma unroll
+    for (int u = 0; u < LL; ++u) M = fmaxf(M, mi[u]);
+    M = wave_allreduce(M, fmx);
+    double S = 0.0;
+#pragma unroll
+    for (int u = 0; u < LL; ++u) {                             // relative to the row's maximum
+        if (u * WAVE >= lists) break;                          // uniform
+        S += mi[u] == M ? si[u] : M < __builtin_huge_valf() ? si[u] * exp(((double)mi[u] - (double)M) / (double)T) : 0.0;
+    }
+    S = wave_allreduce(S, addf);
+    ab = wave_allreduce(ab, addu);
     const double z = log(S);                                   // (no token takes part: not used)
     auto lp_of = [&](float v) {
         return v > LP_NONE ? (float)((v == M ? 0.0 : ((double)v - (double)M) / (double)T) - z) : LP_NONE;
@@ -478,10 +400,77 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
         if (a.lp) a.lp[row] = lp_of(xv);
         if (a.rank) a.rank[row] = xv > LP_NONE ? (has ? (int)ab + 1 : 1) : 0;
     }
-    if (TOP && lane < n) {
-        const uint64_t acc = s.top[lane];
-        if (a.ids) a.ids[(int64_t)row * n + lane] = acc != 0ull ? (int)comp_id(acc) : -1;
-        if (a.top) a.top[(int64_t)row * n + lane] = acc != 0ull ? lp_of(val_of(comp_key(acc))) : LP_NONE;
+    if (TOP) {
+        float best = LP_LOWEST;
+#pragma unroll
+        for (int u = 0; u < LL; ++u) best = fmaxf(best, bi[u]);
+        best = wave_allreduce(best, fmx);
+        const uint32_t least = lp_nth(key, key_of(best), n);
+        // the tokens that reach it, gathered in LDS (one copy of the sort in the code: with one per batch of lists the end
+        // took 3 us more, most of it for instructions)
+        constexpr int ROOM = sizeof(s.gval) / sizeof(uint64_t);
+        uint64_t* join = reinterpret_cast<uint64_t*>(&s.gval[0][0]);
+        int cnt = 0;
+        uint64_t acc = 0ull;
+        auto gather = [&](uint64_t c) {                        // (0: no token; the bound is above it)
+            const bool in = comp_key(c) >= least;
+            const uint64_t m = __ballot(in);
+            if (in) join[cnt + (int)mbcnt(m)] = c;
+            cnt += __popcll(m);
+        };
+        // the lists of waves whose largest logit reaches it (about 17 of 64 for n = 20; reading all of them took 3 us)
+        int* at = s.gid[0];                                    // [LP_PARTS * SK_NW] their numbers, above their lengths
+        int k = 0;
+#pragma unroll
+        for (int u = 0; u < LL; ++u) {
+            const bool in = len[u] > 0 && key_of(mi[u]) >= least;
+            const uint64_t m = __ballot(in);
+            if (in) at[k + (int)mbcnt(m)] = ((u * WAVE + lane) << 8) | len[u];
+            k += __popcll(m);
+        }
+        lp_wave_sync();
+        // half a wave per list, sixteen lists in flight
+        constexpr int U = 8;
+        static_assert(4 * U * WAVE <= ROOM, "a batch fits behind what has to be sorted first");
+        const int half = lane >> 5, pos = lane & 31;
+#pragma unroll 1
+        for (int i0 = 0; i0 < k || cnt > 0; i0 += 2 * U) {
+            if (i0 < k) {
+                int to[U];
+                uint64_t e[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int i = i0 + 2 * u + half;
+                    to[u] = i < k ? at[i] : 0;
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) e[u] = pos < (to[u] & 255) ? rl[(to[u] >> 8) * LP_TOP + pos] : 0ull;
+#pragma unroll
+                for (int u = 0; u < U; ++u) gather(e[u]);
+                bool more = false;                             // lists of more than 32
+#pragma unroll
+                for (int u = 0; u < U; ++u) more |= (to[u] & 255) > 32;
+                if (__ballot(more) != 0ull) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        e[u] = pos + 32 < (to[u] & 255) ? rl[(to[u] >> 8) * LP_TOP + pos + 32] : 0ull;
+#pragma unroll
+                    for (int u = 0; u < U; ++u) gather(e[u]);
+                }
+            }
+            if (cnt > 2 * U * WAVE || i0 + 2 * U >= k) {
+                lp_wave_sync();
+#pragma unroll 1
+                for (int i = 0; i < cnt; i += WAVE)
+                    acc = merge_top64(acc, sort64<false>(i + lane < cnt ? join[i + lane] : 0ull));
+                cnt = 0;
+                lp_wave_sync();
+            }
+        }
+        if (lane < n) {
+            if (a.ids) a.ids[(int64_t)row * n + lane] = acc != 0ull ? (int)comp_id(acc) : -1;
+            if (a.top) a.top[(int64_t)row * n + lane] = acc != 0ull ? lp_of(val_of(comp_key(acc))) : LP_NONE;
+        }
     }
 }
 

@@ -160,10 +160,9 @@ struct fs_context {
     double* ed_u = nullptr;            //   [ed_u_rows] a decode step's draws,
     int64_t* ed_off = nullptr;         //   [ed_off_rows] zeros: the offsets of empty histories
     size_t ed_logits = 0, ed_param_rows = 0, ed_any_rows = 0, ed_u_rows = 0, ed_off_rows = 0;
-    fs::LpPart* lp_part = nullptr;     // fs_logprobs: [lp_segs] segments' sums,
-    uint64_t* lp_lists = nullptr;      //   [lp_list_segs][SK_NW][LP_TOP] their waves' lists,
-    uint32_t* lp_ticket = nullptr;     //   [lp_rows] segment tickets, left at 0
-    size_t lp_segs = 0, lp_list_segs = 0, lp_rows = 0;
+    fs::LpRow* lp_row = nullptr;       // fs_logprobs: [lp_row_rows] what the rows' waves publish,
+    uint64_t* lp_lists = nullptr;      //   [lp_list_segs][SK_NW][LP_TOP] their lists
+    size_t lp_row_rows = 0, lp_list_segs = 0;
     int static_dev = -1;       // device whose static workspace fs_sample_batch_static used with this context
     uint64_t* trace = nullptr; // FS_TRACE builds: phase timestamps, trace_cap entries (fs_trace_set)
     int64_t trace_cap = 0;
@@ -964,9 +963,8 @@ int fs_destroy(fs_context* c) {
     (void)hipFree(c->ed_any);
     (void)hipFree(c->ed_u);
     (void)hipFree(c->ed_off);
-    (void)hipFree(c->lp_part);
+    (void)hipFree(c->lp_row);
     (void)hipFree(c->lp_lists);
-    (void)hipFree(c->lp_ticket);
     for (void* p : c->retired) (void)hipFree(p);
     if (c->hflag) (void)hipHostFree(c->hflag);
     delete c;
@@ -1256,15 +1254,14 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
     std::lock_guard<std::mutex> g(ctx->mu);
     a.nseg = logprob_parts(ctx, B, V, type);
     if (((int64_t)B + fs::XCDS) * a.nseg > 0x7fffffff) return FS_E_INVALID;
-    const size_t segs = a.nseg > 1 ? (size_t)B * a.nseg : 0;   // (a row of one part needs no workspace)
+    const size_t segs = (size_t)B * a.nseg;
     rc = grow(ctx, 0, 0, 0);
-    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_part, ctx->lp_segs, segs, 1, false);
+    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_row, ctx->lp_row_rows, (size_t)B, 1, true);
     if (rc == FS_OK && top > 0) rc = grow_buffer(ctx, ctx->lp_lists, ctx->lp_list_segs, segs, fs::SK_NW * fs::LP_TOP, false);
-    if (rc == FS_OK && segs > 0) rc = grow_buffer(ctx, ctx->lp_ticket, ctx->lp_rows, (size_t)B, 1, true);
     if (rc != FS_OK) return rc;
     a.logits = d_logits; a.ld = ld; a.B = B; a.V = V; a.n = top; a.params = d_params; a.tok = d_tok;
     a.lp = d_lp; a.rank = d_rank; a.ids = d_top_ids; a.top = d_top_lp;
-    a.part = ctx->lp_part; a.lists = ctx->lp_lists; a.ticket = ctx->lp_ticket; a.err = ctx->err;
+    a.rows = ctx->lp_row; a.lists = ctx->lp_lists; a.err = ctx->err;
     return fs::launch_logprobs(type, a, st) == hipSuccess ? FS_OK : FS_E_HIP;
 }
 

@@ -137,13 +137,15 @@ hipError_t launch_edit_end(const EditEnd& e, hipStream_t st);
 constexpr int LP_TOP = 64;                 // largest n: one entry per lane of the finishing wave
 constexpr int LP_PARTS = 64;               // parts per row: the join holds one per lane
 constexpr int LP_NL(int type) { return type == FS_F32 ? 4 : 8; }   // groups of four per thread in a chunk of 16 KB
-struct LpPart {                            // a part's share of its row
-    double sum;                            // of exp((x - max) / T)
-    uint32_t above;                        // logits above the chosen token's
-    float max;
-    float bound;                           // n of its logits reach it
-    int cnt[SK_NW];                        // tokens in its waves' lists
-    uint32_t key[64];                      // the largest logits (as keys) of groups of its lanes
+struct alignas(128) LpRow {                // what a row's waves publish, by part and wave
+    uint32_t ticket;                       // parts that have (left at 0), in a line of its own
+    uint32_t unused[31];
+    double sum[LP_PARTS * SK_NW];          // of exp((x - max) / T)
+    float max[LP_PARTS * SK_NW];
+    uint32_t above[LP_PARTS * SK_NW];      // logits above the chosen token's
+    float bound[LP_PARTS * SK_NW];         // n of the part's logits reach it
+    int cnt[LP_PARTS * SK_NW];             // tokens in the wave's list
+    uint32_t key[LP_PARTS * SK_NW];        // the largest logits (as keys) of groups of lanes
 };
 struct LpArgs {
     const void* logits;
@@ -156,9 +158,8 @@ struct LpArgs {
     int32_t* rank;
     int32_t* ids;                          // [B][n]
     float* top;
-    LpPart* part;                          // [B][nseg]
+    LpRow* rows;                           // [B]
     uint64_t* lists;                       // [B][nseg][SK_NW][LP_TOP]
-    uint32_t* ticket;                      // [B], left at 0
     int32_t* err;
 };
 hipError_t launch_logprobs(int type, const LpArgs& a, hipStream_t st);
