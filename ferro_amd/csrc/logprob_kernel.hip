@@ -380,6 +380,40 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
             key[u] = i < (lists << 6) >> lp_group(nseg) ? rw->key[i] : 0u;
         }
     }
+    // TOP: the tokens' lists. Half a wave reads a list, sixteen lists in flight; the first of them behind the sums
+    constexpr int U = 8, ROOM = sizeof(s.gval) / sizeof(uint64_t);
+    static_assert(4 * U * WAVE <= ROOM, "a batch fits behind what has to be sorted first");
+    const int half = lane >> 5, pos = lane & 31;
+    int* at = s.gid[0];                                        // [LP_PARTS * SK_NW] lists: number, length
+    uint64_t* join = reinterpret_cast<uint64_t*>(&s.gval[0][0]);
+    uint32_t least = 0u;
+    int k = 0, to[U];
+    uint64_t e[U];
+    auto fetch = [&](int i0, int skip) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + 2 * u + half;
+            to[u] = i < k ? at[i] : 0;
+            e[u] = pos + skip < (to[u] & 255) ? rl[(to[u] >> 8) * LP_TOP + pos + skip] : 0ull;
+        }
+    };
+    if (TOP) {
+        float best = LP_LOWEST;
+#pragma unroll
+        for (int u = 0; u < LL; ++u) best = fmaxf(best, bi[u]);
+        best = wave_allreduce(best, fmx);
+        least = lp_nth(key, key_of(best), n);
+        // of waves whose largest logit reaches the bound (about 17 of 64 for n = 20; reading all of them took 3 us)
+#pragma unroll
+        for (int u = 0; u < LL; ++u) {
+            const bool in = len[u] > 0 && key_of(mi[u]) >= least;
+            const uint64_t m = __ballot(in);
+            if (in) at[k + (int)mbcnt(m)] = ((u * WAVE + lane) << 8) | len[u];
+            k += __popcll(m);
+        }
+        lp_wave_sync();
+        fetch(0, 0);
+    }
     float M = LP_LOWEST;
 #pragma unroll
     for (int u = 0; u < LL; ++u) M = fmaxf(M, mi[u]);
@@ -401,69 +435,49 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
         if (a.rank) a.rank[row] = xv > LP_NONE ? (has ? (int)ab + 1 : 1) : 0;
     }
     if (TOP) {
-        float best = LP_LOWEST;
-#pragma unroll
-        for (int u = 0; u < LL; ++u) best = fmaxf(best, bi[u]);
-        best = wave_allreduce(best, fmx);
-        const uint32_t least = lp_nth(key, key_of(best), n);
-        // the tokens that reach it, gathered in LDS (one copy of the sort in the code: with one per batch of lists the end
-        // took 3 us more, most of it for instructions)
-        constexpr int ROOM = sizeof(s.gval) / sizeof(uint64_t);
-        uint64_t* join = reinterpret_cast<uint64_t*>(&s.gval[0][0]);
+        // the tokens that reach the bound, gathered in LDS
         int cnt = 0;
         uint64_t acc = 0ull;
-        auto gather = [&](uint64_t c) {                        // (0: no token; the bound is above it)
-            const bool in = comp_key(c) >= least;
-            const uint64_t m = __ballot(in);
-            if (in) join[cnt + (int)mbcnt(m)] = c;
-            cnt += __popcll(m);
-        };
-        // the lists of waves whose largest logit reaches it (about 17 of 64 for n = 20; reading all of them took 3 us)
-        int* at = s.gid[0];                                    // [LP_PARTS * SK_NW] their numbers, above their lengths
-        int k = 0;
+        bool sorted = false;
+        auto gather = [&]() {                                  // (0: no token; the bound is above it)
 #pragma unroll
-        for (int u = 0; u < LL; ++u) {
-            const bool in = len[u] > 0 && key_of(mi[u]) >= least;
-            const uint64_t m = __ballot(in);
-            if (in) at[k + (int)mbcnt(m)] = ((u * WAVE + lane) << 8) | len[u];
-            k += __popcll(m);
-        }
-        lp_wave_sync();
-        // half a wave per list, sixteen lists in flight
-        constexpr int U = 8;
-        static_assert(4 * U * WAVE <= ROOM, "a batch fits behind what has to be sorted first");
-        const int half = lane >> 5, pos = lane & 31;
-#pragma unroll 1
-        for (int i0 = 0; i0 < k || cnt > 0; i0 += 2 * U) {
-            if (i0 < k) {
-                int to[U];
-                uint64_t e[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int i = i0 + 2 * u + half;
-                    to[u] = i < k ? at[i] : 0;
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) e[u] = pos < (to[u] & 255) ? rl[(to[u] >> 8) * LP_TOP + pos] : 0ull;
-#pragma unroll
-                for (int u = 0; u < U; ++u) gather(e[u]);
-                bool more = false;                             // lists of more than 32
-#pragma unroll
-                for (int u = 0; u < U; ++u) more |= (to[u] & 255) > 32;
-                if (__ballot(more) != 0ull) {
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        e[u] = pos + 32 < (to[u] & 255) ? rl[(to[u] >> 8) * LP_TOP + pos + 32] : 0ull;
-#pragma unroll
-                    for (int u = 0; u < U; ++u) gather(e[u]);
-                }
+            for (int u = 0; u < U; ++u) {
+                const bool in = comp_key(e[u]) >= least;
+                const uint64_t m = __ballot(in);
+                if (in) join[cnt + (int)mbcnt(m)] = e[u];
+                cnt += __popcll(m);
             }
-            if (cnt > 2 * U * WAVE || i0 + 2 * U >= k) {
+        };
+#pragma unroll 1
+        for (int i0 = 0; i0 < k; i0 += 2 * U) {
+            if (i0 > 0) fetch(i0, 0);
+            gather();
+            bool more = false;                                 // lists of more than 32
+#pragma unroll
+            for (int u = 0; u < U; ++u) more |= (to[u] & 255) > 32;
+            if (__ballot(more) != 0ull) {
+                fetch(i0, 32);
+                gather();
+            }
+            lp_wave_sync();
+            const bool last = i0 + 2 * U >= k;
+            if (last && !sorted && cnt <= WAVE) {              // ranks: an eighth of a sort's instructions
+                const uint64_t c = lane < cnt ? join[lane] : 0ull;
+                int r = 0;
+#pragma unroll 4
+                for (int i = 0; i < cnt; ++i) r += join[i] > c ? 1 : 0;
                 lp_wave_sync();
+                join[lane] = 0ull;
+                lp_wave_sync();
+                if (c != 0ull) join[r] = c;
+                lp_wave_sync();
+                acc = join[lane];
+            } else if (last || cnt > 2 * U * WAVE) {
 #pragma unroll 1
                 for (int i = 0; i < cnt; i += WAVE)
                     acc = merge_top64(acc, sort64<false>(i + lane < cnt ? join[i + lane] : 0ull));
                 cnt = 0;
+                sorted = true;
                 lp_wave_sync();
             }
         }
