@@ -99,29 +99,37 @@ __device__ __forceinline__ int64_t ed_lower(const EdRow& r, int id) {
     }
     return lo + __popcll(__ballot(lo + lane_id() < hi && r.ids[lo + lane_id()] < id));
 }
-// A row's biases in registers, one per lane, where it has no more of them (held by kernels that pass over several chunks).
+// A row's biases, the first 64 of them in registers, one per lane: requested early, used when the logits are there.
 struct EdList {
+    int64_t nb;
     int id;
     float val;
 };
 __device__ __forceinline__ EdList ed_list(const EdRow& r) {
-    EdList l = {0x7fffffff, 0.0f};
-    if (lane_id() < r.nb && r.nb <= WAVE) l = {r.ids[lane_id()], r.val[lane_id()]};
+    EdList l = {r.nb, 0x7fffffff, 0.0f};
+    if (lane_id() < r.nb) {
+        l.id = r.ids[lane_id()];
+        l.val = r.val[lane_id()];
+    }
     return l;
 }
-// Adds the row's biases to the wave's logits of the segment, one after another in list order (equal ids add up): each is
-// read by one lane, and the wave gives it to the lane whose logit it is. x(q, c): the lane's logits.
+// Adds the biases of record rec to the wave's logits of the segment, one after another in list order (equal ids add up):
+// each is held by one lane, and the wave gives it to the lane whose logit it is, group by group (with all groups in one
+// loop the kernels spilled their logits). x(q, c): the lane's logits.
 template <int NL, class X>
-__device__ __forceinline__ void ed_add(const EdRow& r, const EdList* held, int seg_lo, int n_in, X x) {
+__device__ __forceinline__ void ed_add(const EdArgs& ed, int rec, const EdList& list, int seg_lo, int n_in, X x) {
     const int lane = lane_id(), w = (int)threadIdx.x / WAVE;
+    EdRow r = {nullptr, false, nullptr, nullptr, list.nb};
+    int64_t i = 0;
+    if (list.nb > WAVE) {
+        ed_bias(r, ed, rec);
+        if (r.nb > 4 * WAVE) i = ed_lower(r, seg_lo);
+    }
 #pragma unroll 1
-    for (int64_t i = r.nb > 4 * WAVE ? ed_lower(r, seg_lo) : 0; i < r.nb; i += WAVE) {
-        int id = 0x7fffffff;
-        float val = 0.0f;
-        if (held && r.nb <= WAVE) {
-            id = held->id;
-            val = held->val;
-        } else if (i + lane < r.nb) {
+    for (; i < r.nb; i += WAVE) {
+        int id = i == 0 ? list.id : 0x7fffffff;
+        float val = list.val;
+        if (i > 0 && i + lane < r.nb) {
             id = r.ids[i + lane];
             val = r.val[i + lane];
         }
@@ -134,11 +142,10 @@ __device__ __forceinline__ void ed_add(const EdRow& r, const EdList* held, int s
                     const int from = __ffsll((unsigned long long)m) - 1;
                     const uint32_t at = (uint32_t)read_lane((int)rel, from);
                     const float d = read_lane(val, from);
-                    if ((int)((at >> 2) & (WAVE - 1)) == lane) {
+                    const bool mine = (int)((at >> 2) & (WAVE - 1)) == lane;
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            if ((int)(at & 3u) == c) x(q, c) = __fadd_rn(x(q, c), d);
-                    }
+                    for (int c = 0; c < 4; ++c)                // (-0 leaves every number as it is)
+                        x(q, c) = __fadd_rn(x(q, c), mine && (int)(at & 3u) == c ? d : -0.0f);
                 }
             }
         }
@@ -149,7 +156,7 @@ __device__ __forceinline__ void ed_add(const EdRow& r, const EdList* held, int s
 // Token id's logit l with its mask and biases, on every lane (whole wave): NaN where it is not allowed.
 __device__ __forceinline__ float ed_one(const EdRow& r, const EdList& list, float l, int id) {
     for (int64_t i = r.nb <= WAVE ? 0 : ed_lower(r, id); i < r.nb; i += WAVE) {
-        const bool held = r.nb <= WAVE, in = i + lane_id() < r.nb;
+        const bool held = i == 0, in = i + lane_id() < r.nb;
         const int at = held ? list.id : in ? r.ids[i + lane_id()] : 0x7fffffff;
         const float val = held ? list.val : in ? r.val[i + lane_id()] : 0.0f;
         uint64_t m = __ballot(at == id);

@@ -48,6 +48,7 @@ __global__ __launch_bounds__(SK_LT) void edit_kernel(EditArgs e) {
     if (e.params) p = ld_const(e.params + rec);
     const EdRow r = ed_row(e.ed, row, rec, e.err);
     const EdBits bits = ed_bits<NL>(r, seg_lo, V);
+    const EdList few = ed_list(r);
 
     const bool rep_on = p.repetition_penalty != 1.0f;
     const bool fp_on = p.frequency_penalty != 0.0f || p.presence_penalty != 0.0f;
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(SK_LT) void edit_kernel(EditArgs e) {
         L::floats(raw[q], x[q]);
         if (p.softcap > 0.0f) softcap_vals(x[q], p.softcap);
     }
-    if (r.nb > 0) ed_add<NL>(r, nullptr, seg_lo, n_in, [&](int q, int c) -> float& { return x[q][c]; });
+    if (few.nb > 0) ed_add<NL>(e.ed, rec, few, seg_lo, n_in, [&](int q, int c) -> float& { return x[q][c]; });
     const bool greedy = p.temperature <= 0.0f || p.top_k == 1;
     const uint32_t none = e.any ? 0x7FC00000u : 0xFF800000u;   // the sampling kernels' rows: NaN, never a candidate
     float* out = e.out + (int64_t)row * e.out_ld + seg_lo;
@@ -148,7 +149,8 @@ hipError_t launch_edit(int nl, const EditArgs& e, hipStream_t st) {
         constexpr int T = decltype(type)::value;
         const dim3 grid((unsigned)((int64_t)e.B * e.nseg)), block(SK_LT);
         if (nl == 8) hipLaunchKernelGGL((edit_kernel<T, 8>), grid, block, 0, st, e);
-        else hipLaunchKernelGGL((edit_kernel<T, 4>), grid, block, 0, st, e);
+        else if (nl == 4) hipLaunchKernelGGL((edit_kernel<T, 4>), grid, block, 0, st, e);
+        else hipLaunchKernelGGL((edit_kernel<T, 2>), grid, block, 0, st, e);
     };
     if (e.type == FS_F32) go(std::integral_constant<int, FS_F32>{});
     else if (e.type == FS_BF16) go(std::integral_constant<int, FS_BF16>{});

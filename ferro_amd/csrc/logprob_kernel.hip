@@ -195,7 +195,7 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
 #pragma unroll
             for (int q = 0; q < NL; ++q) softcap_vals(x[q], cap);
         }
-        if (r.nb > 0) ed_add<NL>(r, &few, lo, n_in, [&](int q, int c_) -> float& { return x[q][c_]; });
+        if (few.nb > 0) ed_add<NL>(a.ed, row, few, lo, n_in, [&](int q, int c_) -> float& { return x[q][c_]; });
         if (masked) {
 #pragma unroll
             for (int q = 0; q < NL; ++q) {

@@ -1628,14 +1628,7 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
     float v[NL][4];
     EdBits eb = {~0u, ~0u};
     bool masked = false;
-    if constexpr (ED) {                                        // the row's mask first: it decides which loads are made
-        const MkArgs& em = *(const MkArgs*)((const __attribute__((address_space(4))) char*)
-                                            __builtin_amdgcn_kernarg_segment_ptr() + MK_ARGS_OFF);
-        EdRow er;
-        ed_mask(er, em.a.ed, row, em.a.err);
-        eb = ed_bits<NL>(er, seg_lo, V);
-        masked = er.words || er.closed;
-    }
+    EdList few = {0, 0x7fffffff, 0.0f};
     auto load = [&](int q) {
         int at = (q * SK_LT + tid) * 16;
         if (ED && masked) at = ed_nibble(eb, q) != 0u ? at : 0x7ffffff0;           // (past the buffer: no read, zeros)
@@ -1644,10 +1637,23 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
     };
     // the first half, then the window's ids, then the rest: a wave's loads return in order, and so the bitmap is built
     // while the rest streams in (segments of 4096 logits are all requested at once: their ids come last anyway)
-    constexpr int NL0 = NL > 4 ? NL / 2 : NL;
+    constexpr int NL0 = NL > 4 ? NL / 2 : NL, NL1 = ED && NL0 > ED_FIRST ? ED_FIRST : NL0;
 #pragma unroll
-    for (int q = 0; q < NL0; ++q) load(q);
+    for (int q = 0; q < NL1; ++q) load(q);
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (ED) {                                        // (the mask decides which of the others are made)
+        if (flags & ED_MASKS) {
+            const MkArgs& em = *(const MkArgs*)((const __attribute__((address_space(4))) char*)
+                                                __builtin_amdgcn_kernarg_segment_ptr() + MK_ARGS_OFF);
+            EdRow er;
+            ed_mask(er, em.a.ed, row, em.a.err);
+            eb = ed_bits<NL>(er, seg_lo, V);
+            masked = er.words || er.closed;
+        }
+#pragma unroll
+        for (int q = NL1; q < NL0; ++q) load(q);
+        __builtin_amdgcn_sched_barrier(0);
+    }
     // the other arguments through a pointer the compiler cannot trace (it would load some of them before the logits)
     const __attribute__((address_space(4))) char* kseg =
         (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
@@ -1711,6 +1717,11 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
     const bool cp_on = (flags & SK_COPY) != 0;
     SkCopy cp = {};
     if (cp_on) cp = sk_cp_load(hist_off, hist, row, seg, nseg);
+    if (ED && !CAP && (flags & ED_BIASES)) {
+        EdRow er = {nullptr, false, nullptr, nullptr, 0};
+        ed_bias(er, a.ed, pidx);
+        few = ed_list(er);
+    }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int q = NL0; q < NL; ++q) load(q);
@@ -1726,11 +1737,8 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
     // the logits under the mask and the biases (-inf, too, is no candidate; with a softcap it is: the cap makes it a number)
     auto edit = [&]() {
         if constexpr (ED) {
-            if (!CAP) {
-                EdRow er;
-                ed_bias(er, a.ed, pidx);
-                if (er.nb > 0) ed_add<NL>(er, nullptr, seg_lo, n_in, [&](int q, int c) -> float& { return v[q][c]; });
-            }
+            if (!CAP && few.nb > 0)
+                ed_add<NL>(a.ed, pidx, few, seg_lo, n_in, [&](int q, int c) -> float& { return v[q][c]; });
             if (masked) {
                 asm volatile("" : "+v"(eb.a), "+v"(eb.b));         // (the nibbles again: kept from the loads they spill)
 #pragma unroll

@@ -479,6 +479,10 @@ fs::SkArgs row_args(const fs_context* ctx, const fs::Args& a, int nseg) {
     return k;
 }
 
+int edit_flags(const fs::EdArgs* ed) {
+    return !ed ? 0 : (ed->mask ? fs::ED_MASKS : 0) | (ed->bias_off ? fs::ED_BIASES : 0);
+}
+
 // Launches the small-k kernel when the batch fits it; *used = false (nothing launched) otherwise. a.mode selects
 // sampling (h_params: B records) or verification windows (h_params: n_streams records).
 // h_params NULL: every row greedy without penalties (fs_argmax_batch without parameters): the context's greedy
@@ -523,7 +527,7 @@ int launch_small(fs_context* ctx, const fs::Args& a_in, const fs_row_params* h_p
     bool may_pen = ch.may_pen;
     // a verification window reaches this kernel only without an active penalty (small_k_windows)
     may_pen = may_pen && !verify && a.hist && a.hist_off;
-    const int flags = (may_pen ? fs::SK_MAY_PEN : 0) | (a.out_hist_off ? fs::SK_COPY : 0);
+    const int flags = (may_pen ? fs::SK_MAY_PEN : 0) | (a.out_hist_off ? fs::SK_COPY : 0) | edit_flags(ed);
     if (fs::launch_small_k(nl, capped, all_greedy, ed != nullptr, (unsigned)grid, flags, k, st) != hipSuccess) return FS_E_HIP;
     used = true;
     return FS_OK;
@@ -676,7 +680,7 @@ int launch_mid(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params
     if (ctx->trace && grid * fs::TRACE_W <= ctx->trace_cap) m.a.trace = ctx->trace;
 #endif
     const int flags = (ch.may_pen ? fs::SK_MAY_PEN : 0) | (a.out_hist_off ? fs::SK_COPY : 0) |
-                      (verify ? fs::MK_VERIFY : 0);
+                      (verify ? fs::MK_VERIFY : 0) | edit_flags(ed);
     if (fs::launch_mid_k(ch.nl, ch.capped, ch.all, ed != nullptr, (unsigned)grid, flags, m, st) != hipSuccess) return FS_E_HIP;
     used = true;
     return FS_OK;
@@ -733,11 +737,15 @@ struct Edited {
     ~Edited() { c->frozen = false; }
 };
 
-// Logits per thread and segments per row of the edit kernel: the larger segments where they fill the device.
+// Groups of four logits per thread and segments per row of the edit kernel: the largest segments that still give every CU
+// four workgroups.
 int edit_plan(int cus, int64_t B, int32_t V, int& nseg) {
-    int nl = 8;
-    if (B * (((int64_t)V + fs::SK_LT * 32 - 1) / (fs::SK_LT * 32)) < cus) nl = 4;
-    nseg = (int)(((int64_t)V + fs::SK_LT * nl * 4 - 1) / (fs::SK_LT * nl * 4));
+    int nl = 2;
+    for (const int l : {8, 4, 2}) {
+        nl = l;
+        nseg = (int)(((int64_t)V + fs::SK_LT * l * 4 - 1) / (fs::SK_LT * l * 4));
+        if (B * nseg >= 4 * (int64_t)cus) break;
+    }
     return nl;
 }
 

@@ -66,8 +66,9 @@ struct SkArgs {
 };
 
 // flags of a launch: some row has an active penalty window; a decode step (the histories are copied); a verification
-// window (mid-k kernel)
-constexpr int SK_MAY_PEN = 1, SK_COPY = 2, MK_VERIFY = 4;
+// window (mid-k kernel); a call with masks, with biases
+constexpr int SK_MAY_PEN = 1, SK_COPY = 2, MK_VERIFY = 4, ED_MASKS = 8, ED_BIASES = 16;
+constexpr int ED_FIRST = 4;                // float4 loads per thread that do not wait for the row's mask
 // nl: float4 loads per thread (4, 8 or 16); the grid and k's layout come from the small-k plan. edited: under k.ed.
 hipError_t launch_small_k(int nl, bool capped, bool all_greedy, bool edited, unsigned grid, int flags, const SkArgs& k,
                           hipStream_t st);
@@ -95,7 +96,7 @@ struct MkArgs {
 hipError_t launch_mid_k(int nl, bool capped, bool all, bool edited, unsigned grid, int flags, const MkArgs& m,
                         hipStream_t st);
 
-// Edited logits written out (edit_kernels.hip). nl: groups of four logits per thread (4 or 8).
+// Edited logits written out (edit_kernels.hip). nl: groups of four logits per thread (2, 4 or 8).
 struct EditArgs {
     const void* logits;
     int type;                              // FS_F32, FS_BF16, FS_F16

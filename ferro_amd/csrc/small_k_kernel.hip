@@ -225,20 +225,32 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
     float4 v[NL];
     EdBits eb = {~0u, ~0u};
     bool masked = false;
-    if constexpr (ED) {
-        const SkArgs& ea = *(const SkArgs*)((const __attribute__((address_space(4))) char*)
-                                            __builtin_amdgcn_kernarg_segment_ptr() + SK_ARGS_OFF);
-        EdRow er;
-        ed_mask(er, ea.ed, row, ea.err);
-        eb = ed_bits<NL>(er, seg_lo, V);
-        masked = er.words || er.closed;
-    }
-#pragma unroll
-    for (int q = 0; q < NL; ++q) {
+    EdList few = {0, 0x7fffffff, 0.0f};
+    auto load = [&](int q) {
         int at = (q * SK_LT + tid) * 16;
-        if (ED && masked) at = ed_nibble(eb, q) != 0u ? at : 0x7ffffff0;           // (past the buffer: no read, zeros)
+        if (ED && masked) at = ed_nibble(eb, q) != 0u ? at : 0x7ffffff0;             // (past the buffer: no read, zeros)
         const f32x4 t = raw_buffer_load_f32x4(rs, at, 0, 2);       // nontemporal: read once
         v[q] = make_float4(t.x, t.y, t.z, t.w);
+    };
+    constexpr int NL0 = ED && NL > ED_FIRST ? ED_FIRST : NL;
+#pragma unroll
+    for (int q = 0; q < NL0; ++q) load(q);
+    if constexpr (ED) {
+        __builtin_amdgcn_sched_barrier(0);
+        const SkArgs& ea = *(const SkArgs*)((const __attribute__((address_space(4))) char*)
+                                            __builtin_amdgcn_kernarg_segment_ptr() + SK_ARGS_OFF);
+        EdRow er = {nullptr, false, nullptr, nullptr, 0};
+        if (flags & ED_MASKS) {
+            ed_mask(er, ea.ed, row, ea.err);
+            eb = ed_bits<NL>(er, seg_lo, V);
+            masked = er.words || er.closed;
+        }
+#pragma unroll
+        for (int q = NL0; q < NL; ++q) load(q);
+        if (!CAP && (flags & ED_BIASES) && ea.mode != MODE_VERIFY) {   // (a window's biases are its stream's: below)
+            ed_bias(er, ea.ed, row);
+            few = ed_list(er);
+        }
     }
     __builtin_amdgcn_sched_barrier(0);
 
@@ -291,6 +303,11 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
             if (ld_const(a.row_off + m) <= row) s0 = m; else s1 = m;
         }
         pidx = s0;
+        if (ED && !CAP && (flags & ED_BIASES)) {
+            EdRow er = {nullptr, false, nullptr, nullptr, 0};
+            ed_bias(er, a.ed, pidx);
+            few = ed_list(er);
+        }
     }
     const fs_row_params* pp = params + pidx;
     const float temp = ld_const(&pp->temperature);
@@ -408,14 +425,10 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
     const bool wpen = __ballot(pm != 0ull) != 0ull;
     const bool tail = n_in < SEG;
     if constexpr (ED) {
-        if (!CAP) {
-            EdRow er;
-            ed_bias(er, a.ed, pidx);
-            if (er.nb > 0)
-                ed_add<NL>(er, nullptr, seg_lo, n_in, [&](int q, int c) -> float& {
-                    return c == 0 ? v[q].x : c == 1 ? v[q].y : c == 2 ? v[q].z : v[q].w;
-                });
-        }
+        if (!CAP && few.nb > 0)
+            ed_add<NL>(a.ed, pidx, few, seg_lo, n_in, [&](int q, int c) -> float& {
+                return c == 0 ? v[q].x : c == 1 ? v[q].y : c == 2 ? v[q].z : v[q].w;
+            });
         if (masked) {
             asm volatile("" : "+v"(eb.a), "+v"(eb.b));         // (the nibbles again: kept from the loads they spill)
 #pragma unroll
