@@ -48,7 +48,7 @@ __global__ __launch_bounds__(SK_LT) void edit_kernel(EditArgs e) {
     if (e.params) p = ld_const(e.params + rec);
     const EdRow r = ed_row(e.ed, row, rec, e.err);
     const EdBits bits = ed_bits<NL>(r, seg_lo, V);
-    const EdList few = ed_list(r);
+    const EdList few = ed_list<false>(r);
 
     const bool rep_on = p.repetition_penalty != 1.0f;
     const bool fp_on = p.frequency_penalty != 0.0f || p.presence_penalty != 0.0f;
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(SK_LT) void edit_kernel(EditArgs e) {
         L::floats(raw[q], x[q]);
         if (p.softcap > 0.0f) softcap_vals(x[q], p.softcap);
     }
-    if (few.nb > 0) ed_add<NL>(e.ed, rec, few, seg_lo, n_in, [&](int q, int c) -> float& { return x[q][c]; });
+    if (few.nb > 0) ed_add<NL, false>(e.ed, rec, few, nullptr, seg_lo, n_in, [&](int q, int c) -> float& { return x[q][c]; });
     const bool greedy = p.temperature <= 0.0f || p.top_k == 1;
     const uint32_t none = e.any ? 0x7FC00000u : 0xFF800000u;   // the sampling kernels' rows: NaN, never a candidate
     float* out = e.out + (int64_t)row * e.out_ld + seg_lo;

@@ -153,7 +153,7 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
         if (c0 + 1 < c1) next = ed_bits<NL>(r, (c0 + 1) * CHUNK, V);
     }
     ed_bias(r, a.ed, row);
-    const EdList few = ed_list(r);
+    const EdList few = ed_list<false>(r);
     const int t = a.tok ? ld_const(a.tok + row) : -1;
     float cap = 0.0f, T = 1.0f;
     if (a.params) {
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
 #pragma unroll
             for (int q = 0; q < NL; ++q) softcap_vals(x[q], cap);
         }
-        if (few.nb > 0) ed_add<NL>(a.ed, row, few, lo, n_in, [&](int q, int c_) -> float& { return x[q][c_]; });
+        if (few.nb > 0) ed_add<NL, false>(a.ed, row, few, nullptr, lo, n_in, [&](int q, int c_) -> float& { return x[q][c_]; });
         if (masked) {
 #pragma unroll
             for (int q = 0; q < NL; ++q) {

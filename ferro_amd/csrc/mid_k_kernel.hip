@@ -87,7 +87,7 @@ struct MkShared {
         uint32_t rk[SK_LT];                // partial ranks of a short list
         uint32_t srt[SK_NW][WAVE];         // the waves' sorted lane maxima
         double2 pow2[64];                  // every token a candidate: 2^(j/64) in two parts
-    } h;
+    } h;                                   // (the upper half: first the row's biases)
     union {
         uint32_t bmp[SK_LT * 2];           // one bit per logit of the window's ids: 64 bits per thread; mk_slow: by id
         float pv[MK_PC];                   // (the bits are read) the flagged logits, raw, then penalised
@@ -1720,7 +1720,7 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
     if (ED && !CAP && (flags & ED_BIASES)) {
         EdRow er = {nullptr, false, nullptr, nullptr, 0};
         ed_bias(er, a.ed, pidx);
-        few = ed_list(er);
+        few = ed_list<true>(er);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -1738,7 +1738,7 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
     auto edit = [&]() {
         if constexpr (ED) {
             if (!CAP && few.nb > 0)
-                ed_add<NL>(a.ed, pidx, few, seg_lo, n_in, [&](int q, int c) -> float& { return v[q][c]; });
+                ed_add<NL, true>(a.ed, pidx, few, s.h.hist + MK_H / 2, seg_lo, n_in, [&](int q, int c) -> float& { return v[q][c]; });
             if (masked) {
                 asm volatile("" : "+v"(eb.a), "+v"(eb.b));         // (the nibbles again: kept from the loads they spill)
 #pragma unroll

@@ -27,7 +27,7 @@ namespace fs {
 struct SkShared {
     float4 gval[SK_NW][SK_GCAP + 1];       // groups of four whose maximum reaches the bound (+ a dummy slot)
     int32_t gidx[SK_NW][SK_GCAP + 1];      //   and the segment offset of their first logit
-    uint64_t cand[SK_CAP];                 // the segment's candidates (composites)
+    uint64_t cand[SK_CAP];                 // the segment's candidates (composites; before, the row's biases)
     uint64_t wl[SK_NW][SK_K];              // per-wave sorted lists (segment sort, row merge)
     uint32_t bmp[SK_LT * 16 * 4 / 32];     // repetition window ids in the segment (largest segment: NL = 16)
     uint32_t hist[16];                     // radix select digits (exact fallback)
@@ -188,8 +188,9 @@ constexpr unsigned SK_PAD_LDS = 16384;
 // MANY: more than 4 * SK_NW lists per row (sk_merge_many; left out of the others, which it cost 0.2 us of 8.4).
 // GREEDY: every row of the batch is greedy (the selection code is left out: fewer registers, more workgroups per CU).
 // ED: the rows have masks and biases (fs_edits; no biases with a softcap, which comes before them but is applied to the
-// candidates alone). A row's mask is read first and the logits' loads then skip the groups of four without an allowed
-// token. A logit that is not allowed becomes NaN, which nothing below takes; candidates are above -inf; a row without one
+// candidates alone). The loads from the ED_FIRST-th on wait for the row's mask and skip the groups of four without an
+// allowed token (64 rows of 262144, k 64: 17.8 us where the masks allow few tokens, 22.5 where they allow most, 20.8
+// without; with all loads behind the mask 17.2 / 22.6 / 21.2 and one more round trip for a single row). A logit that is not allowed becomes NaN, which nothing below takes; candidates are above -inf; a row without one
 // has token -1.
 template <int NL, bool CAP, bool GREEDY, bool MANY, bool ED>
 __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, int64_t ld, int B, int V, int nseg,
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
         for (int q = NL0; q < NL; ++q) load(q);
         if (!CAP && (flags & ED_BIASES) && ea.mode != MODE_VERIFY) {   // (a window's biases are its stream's: below)
             ed_bias(er, ea.ed, row);
-            few = ed_list(er);
+            few = ed_list<true>(er);
         }
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
         if (ED && !CAP && (flags & ED_BIASES)) {
             EdRow er = {nullptr, false, nullptr, nullptr, 0};
             ed_bias(er, a.ed, pidx);
-            few = ed_list(er);
+            few = ed_list<true>(er);
         }
     }
     const fs_row_params* pp = params + pidx;
@@ -426,7 +427,7 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
     const bool tail = n_in < SEG;
     if constexpr (ED) {
         if (!CAP && few.nb > 0)
-            ed_add<NL>(a.ed, pidx, few, seg_lo, n_in, [&](int q, int c) -> float& {
+            ed_add<NL, true>(a.ed, pidx, few, reinterpret_cast<uint32_t*>(&s.cand[0]), seg_lo, n_in, [&](int q, int c) -> float& {
                 return c == 0 ? v[q].x : c == 1 ? v[q].y : c == 2 ? v[q].z : v[q].w;
             });
         if (masked) {
