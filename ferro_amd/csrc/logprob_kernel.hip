@@ -96,11 +96,6 @@ __device__ __forceinline__ uint64_t lp_cut(LpShared& s, int& g, bool& cut, float
     return acc;
 }
 
-// The lanes (a power of two, its logarithm) whose largest logit a wave publishes: 256 groups in a row of up to 64 parts.
-__device__ __forceinline__ int lp_group(int nseg) {
-    return nseg <= 4 ? 2 : nseg <= 8 ? 3 : nseg <= 16 ? 4 : nseg <= 32 ? 5 : 6;
-}
-
 // The kernel's argument list as a struct: the argument segment follows the same layout rules
 struct LpKernargs {
     const void* logits;
@@ -296,8 +291,15 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
     // ---- the wave's end
     auto addu = [](uint32_t u, uint32_t v) { return u + v; };
     auto addf = [](double u, double v) { return u + v; };
-    LpRow* rw = a.rows + row;
     const int lists = nseg * SK_NW, me = part * SK_NW + w;
+    char* rw = a.rows + (int64_t)row * (int64_t)lp_row_bytes(nseg);
+    uint32_t* ticket = a.ticket + (int64_t)row * LP_LINE;
+    double* p_sum = reinterpret_cast<double*>(rw);
+    float* p_max = reinterpret_cast<float*>(p_sum + lists);
+    uint32_t* p_above = reinterpret_cast<uint32_t*>(p_max + lists);
+    float* p_bound = reinterpret_cast<float*>(p_above + lists);
+    int* p_cnt = reinterpret_cast<int*>(p_bound + lists);
+    uint32_t* p_key = reinterpret_cast<uint32_t*>(p_cnt + lists);
     uint64_t* rl = a.lists + (int64_t)row * lists * LP_TOP;
     sum = wave_allreduce(sum, addf);
     if (TOP) {                                                 // the wave's tokens that reach the best of the part's bounds
@@ -343,25 +345,25 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
         if (nseg > 16) top = both(top, xor_lane32<16>(top));
         if (nseg > 32) top = both(top, xor_lane32<32>(top));
         const int lg = lp_group(nseg);
-        if ((lane & ((1 << lg) - 1)) == 0) rw->key[((me << 6) + lane) >> lg] = top;
+        if ((lane & ((1 << lg) - 1)) == 0) p_key[((me << 6) + lane) >> lg] = top;
         if (lane == 0) {
-            rw->cnt[me] = cnt;
-            rw->bound[me] = reach;
+            p_cnt[me] = cnt;
+            p_bound[me] = reach;
         }
     }
     uint32_t turn = 0u;
     if (lane == 0) {
-        rw->sum[me] = sum;
-        rw->max[me] = mx;
-        rw->above[me] = above;
+        p_sum[me] = sum;
+        p_max[me] = mx;
+        p_above[me] = above;
     }
     vm_drain();                                                // the wave's results are in the L2
     __syncthreads();
     if (w != 0) return;
-    if (lane == 0) turn = __hip_atomic_fetch_add(&rw->ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    if (lane == 0) turn = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     if (read_lane(turn, 0) != (uint32_t)nseg - 1u) return;
     // ---- the row's end, by its last part's first wave
-    if (lane == 0) rw->ticket = 0u;
+    if (lane == 0) *ticket = 0u;
     constexpr int LL = LP_PARTS * SK_NW / WAVE;                // waves' results per lane
     double si[LL];
     float mi[LL], bi[LL];
@@ -371,13 +373,13 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
     for (int u = 0; u < LL; ++u) {
         const int i = u * WAVE + lane;
         const bool in = i < lists;
-        si[u] = in ? rw->sum[i] : 0.0;
-        mi[u] = in ? rw->max[i] : LP_LOWEST;
-        ab += in ? rw->above[i] : 0u;
+        si[u] = in ? p_sum[i] : 0.0;
+        mi[u] = in ? p_max[i] : LP_LOWEST;
+        ab += in ? p_above[i] : 0u;
         if (TOP) {
-            bi[u] = in ? rw->bound[i] : LP_LOWEST;
-            len[u] = in ? rw->cnt[i] : 0;
-            key[u] = i < (lists << 6) >> lp_group(nseg) ? rw->key[i] : 0u;
+            bi[u] = in ? p_bound[i] : LP_LOWEST;
+            len[u] = in ? p_cnt[i] : 0;
+            key[u] = i < (lists << 6) >> lp_group(nseg) ? p_key[i] : 0u;
         }
     }
     // TOP: the tokens' lists. Half a wave reads a list, sixteen lists in flight; the first of them behind the sums

@@ -274,11 +274,17 @@ struct MkPen {
 };
 
 // f(logit, place) for a chunk of n logits of a row that one workgroup selects alone: eight loads in flight per thread.
-// ED: under the row's masks and biases (first: the chunk's first token).
+// ED: under the row's masks and biases (first: the chunk's first token); 2048 logits without an allowed token are passed over
+// (64 rows of 262144, k 300, one run of 5000 ids allowed: 1975 us -> 190).
 template <bool ED, class F>
 __device__ __forceinline__ void slow_each(const float* p, int n, const EdRow& er, int first, F f) {
 #pragma unroll 1
-    for (int i0 = threadIdx.x; i0 < n; i0 += 8 * SK_LT) {
+    for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < n; i0 += 8 * SK_LT) {
+        if (ED && er.words) {
+            static_assert(8 * SK_LT == 32 * WAVE, "a word of the mask per lane");
+            const int at = i0 - (int)threadIdx.x + 32 * lane_id();
+            if (__ballot(at < n && er.words[(first + at) >> 5] != 0u) == 0ull) continue;
+        }
         float x[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) x[q] = i0 + q * SK_LT < n ? p[i0 + q * SK_LT] : 0.0f;

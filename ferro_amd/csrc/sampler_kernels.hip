@@ -160,9 +160,10 @@ struct fs_context {
     double* ed_u = nullptr;            //   [ed_u_rows] a decode step's draws,
     int64_t* ed_off = nullptr;         //   [ed_off_rows] zeros: the offsets of empty histories
     size_t ed_logits = 0, ed_param_rows = 0, ed_any_rows = 0, ed_u_rows = 0, ed_off_rows = 0;
-    fs::LpRow* lp_row = nullptr;       // fs_logprobs: [lp_row_rows] what the rows' waves publish,
+    char* lp_row = nullptr;            // fs_logprobs: [lp_row_bytes] what the rows' waves publish,
+    uint32_t* lp_ticket = nullptr;     //   [lp_rows][LP_LINE] their tickets, left at 0,
     uint64_t* lp_lists = nullptr;      //   [lp_list_segs][SK_NW][LP_TOP] their lists
-    size_t lp_row_rows = 0, lp_list_segs = 0;
+    size_t lp_row_bytes = 0, lp_rows = 0, lp_list_segs = 0;
     int static_dev = -1;       // device whose static workspace fs_sample_batch_static used with this context
     uint64_t* trace = nullptr; // FS_TRACE builds: phase timestamps, trace_cap entries (fs_trace_set)
     int64_t trace_cap = 0;
@@ -773,6 +774,10 @@ int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_p
     if (verify) { e.rows = a.rows; e.row_off = a.row_off; e.n_streams = a.n_streams; }
     e.out = ctx->ed_rows; e.out_ld = (int64_t)ld; e.err = ctx->err; e.any = ctx->ed_any; e.rparams = ctx->ed_params;
     if (fs::launch_edit(nl, e, st) != hipSuccess) return FS_E_HIP;
+    auto failed = [&](int rc) {                    // (the rows' marks are left at 0)
+        clear_words(st, ctx->ed_any, (int64_t)B);
+        return rc;
+    };
 
     fs::Args s = {};
     s.logits = ctx->ed_rows; s.ld = (int64_t)ld; s.B = a.B; s.V = a.V; s.params = ctx->ed_params; s.u = a.u; s.tok = a.tok;
@@ -781,7 +786,7 @@ int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_p
     if (decode) {
         hipLaunchKernelGGL(fs::drng_draw_kernel, dim3((unsigned)((B + 63) / 64)), dim3(64), 0, st, a.dmt, a.didx, a.B,
                            (const int64_t*)nullptr, a.params, ctx->ed_u, 0, ctx->err);
-        if (hipGetLastError() != hipSuccess) return FS_E_HIP;
+        if (hipGetLastError() != hipSuccess) return failed(FS_E_HIP);
         s.u = ctx->ed_u;
     }
     int rc = FS_OK;
@@ -789,7 +794,7 @@ int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_p
     std::unique_ptr<fs_row_params[]> h;
     if (h_params && !verify) {                     // (a window's rows have their streams' parameters, known on the device)
         h.reset(new (std::nothrow) fs_row_params[B]);
-        if (!h) return FS_E_NOMEM;
+        if (!h) return failed(FS_E_NOMEM);
         for (size_t b = 0; b < B; ++b) {
             h[b] = h_params[b];
             h[b].repetition_penalty = 1.0f; h[b].frequency_penalty = 0.0f; h[b].presence_penalty = 0.0f;
@@ -797,10 +802,10 @@ int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_p
         }
         rc = launch_small(ctx, s, h.get(), st, used);
         if (rc == FS_OK && !used) rc = launch_mid(ctx, s, h.get(), st, used, mixed_merges(h.get(), a.B, a.V) ? 4 : 2);
-        if (rc < 0) return rc;
+        if (rc < 0) return failed(rc);
     }
     if (!used) rc = launch(ctx, s, a.B, 0, st, h ? (mixed_merges(h.get(), a.B, a.V) ? 4 : 2) : 2);
-    if (rc < 0) return rc;
+    if (rc < 0) return failed(rc);
 
     fs::EditEnd f = {};
     f.B = a.B; f.any = ctx->ed_any; f.rparams = ctx->ed_params; f.tok = a.tok; f.keep = a.keep;
@@ -972,6 +977,7 @@ int fs_destroy(fs_context* c) {
     (void)hipFree(c->ed_u);
     (void)hipFree(c->ed_off);
     (void)hipFree(c->lp_row);
+    (void)hipFree(c->lp_ticket);
     (void)hipFree(c->lp_lists);
     for (void* p : c->retired) (void)hipFree(p);
     if (c->hflag) (void)hipHostFree(c->hflag);
@@ -1264,12 +1270,14 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
     if (((int64_t)B + fs::XCDS) * a.nseg > 0x7fffffff) return FS_E_INVALID;
     const size_t segs = (size_t)B * a.nseg;
     rc = grow(ctx, 0, 0, 0);
-    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_row, ctx->lp_row_rows, (size_t)B, 1, true);
+    if (rc == FS_OK)
+        rc = grow_buffer(ctx, ctx->lp_row, ctx->lp_row_bytes, (size_t)B * fs::lp_row_bytes(a.nseg), 1, false);
+    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_ticket, ctx->lp_rows, (size_t)B, fs::LP_LINE, true);
     if (rc == FS_OK && top > 0) rc = grow_buffer(ctx, ctx->lp_lists, ctx->lp_list_segs, segs, fs::SK_NW * fs::LP_TOP, false);
     if (rc != FS_OK) return rc;
     a.logits = d_logits; a.ld = ld; a.B = B; a.V = V; a.n = top; a.params = d_params; a.tok = d_tok;
     a.lp = d_lp; a.rank = d_rank; a.ids = d_top_ids; a.top = d_top_lp;
-    a.rows = ctx->lp_row; a.lists = ctx->lp_lists; a.err = ctx->err;
+    a.rows = ctx->lp_row; a.ticket = ctx->lp_ticket; a.lists = ctx->lp_lists; a.err = ctx->err;
     return fs::launch_logprobs(type, a, st) == hipSuccess ? FS_OK : FS_E_HIP;
 }
 

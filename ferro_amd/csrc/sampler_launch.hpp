@@ -136,18 +136,18 @@ hipError_t launch_edit_end(const EditEnd& e, hipStream_t st);
 
 // Log-probabilities (logprob_kernel.hip).
 constexpr int LP_TOP = 64;                 // largest n: one entry per lane of the finishing wave
+constexpr int LP_LINE = 32;                // words of a 128-byte line
 constexpr int LP_PARTS = 64;               // parts per row: the join holds one per lane
 constexpr int LP_NL(int type) { return type == FS_F32 ? 4 : 8; }   // groups of four per thread in a chunk of 16 KB
-struct alignas(128) LpRow {                // what a row's waves publish, by part and wave
-    uint32_t ticket;                       // parts that have (left at 0), in a line of its own
-    uint32_t unused[31];
-    double sum[LP_PARTS * SK_NW];          // of exp((x - max) / T)
-    float max[LP_PARTS * SK_NW];
-    uint32_t above[LP_PARTS * SK_NW];      // logits above the chosen token's
-    float bound[LP_PARTS * SK_NW];         // n of the part's logits reach it
-    int cnt[LP_PARTS * SK_NW];             // tokens in the wave's list
-    uint32_t key[LP_PARTS * SK_NW];        // the largest logits (as keys) of groups of lanes
-};
+constexpr int lp_group(int nseg) {         // logarithm of the lanes whose largest logit a wave publishes: 256 groups in a
+    return nseg <= 4 ? 2 : nseg <= 8 ? 3 : nseg <= 16 ? 4 : nseg <= 32 ? 5 : 6;   // row of up to 64 parts
+}
+// What a row's waves publish: by part and wave [lists] the sums, their references, the logits above the chosen token's,
+// bounds and list lengths, then the groups' largest logits.
+constexpr size_t lp_row_bytes(int nseg) {
+    const size_t lists = (size_t)nseg * SK_NW, keys = (lists * 64) >> lp_group(nseg);
+    return (lists * (8 + 4 * 4) + keys * 4 + 127) / 128 * 128;
+}
 struct LpArgs {
     const void* logits;
     int64_t ld;
@@ -159,8 +159,9 @@ struct LpArgs {
     int32_t* rank;
     int32_t* ids;                          // [B][n]
     float* top;
-    LpRow* rows;                           // [B]
+    char* rows;                            // [B][lp_row_bytes(nseg)]
     uint64_t* lists;                       // [B][nseg][SK_NW][LP_TOP]
+    uint32_t* ticket;                      // [B][LP_LINE]: parts that have published (left at 0), in lines of their own
     int32_t* err;
 };
 hipError_t launch_logprobs(int type, const LpArgs& a, hipStream_t st);

@@ -343,6 +343,10 @@ class Edits:
         a = np.pad(a, ((0, 0), (0, (-a.shape[1]) % 32)))
         return np.packbits(a, axis=1, bitorder="little").view(np.int32)
 
+    def tensors(self):
+        """The device tensors of the masks and biases."""
+        return [t for t in (self.mask, self.mask_of, self.bias_ids, self.bias, self.bias_off) if t is not None]
+
     def _ref(self, rows: int, records: int, V: int, dev):
         """The checked fs_edits for a call of `rows` logits rows and `records` records."""
         if dev != self.device:
@@ -397,7 +401,8 @@ def sample_batch(logits, params, u, hist=None, hist_off=None, V=None, kcap=0, ct
         with torch.cuda.device(dev), ctx.lock:
             check(lib().fs_sample_edited(ctx.h, _lptr(logits), ld, B, n, _ptr(hist), _ptr(hist_off), _ptr(p), _hptr(hp),
                                          edits._ref(B, B, n, dev), _ptr(u), _ptr(tok), kcap, _ptr(ids), _ptr(probs),
-                                         _ptr(keep), _on(stream, dev, logits, p, u, hist, hist_off, tok, keep, ids, probs)),
+                                         _ptr(keep), _on(stream, dev, logits, p, u, hist, hist_off, tok, keep, ids, probs,
+                                                             *edits.tensors())),
                   "fs_sample_edited")
         return dict(tok=tok, keep=keep, cand_ids=ids, cand_probs=probs, _keepalive=(p, u, hist, hist_off))
     with ctx.lock:
@@ -468,7 +473,8 @@ def verify(logits, rows, row_off, params, u=None, hist=None, hist_off=None, eos_
             check(lib().fs_verify_edited(ctx.h, _lptr(logits), ld, S, R, n, _ptr(rows), _ptr(row_off), _ptr(hist),
                                          _ptr(hist_off), _ptr(p), _hptr(hp), edits._ref(R, S, n, dev), _ptr(u), int(eos_id),
                                          _ptr(tok), _ptr(acc),
-                                         _on(stream, dev, logits, rows, row_off, p, u, hist, hist_off, tok, acc)),
+                                         _on(stream, dev, logits, rows, row_off, p, u, hist, hist_off, tok, acc,
+                                             *edits.tensors())),
                   "fs_verify_edited")
         return tok, acc
     with ctx.lock:
@@ -582,7 +588,8 @@ def decode_step(logits, params, rng, hist=None, hist_off=None, out_cap=None, V=N
             check(lib().fs_decode_step_edited(ctx.h, rng.h, _lptr(logits), ld, B, n, _ptr(hist), _ptr(hist_off), _ptr(p),
                                               _hptr(hp), edits._ref(B, B, n, dev), _ptr(tok), _ptr(keep), _ptr(out),
                                               _ptr(out_off), int(out_cap),
-                                              _on(stream, dev, logits, p, hist, hist_off, tok, keep, out, out_off)),
+                                              _on(stream, dev, logits, p, hist, hist_off, tok, keep, out, out_off,
+                                                  *edits.tensors())),
                   "fs_decode_step_edited")
         return tok, keep, out, out_off
     with ctx.lock:
@@ -645,7 +652,8 @@ def edit_batch(logits, params=None, hist=None, hist_off=None, edits=None, V=None
     with torch.cuda.device(dev), ctx.lock:
         check(lib().fs_edit_batch(ctx.h, _lptr(logits), kind, ld, B, n, _ptr(hist), _ptr(hist_off), _ptr(p),
                                   None if edits is None else edits._ref(B, B, n, dev), ctypes.c_void_p(o2.data_ptr()),
-                                  out_ld, _on(stream, dev, logits, p, hist, hist_off, out)), "fs_edit_batch")
+                                  out_ld, _on(stream, dev, logits, p, hist, hist_off, out,
+                                               *(edits.tensors() if edits is not None else []))), "fs_edit_batch")
     return out
 
 
@@ -677,7 +685,8 @@ def logprobs(logits, tok=None, n=0, params=None, edits=None, V=None, ctx=None, s
     with torch.cuda.device(dev), ctx.lock:
         check(lib().fs_logprobs(ctx.h, _lptr(logits), kind, ld, B, v, _ptr(p),
                                 None if edits is None else edits._ref(B, B, v, dev), _ptr(t), n, _ptr(lp), _ptr(rank),
-                                _ptr(ids), _ptr(top), _on(stream, dev, logits, p, t, lp, rank, ids, top)), "fs_logprobs")
+                                _ptr(ids), _ptr(top), _on(stream, dev, logits, p, t, lp, rank, ids, top,
+                                                         *(edits.tensors() if edits is not None else []))), "fs_logprobs")
     return dict(lp=lp, rank=rank, ids=ids, top=top)
 
 

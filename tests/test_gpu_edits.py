@@ -324,10 +324,10 @@ def test_decode_loop_edited(name, route):
 
 # ------------------------------------------------------------------------------------------------ log-probabilities
 def lp_tolerance(lp):
-    """fp32 terms: the difference to the maximum (u = 2^-24), its product with 1 / T (2u) and with log2 e inside the
-    exponential (u), each relative to an argument of at most 30 where a term matters (below e^-30 they sum to less than
-    u), the exponential (an ulp, 2u) and 64 additions (u each): the sum is off by at most (4 * 30 + 2 + 64) u relative, its
-    logarithm by as much absolutely. The result is rounded to fp32."""
+    """fp32 terms: the difference to the maximum (u = 2^-24) and its product with log2 e / T, itself rounded (2u), relative to
+    an argument of at most 30 where a term matters (below e^-30 they sum to less than u), the exponential (an ulp, 2u) and
+    at most 10 additions (u each; the chunks' sums are added in fp64): the sum is off by at most (3 * 30 + 2 + 10) u relative,
+    its logarithm by as much absolutely, and 200u is above it. The result is rounded to fp32."""
     return 200 * 2.0 ** -24 + np.abs(lp) * 2.0 ** -24
 
 
