@@ -87,7 +87,7 @@ __global__ __launch_bounds__(SK_LT) void edit_kernel(EditArgs e) {
 #pragma unroll
     for (int q = 0; q < NL; ++q) {
         L::floats(raw[q], x[q]);
-        if (p.softcap > 0.0f) softcap_vals(x[q], p.softcap);
+        if (p.softcap > 0.0f) softcap_vals_unrolled(x[q], p.softcap);
     }
     if (few.nb > 0) ed_add<NL, false>(e.ed, rec, few, nullptr, seg_lo, n_in, [&](int q, int c) -> float& { return x[q][c]; });
     const bool greedy = p.temperature <= 0.0f || p.top_k == 1;
