@@ -304,7 +304,9 @@ class Edits:
         self.device = dev
         self.c = FsEdits()
         if self.mask is not None:
-            self.c.d_mask = self.mask.data_ptr()
+            if self.mask.numel() == 0:                        # no mask at all: a valid pointer, never read
+                self._no_mask = torch.zeros(1, dtype=torch.int32, device=dev)
+            self.c.d_mask = (self.mask if self.mask.numel() else self._no_mask).data_ptr()
             self.c.mask_ld = self.mask.stride(0) if self.mask.shape[0] > 1 else self.mask.shape[1]
             self.c.n_masks = self.mask.shape[0]
             self.c.d_mask_of = self.mask_of.data_ptr() if self.mask_of is not None else None

@@ -129,3 +129,14 @@ def test_edits_handle_checks():
         F.Edits(mask=np.zeros((2, 3), np.int32), mask_of=[0, 1, 0], **cpu)._ref(2, 2, 96, torch.device("cpu"))
     with pytest.raises(SamplerError):
         F.Edits(bias=[{}], **cpu)._ref(2, 2, 96, torch.device("cpu"))
+
+
+def test_a_table_without_masks_is_a_valid_pointer():
+    """A step in which no row has a grammar: a table of no masks, every row's index negative."""
+    e = F.Edits(mask=np.zeros((0, 3), np.int32), mask_of=[-1, -1], device="cpu")
+    assert e.c.d_mask and e.c.d_mask_of and (e.c.n_masks, e.c.mask_ld) == (0, 3)
+    e._ref(2, 2, 96, torch.device("cpu"))
+    with pytest.raises(SamplerError):
+        e._ref(2, 2, 97, torch.device("cpu"))
+    with pytest.raises(SamplerError, match="one mask per row"):
+        F.Edits(mask=np.zeros((0, 3), np.int32), device="cpu")._ref(2, 2, 96, torch.device("cpu"))

@@ -301,3 +301,20 @@ def test_edits_used_on_a_side_stream_may_go():
     torch.cuda.synchronize()
     for t in got:
         assert torch.equal(t, want)
+
+
+@pytest.mark.parametrize("name", ["greedy", "small_k", "mid_k", "every", "large_k"])
+def test_a_step_without_masks_biases_and_histories(name):
+    """A table of no masks, empty bias lists and empty histories do what no edits do, in every call."""
+    B, V = 3, 9001
+    b = Batch(91, B, V, "none", nb=0, **SETS[name])
+    x, off = cuda(b.x), np.zeros(B + 1, np.int64)
+    words = torch.zeros((0, (V + 31) // 32), dtype=torch.int32, device="cuda")
+    ed = F.Edits(mask=words, mask_of=np.full(B, -1), bias=[{}] * B)
+    want = F.sample_batch(x, b.p, b.u)["tok"]
+    assert torch.equal(F.sample_batch(x, b.p, b.u, edits=ed)["tok"], want)
+    assert torch.equal(F.sample_batch(x, b.p, b.u, np.zeros(0, np.int32), off, edits=ed)["tok"], want)
+    assert torch.equal(F.argmax_batch(x, edits=ed), F.argmax_batch(x))
+    assert torch.equal(F.edit_batch(x, edits=ed), x)
+    for got, plain in zip(F.logprobs(x, want, 4, edits=ed).values(), F.logprobs(x, want, 4).values()):
+        assert torch.equal(got, plain)
