@@ -318,3 +318,26 @@ def test_a_step_without_masks_biases_and_histories(name):
     assert torch.equal(F.edit_batch(x, edits=ed), x)
     for got, plain in zip(F.logprobs(x, want, 4, edits=ed).values(), F.logprobs(x, want, 4).values()):
         assert torch.equal(got, plain)
+
+
+@pytest.mark.parametrize("B", [520, 700, 1100])
+def test_logprobs_of_rows_in_parts_past_the_first_round(B):
+    """More rows than workgroups run at once, or more than half as many: parts that fill a last round (3, 1 and 2 of 15
+    chunks)."""
+    V = 60011
+    g = torch.Generator("cuda").manual_seed(B)
+    x = torch.randn((B, V + 1), device="cuda", generator=g)[:, :V] * 4
+    tok = torch.randint(0, V, (B,), device="cuda", generator=g, dtype=torch.int32)
+    ctx = F.Context()
+    a = F.logprobs(x, tok, 3, ctx=ctx)
+    b = F.logprobs(x, tok, 3, ctx=ctx)
+    for r in range(0, B, 37):                          # (the reference a few rows at a time)
+        s = slice(r, min(r + 37, B))
+        want = torch.log_softmax(x[s].double(), 1)
+        lp = want.gather(1, tok[s].long()[:, None])[:, 0]
+        assert torch.all((a["lp"][s].double() - lp).abs() <= 200 * 2.0 ** -24 + lp.abs() * 2.0 ** -24)
+        assert torch.equal(a["rank"][s].long(), 1 + (x[s] > x[s].gather(1, tok[s].long()[:, None])).sum(1))
+        v, i = torch.sort(x[s], dim=1, descending=True, stable=True)
+        assert torch.equal(a["ids"][s].long(), i[:, :3])
+    for k in a:
+        assert torch.equal(a[k], b[k])
