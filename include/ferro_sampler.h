@@ -281,7 +281,7 @@ typedef struct fs_edits {
  * tokens whose edited logit is above -inf: k, min-p and top-p count those alone. A row without a candidate has token -1
  * and 0 kept (a greedy row's candidate outputs are -1 and 0); -1 ends a verification window at its row, and fs_decode_step_
  * edited appends it to the history, where the penalties ignore it. With h_params, batches that the small-k or the mid-k
- * kernel takes (fs_route_plan, fs_mid_k_plan) and that have no biases beside a softcap read their logits once, where they
+ * kernel takes (fs_route_plan, fs_mid_k_plan, and some of shorter rows with a large k) and that have no biases beside a softcap read their logits once, where they
  * are, and of masked rows only the groups of four with an allowed token; others are edited into a workspace of V * 4 bytes
  * a row first, which grows as a context's other buffers do. A call under graph capture whose workspace would have to grow
  * returns FS_E_NOMEM and leaves the capture as it was. */

@@ -341,3 +341,17 @@ def test_logprobs_of_rows_in_parts_past_the_first_round(B):
         assert torch.equal(a["ids"][s].long(), i[:, :3])
     for k in a:
         assert torch.equal(a[k], b[k])
+
+
+@pytest.mark.parametrize("B,V", [(60, 70001), (20, 140003)])
+def test_large_k_on_more_segments_than_run_at_once(B, V):
+    """k up to 2048 on rows too short for the largest segments: smaller ones, more of them than run at once; the same tokens
+    as from rows written out first (device parameters)."""
+    b = Batch(B, B, V, ("most", "few", "block"), nb=40, **dict(SETS["mid_k"], frequency_penalty=0.2))
+    b.p["top_k"] = np.exp(b.rng.uniform(0.0, np.log(2048.0), B)).astype(np.int32).clip(1, 2048)
+    b.p["top_k"][:2] = 2048
+    x = cuda(b.x)
+    out = F.sample_batch(x, b.p, b.u, b.hist, b.off, edits=b.ed)
+    assert check_rows(b, out["tok"].cpu().numpy(), out["keep"].cpu().numpy()) <= 3
+    other = F.sample_batch(x, b.p, b.u, b.hist, b.off, edits=b.ed, route="device")
+    assert torch.equal(out["tok"], other["tok"]) and torch.equal(out["keep"], other["keep"])
