@@ -397,6 +397,23 @@ int small_k_plan(int cus, int64_t B, int32_t V, int& nl, int& nseg) {
     return nl > 0 ? FS_OK : FS_E_INVALID;
 }
 
+// The same for calls under edits: the smallest segments that leave few lists to a row's end and do not crowd the tickets, two
+// workgroups per CU of 4096 logits or three of 8192 (greedy rows, whose lists are one entry: four), else 16384. Measured with
+// 4, 8 and 16 loads, k 64: 1 row of 65536 logits 9.9, 10.1, 11.2 us; 32 rows 12.6, 12.6, 13.5; 64 rows 15.5, 13.5, 14.4; 200
+// rows 31.8, 23.7, 19.3; 1 row of 151936 18.9, 11.3, 11.3; 30 rows of 262144 33.4, 19.6, 16.2; 48 rows 42.6, 26.4, 18.6; 40 of
+// 131072 22.9, 14.7, 15.4. Greedy: 1 row of 262144 6.5, 7.1, 8.5; 12 rows 14.6, 10.6, 11.1; 128 of 65536 16.9, 12.7, 13.7.
+int small_k_edited_plan(int cus, int64_t B, int32_t V, bool greedy, int& nl, int& nseg) {
+    for (const int l : {4, 8, 16}) {
+        const int64_t seg = (int64_t)fs::SK_LT * l * 4, n = ((int64_t)V + seg - 1) / seg;
+        if (n > fs::SK_MAX_SEGS) continue;
+        const int per_cu = l == 4 ? 2 : greedy ? 4 : 3;
+        nl = l;
+        nseg = (int)n;
+        if ((greedy || n <= 16) && B * n <= per_cu * (int64_t)cus) break;
+    }
+    return nl > 0 ? FS_OK : FS_E_INVALID;
+}
+
 int grow_small(fs_context* c, size_t slots, size_t rows) {
     if (c->frozen && (slots > c->sk_slots || rows > c->sk_rows)) return FS_E_NOMEM;
     if (slots > c->sk_slots) {
@@ -452,10 +469,10 @@ struct SmallKChoice {
     int nl = 0, nseg = 0;
     bool all_greedy = true, capped = false, may_pen = false;
 };
-bool small_k_choice(int cus, const fs_row_params* h, int64_t n, int64_t B, int32_t V, bool verify, SmallKChoice& c) {
+bool small_k_choice(int cus, const fs_row_params* h, int64_t n, int64_t B, int32_t V, bool verify, SmallKChoice& c,
+                    bool edited = false) {
     if (verify ? !small_k_windows(h, n, V) : !small_k_batch(h, n, V)) return false;
     if (small_k_plan(cus, B, V, c.nl, c.nseg) != FS_OK) return false;
-    if ((int64_t)fs::XCDS * c.nseg * ((B + fs::XCDS - 1) / fs::XCDS) > 0x7fffffff) return false;
     bool counts = false;
     for (int64_t b = 0; b < n; ++b) {
         const fs_row_params& p = h[b];
@@ -465,6 +482,8 @@ bool small_k_choice(int cus, const fs_row_params* h, int64_t n, int64_t B, int32
         c.may_pen |= (p.repetition_penalty != 1.0f || fp) && p.repeat_last_n != 0;
         counts |= fp && p.repeat_last_n != 0;
     }
+    if (edited && !counts) (void)small_k_edited_plan(cus, B, V, c.all_greedy, c.nl, c.nseg);
+    if ((int64_t)fs::XCDS * c.nseg * ((B + fs::XCDS - 1) / fs::XCDS) > 0x7fffffff) return false;
     return !(counts && c.nl != 4);               // count tables fit segments of 4096 logits only: the fused kernel
 }
 
@@ -504,7 +523,8 @@ int launch_small(fs_context* ctx, const fs::Args& a_in, const fs_row_params* h_p
     const bool verify = a.mode == fs::MODE_VERIFY;
     if (!ctx->seg_layout) return FS_OK;
     SmallKChoice ch;
-    if (!small_k_choice(ctx->cus, h_params, verify ? (int64_t)a.n_streams : (int64_t)a.B, a.B, a.V, verify, ch))
+    if (!small_k_choice(ctx->cus, h_params, verify ? (int64_t)a.n_streams : (int64_t)a.B, a.B, a.V, verify, ch,
+                        ed != nullptr))
         return FS_OK;
     if (ed && ed->bias_off && ch.capped) return FS_OK;     // (the softcap, late in this kernel, comes before the biases)
     const int nl = ch.nl, nseg = ch.nseg;
@@ -514,7 +534,14 @@ int launch_small(fs_context* ctx, const fs::Args& a_in, const fs_row_params* h_p
     // longer than 32 rows
     rc = grow(ctx, 0, 0, verify ? 3 * (size_t)a.n_streams : 0);
     if (rc != FS_OK) return rc;
-    rc = grow_small(ctx, (size_t)a.B * nseg, (size_t)a.B);
+    int most = nseg;
+    if (ed && !ctx->frozen) {                      // (a shape warmed up with any parameters records with others)
+        int l = 0, n = 0;
+        for (const bool greedy : {false, true})
+            if (small_k_edited_plan(ctx->cus, a.B, a.V, greedy, l, n) == FS_OK) most = std::max(most, n);
+        if (small_k_plan(ctx->cus, a.B, a.V, l, n) == FS_OK) most = std::max(most, n);
+    }
+    rc = grow_small(ctx, (size_t)a.B * most, (size_t)a.B);
     if (rc != FS_OK) return rc;
     if (capturing(st)) ctx->captured = true;
     fs::SkArgs k = row_args(ctx, a, nseg);

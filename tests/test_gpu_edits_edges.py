@@ -1,6 +1,8 @@
 """GPU: edited calls where they can go wrong - long bias lists, masks that leave the kernels' bounds without logits, capped
 rows, ties, far offsets, contexts and streams side by side."""
 
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -10,6 +12,7 @@ torch = pytest.importorskip("torch")
 
 import ferro_amd as F  # noqa: E402
 from ferro_amd import workloads as W  # noqa: E402
+from ferro_amd._lib import check, lib  # noqa: E402
 from tests import edit_util as U  # noqa: E402
 from tests.test_gpu_edits import SETS, Batch, U_pack, check_rows, cuda, lp_tolerance  # noqa: E402
 
@@ -355,3 +358,34 @@ def test_large_k_on_more_segments_than_run_at_once(B, V):
     assert check_rows(b, out["tok"].cpu().numpy(), out["keep"].cpu().numpy()) <= 3
     other = F.sample_batch(x, b.p, b.u, b.hist, b.off, edits=b.ed, route="device")
     assert torch.equal(out["tok"], other["tok"]) and torch.equal(out["keep"], other["keep"])
+
+
+@pytest.mark.parametrize("B,V", [(2, 65536), (7, 131072), (24, 65540), (40, 131072), (90, 40000), (130, 16384)])
+@pytest.mark.parametrize("name", ["greedy", "small_k"])
+def test_batches_on_every_segment_size(name, B, V):
+    """Segments of 4096, 8192 and 16384 logits, full ones and a last one of four; a context warmed up with greedy rows
+    records sampled ones, and the other way round."""
+    other = "small_k" if name == "greedy" else "greedy"
+    b = Batch(B, B, V, ("most", "few", "block"), nb=9, **SETS[name])
+    w = Batch(B, B, V, ("most", "few", "block"), nb=9, **SETS[other])
+    x, ctx = cuda(b.x), F.Context()
+    F.sample_batch(x, w.p, b.u, edits=b.ed, ctx=ctx)
+    p, u = b.p, cuda(b.u)
+    hist, off = cuda(b.hist), cuda(b.off)
+    torch.cuda.synchronize()
+    g, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    dev = torch.from_numpy(p.view(np.uint8).copy()).cuda()
+    tok = torch.full((B,), -7, dtype=torch.int32, device="cuda")
+    keep = torch.zeros(B, dtype=torch.int32, device="cuda")
+    ptr = lambda t: ctypes.c_void_p(t.data_ptr())      # noqa: E731
+    with torch.cuda.graph(g, stream=st):
+        check(lib().fs_sample_edited(ctx.h, ptr(x), x.stride(0), B, V, ptr(hist), ptr(off),
+                                     ptr(dev), p.ctypes.data_as(ctypes.c_void_p), b.ed._ref(B, B, V, x.device), ptr(u),
+                                     ptr(tok), 0, None, None, ptr(keep), ctypes.c_void_p(st.cuda_stream)), "edited")
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert check_rows(b, tok.cpu().numpy(), keep.cpu().numpy()) <= 3
+        again = F.sample_batch(x, b.p, b.u, b.hist, b.off, edits=b.ed)
+        assert torch.equal(again["tok"], tok) and torch.equal(again["keep"], keep)
+        tok.fill_(-7)
