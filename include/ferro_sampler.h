@@ -112,7 +112,8 @@ int fs_sample_batch_hp(fs_context* ctx, const float* d_logits, int64_t ld, int32
 
 /* Host-only: the small-k kernel's layout for B rows of V logits on a device with `cus` compute units: *nl float4
  * loads per thread (segments of 1024 * nl logits) and *nseg segments per row; FS_E_LIMIT when V needs more than 64
- * segments (fs_sample_batch_hp then runs fs_sample_batch). No counterpart in the reference (a planner check). */
+ * segments (fs_sample_batch_hp then runs fs_sample_batch). Calls under edits split their rows by a rule of their own. No
+ * counterpart in the reference (a planner check). */
 int fs_small_k_plan(int32_t cus, int32_t B, int32_t V, int32_t* nl, int32_t* nseg);
 
 /* Host-only: the kernel fs_sample_batch_hp (verify = 0: n = total_rows = B row records) or fs_verify_hp (verify != 0:
