@@ -205,6 +205,12 @@ void release(fs_context* c, void* p) {
     else (void)hipFree(p);
 }
 
+// A failed allocation is this call's answer, not the next launch's (whose error check would still find it).
+int no_memory() {
+    (void)hipGetLastError();
+    return FS_E_NOMEM;
+}
+
 int grow(fs_context* c, size_t slots, size_t rows, size_t streams) {
     if (c->frozen && (slots > c->cand_slots || rows > c->row_cap || streams > c->stream_cap || !c->hflag || !c->err))
         return FS_E_NOMEM;
@@ -212,29 +218,29 @@ int grow(fs_context* c, size_t slots, size_t rows, size_t streams) {
         release(c, c->cand);
         release(c, c->meta);
         c->cand = nullptr; c->meta = nullptr; c->cand_slots = 0;
-        if (hipMalloc(&c->cand, slots * fs::CAP * sizeof(uint64_t)) != hipSuccess) return FS_E_NOMEM;
-        if (hipMalloc(&c->meta, slots * 2 * sizeof(uint32_t)) != hipSuccess) return FS_E_NOMEM;
+        if (hipMalloc(&c->cand, slots * fs::CAP * sizeof(uint64_t)) != hipSuccess) return no_memory();
+        if (hipMalloc(&c->meta, slots * 2 * sizeof(uint32_t)) != hipSuccess) return no_memory();
         c->cand_slots = slots;
     }
     if (rows > c->row_cap) {
         release(c, c->rhist);
         release(c, c->rmass);
         c->rhist = nullptr; c->rmass = nullptr; c->row_cap = 0;
-        if (hipMalloc(&c->rhist, rows * fs::RBINS * sizeof(uint32_t)) != hipSuccess) return FS_E_NOMEM;
+        if (hipMalloc(&c->rhist, rows * fs::RBINS * sizeof(uint32_t)) != hipSuccess) return no_memory();
         if (hipMemset(c->rhist, 0, rows * fs::RBINS * sizeof(uint32_t)) != hipSuccess) return FS_E_HIP;
-        if (hipMalloc(&c->rmass, rows * fs::LB * sizeof(uint64_t)) != hipSuccess) return FS_E_NOMEM;
+        if (hipMalloc(&c->rmass, rows * fs::LB * sizeof(uint64_t)) != hipSuccess) return no_memory();
         if (hipMemset(c->rmass, 0, rows * fs::LB * sizeof(uint64_t)) != hipSuccess) return FS_E_HIP;
         c->row_cap = rows;
     }
     if (streams > c->stream_cap) {
         release(c, c->stream_cnt);
         c->stream_cnt = nullptr; c->stream_cap = 0;
-        if (hipMalloc(&c->stream_cnt, streams * sizeof(uint32_t)) != hipSuccess) return FS_E_NOMEM;
+        if (hipMalloc(&c->stream_cnt, streams * sizeof(uint32_t)) != hipSuccess) return no_memory();
         if (hipMemset(c->stream_cnt, 0, streams * sizeof(uint32_t)) != hipSuccess) return FS_E_HIP;
         c->stream_cap = streams;
     }
     if (!c->hflag) {
-        if (hipHostMalloc((void**)&c->hflag, sizeof(int32_t), hipHostMallocMapped) != hipSuccess) return FS_E_NOMEM;
+        if (hipHostMalloc((void**)&c->hflag, sizeof(int32_t), hipHostMallocMapped) != hipSuccess) return no_memory();
         *(volatile int32_t*)c->hflag = 0;
         if (hipHostGetDevicePointer((void**)&c->hflag_dev, c->hflag, 0) != hipSuccess) return FS_E_HIP;
     }
@@ -243,7 +249,7 @@ int grow(fs_context* c, size_t slots, size_t rows, size_t streams) {
         int32_t h[4] = {0, 0, 0, 0};
         const uint64_t fa = (uint64_t)(uintptr_t)c->hflag_dev;
         memcpy(h + 2, &fa, sizeof(fa));
-        if (hipMalloc(&c->err, sizeof(h)) != hipSuccess) return FS_E_NOMEM;
+        if (hipMalloc(&c->err, sizeof(h)) != hipSuccess) return no_memory();
         if (hipMemcpy(c->err, h, sizeof(h), hipMemcpyHostToDevice) != hipSuccess) return FS_E_HIP;
     }
     return FS_OK;
@@ -419,13 +425,13 @@ int grow_small(fs_context* c, size_t slots, size_t rows) {
     if (slots > c->sk_slots) {
         release(c, c->sk_lists);
         c->sk_lists = nullptr; c->sk_slots = 0;
-        if (hipMalloc(&c->sk_lists, slots * fs::SK_K * sizeof(uint64_t)) != hipSuccess) return FS_E_NOMEM;
+        if (hipMalloc(&c->sk_lists, slots * fs::SK_K * sizeof(uint64_t)) != hipSuccess) return no_memory();
         c->sk_slots = slots;
     }
     if (rows > c->sk_rows) {
         release(c, c->sk_ticket);
         c->sk_ticket = nullptr; c->sk_rows = 0;
-        if (hipMalloc(&c->sk_ticket, rows * sizeof(uint32_t)) != hipSuccess) return FS_E_NOMEM;
+        if (hipMalloc(&c->sk_ticket, rows * sizeof(uint32_t)) != hipSuccess) return no_memory();
         if (hipMemset(c->sk_ticket, 0, rows * sizeof(uint32_t)) != hipSuccess) return FS_E_HIP;
         c->sk_rows = rows;
     }
@@ -451,7 +457,7 @@ int greedy_params(fs_context* ctx, int64_t B, hipStream_t st) {
     release(ctx, ctx->greedy);
     ctx->greedy = nullptr;
     ctx->greedy_cap = 0;
-    if (hipMalloc(&ctx->greedy, cap * sizeof(fs_row_params)) != hipSuccess) return FS_E_NOMEM;
+    if (hipMalloc(&ctx->greedy, cap * sizeof(fs_row_params)) != hipSuccess) return no_memory();
     const int64_t blocks = std::min<int64_t>(1024, ((int64_t)cap + 255) / 256);
     hipLaunchKernelGGL(fs::greedy_params_kernel, dim3((unsigned)blocks), dim3(256), 0, st, ctx->greedy, (int64_t)cap);
     if (hipGetLastError() != hipSuccess) return FS_E_HIP;
@@ -503,6 +509,33 @@ int edit_flags(const fs::EdArgs* ed) {
     return !ed ? 0 : (ed->mask ? fs::ED_MASKS : 0) | (ed->bias_off ? fs::ED_BIASES : 0);
 }
 
+// Whether the batch fits the small-k kernel (fits; else nothing grows), and the workspace it needs there. ed: the rows'
+// masks and biases. The caller holds ctx->mu and has the context's device.
+int reserve_small(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params, const fs::EdArgs* ed, SmallKChoice& ch,
+                  bool& fits) {
+    fits = false;
+    const bool verify = a.mode == fs::MODE_VERIFY;
+    if (!ctx->seg_layout) return FS_OK;
+    if (!small_k_choice(ctx->cus, h_params, verify ? (int64_t)a.n_streams : (int64_t)a.B, a.B, a.V, verify, ch,
+                        ed != nullptr))
+        return FS_OK;
+    if (ed && ed->bias_off && ch.capped) return FS_OK;     // (the softcap, late in this kernel, comes before the biases)
+    // the error word and the verify stream counters: a 64-bit word per stream, then the 32-bit counters of streams
+    // longer than 32 rows
+    int rc = grow(ctx, 0, 0, verify ? 3 * (size_t)a.n_streams : 0);
+    if (rc != FS_OK) return rc;
+    int most = ch.nseg;
+    if (ed && !ctx->frozen) {                      // (a shape warmed up with any parameters records with others)
+        int l = 0, n = 0;
+        for (const bool greedy : {false, true})
+            if (small_k_edited_plan(ctx->cus, a.B, a.V, greedy, l, n) == FS_OK) most = std::max(most, n);
+        if (small_k_plan(ctx->cus, a.B, a.V, l, n) == FS_OK) most = std::max(most, n);
+    }
+    rc = grow_small(ctx, (size_t)a.B * most, (size_t)a.B);
+    fits = rc == FS_OK;
+    return rc;
+}
+
 // Launches the small-k kernel when the batch fits it; *used = false (nothing launched) otherwise. a.mode selects
 // sampling (h_params: B records) or verification windows (h_params: n_streams records).
 // h_params NULL: every row greedy without penalties (fs_argmax_batch without parameters): the context's greedy
@@ -521,28 +554,13 @@ int launch_small(fs_context* ctx, const fs::Args& a_in, const fs_row_params* h_p
         a.params = ctx->greedy;
     }
     const bool verify = a.mode == fs::MODE_VERIFY;
-    if (!ctx->seg_layout) return FS_OK;
     SmallKChoice ch;
-    if (!small_k_choice(ctx->cus, h_params, verify ? (int64_t)a.n_streams : (int64_t)a.B, a.B, a.V, verify, ch,
-                        ed != nullptr))
-        return FS_OK;
-    if (ed && ed->bias_off && ch.capped) return FS_OK;     // (the softcap, late in this kernel, comes before the biases)
+    bool fits = false;
+    rc = reserve_small(ctx, a, h_params, ed, ch, fits);
+    if (rc != FS_OK || !fits) return rc;
     const int nl = ch.nl, nseg = ch.nseg;
     const int64_t per_x = ((int64_t)a.B + fs::XCDS - 1) / fs::XCDS;
     const int64_t grid = (int64_t)fs::XCDS * nseg * per_x;
-    // the error word and the verify stream counters: a 64-bit word per stream, then the 32-bit counters of streams
-    // longer than 32 rows
-    rc = grow(ctx, 0, 0, verify ? 3 * (size_t)a.n_streams : 0);
-    if (rc != FS_OK) return rc;
-    int most = nseg;
-    if (ed && !ctx->frozen) {                      // (a shape warmed up with any parameters records with others)
-        int l = 0, n = 0;
-        for (const bool greedy : {false, true})
-            if (small_k_edited_plan(ctx->cus, a.B, a.V, greedy, l, n) == FS_OK) most = std::max(most, n);
-        if (small_k_plan(ctx->cus, a.B, a.V, l, n) == FS_OK) most = std::max(most, n);
-    }
-    rc = grow_small(ctx, (size_t)a.B * most, (size_t)a.B);
-    if (rc != FS_OK) return rc;
     if (capturing(st)) ctx->captured = true;
     fs::SkArgs k = row_args(ctx, a, nseg);
     k.lists = ctx->sk_lists; k.ticket = ctx->sk_ticket;
@@ -621,10 +639,7 @@ int grow_buffer(fs_context* c, T*& p, size_t& cap, size_t n, size_t per, bool ze
     size_t m = std::max(n, cap + cap / 2);
     if (hipMalloc(&q, m * per * sizeof(T)) != hipSuccess) {
         m = n;
-        if (hipMalloc(&q, m * per * sizeof(T)) != hipSuccess) {
-            (void)hipGetLastError();
-            return FS_E_NOMEM;
-        }
+        if (hipMalloc(&q, m * per * sizeof(T)) != hipSuccess) return no_memory();
     }
     if (zero && hipMemset(q, 0, m * per * sizeof(T)) != hipSuccess) {
         (void)hipFree(q);
@@ -668,20 +683,17 @@ int grow_fused(fs_context* ctx, fs::Args& a, int64_t rows, int64_t streams, int 
     return grow(ctx, (size_t)(items > 0 ? items : 1), (size_t)rows, (size_t)(streams > 0 ? 3 * streams : 1));
 }
 
-// Launches the mid-k kernel when the batch fits it; *used = false (nothing launched) otherwise. Under capture a
-// workspace that would have to grow leaves the batch to the fused kernel (no allocation in a capture that worked
-// without one), and so does one that the device has no room for.
+// Whether the batch fits the mid-k kernel (fits), and the workspace it needs there. Under capture a workspace that would
+// have to grow leaves the batch to the fused kernel (no allocation in a capture that worked without one), and so does one
+// that the device has no room for: fits is false.
 // per_cu: as launch's; the fused kernel's workspace grows as launch would grow it, so that a context warmed up with any
-// parameters of a shape allocates nothing when a call of that shape with others is recorded.
-int launch_mid(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params, hipStream_t st, bool& used, int per_cu = 2,
-               const fs::EdArgs* ed = nullptr) {
-    used = false;
-    std::lock_guard<std::mutex> g(ctx->mu);
-    int rc = device_of(ctx);
-    if (rc != FS_OK) return rc;
+// parameters of a shape allocates nothing when a call of that shape with others is recorded. The caller holds ctx->mu and
+// has the context's device.
+int reserve_mid(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params, hipStream_t st, int per_cu,
+                const fs::EdArgs* ed, MidKChoice& ch, bool& fits) {
+    fits = false;
     if (!ctx->seg_layout) return FS_OK;
     const bool verify = a.mode == fs::MODE_VERIFY;
-    MidKChoice ch;
     if (!mid_k_choice(ctx->cus, h_params, verify ? (int64_t)a.n_streams : (int64_t)a.B, a.B, a.V,
                       a.cand_ids || a.cand_probs, ed != nullptr, ch))
         return FS_OK;
@@ -689,6 +701,7 @@ int launch_mid(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params
     const size_t streams = verify ? 3 * (size_t)a.n_streams : 0;
     const bool cap = capturing(st);
     if (cap && (mid_grows(ctx, ch, (size_t)a.B) || streams > ctx->stream_cap || !ctx->err)) return FS_OK;
+    int rc = FS_OK;
     if (!cap) {
         fs::Args fused = a;
         int64_t fused_grid = 0;
@@ -700,9 +713,23 @@ int launch_mid(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params
     }
     if (rc != FS_OK) return rc;
     rc = grow_mid(ctx, ch, (size_t)a.B);
-    if (rc == FS_E_NOMEM) return FS_OK;
+    fits = rc == FS_OK;
+    return rc == FS_E_NOMEM ? FS_OK : rc;
+}
+
+// Launches the mid-k kernel when the batch fits it; *used = false (nothing launched) otherwise.
+int launch_mid(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params, hipStream_t st, bool& used, int per_cu = 2,
+               const fs::EdArgs* ed = nullptr) {
+    used = false;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    int rc = device_of(ctx);
     if (rc != FS_OK) return rc;
-    if (cap) ctx->captured = true;
+    const bool verify = a.mode == fs::MODE_VERIFY;
+    MidKChoice ch;
+    bool fits = false;
+    rc = reserve_mid(ctx, a, h_params, st, per_cu, ed, ch, fits);
+    if (rc != FS_OK || !fits) return rc;
+    if (capturing(st)) ctx->captured = true;
     fs::MkArgs m = {};
     m.a = row_args(ctx, a, ch.nseg);
     m.ctr = ctx->mk_ctr; m.qk = ctx->mk_qk; m.list = ctx->mk_list; m.spill = ctx->mk_spill;
@@ -784,11 +811,29 @@ int edit_plan(int cus, int64_t B, int32_t V, int& nseg) {
 }
 
 // The rows edited into the workspace, sampled there without penalties by whichever kernel takes them, and the call's end:
-// rows without a candidate, a window's accepted prefix. Right for every batch.
+// rows without a candidate, a window's accepted prefix. Right for every batch. Every buffer of the call, the sampling
+// kernel's among them, is there before the first launch: a call that is refused leaves nothing on its stream (or in the
+// graph that records it), and no draw is taken.
 int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params, const fs::EdArgs& ed, hipStream_t st) {
     const bool verify = a.mode == fs::MODE_VERIFY, decode = a.dmt != nullptr;
     const size_t B = (size_t)a.B, ld = ((size_t)a.V + 3) & ~(size_t)3;
+    std::unique_ptr<fs_row_params[]> h;
+    if (h_params && !verify) {                     // (a window's rows have their streams' parameters, known on the device)
+        h.reset(new (std::nothrow) fs_row_params[B]);
+        if (!h) return FS_E_NOMEM;
+        for (size_t b = 0; b < B; ++b) {
+            h[b] = h_params[b];
+            h[b].repetition_penalty = 1.0f; h[b].frequency_penalty = 0.0f; h[b].presence_penalty = 0.0f;
+            h[b].repeat_last_n = 0; h[b].penalty_from = 0; h[b].softcap = 0.0f;
+        }
+    }
+    const int per_cu = h && mixed_merges(h.get(), a.B, a.V) ? 4 : 2;
+    fs::Args s = {};
+    s.ld = (int64_t)ld; s.B = a.B; s.V = a.V; s.u = a.u; s.tok = a.tok;
+    s.kcap = a.kcap; s.cand_ids = a.cand_ids; s.cand_probs = a.cand_probs; s.keep = a.keep;
+    s.mode = fs::MODE_SAMPLE; s.eos = -1;
     int nseg = 0, nl = 0;
+    bool small = false, mid = false;               // the kernel that samples the rows (neither: the fused one)
     {
         std::lock_guard<std::mutex> g(ctx->mu);
         nl = edit_plan(ctx->cus, a.B, a.V, nseg);
@@ -799,6 +844,19 @@ int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_p
         if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_any, ctx->ed_any_rows, B, 1, true);
         if (rc == FS_OK && decode) rc = grow_buffer(ctx, ctx->ed_u, ctx->ed_u_rows, B, 1, false);
         if (rc == FS_OK && decode && !a.hist_off) rc = grow_buffer(ctx, ctx->ed_off, ctx->ed_off_rows, B + 1, 1, true);
+        if (rc == FS_OK && h) {
+            SmallKChoice sc;
+            MidKChoice mc;
+            rc = reserve_small(ctx, s, h.get(), nullptr, sc, small);
+            if (rc == FS_E_NOMEM && ctx->frozen) rc = FS_OK;       // (another kernel's workspace may be there)
+            if (rc == FS_OK && !small) rc = reserve_mid(ctx, s, h.get(), st, per_cu, nullptr, mc, mid);
+        }
+        if (rc == FS_OK && (!(small || mid) || !ctx->frozen)) {    // (a shape warmed up so records with other parameters)
+            fs::Args f = s;
+            int64_t grid = 0;
+            rc = grow_fused(ctx, f, a.B, 0, per_cu, &grid);
+            if ((small || mid) && (rc == FS_E_NOMEM || rc == FS_E_INVALID)) rc = FS_OK;
+        }
         if (rc != FS_OK) return rc;
     }
     fs::EditArgs e = {};
@@ -812,10 +870,7 @@ int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_p
         return rc;
     };
 
-    fs::Args s = {};
-    s.logits = ctx->ed_rows; s.ld = (int64_t)ld; s.B = a.B; s.V = a.V; s.params = ctx->ed_params; s.u = a.u; s.tok = a.tok;
-    s.kcap = a.kcap; s.cand_ids = a.cand_ids; s.cand_probs = a.cand_probs; s.keep = a.keep;
-    s.mode = fs::MODE_SAMPLE; s.eos = -1;
+    s.logits = ctx->ed_rows; s.params = ctx->ed_params;
     if (decode) {
         hipLaunchKernelGGL(fs::drng_draw_kernel, dim3((unsigned)((B + 63) / 64)), dim3(64), 0, st, a.dmt, a.didx, a.B,
                            (const int64_t*)nullptr, a.params, ctx->ed_u, 0, ctx->err);
@@ -824,20 +879,9 @@ int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_p
     }
     int rc = FS_OK;
     bool used = false;
-    std::unique_ptr<fs_row_params[]> h;
-    if (h_params && !verify) {                     // (a window's rows have their streams' parameters, known on the device)
-        h.reset(new (std::nothrow) fs_row_params[B]);
-        if (!h) return failed(FS_E_NOMEM);
-        for (size_t b = 0; b < B; ++b) {
-            h[b] = h_params[b];
-            h[b].repetition_penalty = 1.0f; h[b].frequency_penalty = 0.0f; h[b].presence_penalty = 0.0f;
-            h[b].repeat_last_n = 0; h[b].penalty_from = 0; h[b].softcap = 0.0f;
-        }
-        rc = launch_small(ctx, s, h.get(), st, used);
-        if (rc == FS_OK && !used) rc = launch_mid(ctx, s, h.get(), st, used, mixed_merges(h.get(), a.B, a.V) ? 4 : 2);
-        if (rc < 0) return failed(rc);
-    }
-    if (!used) rc = launch(ctx, s, a.B, 0, st, h ? (mixed_merges(h.get(), a.B, a.V) ? 4 : 2) : 2);
+    if (small) rc = launch_small(ctx, s, h.get(), st, used);
+    else if (mid) rc = launch_mid(ctx, s, h.get(), st, used, per_cu);
+    if (rc == FS_OK && !used) rc = launch(ctx, s, a.B, 0, st, per_cu);
     if (rc < 0) return failed(rc);
 
     fs::EditEnd f = {};
