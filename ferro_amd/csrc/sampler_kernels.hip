@@ -123,7 +123,7 @@ __global__ __launch_bounds__(64) void drng_skip_kernel(uint64_t* mts, int32_t* i
 
 // ================================================================================================ host side
 struct fs_context {
-    std::mutex mu;
+    std::recursive_mutex mu;   // (an edited call holds it while the launches it is made of take it)
     int device = -1;
     int cus = 0;               // compute units of the device
     int xccs = 0;              // XCDs of the device (hipDeviceAttributeNumberOfXccs)
@@ -543,7 +543,7 @@ int reserve_small(fs_context* ctx, const fs::Args& a, const fs_row_params* h_par
 int launch_small(fs_context* ctx, const fs::Args& a_in, const fs_row_params* h_params, hipStream_t st, bool& used,
                  const fs::EdArgs* ed = nullptr) {
     used = false;
-    std::lock_guard<std::mutex> g(ctx->mu);
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
     int rc = device_of(ctx);
     if (rc != FS_OK) return rc;
     fs::Args a = a_in;
@@ -721,7 +721,7 @@ int reserve_mid(fs_context* ctx, const fs::Args& a, const fs_row_params* h_param
 int launch_mid(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params, hipStream_t st, bool& used, int per_cu = 2,
                const fs::EdArgs* ed = nullptr) {
     used = false;
-    std::lock_guard<std::mutex> g(ctx->mu);
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
     int rc = device_of(ctx);
     if (rc != FS_OK) return rc;
     const bool verify = a.mode == fs::MODE_VERIFY;
@@ -747,7 +747,7 @@ int launch_mid(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params
 }
 
 int launch(fs_context* ctx, fs::Args a, int64_t rows, int64_t streams, hipStream_t st, int per_cu = 2) {
-    std::lock_guard<std::mutex> g(ctx->mu);
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
     int rc = device_of(ctx);
     if (rc != FS_OK) return rc;
     int64_t seg_grid = 0;
@@ -781,20 +781,21 @@ int launch(fs_context* ctx, fs::Args a, int64_t rows, int64_t streams, hipStream
 }
 
 // ---- calls under edits (fs_sample_edited, fs_verify_edited, fs_decode_step_edited)
-// For such a call's time: the context is on the current device, and no workspace grows where the call is being recorded (an
-// allocation would end the capture).
+// For such a call's time: the context's lock is held (a composed call's launches follow one another and bind one set of
+// workspace pointers, whatever other host threads enqueue on the context), the context is on the current device, and no
+// workspace grows where the call is being recorded (an allocation would end the capture).
 struct Edited {
+    std::lock_guard<std::recursive_mutex> lock;
     fs_context* c;
     int rc = FS_OK;
-    Edited(fs_context* ctx, hipStream_t st) : c(ctx) {
-        std::lock_guard<std::mutex> g(c->mu);
+    Edited(fs_context* ctx, hipStream_t st) : lock(ctx->mu), c(ctx) {
         rc = device_of(c);
         int dev = -1;
         if (rc == FS_OK && hipGetDevice(&dev) != hipSuccess) rc = FS_E_HIP;
         if (rc == FS_OK && dev != c->device) rc = FS_E_INVALID;
         if (rc == FS_OK && capturing(st)) c->frozen = c->captured = true;
     }
-    ~Edited() { c->frozen = false; }
+    ~Edited() { c->frozen = false; }               // (before the lock goes)
 };
 
 // Groups of four logits per thread and segments per row of the edit kernel: the largest segments that still give every CU
@@ -813,7 +814,7 @@ int edit_plan(int cus, int64_t B, int32_t V, int& nseg) {
 // The rows edited into the workspace, sampled there without penalties by whichever kernel takes them, and the call's end:
 // rows without a candidate, a window's accepted prefix. Right for every batch. Every buffer of the call, the sampling
 // kernel's among them, is there before the first launch: a call that is refused leaves nothing on its stream (or in the
-// graph that records it), and no draw is taken.
+// graph that records it), and no draw is taken. Inside an Edited.
 int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_params, const fs::EdArgs& ed, hipStream_t st) {
     const bool verify = a.mode == fs::MODE_VERIFY, decode = a.dmt != nullptr;
     const size_t B = (size_t)a.B, ld = ((size_t)a.V + 3) & ~(size_t)3;
@@ -832,33 +833,30 @@ int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_p
     s.ld = (int64_t)ld; s.B = a.B; s.V = a.V; s.u = a.u; s.tok = a.tok;
     s.kcap = a.kcap; s.cand_ids = a.cand_ids; s.cand_probs = a.cand_probs; s.keep = a.keep;
     s.mode = fs::MODE_SAMPLE; s.eos = -1;
-    int nseg = 0, nl = 0;
     bool small = false, mid = false;               // the kernel that samples the rows (neither: the fused one)
-    {
-        std::lock_guard<std::mutex> g(ctx->mu);
-        nl = edit_plan(ctx->cus, a.B, a.V, nseg);
-        if ((int64_t)a.B * nseg > 0x7fffffff) return FS_E_INVALID;
-        int rc = grow(ctx, 0, 0, 0);
-        if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_rows, ctx->ed_logits, B * ld, 1, false);
-        if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_params, ctx->ed_param_rows, B, 1, false);
-        if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_any, ctx->ed_any_rows, B, 1, true);
-        if (rc == FS_OK && decode) rc = grow_buffer(ctx, ctx->ed_u, ctx->ed_u_rows, B, 1, false);
-        if (rc == FS_OK && decode && !a.hist_off) rc = grow_buffer(ctx, ctx->ed_off, ctx->ed_off_rows, B + 1, 1, true);
-        if (rc == FS_OK && h) {
-            SmallKChoice sc;
-            MidKChoice mc;
-            rc = reserve_small(ctx, s, h.get(), nullptr, sc, small);
-            if (rc == FS_E_NOMEM && ctx->frozen) rc = FS_OK;       // (another kernel's workspace may be there)
-            if (rc == FS_OK && !small) rc = reserve_mid(ctx, s, h.get(), st, per_cu, nullptr, mc, mid);
-        }
-        if (rc == FS_OK && (!(small || mid) || !ctx->frozen)) {    // (a shape warmed up so records with other parameters)
-            fs::Args f = s;
-            int64_t grid = 0;
-            rc = grow_fused(ctx, f, a.B, 0, per_cu, &grid);
-            if ((small || mid) && (rc == FS_E_NOMEM || rc == FS_E_INVALID)) rc = FS_OK;
-        }
-        if (rc != FS_OK) return rc;
+    int nseg = 0;
+    const int nl = edit_plan(ctx->cus, a.B, a.V, nseg);
+    if ((int64_t)a.B * nseg > 0x7fffffff) return FS_E_INVALID;
+    int rc = grow(ctx, 0, 0, 0);
+    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_rows, ctx->ed_logits, B * ld, 1, false);
+    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_params, ctx->ed_param_rows, B, 1, false);
+    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->ed_any, ctx->ed_any_rows, B, 1, true);
+    if (rc == FS_OK && decode) rc = grow_buffer(ctx, ctx->ed_u, ctx->ed_u_rows, B, 1, false);
+    if (rc == FS_OK && decode && !a.hist_off) rc = grow_buffer(ctx, ctx->ed_off, ctx->ed_off_rows, B + 1, 1, true);
+    if (rc == FS_OK && h) {
+        SmallKChoice sc;
+        MidKChoice mc;
+        rc = reserve_small(ctx, s, h.get(), nullptr, sc, small);
+        if (rc == FS_E_NOMEM && ctx->frozen) rc = FS_OK;       // (another kernel's workspace may be there)
+        if (rc == FS_OK && !small) rc = reserve_mid(ctx, s, h.get(), st, per_cu, nullptr, mc, mid);
     }
+    if (rc == FS_OK && (!(small || mid) || !ctx->frozen)) {    // (a shape warmed up so records with other parameters)
+        fs::Args f = s;
+        int64_t grid = 0;
+        rc = grow_fused(ctx, f, a.B, 0, per_cu, &grid);
+        if ((small || mid) && (rc == FS_E_NOMEM || rc == FS_E_INVALID)) rc = FS_OK;
+    }
+    if (rc != FS_OK) return rc;
     fs::EditArgs e = {};
     e.logits = a.logits; e.type = FS_F32; e.ld = a.ld; e.B = a.B; e.V = a.V; e.nseg = nseg;
     e.hist = a.hist; e.hist_off = a.hist_off; e.params = a.params; e.ed = ed;
@@ -877,7 +875,6 @@ int launch_composed(fs_context* ctx, const fs::Args& a, const fs_row_params* h_p
         if (hipGetLastError() != hipSuccess) return failed(FS_E_HIP);
         s.u = ctx->ed_u;
     }
-    int rc = FS_OK;
     bool used = false;
     if (small) rc = launch_small(ctx, s, h.get(), st, used);
     else if (mid) rc = launch_mid(ctx, s, h.get(), st, used, per_cu);
@@ -1193,7 +1190,7 @@ int fs_sample_batch_static(fs_context* ctx, const float* d_logits, int64_t ld, i
     a.u = d_u; a.tok = d_tok; a.kcap = kcap; a.cand_ids = d_cand_ids; a.cand_probs = d_cand_probs; a.keep = d_keep;
     a.mode = fs::MODE_SAMPLE; a.eos = -1;
     const hipStream_t st = (hipStream_t)stream;
-    std::lock_guard<std::mutex> g(ctx->mu);
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
     rc = device_of(ctx);
     if (rc != FS_OK) return rc;
     int dev = -1;
@@ -1321,15 +1318,11 @@ int fs_edit_batch(fs_context* ctx, const void* d_logits, int32_t type, int64_t l
         const uintptr_t o0 = (uintptr_t)d_out, o1 = o0 + ((size_t)(B - 1) * (size_t)out_ld + (size_t)V) * sizeof(float);
         if (i0 < o1 && o0 < i1) return FS_E_INVALID;
     }
-    int nl = 0;
     const Edited call(ctx, (hipStream_t)stream);
     if (call.rc != FS_OK) return call.rc;
-    {
-        std::lock_guard<std::mutex> g(ctx->mu);
-        rc = grow(ctx, 0, 0, 0);                               // the error word
-        if (rc != FS_OK) return rc;
-        nl = edit_plan(ctx->cus, B, V, e.nseg);
-    }
+    rc = grow(ctx, 0, 0, 0);                                   // the error word
+    if (rc != FS_OK) return rc;
+    const int nl = edit_plan(ctx->cus, B, V, e.nseg);
     if ((int64_t)B * e.nseg > 0x7fffffff) return FS_E_INVALID;
     e.logits = d_logits; e.type = type; e.ld = ld; e.B = B; e.V = V;
     e.hist = d_hist; e.hist_off = d_hist_off; e.params = d_params;
@@ -1352,7 +1345,6 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
     const int top = d_top_ids || d_top_lp ? n : 0;
     const Edited call(ctx, st);
     if (call.rc != FS_OK) return call.rc;
-    std::lock_guard<std::mutex> g(ctx->mu);
     a.nseg = logprob_parts(ctx, B, V, type);
     if (((int64_t)B + fs::XCDS) * a.nseg > 0x7fffffff) return FS_E_INVALID;
     const size_t segs = (size_t)B * a.nseg;
@@ -1377,7 +1369,7 @@ int fs_penalize_batch(fs_context* ctx, float* d_logits, int64_t ld, int32_t B, i
     const int64_t nchunk = ((int64_t)V + fs::PEN_CHUNK - 1) / fs::PEN_CHUNK;
     if ((int64_t)B * nchunk > 0x7fffffff) return FS_E_INVALID;
     {
-        std::lock_guard<std::mutex> g(ctx->mu);
+        std::lock_guard<std::recursive_mutex> g(ctx->mu);
         rc = grow(ctx, 0, 0, 0);
         if (rc != FS_OK) return rc;
     }
@@ -1413,7 +1405,7 @@ int fs_hist_append(fs_context* ctx, int32_t n_streams, const int32_t* d_hist, co
     if (out_cap > 0 && !d_out_hist) return FS_E_INVALID;
     if (d_out_hist_off == d_hist_off || (d_out_hist && d_out_hist == d_hist)) return FS_E_INVALID;   // out of place
     {
-        std::lock_guard<std::mutex> g(ctx->mu);
+        std::lock_guard<std::recursive_mutex> g(ctx->mu);
         const int rc = grow(ctx, 1, 1, 1);               // the device error word
         if (rc != FS_OK) return rc;
     }
@@ -1424,7 +1416,7 @@ int fs_hist_append(fs_context* ctx, int32_t n_streams, const int32_t* d_hist, co
 int fs_device_error(fs_context* ctx, void* stream, int32_t* bits) {
     if (!ctx || !bits) return FS_E_INVALID;
     *bits = 0;
-    std::lock_guard<std::mutex> g(ctx->mu);
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
     if (!ctx->err && ctx->static_dev < 0) return FS_OK;
     if (hipStreamSynchronize((hipStream_t)stream) != hipSuccess) return FS_E_HIP;
     if (ctx->err) {
@@ -1480,7 +1472,7 @@ int fs_plan_layout(int32_t cus, int32_t xccs, int32_t B, int32_t V, int32_t stat
 
 int fs_error_word(fs_context* ctx, const int32_t** d_bits) {
     if (!ctx || !d_bits) return FS_E_INVALID;
-    std::lock_guard<std::mutex> g(ctx->mu);
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
     const int rc = grow(ctx, 0, 0, 0);
     if (rc != FS_OK) return rc;
     *d_bits = ctx->err;
@@ -1489,7 +1481,7 @@ int fs_error_word(fs_context* ctx, const int32_t** d_bits) {
 
 int fs_set_wait_limit(fs_context* ctx, uint32_t polls) {
     if (!ctx) return FS_E_INVALID;
-    std::lock_guard<std::mutex> g(ctx->mu);
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
     ctx->merge_spins = polls == FS_WAIT_GIVE_UP ? 0u : (polls ? polls : fs::MERGE_SPINS);
     return FS_OK;
 }
@@ -1666,7 +1658,7 @@ int fs_drng_error(fs_drng* r, void* stream, int32_t* bits) {
 // entries, TRACE_W per workgroup); a grid larger than the buffer runs untraced.
 int fs_trace_set(fs_context* ctx, uint64_t* d_buf, int64_t cap) {
     if (!ctx || cap < 0) return FS_E_INVALID;
-    std::lock_guard<std::mutex> g(ctx->mu);
+    std::lock_guard<std::recursive_mutex> g(ctx->mu);
     ctx->trace = d_buf;
     ctx->trace_cap = d_buf ? cap : 0;
     return FS_OK;

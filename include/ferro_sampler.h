@@ -9,7 +9,8 @@
  *   - work is enqueued asynchronously on `stream` (a hipStream_t; NULL = the default stream);
  *   - the return value is FS_OK or a negative FS_E_* code; nothing throws across the ABI;
  *   - a context may be used from any thread, but calls on one context must not overlap in time (they share its
- *     device workspace): serialise them on one stream, or use one context per stream;
+ *     device workspace): serialise them on one stream, or use one context per stream. Host threads may make calls on one
+ *     context and one stream at the same time: each call's launches stay together;
  *   - logits rows are fp32, row b starts at d_logits + b*ld, ld >= V, ld % 4 == 0, d_logits 16-byte aligned;
  *     only elements [0, V) of each row are read. Logits are read only: the penalty is applied on the fly and
  *     never written back (ferro's sample() penalises its host row in place).

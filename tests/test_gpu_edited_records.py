@@ -1,6 +1,7 @@
 """GPU: edited calls recorded into graphs on contexts that were warmed up with other calls - those that are refused leave
 nothing behind, the others replay like the eager call."""
 import ctypes
+import threading
 
 import numpy as np
 import pytest
@@ -115,3 +116,43 @@ def test_a_shape_warmed_up_with_one_kind_of_parameters_records_the_other(first):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+def test_two_threads_on_one_context_and_stream():
+    """Host calls that overlap on one context, their work in the order of one stream: composed calls of two threads, each
+    with rows, masks and biases of its own, do not take each other's edited rows."""
+    ctx = F.Context()
+    st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    ptr = lambda t: ctypes.c_void_p(t.data_ptr())              # noqa: E731
+
+    def worker(seed):
+        """Calls of growing sizes (the workspaces are replaced under the other thread) and what they have to give."""
+        work = []
+        for i, (B, V) in enumerate(((3, 4000), (9, 8000), (20, 12000), (40, 16000))):
+            s = Step(seed + i, B, V, **dict(COMPOSED, top_k=40 if i % 2 else 0))
+            u = cuda(np.random.default_rng(seed + i).random(B))
+            want = F.sample_batch(s.x, s.p, u, edits=s.ed, ctx=F.Context())["tok"]
+            work.append((s, u, want))
+
+        def run(out):
+            for s, u, want in work:
+                B, V = s.x.shape
+                for _ in range(10):
+                    tok = torch.full((B,), -7, dtype=torch.int32, device="cuda")
+                    rc = lib().fs_sample_edited(ctx.h, ptr(s.x), V, B, V, None, None, ptr(s.dev), s.p.ctypes.data_as(ctypes.c_void_p),
+                                                s.ed._ref(B, B, V, s.x.device), ptr(u), ptr(tok), 0, None, None, None, st)
+                    out.append((rc, tok, want))
+        return run
+
+    runs, outs = [worker(100), worker(200)], ([], [])
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=r, args=(o,)) for r, o in zip(runs, outs)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for out in outs:
+        assert len(out) == 40
+        for rc, tok, want in out:
+            assert rc == 0 and torch.equal(tok, want)
