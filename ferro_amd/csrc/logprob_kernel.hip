@@ -8,7 +8,10 @@
 // requested before the present one is worked on. Every wave works by itself until its part ends (no barrier in between):
 //   - the sum: exponentials of c (x - m), c = log2 e / T and m the wave's largest x so far (the largest term is 1, exactly).
 //     A chunk's 16 or 32 terms of a lane are added in fp32, chunks in fp64, and a new m scales the lanes' sums in fp64; a
-//     subtraction, a product, an exponential and an addition a logit;
+//     subtraction, a product, an exponential and an addition a logit. A chunk with a term that is 1 is added in fp64
+//     throughout: beside a 1, fp32 loses what a near-certain token's log-probability consists of (1 and e^-18 in one lane:
+//     0 for -1.5e-8). 1024 rows of 151936 bf16 with heavy tails, about 3.5 of 19 chunks: 62.0 us with fp32 alone, 63.8 so,
+//     64.8 with every chunk in fp64;
 //   - a chunk whose sum is NaN (NaN or infinite logits) is added again with NaN left out; once the largest logit is
 //     infinite its tokens are counted instead;
 //   - the n largest: a bound that n of the wave's 64 lane maxima so far reach (bisected with a compare a step; sorting them
@@ -214,24 +217,35 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
 #pragma unroll
             for (int q = 0; q < NL; ++q) cm = lp_max3(lp_max3(cm, x[q][0], x[q][1]), x[q][2], x[q][3]);
         };
-        auto add = [&]() {
-            if (__ballot(cm > mx) != 0ull) {
-                const float m = wave_allreduce(cm, fmx);
-                sum *= exp(((double)mx - (double)m) / (double)T);
-                mx = m;
+        auto add = [&]() {                                     // the lane's terms
+            if (__ballot(cm >= mx) != 0ull) {                  // one of them is 1 (the first chunk, and few others)
+                float m = wave_allreduce(cm, fmx);
+                if (__ballot(m > mx) != 0ull) {
+                    if (__ballot(sum != 0.0) != 0ull) sum *= exp(((double)mx - (double)m) / (double)T);
+                    mx = m;
+                }
+                asm volatile("" : "+v"(m));                    // (differences shared with the other branch are spilled)
+                double d[2] = {0.0, 0.0};
+#pragma unroll
+                for (int q = 0; q < NL; ++q) {
+#pragma unroll
+                    for (int c_ = 0; c_ < 4; ++c_) d[c_ & 1] += (double)__builtin_amdgcn_exp2f((x[q][c_] - m) * c2);
+                    __builtin_amdgcn_sched_barrier(0);         // (all exponentials at once need more registers)
+                }
+                return d[0] + d[1];
             }
             float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int q = 0; q < NL; ++q) {
 #pragma unroll
                 for (int c_ = 0; c_ < 4; ++c_) e[c_] += __builtin_amdgcn_exp2f((x[q][c_] - mx) * c2);
-                __builtin_amdgcn_sched_barrier(0);             // (all exponentials at once need more registers)
+                __builtin_amdgcn_sched_barrier(0);
             }
-            return (e[0] + e[1]) + (e[2] + e[3]);
+            return (double)((e[0] + e[1]) + (e[2] + e[3]));
         };
         lane_max();
-        float e = add();
-        if (__ballot(!(e < __builtin_huge_valf()) || cm != cm) != 0ull) {    // NaN or infinite logits
+        double e = add();
+        if (__ballot(!(e < __builtin_huge_val()) || cm != cm) != 0ull) {    // NaN or infinite logits
 #pragma unroll
             for (int q = 0; q < NL; ++q)
 #pragma unroll
@@ -239,14 +253,15 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
             lane_max();
             e = add();
             if (!(mx < __builtin_huge_valf())) {
-                e = 0.0f;
+                float ones = 0.0f;
 #pragma unroll
                 for (int q = 0; q < NL; ++q)
 #pragma unroll
-                    for (int c_ = 0; c_ < 4; ++c_) e += x[q][c_] == mx ? 1.0f : 0.0f;
+                    for (int c_ = 0; c_ < 4; ++c_) ones += x[q][c_] == mx ? 1.0f : 0.0f;
+                e = (double)ones;
             }
         }
-        sum += (double)e;
+        sum += e;
         if (has && __ballot(cm > xv) != 0ull) {
 #pragma unroll
             for (int q = 0; q < NL; ++q)

@@ -315,7 +315,7 @@ int fs_edit_batch(fs_context* ctx, const void* d_logits, int32_t type, int64_t l
  * whose logit is NaN or -inf, or that is outside [0, V) has -inf and rank 0; places past a row's tokens have id -1 and
  * -inf. Where the largest logit is +inf, its tokens share the probability. n <= FS_MAX_TOP; each output may be NULL
  * (d_lp and d_rank need d_tok). Rows and types as in fs_edit_batch. A lane's 16 or 32 exponentials of a 16 KB chunk are added in
- * fp32, those sums in fp64. */
+ * fp32 (in fp64 where the largest logit so far is among the wave's), those sums in fp64. */
 #define FS_MAX_TOP 64
 int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld, int32_t B, int32_t V,
                 const fs_row_params* d_params, const fs_edits* edits, const int32_t* d_tok, int32_t n, float* d_lp,
