@@ -163,7 +163,11 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
         if (!(T > 0.0f)) T = 1.0f;                             // greedy rows: the distribution itself
     }
     auto fmx = [](float u, float v) { return fmaxf(u, v); };
-    const float c2 = (float)(1.4426950408889634 / (double)T);
+    // Where fp32 holds neither log2 e / T nor what a difference past its range comes to, the terms' arguments are fp64. (T
+    // infinite: a c that takes every finite difference to 0, and -inf to -inf)
+    const double c2d = fmax(1.4426950408889634 / (double)T, 1e-300);
+    const float c2 = (float)c2d;
+    const bool far = !(T >= 0x1p-100f && T <= 0x1p100f);
     // the chosen token's logit (NaN: it takes no part), and what the others are compared with
     float xv = __builtin_nanf("");
     if (t >= 0 && t < V) {
@@ -218,14 +222,26 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
             for (int q = 0; q < NL; ++q) cm = lp_max3(lp_max3(cm, x[q][0], x[q][1]), x[q][2], x[q][3]);
         };
         auto add = [&]() {                                     // the lane's terms
-            if (__ballot(cm >= mx) != 0ull) {                  // one of them is 1 (the first chunk, and few others)
+            if (__ballot(cm >= mx) != 0ull || far) {           // one of them is 1 (the first chunk, and few others)
                 float m = wave_allreduce(cm, fmx);
                 if (__ballot(m > mx) != 0ull) {
-                    if (__ballot(sum != 0.0) != 0ull) sum *= exp(((double)mx - (double)m) / (double)T);
+                    if (__ballot(sum != 0.0) != 0ull)
+                        sum *= m < __builtin_huge_valf() ? exp(((double)mx - (double)m) / (double)T) : 0.0;
                     mx = m;
                 }
+                m = mx;
                 asm volatile("" : "+v"(m));                    // (differences shared with the other branch are spilled)
                 double d[2] = {0.0, 0.0};
+                if (far) {
+#pragma unroll
+                    for (int q = 0; q < NL; ++q) {
+#pragma unroll
+                        for (int c_ = 0; c_ < 4; ++c_)
+                            d[c_ & 1] += (double)__builtin_amdgcn_exp2f((float)(((double)x[q][c_] - (double)m) * c2d));
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    return d[0] + d[1];
+                }
 #pragma unroll
                 for (int q = 0; q < NL; ++q) {
 #pragma unroll
@@ -448,7 +464,8 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
     ab = wave_allreduce(ab, addu);
     const double z = log(S);                                   // (no token takes part: not used)
     auto lp_of = [&](float v) {
-        return v > LP_NONE ? (float)((v == M ? 0.0 : ((double)v - (double)M) / (double)T) - z) : LP_NONE;
+        if (!(v > LP_NONE) || (v < M && !(M < __builtin_huge_valf()))) return LP_NONE;
+        return (float)((v == M ? 0.0 : ((double)v - (double)M) / (double)T) - z);
     };
     if (lane == 0) {
         if (a.lp) a.lp[row] = lp_of(xv);

@@ -10,6 +10,8 @@ torch = pytest.importorskip("torch")
 
 import ferro_amd as F  # noqa: E402
 from ferro_amd import workloads as W  # noqa: E402
+from tests.edit_util import logprob_row  # noqa: E402
+from tests.test_gpu_edits import lp_tolerance  # noqa: E402
 
 DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 U = 2.0 ** -24
@@ -87,3 +89,40 @@ def test_near_certain_tokens_among_noise():
             for r in range(4):
                 want = lp_of_largest(y[r].cpu().numpy())
                 assert abs(float(out["lp"][r]) - want) <= near_certain_tolerance(want), (V, up, r, float(out["lp"][r]), want)
+
+
+TINY = np.float32(2.0 ** -149)
+
+
+@pytest.mark.parametrize("T", [float(TINY), 1e-42, 2.0 ** -127, 1e-33, 1e33, 3e38, math.inf])
+@pytest.mark.parametrize("V", [5, 4096, 30011])
+def test_log_probabilities_at_the_ends_of_the_temperatures(T, V):
+    """Temperatures whose reciprocal, or whose share of the logits' differences, fp32 does not hold; infinite ones (every
+    token that takes part is equally likely)."""
+    T = float(np.float32(T))
+    rng = np.random.default_rng(V)
+    x = (rng.standard_normal((7, V)) * 3).astype(np.float32)
+    x[1, 2:] = x[1, 0]                                         # ties
+    x[2] = np.where(np.arange(V) % 3 == 0, 3e38, -3e38)        # a difference that fp32 does not hold
+    x[3, ::2] = np.nan
+    x[4] = np.arange(V) * np.float32(1e-40)                    # and differences below its normal numbers
+    x[5, ::2] = -np.inf
+    x[6, 3] = np.inf
+    allowed = rng.random((7, V)) < 0.8
+    allowed[:, :4] = True
+    ed = F.Edits(mask=F.Edits.pack(allowed))
+    p = W.make_params(7, temperature=T, repetition_penalty=1.0)
+    tok = np.array([1, 1, 1, 1, 2, 1, 3], np.int32)
+    n = min(V, 4)
+    for dtype in (torch.float32, torch.bfloat16):
+        t = torch.from_numpy(x).cuda().to(dtype)
+        xs = t.float().cpu().numpy()
+        out = {k: v.cpu().numpy() for k, v in F.logprobs(t, tok, n, params=p, edits=ed).items()}
+        for r in range(7):
+            lp, rank, ids, top = logprob_row(xs[r], int(tok[r]), n, T=T, allowed=allowed[r])
+            assert out["ids"][r].tolist() == ids.tolist() and int(out["rank"][r]) == rank, r
+            for got, want in zip([out["lp"][r], *out["top"][r]], [lp, *top]):
+                if want < -3.4028235e38:
+                    assert got == -math.inf, (r, got, want)
+                else:
+                    assert abs(float(got) - want) <= lp_tolerance(want), (r, got, want)
