@@ -262,7 +262,9 @@ class Edits:
     t // 32 is set (as grammar engines write them; `pack` makes them from truth values). mask_of: each logits row's mask,
     negative: every token is allowed (default: row r takes mask r). bias: one {token: bias} per record, or CSR (ids,
     values, offsets) with ids ascending within a record; a record per row, per stream in verify. Arrays go to `device`
-    here; device tensors are used in place, so a program may write the next step's masks into them."""
+    here. Device tensors are read by each call, so a program may write the next step's masks into them: in place where
+    they are packed int32 words (rows any stride apart), int32 mask_of and ids, float32 values and int64 offsets, else
+    converted by every call."""
 
     def __init__(self, mask=None, mask_of=None, bias=None, device=None):
         dev = torch.device("cuda" if device is None else device)
@@ -271,7 +273,9 @@ class Edits:
             dev = next((t.device for t in given if isinstance(t, torch.Tensor) and t.is_cuda), dev)
         if dev.type == "cuda" and dev.index is None:
             dev = torch.device("cuda", torch.cuda.current_device())
+        self.device = dev
         self.mask = self.mask_of = self.bias_ids = self.bias = self.bias_off = None
+        self._given = {}                                      # device tensors that each call converts
         if mask is not None:
             if isinstance(mask, np.ndarray) and mask.dtype == np.uint32:
                 mask = mask.view(np.int32)
@@ -280,39 +284,62 @@ class Edits:
                 mask = mask.view(torch.int32)
             if mask.dtype != torch.int32 or mask.dim() not in (1, 2):
                 raise SamplerError("masks must be int32 or uint32 words [n, W]")
-            mask = (mask.unsqueeze(0) if mask.dim() == 1 else mask).to(dev)
-            if mask.shape[1] > 1 and mask.stride(1) != 1 or (mask.shape[0] > 1 and mask.stride(0) < mask.shape[1]):
-                mask = mask.contiguous()
-            self.mask = mask
+            self._take("mask", mask.unsqueeze(0) if mask.dim() == 1 else mask)
         if mask_of is not None:
             if mask is None:
                 raise SamplerError("mask_of needs masks")
-            self.mask_of = _dev(mask_of, torch.int32, dev)
+            self._take("mask_of", mask_of)
         if bias is not None:
             if not isinstance(bias, tuple):
                 bias = self._csr(bias)
             ids, val, off = bias
             if not any(isinstance(t, torch.Tensor) and t.is_cuda for t in bias):
                 self._check(np.asarray(ids, np.int64), np.asarray(val), np.asarray(off, np.int64))
-            self.bias_ids, self.bias = _dev(ids, torch.int32, dev), _dev(val, torch.float32, dev)
-            self.bias_off = _dev(off, torch.int64, dev)
+            self._take("bias_ids", ids)
+            self._take("bias", val)
+            self._take("bias_off", off)
             if self.bias_ids.numel() != self.bias.numel() or self.bias_off.numel() < 1:
                 raise SamplerError("biases are CSR lists (ids, values, offsets)")
-            if self.bias_ids.numel() == 0:                    # no bias at all: valid pointers, never read
-                self.bias_ids = torch.zeros(1, dtype=torch.int32, device=dev)
-                self.bias = torch.zeros(1, dtype=torch.float32, device=dev)
-        self.device = dev
-        self.c = FsEdits()
-        if self.mask is not None:
-            if self.mask.numel() == 0:                        # no mask at all: a valid pointer, never read
-                self._no_mask = torch.zeros(1, dtype=torch.int32, device=dev)
-            self.c.d_mask = (self.mask if self.mask.numel() else self._no_mask).data_ptr()
-            self.c.mask_ld = self.mask.stride(0) if self.mask.shape[0] > 1 else self.mask.shape[1]
-            self.c.n_masks = self.mask.shape[0]
-            self.c.d_mask_of = self.mask_of.data_ptr() if self.mask_of is not None else None
-        if self.bias_off is not None:
-            self.c.d_bias_ids, self.c.d_bias = self.bias_ids.data_ptr(), self.bias.data_ptr()
-            self.c.d_bias_off = self.bias_off.data_ptr()
+        self.c = self._struct(self._held())
+
+    def _as(self, name, x):
+        """The array or tensor as the kernels read it."""
+        if name != "mask":
+            return _dev(x, {"bias": torch.float32, "bias_off": torch.int64}.get(name, torch.int32), self.device)
+        x = x.to(self.device)
+        packed = x.shape[1] <= 1 or x.stride(1) == 1
+        return x if packed and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
+
+    def _take(self, name, x):
+        t = self._as(name, x)
+        setattr(self, name, t)
+        if isinstance(x, torch.Tensor) and x.device.type == self.device.type and t.data_ptr() != x.data_ptr():
+            self._given[name] = x
+
+    def _held(self):
+        return {n: getattr(self, n) for n in ("mask", "mask_of", "bias_ids", "bias", "bias_off")
+                if getattr(self, n) is not None}
+
+    def _struct(self, held):
+        """The fs_edits of device tensors, which it keeps."""
+        c = FsEdits()
+        c.tensors = list(held.values())
+
+        def ptr(t):                                           # (no masks, no bias at all: a valid pointer, never read)
+            if t.numel() == 0:
+                t = torch.zeros(1, dtype=t.dtype, device=t.device)
+                c.tensors.append(t)
+            return t.data_ptr()
+
+        mask, off = held.get("mask"), held.get("bias_off")
+        if mask is not None:
+            c.d_mask = ptr(mask)
+            c.mask_ld = mask.stride(0) if mask.shape[0] > 1 else mask.shape[1]
+            c.n_masks = mask.shape[0]
+            c.d_mask_of = held["mask_of"].data_ptr() if "mask_of" in held else None
+        if off is not None:
+            c.d_bias_ids, c.d_bias, c.d_bias_off = ptr(held["bias_ids"]), ptr(held["bias"]), off.data_ptr()
+        return c
 
     @staticmethod
     def _csr(dicts):
@@ -347,10 +374,10 @@ class Edits:
 
     def tensors(self):
         """The device tensors of the masks and biases."""
-        return [t for t in (self.mask, self.mask_of, self.bias_ids, self.bias, self.bias_off) if t is not None]
+        return list(self._held().values())
 
-    def _ref(self, rows: int, records: int, V: int, dev):
-        """The checked fs_edits for a call of `rows` logits rows and `records` records."""
+    def _now(self, rows: int, records: int, V: int, dev):
+        """The checked fs_edits for a call of `rows` logits rows and `records` records, on the current stream."""
         if dev != self.device:
             raise SamplerError(f"edits on {self.device}, logits on {dev}")
         if self.mask is not None:
@@ -360,7 +387,12 @@ class Edits:
                 raise SamplerError("one mask index per row" if self.mask_of is not None else "one mask per row")
         if self.bias_off is not None and self.bias_off.numel() != records + 1:
             raise SamplerError("one bias list per record")
-        return ctypes.byref(self.c)
+        if not self._given:
+            return self.c
+        return self._struct(dict(self._held(), **{n: self._as(n, x) for n, x in self._given.items()}))
+
+    def _ref(self, rows: int, records: int, V: int, dev):
+        return ctypes.byref(self._now(rows, records, V, dev))
 
 
 def _on(stream, dev, *tensors):
@@ -401,10 +433,11 @@ def sample_batch(logits, params, u, hist=None, hist_off=None, V=None, kcap=0, ct
         hp = params_array(params)
     if edits is not None:
         with torch.cuda.device(dev), ctx.lock:
+            ed = edits._now(B, B, n, dev)
             check(lib().fs_sample_edited(ctx.h, _lptr(logits), ld, B, n, _ptr(hist), _ptr(hist_off), _ptr(p), _hptr(hp),
-                                         edits._ref(B, B, n, dev), _ptr(u), _ptr(tok), kcap, _ptr(ids), _ptr(probs),
-                                         _ptr(keep), _on(stream, dev, logits, p, u, hist, hist_off, tok, keep, ids, probs,
-                                                             *edits.tensors())),
+                                         ctypes.byref(ed), _ptr(u), _ptr(tok), kcap, _ptr(ids), _ptr(probs), _ptr(keep),
+                                         _on(stream, dev, logits, p, u, hist, hist_off, tok, keep, ids, probs,
+                                             *ed.tensors)),
                   "fs_sample_edited")
         return dict(tok=tok, keep=keep, cand_ids=ids, cand_probs=probs, _keepalive=(p, u, hist, hist_off))
     with ctx.lock:
@@ -472,11 +505,12 @@ def verify(logits, rows, row_off, params, u=None, hist=None, hist_off=None, eos_
         hp = params_array(params)
     if edits is not None:
         with torch.cuda.device(dev), ctx.lock:
+            ed = edits._now(R, S, n, dev)
             check(lib().fs_verify_edited(ctx.h, _lptr(logits), ld, S, R, n, _ptr(rows), _ptr(row_off), _ptr(hist),
-                                         _ptr(hist_off), _ptr(p), _hptr(hp), edits._ref(R, S, n, dev), _ptr(u), int(eos_id),
+                                         _ptr(hist_off), _ptr(p), _hptr(hp), ctypes.byref(ed), _ptr(u), int(eos_id),
                                          _ptr(tok), _ptr(acc),
                                          _on(stream, dev, logits, rows, row_off, p, u, hist, hist_off, tok, acc,
-                                             *edits.tensors())),
+                                             *ed.tensors)),
                   "fs_verify_edited")
         return tok, acc
     with ctx.lock:
@@ -587,11 +621,12 @@ def decode_step(logits, params, rng, hist=None, hist_off=None, out_cap=None, V=N
     hp = params_array(params) if (route or ROUTE) == "host" and not isinstance(params, torch.Tensor) else None
     if edits is not None:
         with torch.cuda.device(dev), ctx.lock:
+            ed = edits._now(B, B, n, dev)
             check(lib().fs_decode_step_edited(ctx.h, rng.h, _lptr(logits), ld, B, n, _ptr(hist), _ptr(hist_off), _ptr(p),
-                                              _hptr(hp), edits._ref(B, B, n, dev), _ptr(tok), _ptr(keep), _ptr(out),
+                                              _hptr(hp), ctypes.byref(ed), _ptr(tok), _ptr(keep), _ptr(out),
                                               _ptr(out_off), int(out_cap),
                                               _on(stream, dev, logits, p, hist, hist_off, tok, keep, out, out_off,
-                                                  *edits.tensors())),
+                                                  *ed.tensors)),
                   "fs_decode_step_edited")
         return tok, keep, out, out_off
     with ctx.lock:
@@ -652,10 +687,11 @@ def edit_batch(logits, params=None, hist=None, hist_off=None, edits=None, V=None
         out_ld = ld
     ctx = ctx or Context.default(dev)
     with torch.cuda.device(dev), ctx.lock:
+        ed = None if edits is None else edits._now(B, B, n, dev)
         check(lib().fs_edit_batch(ctx.h, _lptr(logits), kind, ld, B, n, _ptr(hist), _ptr(hist_off), _ptr(p),
-                                  None if edits is None else edits._ref(B, B, n, dev), ctypes.c_void_p(o2.data_ptr()),
-                                  out_ld, _on(stream, dev, logits, p, hist, hist_off, out,
-                                               *(edits.tensors() if edits is not None else []))), "fs_edit_batch")
+                                  None if ed is None else ctypes.byref(ed), ctypes.c_void_p(o2.data_ptr()), out_ld,
+                                  _on(stream, dev, logits, p, hist, hist_off, out, *(ed.tensors if ed is not None else []))),
+              "fs_edit_batch")
     return out
 
 
@@ -685,10 +721,11 @@ def logprobs(logits, tok=None, n=0, params=None, edits=None, V=None, ctx=None, s
         top = torch.empty((B, n), dtype=torch.float32, device=dev)
     ctx = ctx or Context.default(dev)
     with torch.cuda.device(dev), ctx.lock:
-        check(lib().fs_logprobs(ctx.h, _lptr(logits), kind, ld, B, v, _ptr(p),
-                                None if edits is None else edits._ref(B, B, v, dev), _ptr(t), n, _ptr(lp), _ptr(rank),
-                                _ptr(ids), _ptr(top), _on(stream, dev, logits, p, t, lp, rank, ids, top,
-                                                         *(edits.tensors() if edits is not None else []))), "fs_logprobs")
+        ed = None if edits is None else edits._now(B, B, v, dev)
+        check(lib().fs_logprobs(ctx.h, _lptr(logits), kind, ld, B, v, _ptr(p), None if ed is None else ctypes.byref(ed),
+                                _ptr(t), n, _ptr(lp), _ptr(rank), _ptr(ids), _ptr(top),
+                                _on(stream, dev, logits, p, t, lp, rank, ids, top, *(ed.tensors if ed is not None else []))),
+              "fs_logprobs")
     return dict(lp=lp, rank=rank, ids=ids, top=top)
 
 
