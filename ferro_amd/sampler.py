@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+from collections.abc import Mapping
 from dataclasses import dataclass
 
 import numpy as np
@@ -268,8 +269,9 @@ class Edits:
 
     def __init__(self, mask=None, mask_of=None, bias=None, device=None):
         dev = torch.device("cuda" if device is None else device)
+        bias = None if bias is None else list(bias)
         if device is None:
-            given = [mask, mask_of] + (list(bias) if isinstance(bias, tuple) else [])
+            given = [mask, mask_of] + (bias or [])
             dev = next((t.device for t in given if isinstance(t, torch.Tensor) and t.is_cuda), dev)
         if dev.type == "cuda" and dev.index is None:
             dev = torch.device("cuda", torch.cuda.current_device())
@@ -290,8 +292,10 @@ class Edits:
                 raise SamplerError("mask_of needs masks")
             self._take("mask_of", mask_of)
         if bias is not None:
-            if not isinstance(bias, tuple):
+            if all(d is None or isinstance(d, Mapping) for d in bias):
                 bias = self._csr(bias)
+            if len(bias) != 3:
+                raise SamplerError("biases are one {token: bias} per record or CSR lists (ids, values, offsets)")
             ids, val, off = bias
             if not any(isinstance(t, torch.Tensor) and t.is_cuda for t in bias):
                 self._check(np.asarray(ids, np.int64), np.asarray(val), np.asarray(off, np.int64))

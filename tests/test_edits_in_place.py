@@ -49,3 +49,20 @@ def test_arrays_are_taken_as_they_are_when_given():
     ed = F.Edits(mask=np.ones((2, 3), np.uint32), mask_of=of, device="cpu")
     of[:] = 1
     assert words_at(ed._now(2, 2, 96, CPU).d_mask_of, 2) == [0, 0]
+
+
+@pytest.mark.parametrize("made", [list, tuple, iter])
+def test_one_dict_per_record_in_any_sequence(made):
+    """Three records, too: they are no CSR lists."""
+    for dicts in ([{9: 1.0, 2: -1.0}, None, {4: 0.5}], [{3: 1.0}], [{}, {}, {}], []):
+        ed = F.Edits(bias=made(dicts), device="cpu")
+        assert ed.bias_ids.tolist() == [t for d in dicts for t in sorted(d or {})]
+        assert ed.bias_off.tolist() == [0, *np.cumsum([len(d or {}) for d in dicts]).tolist()]
+
+
+def test_csr_lists_in_a_list_and_refusals():
+    ed = F.Edits(bias=[np.array([5, 7]), np.ones(2, np.float32), [0, 2]], device="cpu")
+    assert ed.bias_ids.tolist() == [5, 7] and ed.bias_off.tolist() == [0, 2]
+    for bad in ([np.array([5])], (np.array([5]), np.ones(1)), [{}, [1], {}, {}]):
+        with pytest.raises(F.SamplerError):
+            F.Edits(bias=bad, device="cpu")
