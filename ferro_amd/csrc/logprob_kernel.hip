@@ -8,10 +8,10 @@
 // requested before the present one is worked on. Every wave works by itself until its part ends (no barrier in between):
 //   - the sum: exponentials of c (x - m), c = log2 e / T and m the wave's largest x so far (the largest term is 1, exactly).
 //     A chunk's 16 or 32 terms of a lane are added in fp32, chunks in fp64, and a new m scales the lanes' sums in fp64; a
-//     subtraction, a product, an exponential and an addition a logit. A chunk with a term that is 1 is added in fp64
-//     throughout: beside a 1, fp32 loses what a near-certain token's log-probability consists of (1 and e^-18 in one lane:
-//     0 for -1.5e-8). 1024 rows of 151936 bf16 with heavy tails, about 3.5 of 19 chunks: 62.0 us with fp32 alone, 63.8 so,
-//     64.8 with every chunk in fp64;
+//     subtraction, a product, an exponential and an addition a logit. Where a term is 1, a lane's terms are added in fp64:
+//     beside a 1, fp32 loses what a near-certain token's log-probability consists of (1 and e^-18 in one lane: 0 for
+//     -1.5e-8). 1024 rows of 151936 bf16 with heavy tails, 3.5 such chunks of 19: 62.3 us with fp32 alone, 62.8 so, 64.8
+//     with every term in fp64;
 //   - a chunk whose sum is NaN (NaN or infinite logits) is added again with NaN left out; once the largest logit is
 //     infinite its tokens are counted instead;
 //   - the n largest: a bound that n of the wave's 64 lane maxima so far reach (bisected with a compare a step; sorting them
@@ -242,11 +242,38 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
                     }
                     return d[0] + d[1];
                 }
+                if constexpr (NL > 4) {
+                    // a lane's logits by their place in the group: eight terms in fp64 only where one of them is 1 (1024 rows
+                    // of 151936 bf16: 62.8 us; with all in fp64 64.2, as in the shorter chunks of fp32 rows, where that is
+                    // the faster: 64 rows of 262144 25.6 us, by place 25.9)
 #pragma unroll
-                for (int q = 0; q < NL; ++q) {
+                    for (int c_ = 0; c_ < 4; ++c_) {
+                        float most = lp_max3(x[0][c_], x[1][c_], x[2][c_]);
 #pragma unroll
-                    for (int c_ = 0; c_ < 4; ++c_) d[c_ & 1] += (double)__builtin_amdgcn_exp2f((x[q][c_] - m) * c2);
-                    __builtin_amdgcn_sched_barrier(0);         // (all exponentials at once need more registers)
+                        for (int q = 3; q < NL; q += 2) most = lp_max3(most, x[q][c_], x[q + 1 < NL ? q + 1 : q][c_]);
+                        if (__ballot(most == m) != 0ull) {
+#pragma unroll
+                            for (int q = 0; q < NL; ++q) {
+                                d[q & 1] += (double)__builtin_amdgcn_exp2f((x[q][c_] - m) * c2);
+                                if (q % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                            }
+                        } else {
+                            float e[2] = {0.0f, 0.0f};
+#pragma unroll
+                            for (int q = 0; q < NL; ++q) {
+                                e[q & 1] += __builtin_amdgcn_exp2f((x[q][c_] - m) * c2);
+                                if (q % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                            }
+                            d[c_ & 1] += (double)(e[0] + e[1]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < NL; ++q) {
+#pragma unroll
+                        for (int c_ = 0; c_ < 4; ++c_) d[c_ & 1] += (double)__builtin_amdgcn_exp2f((x[q][c_] - m) * c2);
+                        __builtin_amdgcn_sched_barrier(0);     // (all exponentials at once need more registers)
+                    }
                 }
                 return d[0] + d[1];
             }
