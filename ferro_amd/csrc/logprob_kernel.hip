@@ -24,10 +24,10 @@
 // maxima of groups of lanes that the waves publish, and sorts the tokens that reach it (about 1.2 n) in registers.
 // A chunk's mask is read a chunk ahead of its logits, whose groups of four without an allowed token are not read (the
 // part's first chunk is requested whole, at once).
-// Bound: HBM; the arithmetic (about 10 instructions a logit) takes about half of the time of reading 16-bit logits. 1024 rows
-// of 151936 bf16, n 1: 62.2 us (5.0 TB/s of 311 MB). 64 rows of 262144 fp32: 14.6 us for the chosen token's alone, 19.8 with
-// n 5, 25.4 with n 20 under masks and biases: the lists and the row's end, a chain behind the last read. One row of 65536:
-// 8.7 us, of which the read is about 1.
+// Bound: HBM, and for 16-bit logits nearly as much the arithmetic (about 10 instructions a logit: four fifths of a busy CU's
+// cycles). 1024 rows of 151936 bf16: 57.1 us for the chosen token's alone, 62.9 with n 1 (4.9 TB/s of 311 MB). 64 rows of
+// 262144 fp32: 14.8 us, 20.8 with n 5, 24.1 with n 20, and 25.6 with n 20 under masks and biases: the lists and the row's end,
+// a chain behind the last read. One row of 65536 with n 5: 8.7 us, of which the read is about 1.
 #include "edit_device.hpp"
 #include "row_device.hpp"
 

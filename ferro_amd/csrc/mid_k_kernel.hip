@@ -1331,8 +1331,8 @@ __device__ __forceinline__ bool ak_finish(const uint64_t* list, uint32_t n0, uin
 // now 830 (2460 on the fused kernel).
 template <bool CAP, bool ED>
 __device__ __forceinline__ bool ak_values(const float* rowp, int V, bool pen, const MkWin& win, const MkPen& pn,
-                                          const EdRow& er, uint64_t* list, uint32_t above, const AkRow& r, const fs_row_params& p, MkShared& s, int& tok,
-                                          int& keep) {
+                                          const EdRow& er, uint64_t* list, uint32_t above, const AkRow& r,
+                                          const fs_row_params& p, MkShared& s, int& tok, int& keep) {
     constexpr int PT = 32, CH = SK_LT * PT;                    // logits of a thread, of a chunk
     const int tid = threadIdx.x, lane = lane_id();
     const double Td = (double)p.temperature;
@@ -1744,7 +1744,8 @@ __global__ __launch_bounds__(SK_LT, 4) void mid_k_kernel(const float* logits, in
     auto edit = [&]() {
         if constexpr (ED) {
             if (!CAP && few.nb > 0)
-                ed_add<NL, true>(a.ed, pidx, few, s.h.hist + MK_H / 2, seg_lo, n_in, [&](int q, int c) -> float& { return v[q][c]; });
+                ed_add<NL, true>(a.ed, pidx, few, s.h.hist + MK_H / 2, seg_lo, n_in,
+                                 [&](int q, int c) -> float& { return v[q][c]; });
             if (masked) {
                 asm volatile("" : "+v"(eb.a), "+v"(eb.b));         // (the nibbles again: kept from the loads they spill)
 #pragma unroll

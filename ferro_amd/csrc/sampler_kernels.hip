@@ -800,7 +800,9 @@ struct Edited {
 
 // Groups of four logits per thread and segments per row of the edit kernel: the largest segments that still give every CU
 // four workgroups. Measured with 2, 4 and 8 groups, bf16 with masks, 30 biases and a window: 1 row of 262144 4.4, 5.2, 6.7 us;
-// 32 rows 14.3, 12.5, 12.2; 64 rows 23.4, 22.6, 18.5; 256 rows 83.9, 72.0, 75.4; 64 rows of 32000 6.6, 6.8, 8.6.
+// 32 rows 14.3, 12.5, 12.2; 64 rows 23.4, 22.6, 18.5; 256 rows 83.9, 72.0, 75.4; 64 rows of 32000 6.6, 6.8, 8.6. fp16 rows of
+// 100003 with a softcap, windows of 4096 ids and 300 biases, which every segment reads again: 1 row 10.0, 15.0, 24.3; 24 rows
+// 16.9, 20.1, 28.9; 64 rows 30.6, 31.7, 39.9; 64 of 262144 61.9, 59.3, 63.3.
 int edit_plan(int cus, int64_t B, int32_t V, int& nseg) {
     int nl = 2;
     for (const int l : {8, 4, 2}) {
@@ -931,9 +933,9 @@ int edit_args(const fs_edits* edits, int32_t rows, int32_t V, fs::EdArgs& ed) {
 
 // Parts per row of fs_logprobs. Four workgroups fit a CU; p parts take ceil(B p / 4 CUs) rounds of ceil(n / p) chunks of a
 // row's n and of about 4 chunks' time to begin and join, and the p with the shortest of these is taken. For few rows that
-// fills the device once (64 rows of 262144, n 20: 16 parts 25.4 us, 8 30.4, 32 31.0; 256 rows: 4 parts 57.0, 2 78, 8 65);
-// past half of the slots more parts fill a last round (600 rows of 151936: 3 parts 83.1 us, 1 92.1; 1100 rows of bf16, n 1:
-// 2 parts 77.2, 1 85.0; 700 rows: 1 part 51).
+// fills the device once (64 rows of 262144, n 20: 16 parts 25.6 us, 8 30.7, 32 31.2; 256 rows: 4 parts 57.6, 2 78.7, 8 66.3);
+// past half of the slots more parts fill a last round (600 rows of 151936: 3 parts 84.1 us, 1 94.0; 1100 rows of bf16, n 1:
+// 2 parts 79.1, 1 86.1; 700 rows: 1 part 52.5, 2 56.3).
 int logprob_parts(const fs_context* c, int64_t B, int32_t V, int32_t type) {
     if (!c->seg_layout) return 1;                  // (a row's parts would not share an L2)
     const int64_t chunk = (int64_t)fs::SK_LT * 4 * fs::LP_NL(type), n = ((int64_t)V + chunk - 1) / chunk;

@@ -190,8 +190,8 @@ constexpr unsigned SK_PAD_LDS = 16384;
 // ED: the rows have masks and biases (fs_edits; no biases with a softcap, which comes before them but is applied to the
 // candidates alone). The loads from the ED_FIRST-th on wait for the row's mask and skip the groups of four without an
 // allowed token (64 rows of 262144, k 64: 17.8 us where the masks allow few tokens, 22.5 where they allow most, 20.8
-// without; with all loads behind the mask 17.2 / 22.6 / 21.2 and one more round trip for a single row). A logit that is not allowed becomes NaN, which nothing below takes; candidates are above -inf; a row without one
-// has token -1.
+// without; with all loads behind the mask 17.2 / 22.6 / 21.2 and one more round trip for a single row). A logit that is not
+// allowed becomes NaN, which nothing below takes; candidates are above -inf; a row without one has token -1.
 template <int NL, bool CAP, bool GREEDY, bool MANY, bool ED>
 __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, int64_t ld, int B, int V, int nseg,
                                                         int flags, const fs_row_params* params,
@@ -427,9 +427,10 @@ __global__ __launch_bounds__(SK_LT, 4) void small_k_kernel(const float* logits, 
     const bool tail = n_in < SEG;
     if constexpr (ED) {
         if (!CAP && few.nb > 0)
-            ed_add<NL, true>(a.ed, pidx, few, reinterpret_cast<uint32_t*>(&s.cand[0]), seg_lo, n_in, [&](int q, int c) -> float& {
-                return c == 0 ? v[q].x : c == 1 ? v[q].y : c == 2 ? v[q].z : v[q].w;
-            });
+            ed_add<NL, true>(a.ed, pidx, few, reinterpret_cast<uint32_t*>(&s.cand[0]), seg_lo, n_in,
+                             [&](int q, int c) -> float& {
+                                 return c == 0 ? v[q].x : c == 1 ? v[q].y : c == 2 ? v[q].z : v[q].w;
+                             });
         if (masked) {
             asm volatile("" : "+v"(eb.a), "+v"(eb.b));         // (the nibbles again: kept from the loads they spill)
 #pragma unroll

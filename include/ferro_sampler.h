@@ -273,20 +273,24 @@ typedef struct fs_edits {
     int32_t n_masks;
     const int32_t* d_mask_of;   /* [rows] each logits row's mask; negative: every token is allowed; >= n_masks: none is, and
                                    FS_DEVERR_MASK is set. NULL: row r takes mask r */
-    const int32_t* d_bias_ids;  /* biases of record s: [d_bias_off[s], d_bias_off[s+1]), ids ascending within a record; equal */
-    const float* d_bias;        /* ids add up one after another; ids outside [0, V) are ignored. A bias of -inf bans its token */
+    const int32_t* d_bias_ids;  /* biases of record s: [d_bias_off[s], d_bias_off[s+1]), ids ascending within a record; */
+    const float* d_bias;        /* equal ids add up one after another; ids outside [0, V) are ignored. A bias of -inf bans
+                                   its token (+inf forces a greedy row's alone: it leaves a sampled row's weights NaN, as in
+                                   ferro; a mask of one token forces it in both) */
     const int64_t* d_bias_off;  /* [records + 1]: a record per row, per stream in fs_verify_edited. NULL: no biases */
 } fs_edits;
 
 /* Sampling under edits: fs_sample_batch_hp, fs_verify_hp and fs_decode_step_hp on the edited logits, with the same
  * arguments and outputs beside `edits` (h_params may be NULL here too; edits may not). A row's candidates are its allowed
  * tokens whose edited logit is above -inf: k, min-p and top-p count those alone. A row without a candidate has token -1
- * and 0 kept (a greedy row's candidate outputs are -1 and 0); -1 ends a verification window at its row, and fs_decode_step_
- * edited appends it to the history, where the penalties ignore it. With h_params, batches that the small-k or the mid-k
- * kernel takes (fs_route_plan, fs_mid_k_plan, and some of shorter rows with a large k) and that have no biases beside a softcap read their logits once, where they
- * are, and of masked rows only the groups of four with an allowed token; others are edited into a workspace of V * 4 bytes
- * a row first, which grows as a context's other buffers do. A call under graph capture whose workspace would have to grow
- * returns FS_E_NOMEM and leaves the capture as it was. */
+ * and 0 kept (a greedy row's candidate outputs are -1 and 0); -1 ends a verification window at its row, and
+ * fs_decode_step_edited appends it to the history, where the penalties ignore it. With h_params, batches that the small-k or
+ * the mid-k kernel takes (fs_route_plan, fs_mid_k_plan, and some of shorter rows with a large k) and that have no biases
+ * beside a softcap read their logits once, where they are: the first 4096 of every segment of 4096, 8192 or 16384, and of
+ * a masked row's others the groups of four with an allowed token. Others are edited into a workspace of V * 4 bytes a row
+ * first, which grows as a context's other buffers do, and sampled there. A call that is refused for want of memory has
+ * launched nothing and taken no draw; one under graph capture whose workspace would have to grow returns FS_E_NOMEM and
+ * leaves the capture as it was. */
 int fs_sample_edited(fs_context* ctx, const float* d_logits, int64_t ld, int32_t B, int32_t V, const int32_t* d_hist,
                      const int64_t* d_hist_off, const fs_row_params* d_params, const fs_row_params* h_params,
                      const fs_edits* edits, const double* d_u, int32_t* d_tok, int32_t kcap, int32_t* d_cand_ids,
@@ -314,8 +318,9 @@ int fs_edit_batch(fs_context* ctx, const void* d_logits, int32_t type, int64_t l
  * d_params NULL: the logits' own), without penalties (fs_edit_batch writes penalised rows). A token that is not allowed,
  * whose logit is NaN or -inf, or that is outside [0, V) has -inf and rank 0; places past a row's tokens have id -1 and
  * -inf. Where the largest logit is +inf, its tokens share the probability. n <= FS_MAX_TOP; each output may be NULL
- * (d_lp and d_rank need d_tok). Rows and types as in fs_edit_batch. A lane's 16 or 32 exponentials of a 16 KB chunk are added in
- * fp32 (in fp64 where the largest logit so far is among the wave's), those sums in fp64. */
+ * (d_lp and d_rank need d_tok). Rows and types as in fs_edit_batch. A lane's 16 or 32 exponentials of a 16 KB chunk are
+ * added in fp32 (in fp64 beside the largest logit so far), those sums in fp64: a near-certain token's log-probability
+ * is right relative to itself, down to about 1e-15. */
 #define FS_MAX_TOP 64
 int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld, int32_t B, int32_t V,
                 const fs_row_params* d_params, const fs_edits* edits, const int32_t* d_tok, int32_t n, float* d_lp,
