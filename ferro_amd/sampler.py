@@ -426,6 +426,8 @@ def sample_batch(logits, params, u, hist=None, hist_off=None, V=None, kcap=0, ct
     if p.numel() != B * PARAMS_DTYPE.itemsize:
         raise SamplerError("one params record per row")
     u = _dev(u, torch.float64, dev)
+    if u.numel() < B:
+        raise SamplerError("one draw per row")
     hist, hist_off = _hist_tensors(hist, hist_off, B, dev)
     tok = torch.empty(B, dtype=torch.int32, device=dev)
     keep = torch.empty(B, dtype=torch.int32, device=dev)
@@ -493,6 +495,10 @@ def verify(logits, rows, row_off, params, u=None, hist=None, hist_off=None, eos_
     logits, ld, n = _check_logits(logits, V)
     R = logits.shape[0]
     dev = logits.device
+    if not (isinstance(row_off, torch.Tensor) and row_off.is_cuda):
+        o = np.asarray(row_off, np.int64)                 # (a row outside the windows would be counted as one of theirs)
+        if o.ndim != 1 or o.size < 1 or o[0] != 0 or o[-1] != R or np.any(np.diff(o) < 0):
+            raise SamplerError("row_off must ascend from 0 to the logits' rows")
     rows = _dev(rows, torch.int32, dev)
     row_off = _dev(row_off, torch.int64, dev)
     S = row_off.numel() - 1
@@ -500,6 +506,8 @@ def verify(logits, rows, row_off, params, u=None, hist=None, hist_off=None, eos_
     if p.numel() != S * PARAMS_DTYPE.itemsize:
         raise SamplerError("one params record per stream")
     u = _dev(np.zeros(R) if u is None else u, torch.float64, dev)
+    if rows.numel() < R or u.numel() < R:
+        raise SamplerError("one fed token and one draw per row")
     hist, hist_off = _hist_tensors(hist, hist_off, S, dev)
     tok = torch.empty(R, dtype=torch.int32, device=dev)
     acc = torch.empty(S, dtype=torch.int32, device=dev)

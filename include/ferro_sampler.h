@@ -157,7 +157,8 @@ int fs_argmax_batch(fs_context* ctx, const float* d_logits, int64_t ld, int32_t 
                     int32_t* d_tok, void* stream);
 
 /* Speculative verification window (src/server.cpp:613-651). Stream s owns logits rows
- * d_row_off[s] .. d_row_off[s+1]-1 (d_row_off has n_streams+1 entries, total rows = d_row_off[n_streams]);
+ * d_row_off[s] .. d_row_off[s+1]-1 (d_row_off has n_streams+1 entries, ascends from 0, and total_rows =
+ * d_row_off[n_streams]: a row outside the windows would be counted as one of theirs);
  * d_rows[r] is the token fed at row r: d_rows[d_row_off[s]] is the stream's last sampled token, the rest are its
  * drafts. Row r of stream s is sampled with history = d_hist[d_hist_off[s] .. d_hist_off[s+1]) followed by the
  * drafts fed before it (d_rows[d_row_off[s]+1 .. d_row_off[s]+r]), with params d_params[s] and draw d_u[row].
