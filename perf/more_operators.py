@@ -329,7 +329,7 @@ def _plain_select(d):
     # a row's best tokens but eos, and eos by itself (before others of its score)
     if c["eos"]:
         e = score(x[:, d["eos"]:d["eos"] + 1])
-        x = x.clone() if x is d["x"] else x
+        x = x.clone() if x.data_ptr() == d["x"].data_ptr() else x      # (the logits are read only)
         x[:, d["eos"]] = -math.inf
     v, idx = torch.sort(x, dim=1, descending=True, stable=True)
     k = min(n, V)
