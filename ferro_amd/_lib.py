@@ -24,9 +24,12 @@ FS_W_RECOVERED = 1          # success; an earlier call's give-up was cleared (FS
 FS_WAIT_GIVE_UP = 0xFFFFFFFF
 FS_DEVERR_COUNT_OVERFLOW = 1
 FS_DEVERR_INTERNAL = 2
+FS_DEVERR_HIST_APPEND = 4
 FS_DEVERR_MASK = 8
+FS_DEVERR_PARENT = 16
 FS_F32, FS_BF16, FS_F16 = 0, 1, 2
 FS_MAX_TOP = 64
+FS_BEAM_KEEP_SLOTS = 1
 
 # fs_row_params (include/ferro_sampler.h); field order follows ferro's SamplerParams (src/sampler.h:12-21).
 PARAMS_DTYPE = np.dtype([
@@ -42,6 +45,13 @@ class FsEdits(ctypes.Structure):
     _fields_ = [("d_mask", ctypes.c_void_p), ("mask_ld", ctypes.c_int64), ("n_masks", ctypes.c_int32),
                 ("d_mask_of", ctypes.c_void_p), ("d_bias_ids", ctypes.c_void_p), ("d_bias", ctypes.c_void_p),
                 ("d_bias_off", ctypes.c_void_p)]
+
+
+class FsState(ctypes.Structure):
+    """fs_state (include/ferro_sampler.h): one state buffer that follows its beams."""
+    _fields_ = [("d_src", ctypes.c_void_p), ("d_dst", ctypes.c_void_p)] + \
+        [(f"{side}_{unit}", ctypes.c_int64) for side in ("src", "dst") for unit in ("row", "block", "pos")] + \
+        [("pos_bytes", ctypes.c_int64), ("blocks", ctypes.c_int32), ("positions", ctypes.c_int32)]
 
 
 # Every symbol include/ferro_sampler.h declares, with its ctypes signature.
@@ -65,6 +75,10 @@ SIGNATURES = {
     "fs_decode_step_edited": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "fs_edit_batch": (ctypes.c_int, [_P, _P, _I32, _I64, _I32, _I32, _P, _P, _P, _P, _P, _I64, _P]),
     "fs_logprobs": (ctypes.c_int, [_P, _P, _I32, _I64, _I32, _I32, _P, _P, _P, _I32, _P, _P, _P, _P, _P]),
+    "fs_beam_select": (ctypes.c_int, [_P, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _I32, _I32, _I32, _P, _P, _P, _P,
+                                      _P, _P, _P]),
+    "fs_hist_fork": (ctypes.c_int, [_P, _I32, _P, _P, _P, _I32, _P, _P, _P, _I64, _P, _P]),
+    "fs_reorder_states": (ctypes.c_int, [_P, _I32, _P, _I32, _I32, _I32, _P, _P, _P, _P]),
     "fs_penalize_batch": (ctypes.c_int, [_P, _P, _I64, _I32, _I32, _P, _P, _P, _P]),
     "fs_softcap_batch": (ctypes.c_int, [_P, _P, _I64, ctypes.c_float, _P]),
     "fs_device_error": (ctypes.c_int, [_P, _P, _P]),

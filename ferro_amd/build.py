@@ -10,7 +10,7 @@ ROOT = os.path.dirname(PKG)
 # the kernel files, compiled side by side and linked into one library
 SRCS = [os.path.join(PKG, "csrc", f) for f in ("fused_kernel.hip", "sampler_kernels.hip", "small_k_kernel.hip",
                                                   "mid_k_kernel.hip", "history_kernels.hip", "edit_kernels.hip",
-                                                  "logprob_kernel.hip")]
+                                                  "logprob_kernel.hip", "beam_kernels.hip")]
 LIB = os.path.join(PKG, "libferro_sampler.so")
 # the same source with phase timestamps compiled in (-DFS_TRACE, fs_trace_set): read by ferro_amd/trace_phases.py
 TRACE_LIB = os.path.join(PKG, "libferro_sampler_trace.so")

@@ -164,6 +164,9 @@ struct fs_context {
     uint32_t* lp_ticket = nullptr;     //   [lp_rows][LP_LINE] their tickets, left at 0,
     uint64_t* lp_lists = nullptr;      //   [lp_list_segs][SK_NW][LP_TOP] their lists
     size_t lp_row_bytes = 0, lp_rows = 0, lp_list_segs = 0;
+    fs::BeamRow* bm_rows = nullptr;    // fs_beam_select: [bm_row_cap] the rows' sums,
+    uint64_t* bm_lists = nullptr;      //   [bm_list_rows][BM_TOP] their lists
+    size_t bm_row_cap = 0, bm_list_rows = 0;
     int static_dev = -1;       // device whose static workspace fs_sample_batch_static used with this context
     uint64_t* trace = nullptr; // FS_TRACE builds: phase timestamps, trace_cap entries (fs_trace_set)
     int64_t trace_cap = 0;
@@ -949,6 +952,44 @@ int logprob_parts(const fs_context* c, int64_t B, int32_t V, int32_t type) {
     return (int)best;
 }
 
+// ---- fs_reorder_states
+// Bytes per column: what the pointers, the strides and a position's bytes are all multiples of, 16 at most (streams of more
+// than 16 rows, whose columns are all in registers: 8).
+int state_bytes(const fs_state& z, int rows) {
+    const uint64_t all = (uint64_t)(uintptr_t)z.d_src | (uint64_t)(uintptr_t)z.d_dst | (uint64_t)z.src_row |
+                         (uint64_t)z.src_block | (uint64_t)z.src_pos | (uint64_t)z.dst_row | (uint64_t)z.dst_block |
+                         (uint64_t)z.dst_pos | (uint64_t)z.pos_bytes;
+    int vb = rows > 16 ? 8 : 16;
+    while (vb > 1 && (all & (uint64_t)(vb - 1)) != 0) vb >>= 1;
+    return vb;
+}
+int64_t state_cols(const fs_state& z, int vb) {
+    return (int64_t)z.blocks * std::max(1, z.positions) * (z.pos_bytes / vb);
+}
+int check_state(const fs_state& z, int64_t S, int32_t n_src, int32_t n) {
+    const bool empty = z.blocks == 0 || z.pos_bytes == 0 || S == 0;
+    if ((!empty && (!z.d_src || !z.d_dst)) || z.pos_bytes < 0 || z.blocks < 0 || z.positions < 0 || z.src_row < 0 || z.src_block < 0 ||
+        z.src_pos < 0 || z.dst_row < 0 || z.dst_block < 0 || z.dst_pos < 0)
+        return FS_E_INVALID;
+    // columns are counted in 32 bits; nor do spans come near 64
+    const int64_t most = int64_t(1) << 46;
+    const int64_t pos = std::max(1, z.positions);
+    if (z.pos_bytes > 0x7fffffff || (int64_t)z.blocks * pos > 0x7fffffff) return FS_E_INVALID;
+    for (const int64_t stride : {z.src_row, z.src_block, z.src_pos, z.dst_row, z.dst_block, z.dst_pos})
+        if (stride > most) return FS_E_INVALID;
+    if ((double)z.blocks * (double)pos * (double)z.pos_bytes > 2e9 * state_bytes(z, n > n_src ? n : n_src)) return FS_E_INVALID;
+    if (empty) return FS_OK;
+    if (z.d_src == z.d_dst && n == n_src && z.src_row == z.dst_row && z.src_block == z.dst_block && z.src_pos == z.dst_pos)
+        return FS_OK;
+    auto span = [&](int64_t rows, int64_t row, int64_t block, int64_t p) {
+        return (double)(rows - 1) * (double)row + (double)(z.blocks - 1) * (double)block + (double)(pos - 1) * (double)p +
+               (double)z.pos_bytes;
+    };
+    const double s0 = (double)(uintptr_t)z.d_src, s1 = s0 + span(S * n_src, z.src_row, z.src_block, z.src_pos);
+    const double d0 = (double)(uintptr_t)z.d_dst, d1 = d0 + span(S * n, z.dst_row, z.dst_block, z.dst_pos);
+    return s0 < d1 && d0 < s1 ? FS_E_INVALID : FS_OK;
+}
+
 size_t type_size(int32_t type) { return type == FS_F32 ? 4 : type == FS_BF16 || type == FS_F16 ? 2 : 0; }
 
 // Rows of logits of any type: check_rows for FS_F32, four logits' alignment for the others.
@@ -1065,6 +1106,8 @@ int fs_destroy(fs_context* c) {
     (void)hipFree(c->lp_row);
     (void)hipFree(c->lp_ticket);
     (void)hipFree(c->lp_lists);
+    (void)hipFree(c->bm_rows);
+    (void)hipFree(c->bm_lists);
     for (void* p : c->retired) (void)hipFree(p);
     if (c->hflag) (void)hipHostFree(c->hflag);
     delete c;
@@ -1360,6 +1403,85 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
     a.lp = d_lp; a.rank = d_rank; a.ids = d_top_ids; a.top = d_top_lp;
     a.rows = ctx->lp_row; a.ticket = ctx->lp_ticket; a.lists = ctx->lp_lists; a.err = ctx->err;
     return fs::launch_logprobs(type, a, st) == hipSuccess ? FS_OK : FS_E_HIP;
+}
+
+int fs_beam_select(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld, int32_t n_streams, int32_t total_rows,
+                   int32_t V, const int64_t* d_row_off, const float* d_score, const fs_row_params* d_params,
+                   const fs_edits* edits, int32_t eos_id, int32_t n, int32_t flags, int32_t* d_parent, int32_t* d_tok,
+                   float* d_out_score, int32_t* d_done, int32_t* d_done_parent, float* d_done_score, void* stream) {
+    if (!ctx || n_streams < 0 || n < 1 || n > FS_MAX_TOP || (flags & ~FS_BEAM_KEEP_SLOTS) != 0 || !d_parent || !d_tok ||
+        !d_out_score)
+        return FS_E_INVALID;
+    if (!d_row_off && n_streams > 0 && total_rows % n_streams != 0) return FS_E_INVALID;
+    int rc = check_typed(d_logits, type, ld, total_rows, V);
+    if (rc != FS_OK) return rc;
+    fs::BeamArgs a = {};
+    rc = edit_args(edits, total_rows, V, a.ed);
+    if (rc != FS_OK) return rc;
+    if (n_streams == 0) return FS_OK;
+    const hipStream_t st = (hipStream_t)stream;
+    const Edited call(ctx, st);
+    if (call.rc != FS_OK) return call.rc;
+    rc = grow(ctx, 0, 0, 0);
+    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->bm_rows, ctx->bm_row_cap, (size_t)total_rows, 1, false);
+    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->bm_lists, ctx->bm_list_rows, (size_t)total_rows, fs::BM_TOP, false);
+    if (rc != FS_OK) return rc;
+    a.logits = d_logits; a.ld = ld; a.S = n_streams; a.R = total_rows; a.V = V; a.n = n; a.eos = eos_id;
+    a.keep_slots = flags & FS_BEAM_KEEP_SLOTS; a.row_off = d_row_off; a.score = d_score; a.params = d_params;
+    a.parent = d_parent; a.tok = d_tok; a.out_score = d_out_score;
+    a.done = d_done; a.done_parent = d_done_parent; a.done_score = d_done_score;
+    a.rows = ctx->bm_rows; a.lists = ctx->bm_lists; a.err = ctx->err;
+    return fs::launch_beam_select(type, a, st) == hipSuccess ? FS_OK : FS_E_HIP;
+}
+
+int fs_hist_fork(fs_context* ctx, int32_t n_streams, const int32_t* d_hist, const int64_t* d_hist_off,
+                 const int64_t* d_row_off, int32_t n, const int32_t* d_parent, const int32_t* d_tok, int32_t* d_out_hist,
+                 int64_t out_cap, int64_t* d_out_hist_off, void* stream) {
+    if (!ctx || n_streams < 0 || n < 1 || out_cap < 0 || (int64_t)n_streams * n > 0x7fffffff || !d_out_hist_off ||
+        (out_cap > 0 && !d_out_hist))
+        return FS_E_INVALID;
+    if (n_streams > 0 && (!d_hist_off || !d_parent)) return FS_E_INVALID;
+    if (d_out_hist_off == d_hist_off || (d_out_hist && (d_out_hist == d_hist || d_out_hist == d_tok || d_out_hist == d_parent)))
+        return FS_E_INVALID;                                   // out of place
+    const hipStream_t st = (hipStream_t)stream;
+    const Edited call(ctx, st);
+    if (call.rc != FS_OK) return call.rc;
+    const int rc = grow(ctx, 0, 0, 0);
+    if (rc != FS_OK) return rc;
+    fs::ForkArgs a = {};
+    a.hist = d_hist; a.hist_off = d_hist_off; a.row_off = d_row_off; a.S = n_streams; a.n = n; a.parent = d_parent;
+    a.tok = d_tok; a.out = d_out_hist; a.out_cap = out_cap; a.out_off = d_out_hist_off; a.err = ctx->err;
+    return fs::launch_hist_fork(a, st) == hipSuccess ? FS_OK : FS_E_HIP;
+}
+
+int fs_reorder_states(fs_context* ctx, int32_t n_states, const fs_state* states, int32_t n_streams, int32_t n_src, int32_t n,
+                      const int32_t* d_parent, const int32_t* d_from, const int32_t* d_len, void* stream) {
+    if (!ctx || n_states < 0 || (n_states > 0 && !states) || n_streams < 0 || n_src < 1 || n_src > FS_MAX_TOP || n < 1 ||
+        n > FS_MAX_TOP || (n_streams > 0 && !d_parent))
+        return FS_E_INVALID;
+    for (int32_t i = 0; i < n_states; ++i) {
+        const int rc = check_state(states[i], n_streams, n_src, n);
+        if (rc != FS_OK) return rc;
+    }
+    if (n_streams == 0 || n_states == 0) return FS_OK;
+    const hipStream_t st = (hipStream_t)stream;
+    const Edited call(ctx, st);
+    if (call.rc != FS_OK) return call.rc;
+    const int rc = grow(ctx, 0, 0, 0);
+    if (rc != FS_OK) return rc;
+    for (int32_t i = 0; i < n_states;) {           // runs of states whose columns are of one width
+        fs::StateArgs a = {};
+        a.S = n_streams; a.n_src = n_src; a.n = n; a.parent = d_parent; a.from = d_from; a.len = d_len; a.err = ctx->err;
+        const int vb = state_bytes(states[i], n > n_src ? n : n_src);
+        int64_t tiles = 0;
+        int k = 0;
+        for (; i < n_states && k < fs::ST_MAX && state_bytes(states[i], n > n_src ? n : n_src) == vb; ++i) {
+            a.z[k++] = states[i];
+            tiles = std::max(tiles, (state_cols(states[i], vb) + 255) / 256);
+        }
+        if (tiles > 0 && fs::launch_reorder_states(vb, a, k, tiles, st) != hipSuccess) return FS_E_HIP;
+    }
+    return FS_OK;
 }
 
 int fs_penalize_batch(fs_context* ctx, float* d_logits, int64_t ld, int32_t B, int32_t V, const int32_t* d_hist,

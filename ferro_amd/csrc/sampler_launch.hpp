@@ -169,6 +169,60 @@ struct LpArgs {
 };
 hipError_t launch_logprobs(int type, const LpArgs& a, hipStream_t st);
 
+// Beam search (beam_kernels.hip).
+constexpr int BM_TOP = FS_MAX_TOP;         // new beams per stream, at most
+struct BeamRow {                           // a row's sum, and what its candidates' scores follow from
+    double a, z;                           // its score; the logarithm of its sum
+    float M, T, eos;                       // its largest logit, its temperature, the logit that ends the text (-inf: none)
+    int cnt;                               // entries of its list
+};
+struct BeamArgs {
+    const void* logits;
+    int64_t ld;
+    int S, R, V, n, eos;                   // streams, rows
+    int keep_slots;
+    const int64_t* row_off;                // NULL: R / S rows each
+    const float* score;                    // NULL: zeros
+    const fs_row_params* params;           // by stream (NULL: no softcap, temperature 1)
+    EdArgs ed;                             // masks by row, biases by stream
+    int32_t* parent;                       // [S][n]
+    int32_t* tok;
+    float* out_score;
+    int32_t* done;                         // [S]
+    int32_t* done_parent;                  // [S][n]
+    float* done_score;
+    BeamRow* rows;                         // [R]
+    uint64_t* lists;                       // [R][BM_TOP]
+    int32_t* err;
+};
+hipError_t launch_beam_select(int type, const BeamArgs& a, hipStream_t st);
+
+struct ForkArgs {
+    const int32_t* hist;
+    const int64_t* hist_off;
+    const int64_t* row_off;                // NULL: n rows each
+    int S, n;
+    const int32_t* parent;
+    const int32_t* tok;                    // NULL: nothing behind the histories
+    int32_t* out;
+    int64_t out_cap;
+    int64_t* out_off;
+    int32_t* err;
+};
+hipError_t launch_hist_fork(const ForkArgs& a, hipStream_t st);
+
+constexpr int ST_MAX = 32;                 // states per launch (their records travel in the argument segment)
+struct StateArgs {
+    int S, n_src, n;
+    const int32_t* parent;
+    const int32_t* from;
+    const int32_t* len;
+    int32_t* err;
+    fs_state z[ST_MAX];
+};
+// vb: bytes per column (1 to 16); tiles: columns of the largest state over ST_T
+hipError_t launch_reorder_states(int vb, const StateArgs& a, int n_states, int64_t tiles, hipStream_t st);
+
 hipError_t launch_lookup_draft(int n_streams, const int32_t* hist, const int64_t* hist_off, const int32_t* kmax,
                                const int32_t* min_n, int eos, int32_t* draft, int draft_ld, int32_t* ndraft,
                                hipStream_t st);

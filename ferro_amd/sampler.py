@@ -8,6 +8,7 @@
   fs_verify) on torch CUDA tensors, launched on torch's current stream.
 - `Edits` holds masks of allowed tokens and biases (fs_edits) for those calls and `decode_step`; `edit_batch` writes
   edited logits out, `logprobs` gives log-probabilities.
+- `beam_select`, `hist_fork` and `reorder_states` are a beam search's step: the new beams, their histories, their states.
 
 PyTorch only supplies device memory and streams; all sampling arithmetic runs in libferro_sampler.so.
 """
@@ -21,12 +22,14 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from ._lib import FS_BF16, FS_F16, FS_F32, FS_MAX_TOP, PARAMS_DTYPE, FS_OK, FsEdits, SamplerError, check, lib
+from ._lib import (FS_BEAM_KEEP_SLOTS, FS_BF16, FS_F16, FS_F32, FS_MAX_TOP, PARAMS_DTYPE, FS_OK, FsEdits, FsState,
+                   SamplerError, check, lib)
 
 __all__ = ["SamplerParams", "Sampler", "Context", "Rng", "Edits", "params_array", "sample_batch", "argmax_batch", "verify",
-           "edit_batch", "logprobs", "device_error", "PARAMS_DTYPE", "SamplerError"]
+           "edit_batch", "logprobs", "beam_select", "hist_fork", "States", "reorder_states", "device_error", "PARAMS_DTYPE", "SamplerError"]
 
-F32, BF16, F16 = FS_F32, FS_BF16, FS_F16          # types of logits (edit_batch, logprobs)
+F32, BF16, F16 = FS_F32, FS_BF16, FS_F16          # types of logits (edit_batch, logprobs, beam_select)
+BEAM_KEEP_SLOTS = FS_BEAM_KEEP_SLOTS
 
 
 @dataclass
@@ -739,6 +742,182 @@ def logprobs(logits, tok=None, n=0, params=None, edits=None, V=None, ctx=None, s
                                 _on(stream, dev, logits, p, t, lp, rank, ids, top, *(ed.tensors if ed is not None else []))),
               "fs_logprobs")
     return dict(lp=lp, rank=rank, ids=ids, top=top)
+
+
+def _row_off(row_off, rows, dev):
+    """Offsets of streams' rows as a device tensor; host ones are checked."""
+    if not (isinstance(row_off, torch.Tensor) and row_off.is_cuda):
+        o = np.asarray(row_off, np.int64)
+        if o.ndim != 1 or o.size < 1 or o[0] != 0 or o[-1] != rows or np.any(np.diff(o) < 0):
+            raise SamplerError("row_off must ascend from 0 to the last row")
+    return _dev(row_off, torch.int64, dev)
+
+
+def beam_select(logits, score, n, eos_id=-1, params=None, row_off=None, streams=None, keep_slots=False, edits=None, V=None,
+                ctx=None, stream=None):
+    """fs_beam_select: a beam search's step. logits [R, ld] float32, bfloat16 or float16, one row per beam; score [R] (or
+    [S, W]) the beams' sums of log-probabilities, -inf for a beam that has ended (None: zeros). The S streams' rows:
+    row_off (S + 1 offsets), or S alike parts (`streams`, default score.shape[0] of a [S, W] score). params: a record per
+    stream (softcap, temperature); edits: masks by row, biases by stream. Returns dict(parent, tok, score [S, n], done [S],
+    done_parent, done_score [S, n]): the new beams (parent: the row's number in its stream; -1, -1 and -inf past a stream's
+    candidates), best first or, with keep_slots, a parent's best child in its place; and the hypotheses eos_id ends."""
+    logits, ld, v, kind = _typed_logits(logits, V)
+    R, dev = logits.shape[0], logits.device
+    if not 1 <= n <= FS_MAX_TOP:
+        raise SamplerError(f"n must lie in [1, {FS_MAX_TOP}]")
+    if row_off is not None:
+        row_off = _row_off(row_off, R, dev)
+        S = row_off.numel() - 1
+    else:
+        S = streams if streams is not None else score.shape[0] if score is not None and score.dim() == 2 else None
+        if S is None or S < 0 or (R % S if S else R):
+            raise SamplerError("the streams' rows: row_off, streams or a score [streams, rows each]")
+    if score is not None:
+        score = _dev(score, torch.float32, dev)
+        if score.numel() != R:
+            raise SamplerError("one score per row")
+    p = None
+    if params is not None:
+        p = _dev_params(params, dev)
+        if p.numel() != S * PARAMS_DTYPE.itemsize:
+            raise SamplerError("one params record per stream")
+    parent, tok, done_parent = (torch.empty((S, n), dtype=torch.int32, device=dev) for _ in range(3))
+    out, done_score = (torch.empty((S, n), dtype=torch.float32, device=dev) for _ in range(2))
+    done = torch.empty(S, dtype=torch.int32, device=dev)
+    ctx = ctx or Context.default(dev)
+    with torch.cuda.device(dev), ctx.lock:
+        ed = None if edits is None else edits._now(R, S, v, dev)
+        check(lib().fs_beam_select(ctx.h, _lptr(logits), kind, ld, S, R, v, _ptr(row_off), _ptr(score), _ptr(p),
+                                   None if ed is None else ctypes.byref(ed), int(eos_id), n,
+                                   FS_BEAM_KEEP_SLOTS if keep_slots else 0, _ptr(parent), _ptr(tok), _ptr(out), _ptr(done),
+                                   _ptr(done_parent), _ptr(done_score),
+                                   _on(stream, dev, logits, row_off, score, p, parent, tok, out, done, done_parent, done_score,
+                                       *(ed.tensors if ed is not None else []))),
+              "fs_beam_select")
+    return dict(parent=parent, tok=tok, score=out, done=done, done_parent=done_parent, done_score=done_score)
+
+
+def _parents(parent, dev):
+    parent = _dev(parent, torch.int32, dev)
+    if parent.dim() != 2:
+        raise SamplerError("parents are [streams, beams]")
+    return parent
+
+
+def hist_fork(hist, hist_off, parent, tok=None, row_off=None, out_cap=None, ctx=None, stream=None):
+    """fs_hist_fork: the new beams' histories. hist, hist_off: CSR histories of the present beams, whose rows row_off gives
+    (None: as many per stream as there are new ones); parent, tok [S, n] (tok None: nothing is appended), as beam_select
+    returns them. Returns (out_hist, out_off): row s * n + j the history of beam j of stream s; out_hist holds out_cap ids
+    (default: room for any parents). Nothing here waits for the GPU."""
+    dev = parent.device if isinstance(parent, torch.Tensor) and parent.is_cuda else torch.device("cuda", torch.cuda.current_device())
+    parent = _parents(parent, dev)
+    S, n = parent.shape
+    hist, hist_off = _dev(hist, torch.int32, dev), _dev(hist_off, torch.int64, dev)
+    rows = hist_off.numel() - 1
+    if row_off is not None:
+        row_off = _row_off(row_off, rows, dev)
+        if row_off.numel() != S + 1:
+            raise SamplerError("row_off must have an entry per stream and one more")
+    elif rows != S * n:
+        raise SamplerError("hist_off must have an entry per beam and one more")
+    if tok is not None:
+        tok = _dev(tok, torch.int32, dev)
+        if tok.numel() != S * n:
+            raise SamplerError("one token per beam")
+    if out_cap is None:
+        out_cap = hist.numel() * n + S * n
+    out = torch.empty(max(int(out_cap), 1), dtype=torch.int32, device=dev)
+    out_off = torch.empty(S * n + 1, dtype=torch.int64, device=dev)
+    ctx = ctx or Context.default(dev)
+    with torch.cuda.device(dev), ctx.lock:
+        check(lib().fs_hist_fork(ctx.h, S, _ptr(hist), _ptr(hist_off), _ptr(row_off), n, _ptr(parent), _ptr(tok), _ptr(out),
+                                 int(out_cap), _ptr(out_off),
+                                 _on(stream, dev, hist, hist_off, row_off, parent, tok, out, out_off)), "fs_hist_fork")
+    return out, out_off
+
+
+class States:
+    """State buffers that follow their beams (fs_state records), kept from step to step for reorder_states: caches of keys and
+    values, convolution and recurrent states, block tables. Tensors [rows, ...] of any type; dst: the buffers they are
+    written into (default: in place). pos_dim: the dimension of a cache's positions (None: a state without any, which
+    follows whole), one for all or one per tensor. The dimensions behind the positions must be packed, those before them one
+    stride apart; strides are otherwise free."""
+
+    def __init__(self, tensors, dst=None, pos_dim=None):
+        self.src = list(tensors)
+        self.dst = self.src if dst is None else list(dst)
+        if len(self.dst) != len(self.src):
+            raise SamplerError("one buffer to write per state")
+        dims = list(pos_dim) if isinstance(pos_dim, (list, tuple)) else [pos_dim] * len(self.src)
+        if len(dims) != len(self.src):
+            raise SamplerError("one pos_dim per state")
+        self.device = self.src[0].device if self.src else torch.device("cuda")
+        self.src_rows = self.src[0].shape[0] if self.src else 0
+        self.dst_rows = self.dst[0].shape[0] if self.src else 0
+        self.c = (FsState * max(len(self.src), 1))(*[self._state(*a) for a in zip(self.src, self.dst, dims)])
+
+    def __len__(self):
+        return len(self.src)
+
+    def _state(self, a, b, pos):
+        if a.dim() < 1 or a.dtype != b.dtype or a.dim() != b.dim() or a.device != self.device or b.device != self.device:
+            raise SamplerError("states and the buffers they are written into must be alike, on one device")
+        if pos is not None and pos < 0:
+            pos += a.dim()
+        if pos is not None and not 1 <= pos < a.dim():
+            raise SamplerError("pos_dim is a dimension behind the rows")
+        if a.shape[0] != self.src_rows or b.shape[0] != self.dst_rows or \
+                any(a.shape[i] != b.shape[i] for i in range(1, a.dim()) if i != pos):
+            raise SamplerError("states of other rows or shapes")
+        size = a.element_size()
+        z = FsState(d_src=a.data_ptr(), d_dst=b.data_ptr(), src_row=a.stride(0) * size, dst_row=b.stride(0) * size)
+        run, i = size, a.dim() - 1                             # the packed dimensions at the end
+        while i > (0 if pos is None else pos) and (a.shape[i] == 1 or a.stride(i) * size == b.stride(i) * size == run):
+            run, i = run * a.shape[i], i - 1
+        if pos is not None and i > pos:
+            raise SamplerError("the dimensions behind a state's positions must be packed")
+        z.pos_bytes, z.blocks = run, 1
+        if pos is not None:
+            z.positions = min(a.shape[pos], b.shape[pos])
+            z.src_pos, z.dst_pos, i = a.stride(pos) * size, b.stride(pos) * size, pos - 1
+            if z.positions == 0:
+                z.blocks = 0
+        for i in range(i, 0, -1):                              # the others: blocks one stride apart
+            if a.shape[i] == 1:
+                continue
+            if z.blocks > 1 and (a.stride(i) * size != z.blocks * z.src_block or b.stride(i) * size != z.blocks * z.dst_block):
+                raise SamplerError("the dimensions before a state's positions must be one stride apart")
+            if z.blocks == 1:
+                z.src_block, z.dst_block = a.stride(i) * size, b.stride(i) * size
+            z.blocks *= a.shape[i]
+        return z
+
+
+def reorder_states(states, parent, start=None, length=None, ctx=None, stream=None):
+    """fs_reorder_states: row s * n + j of every state gets what row (s, parent[s, j]) held, parent [S, n] as beam_select
+    returns it (below 0: the row stays as it was). states: a States, or tensors without positions. start, length [S]: the
+    positions that follow, from `start` (default 0; what a stream's beams share before it need not move) to `length`
+    (default: all). Returns the tensors written."""
+    if not isinstance(states, States):
+        states = States(states)
+    dev = states.device
+    if dev.type != "cuda":
+        raise SamplerError("states must be CUDA tensors")
+    parent = _parents(parent, dev)
+    S, n = parent.shape
+    if len(states) == 0 or S == 0:
+        return states.dst
+    if states.src_rows % S or states.dst_rows != S * n:
+        raise SamplerError(f"states of {states.src_rows} and {states.dst_rows} rows for {S} streams of {n} beams")
+    lens = [None if t is None else _dev(t, torch.int32, dev) for t in (start, length)]
+    if any(t is not None and t.numel() != S for t in lens):
+        raise SamplerError("one start and one length per stream")
+    ctx = ctx or Context.default(dev)
+    with torch.cuda.device(dev), ctx.lock:
+        check(lib().fs_reorder_states(ctx.h, len(states), states.c, S, states.src_rows // S, n, _ptr(parent), _ptr(lens[0]),
+                                      _ptr(lens[1]), _on(stream, dev, parent, *lens, *states.src, *states.dst)),
+              "fs_reorder_states")
+    return states.dst
 
 
 def device_error(ctx=None, stream=None) -> int:

@@ -48,6 +48,8 @@ extern "C" {
                                         written), or a count lies outside [0, its stream's rows] (clamped) */
 
 #define FS_DEVERR_MASK 8             /* a row's mask index lies past the last mask: no token of the row is allowed */
+#define FS_DEVERR_PARENT 16          /* fs_hist_fork, fs_reorder_states: a parent past its stream's rows (its beam is left
+                                        without a history, its states as they were) */
 
 /* Types of logits (fs_edit_batch, fs_logprobs; the sampling calls read FS_F32). */
 #define FS_F32 0
@@ -326,6 +328,57 @@ int fs_edit_batch(fs_context* ctx, const void* d_logits, int32_t type, int64_t l
 int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld, int32_t B, int32_t V,
                 const fs_row_params* d_params, const fs_edits* edits, const int32_t* d_tok, int32_t n, float* d_lp,
                 int32_t* d_rank, int32_t* d_top_ids, float* d_top_lp, void* stream);
+
+/* Beam search: a step's selection. Stream s (one request) has the beams of the logits rows d_row_off[s] .. d_row_off[s+1]-1
+ * (as fs_verify's; NULL: total_rows / n_streams rows each) with the scores d_score (sums of log-probabilities; NULL: zeros).
+ * Token t of row r is the candidate
+ *     c(r, t) = d_score[r] + log softmax((cap(l) + bias) / T)(t)      (fs_logprobs' distribution, by the stream's record)
+ * in fp64; a token that is not allowed, whose logit is NaN or -inf, or whose c does not round to a fp32 above -inf is none.
+ * Candidates come by c; among equal ones those of eos_id (-1: none) first, then the lower row's, in a row the larger logit's,
+ * then the lower token's. The n best (n <= FS_MAX_TOP) whose token is not eos_id are the new beams: d_parent [n_streams][n]
+ * (the row's number in its stream, from 0), d_tok, d_out_score; places past a stream's candidates hold -1, -1 and -inf. Those
+ * with eos_id that fewer than n candidates come before are ended hypotheses: their number d_done[s] and, in their order,
+ * d_done_parent and d_done_score [n_streams][n], -1 and -inf past them (each may be NULL; min(n, the stream's rows) at most).
+ * Rows whose score is -inf or NaN have no candidate and are not read: the last step's d_out_score is this step's d_score.
+ * flags: FS_BEAM_KEEP_SLOTS puts a parent's best child into the parent's own place (where that is below n) and the others, in
+ * their order, into the free places, ascending: a state then moves for a parent's further children alone; without it the
+ * beams come best first. edits: masks by row, biases by stream, may be NULL; penalties are fs_edit_batch's. d_params NULL: no
+ * softcap, T = 1. Rows and types as in fs_edit_batch. No counterpart in the reference (ferro samples). */
+#define FS_BEAM_KEEP_SLOTS 1
+int fs_beam_select(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld, int32_t n_streams, int32_t total_rows,
+                   int32_t V, const int64_t* d_row_off, const float* d_score, const fs_row_params* d_params,
+                   const fs_edits* edits, int32_t eos_id, int32_t n, int32_t flags, int32_t* d_parent, int32_t* d_tok,
+                   float* d_out_score, int32_t* d_done, int32_t* d_done_parent, float* d_done_score, void* stream);
+
+/* The new beams' histories: beam j of stream s (row s * n + j) gets the history of row d_parent[s * n + j] of the stream
+ * (its rows: d_row_off, NULL: s * n .. s * n + n - 1) and d_tok[s * n + j] behind it (d_tok NULL: nothing); a parent below 0
+ * leaves it empty. Histories are CSR, as fs_hist_append's: d_hist_off has one entry more than there are rows, the new
+ * offsets d_out_hist_off n_streams * n + 1, from 0; ids past out_cap are not written and set FS_DEVERR_HIST_APPEND. Out of
+ * place: the outputs must not overlap the inputs. d_hist may be NULL where every history is empty. */
+int fs_hist_fork(fs_context* ctx, int32_t n_streams, const int32_t* d_hist, const int64_t* d_hist_off,
+                 const int64_t* d_row_off, int32_t n, const int32_t* d_parent, const int32_t* d_tok, int32_t* d_out_hist,
+                 int64_t out_cap, int64_t* d_out_hist_off, void* stream);
+
+/* A model's state by rows: caches of keys and values, convolution and recurrent states, block tables, of any type. A row
+ * holds `blocks` blocks of `positions` positions of pos_bytes bytes each; strides in bytes, none negative. */
+typedef struct fs_state {
+    const void* d_src;
+    void* d_dst;                /* d_src: in place (equal strides, as many rows per stream) */
+    int64_t src_row, src_block, src_pos;   /* from a row, a block (a head), a position to the next */
+    int64_t dst_row, dst_block, dst_pos;
+    int64_t pos_bytes;
+    int32_t blocks;
+    int32_t positions;          /* 0: a state without positions, whose blocks of pos_bytes bytes follow whole */
+} fs_state;
+
+/* States follow their beams: row s * n + j of each d_dst gets what row s * n_src + d_parent[s * n + j] of its d_src held, of
+ * positions [d_from[s], d_len[s]) (NULL: 0, the state's positions; cut to those), the rest of d_dst stays as it was. In place
+ * rows of a stream may change places, be copied more than once or dropped. d_from is for what a stream's beams share (the
+ * prompt), which need not move. A parent below 0 leaves its row as it was. n, n_src <= FS_MAX_TOP; n_src = 1 opens the beams
+ * of prompts. `states` is host memory, read before the call returns; the states' rows must not overlap one another, nor a
+ * d_dst any other state of the call (in place: its own d_src alone). */
+int fs_reorder_states(fs_context* ctx, int32_t n_states, const fs_state* states, int32_t n_streams, int32_t n_src, int32_t n,
+                      const int32_t* d_parent, const int32_t* d_from, const int32_t* d_len, void* stream);
 
 /* Gemma 4's final-logit softcap as the sampler applies it (fs_row_params.softcap): d_out[i] = cap * tanhf(d_in[i] /
  * cap), the host loop of model_gemma4_gpu.cpp:282-283, bit-identical to it on a glibc host (its float tanh is
