@@ -28,6 +28,10 @@
 // cycles). 1024 rows of 151936 bf16: 57.1 us for the chosen token's alone, 62.9 with n 1 (4.9 TB/s of 311 MB). 64 rows of
 // 262144 fp32: 14.8 us, 20.8 with n 5, 24.1 with n 20, and 25.6 with n 20 under masks and biases: the lists and the row's end,
 // a chain behind the last read. One row of 65536 with n 5: 8.7 us, of which the read is about 1.
+//
+// fs_beam_select runs the same kernel (BEAM): a row is a beam, whose lists leave eos out (its logit is kept by itself, as the
+// chosen token's), and whose parts end in their stream's (beam_device.hpp).
+#include "beam_device.hpp"
 #include "edit_device.hpp"
 #include "row_device.hpp"
 
@@ -36,12 +40,18 @@ namespace fs {
 constexpr int LP_GROUPS = 256;             // groups of four in a wave's list
 constexpr int LP_GROWN = 16;               // groups in a list since its bound was taken, after which it is taken again
 
-struct LpShared {
+struct __attribute__((aligned(16))) LpShared {
     float4 gval[SK_NW][LP_GROUPS];         // (the row's end gathers its tokens here)
     int gid[SK_NW][LP_GROUPS];             // the id of a group's first token
     uint64_t kept[SK_NW][LP_TOP];          // what a cut left: sorted, 0 past the entries
     float bound[SK_NW];
 };
+union LpBeamShared {
+    LpShared lp;
+    BeamShared bm;                         // once the part's lists are published
+};
+__device__ __forceinline__ LpShared& lp_shared(LpShared& s) { return s; }
+__device__ __forceinline__ LpShared& lp_shared(LpBeamShared& s) { return s.lp; }
 
 constexpr float LP_NONE = -__builtin_huge_valf(), LP_LOWEST = -3.402823466e+38f;
 
@@ -82,6 +92,22 @@ __device__ __forceinline__ uint32_t lp_nth(const uint32_t (&key)[K], uint32_t lo
     return lo;
 }
 
+// BEAM: of four maxima per lane. A few tokens are found by the lanes' largest alone; for many these are too few, and the least
+// of them lets most of the logits pass (128 rows of 100003 fp16, n 64: 88 us).
+__device__ __forceinline__ uint32_t lp_nth_set(const float (&ls)[4], float reach, int n) {
+    uint32_t from;
+    auto at_least = [&](uint32_t f) { return reach > LP_LOWEST && f < key_of(reach) ? key_of(reach) : f; };
+    if (n <= 16) {
+        const uint32_t key[1] = {key_of(lp_max3(lp_max3(ls[0], ls[1], ls[2]), ls[3], ls[3]))};
+        return lp_nth(key, at_least(wave_min(key[0])), n);
+    }
+    const uint32_t key[4] = {key_of(ls[0]), key_of(ls[1]), key_of(ls[2]), key_of(ls[3])};
+    from = key[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) from = key[i] < from ? key[i] : from;
+    return lp_nth(key, at_least(wave_min(from)), n);
+}
+
 // What the wave keeps of its list of g groups and an earlier cut: its n largest tokens at or above the bound, sorted, one
 // per lane, 0 past them (also in s.kept).
 __device__ __forceinline__ uint64_t lp_cut(LpShared& s, int& g, bool& cut, float bound, int n) {
@@ -103,19 +129,287 @@ __device__ __forceinline__ uint64_t lp_cut(LpShared& s, int& g, bool& cut, float
 }
 
 // The kernel's argument list as a struct: the argument segment follows the same layout rules
+template <class A>
 struct LpKernargs {
     const void* logits;
     int64_t ld;
     int B, V, nseg, n;
-    LpArgs a;
+    A a;
 };
+__device__ __forceinline__ const LpArgs& lp_args(const LpArgs& a) { return a; }
+__device__ __forceinline__ const LpArgs& lp_args(const LpBeamArgs& a) { return a.lp; }
 
-// NL: groups of four per thread and chunk. TOP: the n largest are asked for.
-template <int TYPE, int NL, bool TOP>
+// Where a row's waves publish what they found (lp_row_bytes).
+struct LpRow {
+    double* sum;
+    float* max;
+    uint32_t* above;                       // (BEAM: of wave 0, the logit that ends the text)
+    float* bound;
+    int* cnt;
+    uint32_t* key;
+};
+__device__ __forceinline__ LpRow lp_row(const LpArgs& a, int64_t row, int nseg) {
+    const int lists = nseg * SK_NW;
+    LpRow r;
+    r.sum = reinterpret_cast<double*>(a.rows + row * (int64_t)lp_row_bytes(nseg));
+    r.max = reinterpret_cast<float*>(r.sum + lists);
+    r.above = reinterpret_cast<uint32_t*>(r.max + lists);
+    r.bound = reinterpret_cast<float*>(r.above + lists);
+    r.cnt = reinterpret_cast<int*>(r.bound + lists);
+    r.key = reinterpret_cast<uint32_t*>(r.cnt + lists);
+    return r;
+}
+
+// BEAM: what a wave publishes. Its tokens at or above the best of the part's bounds, BM_LIST of them or the n largest.
+__device__ __forceinline__ void beam_publish(const LpArgs& a, LpShared& s, int row, int part, int nseg, int n, double sum, float mx,
+                                             float xv, const float (&ls)[4], float reach, int g, bool cut) {
+    const int lane = lane_id(), w = (int)threadIdx.x / WAVE, me = part * SK_NW + w;
+    const LpRow p = lp_row(a, row, nseg);
+    uint64_t* out = a.lists + ((int64_t)row * nseg * SK_NW + me) * BM_LIST;
+    sum = wave_allreduce(sum, [](double u, double v) { return u + v; });
+    if (n > 16) {                                              // (many tokens: a fresh bound leaves few to write and to read)
+        const uint32_t nth = lp_nth_set(ls, reach, n);
+        reach = fmaxf(reach, nth > 0x007FFFFFu ? val_of(nth) : LP_LOWEST);
+    }
+    if (lane == 0) s.bound[w] = reach;
+    __syncthreads();
+    reach = fmaxf(fmaxf(s.bound[0], s.bound[1]), fmaxf(s.bound[2], s.bound[3]));
+    int cnt = 0;
+    bool fits = !cut;
+#pragma unroll 1
+    for (int i = 0; fits && i < g; i += WAVE) {
+        const bool in = i + lane < g;
+        const float4 v = in ? s.gval[w][i + lane] : make_float4(LP_NONE, LP_NONE, LP_NONE, LP_NONE);
+        const uint32_t id = in ? (uint32_t)s.gid[w][i + lane] : 0u;
+        const float y[4] = {v.x, v.y, v.z, v.w};
+        uint64_t m[4];
+        int all = cnt;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            m[c] = __ballot(y[c] >= reach);
+            all += __popcll(m[c]);
+        }
+        fits = all <= BM_LIST;
+        if (fits) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (y[c] >= reach) st_agent(out + cnt + (int)mbcnt(m[c]), comp_of(key_of(y[c]), id + (uint32_t)c));
+                cnt += __popcll(m[c]);
+            }
+        }
+    }
+    if (!fits) {                                               // a list that was cut, or equal logits at the bound
+        const uint64_t e = lp_cut(s, g, cut, reach, n);
+        cnt = __popcll(__ballot(e != 0ull));
+        if (lane < cnt) st_agent(out + lane, e);
+    }
+    const float lm = lp_max3(lp_max3(ls[0], ls[1], ls[2]), ls[3], ls[3]);
+    uint32_t top = lm > LP_NONE ? key_of(lm) : 0u;
+    auto both = [](uint32_t u, uint32_t v) { return u > v ? u : v; };
+    top = both(top, xor_lane32<1>(top));
+    top = both(top, xor_lane32<2>(top));
+    if (nseg > 4) top = both(top, xor_lane32<4>(top));
+    if (nseg > 8) top = both(top, xor_lane32<8>(top));
+    if (nseg > 16) top = both(top, xor_lane32<16>(top));
+    if (nseg > 32) top = both(top, xor_lane32<32>(top));
+    const int lg = lp_group(nseg);
+    if ((lane & ((1 << lg) - 1)) == 0) st_agent(p.key + (((me << 6) + lane) >> lg), top);
+    if (lane == 0) {
+        st_agent(reinterpret_cast<uint64_t*>(p.sum + me), (uint64_t)__double_as_longlong(sum));
+        st_agent(reinterpret_cast<uint32_t*>(p.max + me), __float_as_uint(mx));
+        st_agent(p.cnt + me, cnt);
+        if (me == 0) st_agent(p.above, __float_as_uint(xv));
+    }
+}
+
+// BEAM: a row's end, by one wave: its sum, and its n largest tokens (one per lane, in order; 0 past them).
+__device__ __forceinline__ uint64_t beam_row_end(const LpArgs& a, BeamShared& s, int64_t row, int nseg, int n, float score, float T,
+                                                 BeamRow& br) {
+    const int lane = lane_id(), w = (int)threadIdx.x / WAVE, lists = nseg * SK_NW;
+    const LpRow p = lp_row(a, row, nseg);
+    const uint64_t* rl = a.lists + row * lists * BM_LIST;
+    constexpr int LL = LP_PARTS * SK_NW / WAVE;
+    double si[LL];
+    float mi[LL];
+    uint32_t key[LL];
+    int len[LL];
+#pragma unroll
+    for (int u = 0; u < LL; ++u) {
+        const int i = u * WAVE + lane;
+        const bool in = i < lists;
+        si[u] = 0.0;
+        mi[u] = LP_LOWEST;
+        len[u] = 0;
+        key[u] = 0u;
+        if (u * WAVE < lists) {                                // (uniform)
+            si[u] = in ? __longlong_as_double((long long)ld_agent(reinterpret_cast<const uint64_t*>(p.sum + i))) : 0.0;
+            mi[u] = in ? __uint_as_float(ld_agent(reinterpret_cast<const uint32_t*>(p.max + i))) : LP_LOWEST;
+            len[u] = in ? ld_agent(p.cnt + i) : 0;
+        }
+        if (u * WAVE < (lists << 6) >> lp_group(nseg)) key[u] = i < (lists << 6) >> lp_group(nseg) ? ld_agent(p.key + i) : 0u;
+    }
+    const float xv = __uint_as_float(ld_agent(p.above));
+    auto fmx = [](float u, float v) { return fmaxf(u, v); };
+    // a bound that n tokens reach (that there are lists above it which lack tokens that reach it does no harm: they have n)
+    uint32_t least = 1u;
+    if (n <= 16) {
+        uint32_t k1 = key[0];
+#pragma unroll
+        for (int u = 1; u < LL; ++u) k1 = key[u] > k1 ? key[u] : k1;
+        const uint32_t nth = read_lane(sort64_desc_u32(k1), n - 1);
+        least = nth > least ? nth : least;
+    } else {
+        least = lp_nth(key, least, n);
+    }
+    // lists of waves whose largest logit reaches the bound; half a wave reads 32 entries of one
+    constexpr int U = 4, ROOM = sizeof(s.gather[0]) / sizeof(uint64_t);
+    uint16_t* at = s.at[w];
+    uint64_t* join = s.gather[w];
+    int k = 0;
+#pragma unroll
+    for (int u = 0; u < LL; ++u) {
+        if (u * WAVE >= lists) break;                          // uniform
+        const bool in = len[u] > 0 && key_of(mi[u]) >= least;
+        const uint64_t m = __ballot(in);
+        if (in) at[k + (int)mbcnt(m)] = (uint16_t)(((u * WAVE + lane) << 8) | len[u]);
+        k += __popcll(m);
+    }
+    lp_wave_sync();
+    const int half = lane >> 5, pos = lane & 31;
+    int to[U];
+    uint64_t e[U];
+    auto fetch = [&](int i0, int skip) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + 2 * u + half;
+            to[u] = i < k ? at[i] : 0;
+            e[u] = pos + skip < (to[u] & 255) ? ld_agent(rl + (to[u] >> 8) * BM_LIST + pos + skip) : 0ull;
+        }
+    };
+    fetch(0, 0);
+    float M = LP_LOWEST;
+#pragma unroll
+    for (int u = 0; u < LL; ++u) M = fmaxf(M, mi[u]);
+    M = wave_allreduce(M, fmx);
+    double S = 0.0;
+#pragma unroll 1
+    for (int u = 0; u * WAVE < lists; ++u) {                   // relative to the row's maximum
+        const float m_ = u == 0 ? mi[0] : u == 1 ? mi[1] : u == 2 ? mi[2] : mi[3];
+        const double s_ = u == 0 ? si[0] : u == 1 ? si[1] : u == 2 ? si[2] : si[3];
+        S += m_ == M ? s_ : M < __builtin_huge_valf() ? s_ * exp(((double)m_ - (double)M) / (double)T) : 0.0;
+    }
+    S = wave_allreduce(S, [](double u, double v) { return u + v; });
+    br = {(double)score, log(S), M, T, xv > LP_NONE ? xv : LP_NONE, 0};
+    int cnt = 0;
+    uint64_t acc = 0ull;
+    bool sorted = false;
+    auto sort = [&]() {
+        lp_wave_sync();
+#pragma unroll 1
+        for (int i = 0; i < cnt; i += WAVE) acc = merge_top64(acc, sort64<false>(i + lane < cnt ? join[i + lane] : 0ull));
+        lp_wave_sync();
+        cnt = 0;
+        sorted = true;
+    };
+#pragma unroll 1
+    for (int i0 = 0, skip = 0; i0 < k;) {
+        bool more = false;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool in = comp_key(e[u]) >= least;
+            const uint64_t m = __ballot(in);
+            if (in) join[cnt + (int)mbcnt(m)] = e[u];
+            cnt += __popcll(m);
+            more |= (to[u] & 255) > skip + 32;
+        }
+        const bool longer = __ballot(more) != 0ull;            // lists that have more entries
+        skip = longer ? skip + 32 : 0;
+        i0 = longer ? i0 : i0 + 2 * U;
+        const bool last = i0 >= k;
+        if (cnt > ROOM - U * WAVE || (last && (sorted || cnt > WAVE))) sort();
+        if (!last) fetch(i0, skip);
+    }
+    lp_wave_sync();
+    if (!sorted) {                                             // ranks: an eighth of a sort's instructions
+        const uint64_t c = lane < cnt ? join[lane] : 0ull;
+        int r = 0;
+#pragma unroll 4
+        for (int i = 0; i < cnt; ++i) r += join[i] > c ? 1 : 0;
+        lp_wave_sync();
+        join[lane] = 0ull;
+        lp_wave_sync();
+        if (c != 0ull) join[r] = c;
+        lp_wave_sync();
+        acc = join[lane];
+        lp_wave_sync();
+    }
+    return lane < n ? acc : 0ull;
+}
+
+// BEAM: the end of a part. The last part of a stream of few rows ends its rows, a wave each at a time, and the stream; in
+// others a row's last part ends the row and the last row's workgroup the stream.
+__device__ __forceinline__ void beam_end(const LpBeamArgs& args, LpShared& s, BeamShared& bm, const BeamStream& st, int row, int part,
+                                         int nseg, float T, bool dead, double sum, float mx, float xv, const float (&ls)[4],
+                                         float reach, int g, bool cut) {
+    const LpArgs& a = args.lp;
+    const BeamArgs& b = args.b;
+    const int tid = threadIdx.x, lane = lane_id(), w = tid / WAVE, n = b.n, m = st.m;
+    const bool ends = b.eos >= 0 && (b.done || b.done_parent || b.done_score);
+    const bool once = m <= BM_ROWS && bm_is_few(m, n);
+    bool few = once;
+    uint32_t* ticket = b.ticket + (int64_t)st.s * LP_LINE;
+    if (!dead) beam_publish(a, s, row, part, nseg, n, sum, mx, xv, ls, reach, g, cut);
+    if (once) {
+        if (!bm_last(bm, ticket, dead ? (uint32_t)nseg : 1u, (uint32_t)(m * nseg))) return;
+    } else if (!dead) {
+        if (!bm_last(bm, a.ticket + (int64_t)row * LP_LINE, 1u, (uint32_t)nseg)) return;
+    }
+#pragma unroll 1
+    for (int r = once ? w : 0; r < (once ? m : w == 0 && !dead ? 1 : 0); r += SK_NW) {
+        const int64_t q = once ? st.r0 + r : (int64_t)row;
+        const float score = b.score ? ld_const(b.score + q) : 0.0f;
+        BeamRow br = bm_dead_row();
+        uint64_t acc = 0ull;
+        if (score > LP_NONE) acc = beam_row_end(a, bm, q, nseg, n, score, T, br);
+        if (once) {
+            if (lane == 0) bm.row[r] = br;
+            if (lane < n) bm.list[r * n + lane] = acc;
+        } else {
+            if (lane == 0) bm_store_row(b, q, br);
+            if (lane < n) st_agent(b.row_lists + q * BM_TOP + lane, acc);
+        }
+    }
+    if (!once) {
+        if (!bm_last(bm, ticket, 1u, (uint32_t)m)) return;
+        few = bm_is_few(m, n);
+        if (few) {
+            if (tid < m) bm.row[tid] = bm_load_row(b, st.r0 + tid);
+            if (tid < m * n) bm.list[tid] = ld_agent(b.row_lists + (st.r0 + tid / n) * BM_TOP + tid % n);
+        }
+    }
+    __syncthreads();
+    if (few) {
+        bm_few(b, bm, m, ends);
+        __syncthreads();
+    }
+    if (w != 0) return;
+    if (!few) bm_join(b, bm, st.r0, m, ends);
+    bm_finish(b, bm.best, st.s);
+    if (!b.row_off) return;
+    for (int e = st.s + 1; e < b.S && ld_const(b.row_off + e + 1) == st.r0 + m; ++e) bm_nothing(b, e);   // streams without rows
+    if (st.r0 == 0)
+        for (int e = 0; e < st.s; ++e) bm_nothing(b, e);
+}
+
+// NL: groups of four per thread and chunk. TOP: the n largest are asked for. BEAM: the rows are beams (fs_beam_select).
+template <int TYPE, int NL, bool TOP, bool BEAM>
 __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, int64_t ld, int B, int V, int nseg, int n,
-                                                           LpArgs a_) {
+                                                           std::conditional_t<BEAM, LpBeamArgs, LpArgs> a_) {
+    static_assert(TOP || !BEAM, "beams come from lists");
+    using Kernargs = LpKernargs<std::conditional_t<BEAM, LpBeamArgs, LpArgs>>;
     constexpr int CHUNK = SK_LT * NL * 4;
-    __shared__ __align__(16) LpShared s;
+    __shared__ __align__(16) std::conditional_t<BEAM, LpBeamShared, LpShared> shared;
+    LpShared& s = lp_shared(shared);
     const int tid = threadIdx.x, lane = lane_id(), w = tid / WAVE;
     // a row's parts are consecutive workgroups of one index class mod XCDS, as in the small-k kernel
     const int j = (int)(blockIdx.x / (unsigned)XCDS);
@@ -144,8 +438,17 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
     const __attribute__((address_space(4))) char* kseg =       // (as in the small-k kernel: no argument is read earlier)
         (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(kseg) : : "memory");
-    const LpArgs& a = *(const LpArgs*)(kseg + offsetof(LpKernargs, a));
+    const auto& args = *(const decltype(a_)*)(kseg + offsetof(Kernargs, a));
+    const LpArgs& a = lp_args(args);
     (void)a_;
+    int rec = row;                                             // the record of its parameters and biases
+    float score = 0.0f;
+    BeamStream beams = {0, 0, 0};
+    if constexpr (BEAM) {
+        beams = bm_stream(args.b, row, B);
+        rec = beams.s;
+        score = args.b.score ? ld_const(args.b.score + row) : 0.0f;
+    }
     EdRow r = {nullptr, false, nullptr, nullptr, 0};
     ed_mask(r, a.ed, row, a.err);
     const bool masked = r.words || r.closed;
@@ -153,13 +456,15 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
         bits = ed_bits<NL>(r, c0 * CHUNK, V);
         if (c0 + 1 < c1) next = ed_bits<NL>(r, (c0 + 1) * CHUNK, V);
     }
-    ed_bias(r, a.ed, row);
+    ed_bias(r, a.ed, rec);
     const EdList few = ed_list<false>(r);
-    const int t = a.tok ? ld_const(a.tok + row) : -1;
+    int t = -1;
+    if constexpr (BEAM) t = args.b.eos;
+    else t = a.tok ? ld_const(a.tok + row) : -1;
     float cap = 0.0f, T = 1.0f;
     if (a.params) {
-        cap = ld_const(&a.params[row].softcap);
-        T = ld_const(&a.params[row].temperature);
+        cap = ld_const(&a.params[rec].softcap);
+        T = ld_const(&a.params[rec].temperature);
         if (!(T > 0.0f)) T = 1.0f;                             // greedy rows: the distribution itself
     }
     auto fmx = [](float u, float v) { return fmaxf(u, v); };
@@ -176,17 +481,22 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
         xv = ed_one(r, few, xv, t);
         xv = xv > LP_NONE ? xv : __builtin_nanf("");
     }
-    const bool has = xv < __builtin_huge_valf();               // (none is larger than +inf)
+    const bool has = !BEAM && xv < __builtin_huge_valf();      // (none is larger than +inf)
+
+    const bool dead = BEAM && !(score > LP_NONE);              // a dead beam (NaN, too): no candidates
+    if (dead && part != 0) return;
+    const int c_end = dead ? c0 : c1;
 
     float mx = LP_LOWEST;                                      // the wave's largest logit: its sums' reference
     double sum = 0.0;
     uint32_t above = 0u;                                       // the wave's count
     // TOP: the bound of new candidates; what n logits of the wave reach; the lane's largest logit
     float bound = LP_LOWEST, reach = LP_LOWEST, lm = LP_NONE;
+    float ls[4] = {LP_NONE, LP_NONE, LP_NONE, LP_NONE};        // BEAM: of a fourth of its groups each (lm unused)
     int g = 0, bound_at = -LP_GROWN;                           // groups in the list, and when the bound was taken
     bool cut = false;
 #pragma unroll 1
-    for (int c = c0; c < c1; ++c) {
+    for (int c = c0; c < c_end; ++c) {
         const int lo = c * CHUNK, n_in = V - lo < CHUNK ? V - lo : CHUNK;
         float x[NL][4];
 #pragma unroll
@@ -200,7 +510,7 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
 #pragma unroll
             for (int q = 0; q < NL; ++q) softcap_vals(x[q], cap);
         }
-        if (few.nb > 0) ed_add<NL, false>(a.ed, row, few, nullptr, lo, n_in, [&](int q, int c_) -> float& { return x[q][c_]; });
+        if (few.nb > 0) ed_add<NL, false>(a.ed, rec, few, nullptr, lo, n_in, [&](int q, int c_) -> float& { return x[q][c_]; });
         if (masked) {
 #pragma unroll
             for (int q = 0; q < NL; ++q) {
@@ -216,7 +526,15 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
                 for (int c_ = 0; c_ < 4; ++c_) x[q][c_] = (q * SK_LT + tid) * 4 + c_ < n_in ? x[q][c_] : LP_NONE;
         }
         float cm = LP_NONE;                                    // the chunk's largest of the lane
+        float cs[4] = {LP_NONE, LP_NONE, LP_NONE, LP_NONE};
         auto lane_max = [&]() {
+            if constexpr (BEAM) {
+#pragma unroll
+                for (int q = 0; q < NL; ++q)
+                    cs[q & 3] = lp_max3(lp_max3(q < 4 ? LP_NONE : cs[q & 3], x[q][0], x[q][1]), x[q][2], x[q][3]);
+                cm = lp_max3(lp_max3(cs[0], cs[1], cs[2]), cs[3], cs[3]);
+                return;
+            }
             cm = LP_NONE;
 #pragma unroll
             for (int q = 0; q < NL; ++q) cm = lp_max3(lp_max3(cm, x[q][0], x[q][1]), x[q][2], x[q][3]);
@@ -311,14 +629,31 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
 #pragma unroll
                 for (int c_ = 0; c_ < 4; ++c_) above += (uint32_t)__popcll(__ballot(x[q][c_] > xv));
         }
+        if (BEAM && (uint32_t)(t - lo) < (uint32_t)n_in) {     // eos is on no list
+#pragma unroll
+            for (int q = 0; q < NL; ++q)
+#pragma unroll
+                for (int c_ = 0; c_ < 4; ++c_) x[q][c_] = lo + (q * SK_LT + tid) * 4 + c_ == t ? LP_NONE : x[q][c_];
+            lane_max();
+        }
         if (TOP) {
-            lm = fmaxf(lm, cm);
+            if constexpr (BEAM) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ls[i] = fmaxf(ls[i], cs[i]);
+            } else {
+                lm = fmaxf(lm, cm);
+            }
             const bool any = __ballot(cm >= bound) != 0ull;
             if (any && g - bound_at >= LP_GROWN) {
-                const uint32_t key[1] = {key_of(lm)};
-                uint32_t from = wave_min(key[0]);              // (every lane reaches it)
-                from = reach > LP_LOWEST && from < key_of(reach) ? key_of(reach) : from;
-                const uint32_t nth = lp_nth(key, from, n);
+                uint32_t nth;
+                if constexpr (BEAM) {
+                    nth = lp_nth_set(ls, reach, n);
+                } else {
+                    const uint32_t key[1] = {key_of(lm)};
+                    uint32_t from = wave_min(key[0]);          // (every lane reaches it)
+                    from = reach > LP_LOWEST && from < key_of(reach) ? key_of(reach) : from;
+                    nth = lp_nth(key, from, n);
+                }
                 const float b = nth > 0x007FFFFFu ? val_of(nth) : LP_LOWEST;
                 bound = fmaxf(bound, b);
                 reach = fmaxf(reach, b);
@@ -350,6 +685,10 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
         }
     }
     // ---- the wave's end
+    if constexpr (BEAM) {
+        beam_end(args, shared.lp, shared.bm, beams, row, part, nseg, T, dead, sum, mx, xv, ls, reach, g, cut);
+        return;
+    }
     auto addu = [](uint32_t u, uint32_t v) { return u + v; };
     auto addf = [](double u, double v) { return u + v; };
     const int lists = nseg * SK_NW, me = part * SK_NW + w;
@@ -552,20 +891,32 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
     }
 }
 
-hipError_t launch_logprobs(int type, const LpArgs& a, hipStream_t st) {
+template <bool BEAM, class A>
+hipError_t launch_rows(int type, const A& args, const LpArgs& a, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)XCDS * a.nseg * (((int64_t)a.B + XCDS - 1) / XCDS))), block(SK_LT);
     auto go = [&](auto t, auto top) {
         constexpr int T = decltype(t)::value;
-        hipLaunchKernelGGL((logprob_kernel<T, LP_NL(T), decltype(top)::value>), grid, block, 0, st, a.logits, a.ld, a.B,
-                           a.V, a.nseg, a.n, a);
+        hipLaunchKernelGGL((logprob_kernel<T, LP_NL(T), decltype(top)::value, BEAM>), grid, block, 0, st, a.logits, a.ld,
+                           a.B, a.V, a.nseg, a.n, args);
     };
     auto by_top = [&](auto t) {
-        if (a.n > 0) go(t, std::true_type{});
+        if constexpr (BEAM) go(t, std::true_type{});
+        else if (a.n > 0) go(t, std::true_type{});
         else go(t, std::false_type{});
     };
     if (type == FS_F32) by_top(std::integral_constant<int, FS_F32>{});
     else if (type == FS_BF16) by_top(std::integral_constant<int, FS_BF16>{});
     else by_top(std::integral_constant<int, FS_F16>{});
+    return hipGetLastError();
+}
+
+hipError_t launch_logprobs(int type, const LpArgs& a, hipStream_t st) { return launch_rows<false>(type, a, a, st); }
+
+__global__ __launch_bounds__(WAVE) void beam_nothing_kernel(BeamArgs b) { bm_nothing(b, (int)blockIdx.x); }
+
+hipError_t launch_beam_select(int type, const LpBeamArgs& a, hipStream_t st) {
+    if (a.lp.B > 0) return launch_rows<true>(type, a, a.lp, st);
+    hipLaunchKernelGGL(beam_nothing_kernel, dim3((unsigned)a.b.S), dim3(WAVE), 0, st, a.b);
     return hipGetLastError();
 }
 

@@ -162,11 +162,12 @@ struct fs_context {
     size_t ed_logits = 0, ed_param_rows = 0, ed_any_rows = 0, ed_u_rows = 0, ed_off_rows = 0;
     char* lp_row = nullptr;            // fs_logprobs: [lp_row_bytes] what the rows' waves publish,
     uint32_t* lp_ticket = nullptr;     //   [lp_rows][LP_LINE] their tickets, left at 0,
-    uint64_t* lp_lists = nullptr;      //   [lp_list_segs][SK_NW][LP_TOP] their lists
-    size_t lp_row_bytes = 0, lp_rows = 0, lp_list_segs = 0;
-    fs::BeamRow* bm_rows = nullptr;    // fs_beam_select: [bm_row_cap] the rows' sums,
-    uint64_t* bm_lists = nullptr;      //   [bm_list_rows][BM_TOP] their lists
-    size_t bm_row_cap = 0, bm_list_rows = 0;
+    uint64_t* lp_lists = nullptr;      //   [lp_list_cap] entries of their lists
+    size_t lp_row_bytes = 0, lp_rows = 0, lp_list_cap = 0;
+    fs::BeamRow* bm_rows = nullptr;    // fs_beam_select: [bm_row_cap] the rows' results
+    uint64_t* bm_lists = nullptr;      //   [bm_list_cap][BM_TOP] and lists,
+    uint32_t* bm_ticket = nullptr;     //   [bm_streams][LP_LINE] the streams' tickets, left at 0
+    size_t bm_row_cap = 0, bm_list_cap = 0, bm_streams = 0;
     int static_dev = -1;       // device whose static workspace fs_sample_batch_static used with this context
     uint64_t* trace = nullptr; // FS_TRACE builds: phase timestamps, trace_cap entries (fs_trace_set)
     int64_t trace_cap = 0;
@@ -990,6 +991,24 @@ int check_state(const fs_state& z, int64_t S, int32_t n_src, int32_t n) {
     return s0 < d1 && d0 < s1 ? FS_E_INVALID : FS_OK;
 }
 
+// The parts, the rows and the workspace of a log-probability kernel's launch (top: the largest it lists; list: entries of a
+// wave's list).
+int reserve_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld, int32_t B, int32_t V, int32_t top,
+                     int list, fs::LpArgs& a) {
+    a.nseg = logprob_parts(ctx, B, V, type);
+    if (((int64_t)B + fs::XCDS) * a.nseg > 0x7fffffff) return FS_E_INVALID;
+    const size_t entries = (size_t)B * a.nseg * fs::SK_NW * list;
+    int rc = grow(ctx, 0, 0, 0);
+    if (rc == FS_OK)
+        rc = grow_buffer(ctx, ctx->lp_row, ctx->lp_row_bytes, (size_t)B * fs::lp_row_bytes(a.nseg), 1, false);
+    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_ticket, ctx->lp_rows, (size_t)B, fs::LP_LINE, true);
+    if (rc == FS_OK && top > 0) rc = grow_buffer(ctx, ctx->lp_lists, ctx->lp_list_cap, entries, 1, false);
+    if (rc != FS_OK) return rc;
+    a.logits = d_logits; a.ld = ld; a.B = B; a.V = V; a.n = top;
+    a.rows = ctx->lp_row; a.ticket = ctx->lp_ticket; a.lists = ctx->lp_lists; a.err = ctx->err;
+    return FS_OK;
+}
+
 size_t type_size(int32_t type) { return type == FS_F32 ? 4 : type == FS_BF16 || type == FS_F16 ? 2 : 0; }
 
 // Rows of logits of any type: check_rows for FS_F32, four logits' alignment for the others.
@@ -1108,6 +1127,7 @@ int fs_destroy(fs_context* c) {
     (void)hipFree(c->lp_lists);
     (void)hipFree(c->bm_rows);
     (void)hipFree(c->bm_lists);
+    (void)hipFree(c->bm_ticket);
     for (void* p : c->retired) (void)hipFree(p);
     if (c->hflag) (void)hipHostFree(c->hflag);
     delete c;
@@ -1390,18 +1410,9 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
     const int top = d_top_ids || d_top_lp ? n : 0;
     const Edited call(ctx, st);
     if (call.rc != FS_OK) return call.rc;
-    a.nseg = logprob_parts(ctx, B, V, type);
-    if (((int64_t)B + fs::XCDS) * a.nseg > 0x7fffffff) return FS_E_INVALID;
-    const size_t segs = (size_t)B * a.nseg;
-    rc = grow(ctx, 0, 0, 0);
-    if (rc == FS_OK)
-        rc = grow_buffer(ctx, ctx->lp_row, ctx->lp_row_bytes, (size_t)B * fs::lp_row_bytes(a.nseg), 1, false);
-    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->lp_ticket, ctx->lp_rows, (size_t)B, fs::LP_LINE, true);
-    if (rc == FS_OK && top > 0) rc = grow_buffer(ctx, ctx->lp_lists, ctx->lp_list_segs, segs, fs::SK_NW * fs::LP_TOP, false);
+    rc = reserve_logprobs(ctx, d_logits, type, ld, B, V, top, fs::LP_TOP, a);
     if (rc != FS_OK) return rc;
-    a.logits = d_logits; a.ld = ld; a.B = B; a.V = V; a.n = top; a.params = d_params; a.tok = d_tok;
-    a.lp = d_lp; a.rank = d_rank; a.ids = d_top_ids; a.top = d_top_lp;
-    a.rows = ctx->lp_row; a.ticket = ctx->lp_ticket; a.lists = ctx->lp_lists; a.err = ctx->err;
+    a.params = d_params; a.tok = d_tok; a.lp = d_lp; a.rank = d_rank; a.ids = d_top_ids; a.top = d_top_lp;
     return fs::launch_logprobs(type, a, st) == hipSuccess ? FS_OK : FS_E_HIP;
 }
 
@@ -1415,22 +1426,24 @@ int fs_beam_select(fs_context* ctx, const void* d_logits, int32_t type, int64_t 
     if (!d_row_off && n_streams > 0 && total_rows % n_streams != 0) return FS_E_INVALID;
     int rc = check_typed(d_logits, type, ld, total_rows, V);
     if (rc != FS_OK) return rc;
-    fs::BeamArgs a = {};
-    rc = edit_args(edits, total_rows, V, a.ed);
+    fs::LpBeamArgs a = {};
+    rc = edit_args(edits, total_rows, V, a.lp.ed);
     if (rc != FS_OK) return rc;
     if (n_streams == 0) return FS_OK;
     const hipStream_t st = (hipStream_t)stream;
     const Edited call(ctx, st);
     if (call.rc != FS_OK) return call.rc;
-    rc = grow(ctx, 0, 0, 0);
+    rc = reserve_logprobs(ctx, d_logits, type, ld, total_rows, V, n, fs::BM_LIST, a.lp);
     if (rc == FS_OK) rc = grow_buffer(ctx, ctx->bm_rows, ctx->bm_row_cap, (size_t)total_rows, 1, false);
-    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->bm_lists, ctx->bm_list_rows, (size_t)total_rows, fs::BM_TOP, false);
+    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->bm_lists, ctx->bm_list_cap, (size_t)total_rows, fs::BM_TOP, false);
+    if (rc == FS_OK) rc = grow_buffer(ctx, ctx->bm_ticket, ctx->bm_streams, (size_t)n_streams, fs::LP_LINE, true);
     if (rc != FS_OK) return rc;
-    a.logits = d_logits; a.ld = ld; a.S = n_streams; a.R = total_rows; a.V = V; a.n = n; a.eos = eos_id;
-    a.keep_slots = flags & FS_BEAM_KEEP_SLOTS; a.row_off = d_row_off; a.score = d_score; a.params = d_params;
-    a.parent = d_parent; a.tok = d_tok; a.out_score = d_out_score;
-    a.done = d_done; a.done_parent = d_done_parent; a.done_score = d_done_score;
-    a.rows = ctx->bm_rows; a.lists = ctx->bm_lists; a.err = ctx->err;
+    a.lp.params = d_params;
+    fs::BeamArgs& b = a.b;
+    b.S = n_streams; b.W = total_rows / n_streams; b.n = n; b.eos = eos_id; b.keep_slots = flags & FS_BEAM_KEEP_SLOTS;
+    b.row_off = d_row_off; b.score = d_score; b.parent = d_parent; b.tok = d_tok; b.out_score = d_out_score;
+    b.done = d_done; b.done_parent = d_done_parent; b.done_score = d_done_score;
+    b.rows = ctx->bm_rows; b.row_lists = ctx->bm_lists; b.ticket = ctx->bm_ticket;
     return fs::launch_beam_select(type, a, st) == hipSuccess ? FS_OK : FS_E_HIP;
 }
 

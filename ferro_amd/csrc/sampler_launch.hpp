@@ -171,31 +171,32 @@ hipError_t launch_logprobs(int type, const LpArgs& a, hipStream_t st);
 
 // Beam search (beam_kernels.hip).
 constexpr int BM_TOP = FS_MAX_TOP;         // new beams per stream, at most
-struct BeamRow {                           // a row's sum, and what its candidates' scores follow from
+struct BeamRow {                           // a row: what its candidates' scores follow from
     double a, z;                           // its score; the logarithm of its sum
     float M, T, eos;                       // its largest logit, its temperature, the logit that ends the text (-inf: none)
-    int cnt;                               // entries of its list
+    int unused;
 };
+constexpr int BM_LIST = 2 * BM_TOP;        // entries of a wave's list
 struct BeamArgs {
-    const void* logits;
-    int64_t ld;
-    int S, R, V, n, eos;                   // streams, rows
+    int S, W, n, eos;                      // streams; rows of each where row_off is NULL
     int keep_slots;
-    const int64_t* row_off;                // NULL: R / S rows each
+    const int64_t* row_off;
     const float* score;                    // NULL: zeros
-    const fs_row_params* params;           // by stream (NULL: no softcap, temperature 1)
-    EdArgs ed;                             // masks by row, biases by stream
     int32_t* parent;                       // [S][n]
     int32_t* tok;
     float* out_score;
     int32_t* done;                         // [S]
     int32_t* done_parent;                  // [S][n]
     float* done_score;
-    BeamRow* rows;                         // [R]
-    uint64_t* lists;                       // [R][BM_TOP]
-    int32_t* err;
+    BeamRow* rows;                         // [rows]
+    uint64_t* row_lists;                   // [rows][BM_TOP]
+    uint32_t* ticket;                      // [S][LP_LINE]: what has ended of a stream (left at 0)
 };
-hipError_t launch_beam_select(int type, const BeamArgs& a, hipStream_t st);
+struct LpBeamArgs {                        // lp: params and biases by stream; lists of BM_LIST; tok and its outputs unused
+    LpArgs lp;
+    BeamArgs b;
+};
+hipError_t launch_beam_select(int type, const LpBeamArgs& a, hipStream_t st);
 
 struct ForkArgs {
     const int32_t* hist;
