@@ -955,12 +955,12 @@ int logprob_parts(const fs_context* c, int64_t B, int32_t V, int32_t type) {
 
 // ---- fs_reorder_states
 // Bytes per column: what the pointers, the strides and a position's bytes are all multiples of, 16 at most (streams of more
-// than 16 rows, whose columns are all in registers: 8).
+// than 32 rows, whose columns are all in registers: 8).
 int state_bytes(const fs_state& z, int rows) {
     const uint64_t all = (uint64_t)(uintptr_t)z.d_src | (uint64_t)(uintptr_t)z.d_dst | (uint64_t)z.src_row |
                          (uint64_t)z.src_block | (uint64_t)z.src_pos | (uint64_t)z.dst_row | (uint64_t)z.dst_block |
                          (uint64_t)z.dst_pos | (uint64_t)z.pos_bytes;
-    int vb = rows > 16 ? 8 : 16;
+    int vb = rows > 32 ? 8 : 16;
     while (vb > 1 && (all & (uint64_t)(vb - 1)) != 0) vb >>= 1;
     return vb;
 }
@@ -1464,7 +1464,7 @@ int fs_hist_fork(fs_context* ctx, int32_t n_streams, const int32_t* d_hist, cons
     fs::ForkArgs a = {};
     a.hist = d_hist; a.hist_off = d_hist_off; a.row_off = d_row_off; a.S = n_streams; a.n = n; a.parent = d_parent;
     a.tok = d_tok; a.out = d_out_hist; a.out_cap = out_cap; a.out_off = d_out_hist_off; a.err = ctx->err;
-    return fs::launch_hist_fork(a, st) == hipSuccess ? FS_OK : FS_E_HIP;
+    return fs::launch_hist_fork(a, ctx->cus, st) == hipSuccess ? FS_OK : FS_E_HIP;
 }
 
 int fs_reorder_states(fs_context* ctx, int32_t n_states, const fs_state* states, int32_t n_streams, int32_t n_src, int32_t n,
@@ -1486,13 +1486,16 @@ int fs_reorder_states(fs_context* ctx, int32_t n_states, const fs_state* states,
         fs::StateArgs a = {};
         a.S = n_streams; a.n_src = n_src; a.n = n; a.parent = d_parent; a.from = d_from; a.len = d_len; a.err = ctx->err;
         const int vb = state_bytes(states[i], n > n_src ? n : n_src);
-        int64_t tiles = 0;
-        int k = 0;
-        for (; i < n_states && k < fs::ST_MAX && state_bytes(states[i], n > n_src ? n : n_src) == vb; ++i) {
-            a.z[k++] = states[i];
-            tiles = std::max(tiles, (state_cols(states[i], vb) + 255) / 256);
+        int64_t cols = 0;
+        a.alike = 1;
+        for (; i < n_states && a.n_states < fs::ST_MAX && state_bytes(states[i], n > n_src ? n : n_src) == vb; ++i) {
+            const fs_state& z = states[i];
+            a.alike &= z.blocks == a.z[0].blocks && z.positions == a.z[0].positions && z.pos_bytes == a.z[0].pos_bytes ||
+                       a.n_states == 0;
+            a.z[a.n_states++] = z;
+            cols += state_cols(states[i], vb) * n_streams;
         }
-        if (tiles > 0 && fs::launch_reorder_states(vb, a, k, tiles, st) != hipSuccess) return FS_E_HIP;
+        if (cols > 0 && fs::launch_reorder_states(vb, a, cols, ctx->cus, st) != hipSuccess) return FS_E_HIP;
     }
     return FS_OK;
 }

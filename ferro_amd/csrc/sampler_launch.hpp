@@ -210,19 +210,19 @@ struct ForkArgs {
     int64_t* out_off;
     int32_t* err;
 };
-hipError_t launch_hist_fork(const ForkArgs& a, hipStream_t st);
+hipError_t launch_hist_fork(const ForkArgs& a, int cus, hipStream_t st);
 
 constexpr int ST_MAX = 32;                 // states per launch (their records travel in the argument segment)
 struct StateArgs {
-    int S, n_src, n;
+    int n_states, alike, S, n_src, n;      // alike: all states have as many columns
     const int32_t* parent;
     const int32_t* from;
     const int32_t* len;
     int32_t* err;
     fs_state z[ST_MAX];
 };
-// vb: bytes per column (1 to 16); tiles: columns of the largest state over ST_T
-hipError_t launch_reorder_states(int vb, const StateArgs& a, int n_states, int64_t tiles, hipStream_t st);
+// vb: bytes per column (1 to 16); cols: columns of all states' and streams' blocks
+hipError_t launch_reorder_states(int vb, StateArgs a, int64_t cols, int cus, hipStream_t st);
 
 hipError_t launch_lookup_draft(int n_streams, const int32_t* hist, const int64_t* hist_off, const int32_t* kmax,
                                const int32_t* min_n, int eos, int32_t* draft, int draft_ld, int32_t* ndraft,
