@@ -5,8 +5,7 @@
 #ifndef FERRO_BEAM_DEVICE_HPP
 #define FERRO_BEAM_DEVICE_HPP
 
-#include "sampler_device.hpp"
-#include "sampler_launch.hpp"
+#include "row_device.hpp"
 
 namespace fs {
 
@@ -19,27 +18,23 @@ __device__ __forceinline__ double bm_score(const BeamRow& r, float x) {
     return r.a + ((x == r.M ? 0.0 : ((double)x - (double)r.M) / (double)r.T) - r.z);
 }
 // Scores as ordered integers (0: no candidate): the upper 51 bits, 39 of them the mantissa's, are compared; the lower 13 order
-// equal ones where they are sorted, and lead back to the candidate.
+// equal ones by row and place, and make the integers distinct.
 constexpr int BM_LOW = 13;
-constexpr uint32_t BM_OLD = 1u << 12;      // before others: of an earlier batch of rows (and 63 - its place), or the text's end
+constexpr uint32_t BM_OLD = 1u << 12;      // before others: of earlier rows, or the text's end
 __device__ __forceinline__ uint64_t bm_key(double c, uint32_t low) {
     if (!((float)c > -__builtin_huge_valf())) return 0ull;
     const uint64_t u = (uint64_t)__double_as_longlong(c + 0.0);
     return ((u >> 63 ? ~u : u | 0x8000000000000000ull) & ~(uint64_t)((1u << BM_LOW) - 1u)) | low;
 }
 
-constexpr int BM_HELD = 1024;              // entries of the lists kept in LDS
-struct BeamJoin {                          // many rows or candidates
-    BeamRow row[WAVE];
-    uint64_t entry[BM_HELD];
-    int from[2][BM_TOP], token[BM_TOP];    // of earlier batches: the beams (0), the ended (1)
-    float value[2][BM_TOP];
-};
 struct BeamBest {                          // a stream's end
-    union {
-        BeamJoin join;
-        uint64_t key[BM_T + 16];           // few: candidates, then what ends the text, one per thread; 0 past each
-    };
+    uint64_t key[BM_T + 16];               // candidates; 0 up to a multiple of eight (few: then what ends the text)
+    uint64_t ekey[2 * BM_TOP + 8];
+    uint64_t entry[BM_T];
+    int crow[BM_T];
+    uint32_t hi[4][WAVE];
+    float cvalue[BM_TOP];
+    int cnt, again;
     int from[BM_TOP], token[BM_TOP], efrom[BM_TOP], first[BM_TOP], place[BM_TOP];
     float value[BM_TOP], evalue[BM_TOP];
     int n_ends;
@@ -53,6 +48,7 @@ struct BeamShared {
     uint16_t at[SK_NW][LP_PARTS * SK_NW];
     BeamRow row[WAVE];                     // the stream's rows,
     uint64_t list[BM_T];                   // their candidates
+    int cnt[SK_NW];
     uint32_t turn;
 };
 __device__ __forceinline__ void bm_sync() {    // LDS stores and loads of one wave in order
@@ -142,109 +138,160 @@ __device__ __forceinline__ void bm_few(const BeamArgs& a, BeamShared& sh, int m,
     }
 }
 
-// Any number of rows, by one wave: their lists, place by place (the rows' best first), 64 candidates at a time, sorted and
-// merged into the best so far where one of them reaches the n-th. The first 64 of which none does end the walk: what follows
-// is no better. Rows past the 64th are a batch of their own, whose candidates lose to equal ones of earlier batches.
-__device__ __forceinline__ void bm_join(const BeamArgs& a, BeamShared& sh, int64_t r0, int m, bool ends) {
-    BeamJoin& s = sh.best.join;
-    const int lane = lane_id(), n = a.n;
-    uint64_t acc = 0ull, end = 0ull;                           // sorted, one per lane
-    int from = -1, token = -1, efrom = -1;
-    float value = -__builtin_huge_valf(), evalue = value;
+// Any number of rows, 64 at a time (a batch), a row per lane. Of the first four places of the rows' lists, which are in order, n
+// reach a bound (as lp_nth); places further down are read as long as one of them reaches it. The candidates so found (about 1.5 n)
+// are put in order, a thread each, with the best of earlier batches; where there is no room for them, they are before the walk
+// goes on.
+constexpr uint64_t BM_MASK = ~(uint64_t)((1u << BM_LOW) - 1u);
+__device__ __forceinline__ void bm_many(const BeamArgs& a, BeamShared& sh, int64_t r0, int m, bool ends) {
+    BeamBest& s = sh.best;
+    const int t = threadIdx.x, lane = lane_id(), w = t / WAVE, n = a.n;
+    constexpr float NONE = -__builtin_huge_valf();
+    uint32_t least = 1u;                                       // (of the keys' upper halves; the first wave's)
+    int held = 0;                                              // of s.key: the best so far, in order
+    if (t < BM_TOP) {
+        s.ekey[BM_TOP + t] = 0ull;
+        s.efrom[t] = -1;
+        s.evalue[t] = NONE;
+    }
+    if (t == 0) s.cnt = 0;
+    __syncthreads();
 #pragma unroll 1
     for (int b = 0; b < m; b += WAVE) {
         const int k = m - b < WAVE ? m - b : WAVE;             // rows of this batch
-        const uint64_t* lists = a.row_lists + (r0 + b) * BM_TOP;
-        const int all = k * n;
-        constexpr int U = 4;
-        uint64_t e[U];
-        auto fetch = [&](int i0) {
+        const uint64_t* list = a.row_lists + (r0 + b + lane) * BM_TOP;
+        auto fetch = [&](int p) { return lane < k && p < n ? ld_agent(list + p) : (uint64_t)0; };
+        uint64_t next[4] = {0ull, 0ull, 0ull, 0ull};           // places p .. p + 3
+        BeamRow br = bm_dead_row();
+        int p = 0;
+        if (w == 0) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = i0 + u * WAVE + lane, p = i / k, r = i - p * k;
-                e[u] = i < all ? ld_agent(lists + r * BM_TOP + p) : 0ull;
-            }
+            for (int u = 0; u < 4; ++u) next[u] = fetch(u);
+            if (lane < k) br = bm_load_row(a, r0 + b + lane);
+            sh.row[lane] = br;
+            if (b > 0 && lane < s.cnt) s.key[lane] = (s.key[lane] & BM_MASK) | BM_OLD | (uint32_t)(63 - lane);  // before equal ones
+        }
+        auto key_now = [&]() {
+            return bm_key(next[0] ? bm_score(br, val_of(comp_key(next[0]))) : (double)NONE, 4095u - (uint32_t)(lane * 64 + p));
         };
-        BeamRow br = {0.0, 0.0, 0.0f, 1.0f, -__builtin_huge_valf(), 0};
-        if (lane < k) br = bm_load_row(a, r0 + b + lane);
-        fetch(0);
-        s.row[lane] = br;
-        if (b > 0) {
-            s.from[0][lane] = from; s.token[lane] = token; s.value[0][lane] = value;
-            s.from[1][lane] = efrom; s.value[1][lane] = evalue;
-            acc = acc ? (acc & ~(uint64_t)((1u << BM_LOW) - 1u)) | BM_OLD | (uint32_t)(63 - lane) : 0ull;
-            end = end ? (end & ~(uint64_t)((1u << BM_LOW) - 1u)) | BM_OLD | (uint32_t)(63 - lane) : 0ull;
-        }
-        bm_sync();
-        bool more = true;
+        auto advance = [&]() {
+            next[0] = next[1];
+            next[1] = next[2];
+            next[2] = next[3];
+            next[3] = fetch(p + 4);
+            ++p;
+        };
+        bool go = true;
 #pragma unroll 1
-        for (int i0 = 0; more && i0 < all; i0 += U * WAVE) {
-            if (i0 > 0) fetch(i0);
+        for (int round = 0; go; ++round) {
+            if (w == 0) {
+                int cnt = s.cnt;
+                if (round == 0) {
+                    const uint64_t first[4] = {next[0], next[1], next[2], next[3]};
 #pragma unroll 1
-            for (int u = 0; u < U; ++u) {
-                const uint64_t eu = u == 0 ? e[0] : u == 1 ? e[1] : u == 2 ? e[2] : e[3];
-                const int i = i0 + u * WAVE + lane, p = i / k, r = i - p * k;
-                if (i < BM_HELD) s.entry[i] = eu;
-                uint64_t key = 0ull;
-                if (eu != 0ull && i < all) key = bm_key(bm_score(s.row[r], val_of(comp_key(eu))), 4095u - (uint32_t)(r * 64 + p));
-                const uint64_t nth = read_lane(acc, n - 1);
-                if (more && i0 + u * WAVE < all) {             // uniform
-                    if (__ballot(key > nth) != 0ull) acc = merge_top64(acc, sort64<false>(key));
-                    else more = false;
-                }
-            }
-        }
-        bm_sync();
-        // back from the keys to the candidates
-        if (acc != 0ull) {
-            const uint32_t low = (uint32_t)acc & ((1u << BM_LOW) - 1u);
-            if (low & BM_OLD) {
-                const int j = 63 - (int)(low & 63u);
-                from = s.from[0][j]; token = s.token[j]; value = s.value[0][j];
-            } else {
-                const int at = (int)(4095u - low), r = at >> 6, p = at & 63, i = p * k + r;
-                const uint64_t c = i < BM_HELD ? s.entry[i] : ld_agent(lists + r * BM_TOP + p);
-                from = b + r;
-                token = (int)comp_id(c);
-                value = (float)bm_score(s.row[r], val_of(comp_key(c)));
-            }
-        }
-        if (ends) {
-            const uint64_t key = lane < k ? bm_key(bm_score(br, br.eos), 4095u - (uint32_t)(lane * 64)) : 0ull;
-            if (__ballot(key != 0ull) != 0ull) {
-                end = merge_top64(end, sort64<false>(key));
-                if (end != 0ull) {
-                    const uint32_t low = (uint32_t)end & ((1u << BM_LOW) - 1u);
-                    if (low & BM_OLD) {
-                        const int j = 63 - (int)(low & 63u);
-                        efrom = s.from[1][j]; evalue = s.value[1][j];
-                    } else {
-                        const int r = (int)(4095u - low) >> 6;
-                        efrom = b + r;
-                        evalue = (float)bm_score(s.row[r], s.row[r].eos);
+                    for (int u = 0; u < 4; ++u) {
+                        s.hi[u][lane] = (uint32_t)(key_now() >> 32);
+                        next[0] = next[1];
+                        next[1] = next[2];
+                        next[2] = next[3];
+                        ++p;
                     }
+                    p = 0;
+                    bm_sync();
+                    const uint32_t hi[4] = {s.hi[0][lane], s.hi[1][lane], s.hi[2][lane], s.hi[3][lane]};
+                    // (the lists are in order: all of these reach the least of the fourth)
+                    const uint32_t reach = wave_min(lane >= k ? ~0u : hi[3] > 1u ? hi[3] : 1u);
+                    least = lp_nth(hi, 4 * k >= n && reach > least ? reach : least, n);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) next[u] = first[u];
+                }
+#pragma unroll 1
+                while (go) {                                   // a place at a time
+                    const uint64_t key = key_now();
+                    const bool in = (uint32_t)(key >> 32) >= least;
+                    const uint64_t mm = __ballot(in);
+                    go = mm != 0ull && p < n;                  // (in order: no more below places that none reaches)
+                    if (!go || cnt + __popcll(mm) > BM_T) break;       // (no room: the next round)
+                    if (in) {
+                        const int i = cnt + (int)mbcnt(mm);
+                        s.key[i] = key;
+                        s.entry[i] = next[0];
+                        s.crow[i] = b + lane;
+                    }
+                    cnt += __popcll(mm);
+                    advance();
+                }
+                if (lane < 8) s.key[cnt + lane] = 0ull;
+                if (lane == 0) {
+                    s.cnt = cnt;
+                    s.again = go ? 1 : 0;
                 }
             }
+            __syncthreads();
+            const int all = s.cnt;
+            go = s.again != 0;
+            const uint64_t key = t < all ? s.key[t] : 0ull, e = t < all ? s.entry[t] : 0ull;
+            const int row = t < all ? s.crow[t] : -1;
+            float value = t < BM_TOP ? s.cvalue[t] : NONE;     // (of the best of earlier rounds)
+            if (t < all && t >= held) value = (float)bm_score(sh.row[row - b], val_of(comp_key(e)));
+            const int at = key ? bm_above(s.key, all, key) : BM_T;
+            __syncthreads();
+            if (at < n) {
+                s.key[at] = key;
+                s.entry[at] = e;
+                s.crow[at] = row;
+                s.cvalue[at] = value;
+            }
+            held = all < n ? all : n;
+            if (t < 8) s.key[held + t] = 0ull;
+            if (t == 0) s.cnt = held;
+            __syncthreads();
+            if (w == 0 && held == n) least = (uint32_t)(s.key[n - 1] >> 32);
         }
-        bm_sync();
+        if (!ends) continue;
+        // what ends the text: the batch's rows, and the best of earlier ones (which come before equal ones)
+        uint64_t key = 0ull;
+        int from = -1;
+        float value = NONE;
+        if (w == 0) {
+            const double c = bm_score(br, br.eos);
+            key = bm_key(c, 4095u - (uint32_t)(lane * 64));
+            from = b + lane;
+            value = (float)c;
+        } else if (w == 1) {
+            key = s.ekey[BM_TOP + lane];
+            from = s.efrom[lane];
+            value = s.evalue[lane];
+        }
+        if (w == 0) s.ekey[lane] = key;
+        __syncthreads();
+        const int at = key ? bm_above(s.ekey, 2 * BM_TOP, key) : BM_T;
+        __syncthreads();
+        if (w == 1) s.ekey[t] = 0ull;
+        __syncthreads();
+        if (at < n) {
+            s.ekey[BM_TOP + at] = (key & BM_MASK) | BM_OLD | (uint32_t)(63 - at);
+            s.efrom[at] = from;
+            s.evalue[at] = value;
+        }
+        __syncthreads();
     }
-    // ended hypotheses: fewer than n candidates before them, ended ones among these (a prefix of the ended ones' order)
-    int before = 0;
-    if (__ballot(end != 0ull) != 0ull) {
-#pragma unroll 1
-        for (int j = 0; j < n; ++j) before += read_lane(acc, j) >> BM_LOW > end >> BM_LOW ? 1 : 0;
+    if (t < BM_TOP) {
+        const bool live = t < s.cnt;
+        const uint64_t key = s.ekey[BM_TOP + t];
+        s.from[t] = live ? s.crow[t] : -1;
+        s.token[t] = live ? (int)comp_id(s.entry[t]) : -1;
+        s.value[t] = live ? s.cvalue[t] : NONE;
+        // the ended: fewer than n candidates before them, the ended among these (so the first few in their order)
+        bool ended = false;
+        if (__ballot(key != 0ull) != 0ull) ended = key != 0ull && bm_above(s.key, held, key | ~BM_MASK) + t < n;
+        const int d = __popcll(__ballot(ended));
+        if (!ended) {
+            s.efrom[t] = -1;
+            s.evalue[t] = NONE;
+        }
+        if (t == 0) s.n_ends = d;
     }
-    const bool ended = end != 0ull && before + lane < n;
-    const bool live = lane < n && acc != 0ull;
-    BeamBest& o = sh.best;
-    o.from[lane] = live ? from : -1;
-    o.token[lane] = live ? token : -1;
-    o.value[lane] = live ? value : -__builtin_huge_valf();
-    o.efrom[lane] = ended ? efrom : -1;
-    o.evalue[lane] = ended ? evalue : -__builtin_huge_valf();
-    const int d = __popcll(__ballot(ended));
-    if (lane == 0) o.n_ends = d;
-    bm_sync();
 }
 
 // Stream st without a candidate (one wave).

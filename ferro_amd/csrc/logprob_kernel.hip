@@ -65,33 +65,6 @@ __device__ __forceinline__ float lp_max3(float a, float b, float c) {   // (fmax
     return a;
 }
 
-// A key that n of the wave's 64 K keys reach, and about a quarter more at most where they differ; n reach `lo` already.
-// Bisected: K compares a step.
-template <int K>
-__device__ __forceinline__ uint32_t lp_nth(const uint32_t (&key)[K], uint32_t lo, int n) {
-    uint32_t hi = key[0];
-#pragma unroll
-    for (int u = 1; u < K; ++u) hi = key[u] > hi ? key[u] : hi;
-    hi = wave_max(hi);
-    if (n == 1) return hi > lo ? hi : lo;
-    uint32_t step = hi > lo ? hi - lo : 0u;                    // the n-th largest lies in [lo, lo + step]
-#pragma unroll 1
-    while (step > 0u) {
-        const uint32_t up = (step >> 1) + (step & 1u);
-        int c = 0;
-#pragma unroll
-        for (int u = 0; u < K; ++u) c += __popcll(__ballot(key[u] >= lo + up));
-        if (c >= n) {
-            lo += up;
-            step -= up;
-            if (c <= n + n / 4) break;
-        } else {
-            step = up - 1u;
-        }
-    }
-    return lo;
-}
-
 // BEAM: of four maxima per lane. A few tokens are found by the lanes' largest alone; for many these are too few, and the least
 // of them lets most of the logits pass (128 rows of 100003 fp16, n 64: 88 us).
 __device__ __forceinline__ uint32_t lp_nth_set(const float (&ls)[4], float reach, int n) {
@@ -222,10 +195,12 @@ __device__ __forceinline__ void beam_publish(const LpArgs& a, LpShared& s, int r
     }
 }
 
-// BEAM: a row's end, by one wave: its sum, and its n largest tokens (one per lane, in order; 0 past them).
+// BEAM: a row's end: its sum, and its n largest tokens. ALONE: by one wave (returned: one per lane, in order; 0 past them);
+// else by the workgroup, a fourth of the lists per wave (to s.list).
+template <bool ALONE>
 __device__ __forceinline__ uint64_t beam_row_end(const LpArgs& a, BeamShared& s, int64_t row, int nseg, int n, float score, float T,
                                                  BeamRow& br) {
-    const int lane = lane_id(), w = (int)threadIdx.x / WAVE, lists = nseg * SK_NW;
+    const int tid_ = threadIdx.x, lane = lane_id(), w = tid_ / WAVE, lists = nseg * SK_NW;
     const LpRow p = lp_row(a, row, nseg);
     const uint64_t* rl = a.lists + row * lists * BM_LIST;
     constexpr int LL = LP_PARTS * SK_NW / WAVE;
@@ -274,6 +249,9 @@ __device__ __forceinline__ uint64_t beam_row_end(const LpArgs& a, BeamShared& s,
         if (in) at[k + (int)mbcnt(m)] = (uint16_t)(((u * WAVE + lane) << 8) | len[u]);
         k += __popcll(m);
     }
+    constexpr int STEP = ALONE ? 1 : SK_NW;
+    const int k0 = ALONE ? 0 : w;                              // this wave's: k0, k0 + STEP, ..
+    k = (k - k0 + STEP - 1) / STEP;
     lp_wave_sync();
     const int half = lane >> 5, pos = lane & 31;
     int to[U];
@@ -282,7 +260,7 @@ __device__ __forceinline__ uint64_t beam_row_end(const LpArgs& a, BeamShared& s,
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + 2 * u + half;
-            to[u] = i < k ? at[i] : 0;
+            to[u] = i < k ? at[k0 + i * STEP] : 0;
             e[u] = pos + skip < (to[u] & 255) ? ld_agent(rl + (to[u] >> 8) * BM_LIST + pos + skip) : 0ull;
         }
     };
@@ -330,6 +308,24 @@ __device__ __forceinline__ uint64_t beam_row_end(const LpArgs& a, BeamShared& s,
         if (!last) fetch(i0, skip);
     }
     lp_wave_sync();
+    if constexpr (!ALONE) {                                    // up to 64 of each wave, a thread each
+        if (sorted) {
+            acc = lane < n ? acc : 0ull;
+            cnt = __popcll(__ballot(acc != 0ull));
+            join[lane] = acc;
+        }
+        if (lane < 8) join[cnt + lane] = 0ull;                 // (up to a multiple of eight)
+        if (lane == 0) s.cnt[w] = cnt;
+        if (tid_ < BM_TOP) s.list[tid_] = 0ull;
+        __syncthreads();
+        const uint64_t c = lane < cnt ? join[lane] : 0ull;
+        int r = 0;
+#pragma unroll 1
+        for (int i = 0; i < SK_NW; ++i) r += bm_above(s.gather[i], s.cnt[i], c);
+        if (c != 0ull && r < n) s.list[r] = c;
+        __syncthreads();
+        return 0ull;
+    }
     if (!sorted) {                                             // ranks: an eighth of a sort's instructions
         const uint64_t c = lane < cnt ? join[lane] : 0ull;
         int r = 0;
@@ -364,20 +360,35 @@ __device__ __forceinline__ void beam_end(const LpBeamArgs& args, LpShared& s, Be
     } else if (!dead) {
         if (!bm_last(bm, a.ticket + (int64_t)row * LP_LINE, 1u, (uint32_t)nseg)) return;
     }
+    // a row's end by one wave, or, one row's long lists, by all
+    if (n <= 16 || (once && m > 1)) {
 #pragma unroll 1
-    for (int r = once ? w : 0; r < (once ? m : w == 0 && !dead ? 1 : 0); r += SK_NW) {
-        const int64_t q = once ? st.r0 + r : (int64_t)row;
-        const float score = b.score ? ld_const(b.score + q) : 0.0f;
-        BeamRow br = bm_dead_row();
-        uint64_t acc = 0ull;
-        if (score > LP_NONE) acc = beam_row_end(a, bm, q, nseg, n, score, T, br);
-        if (once) {
-            if (lane == 0) bm.row[r] = br;
-            if (lane < n) bm.list[r * n + lane] = acc;
-        } else {
-            if (lane == 0) bm_store_row(b, q, br);
-            if (lane < n) st_agent(b.row_lists + q * BM_TOP + lane, acc);
+        for (int r = w; r < (once ? m : dead ? 0 : 1); r += SK_NW) {
+            const int64_t q = once ? st.r0 + r : (int64_t)row;
+            const float score = b.score ? ld_const(b.score + q) : 0.0f;
+            BeamRow br = bm_dead_row();
+            uint64_t acc = 0ull;
+            if (score > LP_NONE) acc = beam_row_end<true>(a, bm, q, nseg, n, score, T, br);
+            if (once) {
+                if (lane == 0) bm.row[r] = br;
+                if (lane < n) bm.list[r * n + lane] = acc;
+            } else {
+                if (lane == 0) bm_store_row(b, q, br);
+                if (lane < n) st_agent(b.row_lists + q * BM_TOP + lane, acc);
+            }
         }
+    } else if (!dead) {
+        BeamRow br;
+        beam_row_end<false>(a, bm, row, nseg, n, b.score ? ld_const(b.score + row) : 0.0f, T, br);
+        if (once) {
+            if (tid == 0) bm.row[0] = br;
+        } else {
+            if (tid == 0) bm_store_row(b, row, br);
+            if (tid < n) st_agent(b.row_lists + (int64_t)row * BM_TOP + tid, bm.list[tid]);
+        }
+    } else if (once) {
+        if (tid == 0) bm.row[0] = bm_dead_row();
+        if (tid < n) bm.list[tid] = 0ull;
     }
     if (!once) {
         if (!bm_last(bm, ticket, 1u, (uint32_t)m)) return;
@@ -388,12 +399,10 @@ __device__ __forceinline__ void beam_end(const LpBeamArgs& args, LpShared& s, Be
         }
     }
     __syncthreads();
-    if (few) {
-        bm_few(b, bm, m, ends);
-        __syncthreads();
-    }
+    if (few) bm_few(b, bm, m, ends);
+    else bm_many(b, bm, st.r0, m, ends);
+    __syncthreads();
     if (w != 0) return;
-    if (!few) bm_join(b, bm, st.r0, m, ends);
     bm_finish(b, bm.best, st.s);
     if (!b.row_off) return;
     for (int e = st.s + 1; e < b.S && ld_const(b.row_off + e + 1) == st.r0 + m; ++e) bm_nothing(b, e);   // streams without rows

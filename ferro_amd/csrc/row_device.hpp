@@ -172,6 +172,33 @@ __device__ __forceinline__ void sk_rank(const uint64_t* cand, uint32_t* rk, int 
     }
 }
 
+// A key that n of the wave's 64 K keys reach, and about a quarter more at most where they differ; n reach `lo` already.
+// Bisected: K compares a step.
+template <int K>
+__device__ __forceinline__ uint32_t lp_nth(const uint32_t (&key)[K], uint32_t lo, int n) {
+    uint32_t hi = key[0];
+#pragma unroll
+    for (int u = 1; u < K; ++u) hi = key[u] > hi ? key[u] : hi;
+    hi = wave_max(hi);
+    if (n == 1) return hi > lo ? hi : lo;
+    uint32_t step = hi > lo ? hi - lo : 0u;                    // the n-th largest lies in [lo, lo + step]
+#pragma unroll 1
+    while (step > 0u) {
+        const uint32_t up = (step >> 1) + (step & 1u);
+        int c = 0;
+#pragma unroll
+        for (int u = 0; u < K; ++u) c += __popcll(__ballot(key[u] >= lo + up));
+        if (c >= n) {
+            lo += up;
+            step -= up;
+            if (c <= n + n / 4) break;
+        } else {
+            step = up - 1u;
+        }
+    }
+    return lo;
+}
+
 // The row's end, in the merging workgroup's wave 0: its token and kept count, a decode step's append and draw, or the
 // verification window's exchange. w: LDS scratch of MT_N entries.
 __device__ __forceinline__ void sk_finish(const SkArgs& a, int row, int pidx, bool sampled, int tok, int keep,
