@@ -45,7 +45,7 @@ struct BeamShared {
         uint64_t gather[SK_NW][512];       // a row's tokens, by the wave that ends it
         BeamBest best;
     };
-    uint16_t at[SK_NW][LP_PARTS * SK_NW];
+    uint16_t at[SK_NW][BM_PARTS * SK_NW];
     BeamRow row[WAVE];                     // the stream's rows,
     uint64_t list[BM_T];                   // their candidates
     int cnt[SK_NW];

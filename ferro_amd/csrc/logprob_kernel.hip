@@ -203,10 +203,10 @@ __device__ __forceinline__ uint64_t beam_row_end(const LpArgs& a, BeamShared& s,
     const int tid_ = threadIdx.x, lane = lane_id(), w = tid_ / WAVE, lists = nseg * SK_NW;
     const LpRow p = lp_row(a, row, nseg);
     const uint64_t* rl = a.lists + row * lists * BM_LIST;
-    constexpr int LL = LP_PARTS * SK_NW / WAVE;
+    constexpr int LL = BM_PARTS * SK_NW / WAVE, KL = 256 / WAVE;       // waves, groups per lane
     double si[LL];
     float mi[LL];
-    uint32_t key[LL];
+    uint32_t key[KL];
     int len[LL];
 #pragma unroll
     for (int u = 0; u < LL; ++u) {
@@ -215,13 +215,16 @@ __device__ __forceinline__ uint64_t beam_row_end(const LpArgs& a, BeamShared& s,
         si[u] = 0.0;
         mi[u] = LP_LOWEST;
         len[u] = 0;
-        key[u] = 0u;
         if (u * WAVE < lists) {                                // (uniform)
             si[u] = in ? __longlong_as_double((long long)ld_agent(reinterpret_cast<const uint64_t*>(p.sum + i))) : 0.0;
             mi[u] = in ? __uint_as_float(ld_agent(reinterpret_cast<const uint32_t*>(p.max + i))) : LP_LOWEST;
             len[u] = in ? ld_agent(p.cnt + i) : 0;
         }
-        if (u * WAVE < (lists << 6) >> lp_group(nseg)) key[u] = i < (lists << 6) >> lp_group(nseg) ? ld_agent(p.key + i) : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < KL; ++u) {
+        const int i = u * WAVE + lane;
+        key[u] = i < (lists << 6) >> lp_group(nseg) ? ld_agent(p.key + i) : 0u;
     }
     const float xv = __uint_as_float(ld_agent(p.above));
     auto fmx = [](float u, float v) { return fmaxf(u, v); };
@@ -230,7 +233,7 @@ __device__ __forceinline__ uint64_t beam_row_end(const LpArgs& a, BeamShared& s,
     if (n <= 16) {
         uint32_t k1 = key[0];
 #pragma unroll
-        for (int u = 1; u < LL; ++u) k1 = key[u] > k1 ? key[u] : k1;
+        for (int u = 1; u < KL; ++u) k1 = key[u] > k1 ? key[u] : k1;
         const uint32_t nth = read_lane(sort64_desc_u32(k1), n - 1);
         least = nth > least ? nth : least;
     } else {
@@ -270,10 +273,11 @@ __device__ __forceinline__ uint64_t beam_row_end(const LpArgs& a, BeamShared& s,
     for (int u = 0; u < LL; ++u) M = fmaxf(M, mi[u]);
     M = wave_allreduce(M, fmx);
     double S = 0.0;
+    static_assert(LL == 2, "");
 #pragma unroll 1
     for (int u = 0; u * WAVE < lists; ++u) {                   // relative to the row's maximum
-        const float m_ = u == 0 ? mi[0] : u == 1 ? mi[1] : u == 2 ? mi[2] : mi[3];
-        const double s_ = u == 0 ? si[0] : u == 1 ? si[1] : u == 2 ? si[2] : si[3];
+        const float m_ = u == 0 ? mi[0] : mi[1];
+        const double s_ = u == 0 ? si[0] : si[1];
         S += m_ == M ? s_ : M < __builtin_huge_valf() ? s_ * exp(((double)m_ - (double)M) / (double)T) : 0.0;
     }
     S = wave_allreduce(S, [](double u, double v) { return u + v; });

@@ -935,15 +935,15 @@ int edit_args(const fs_edits* edits, int32_t rows, int32_t V, fs::EdArgs& ed) {
     return FS_OK;
 }
 
-// Parts per row of fs_logprobs. Four workgroups fit a CU; p parts take ceil(B p / 4 CUs) rounds of ceil(n / p) chunks of a
+// Parts per row of fs_logprobs and fs_beam_select, at most `parts`. Four workgroups fit a CU; p parts take ceil(B p / 4 CUs) rounds of ceil(n / p) chunks of a
 // row's n and of about 4 chunks' time to begin and join, and the p with the shortest of these is taken. For few rows that
 // fills the device once (64 rows of 262144, n 20: 16 parts 25.6 us, 8 30.7, 32 31.2; 256 rows: 4 parts 57.6, 2 78.7, 8 66.3);
 // past half of the slots more parts fill a last round (600 rows of 151936: 3 parts 84.1 us, 1 94.0; 1100 rows of bf16, n 1:
 // 2 parts 79.1, 1 86.1; 700 rows: 1 part 52.5, 2 56.3).
-int logprob_parts(const fs_context* c, int64_t B, int32_t V, int32_t type) {
+int logprob_parts(const fs_context* c, int64_t B, int32_t V, int32_t type, int parts) {
     if (!c->seg_layout) return 1;                  // (a row's parts would not share an L2)
     const int64_t chunk = (int64_t)fs::SK_LT * 4 * fs::LP_NL(type), n = ((int64_t)V + chunk - 1) / chunk;
-    const int64_t slots = 4 * (int64_t)c->cus, most = std::min<int64_t>(n, fs::LP_PARTS);    // (the join: one part per lane)
+    const int64_t slots = 4 * (int64_t)c->cus, most = std::min<int64_t>(n, parts);
     if (B * most <= slots) return (int)most;
     int64_t best = 1, least = INT64_MAX;
     for (int64_t p = 1; p <= most; ++p) {
@@ -991,11 +991,11 @@ int check_state(const fs_state& z, int64_t S, int32_t n_src, int32_t n) {
     return s0 < d1 && d0 < s1 ? FS_E_INVALID : FS_OK;
 }
 
-// The parts, the rows and the workspace of a log-probability kernel's launch (top: the largest it lists; list: entries of a
-// wave's list).
+// The parts, the rows and the workspace of a log-probability kernel's launch (top: the largest it lists; parts, list: the most
+// parts of a row, entries of a wave's list).
 int reserve_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld, int32_t B, int32_t V, int32_t top,
-                     int list, fs::LpArgs& a) {
-    a.nseg = logprob_parts(ctx, B, V, type);
+                     int parts, int list, fs::LpArgs& a) {
+    a.nseg = logprob_parts(ctx, B, V, type, parts);
     if (((int64_t)B + fs::XCDS) * a.nseg > 0x7fffffff) return FS_E_INVALID;
     const size_t entries = (size_t)B * a.nseg * fs::SK_NW * list;
     int rc = grow(ctx, 0, 0, 0);
@@ -1410,7 +1410,7 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
     const int top = d_top_ids || d_top_lp ? n : 0;
     const Edited call(ctx, st);
     if (call.rc != FS_OK) return call.rc;
-    rc = reserve_logprobs(ctx, d_logits, type, ld, B, V, top, fs::LP_TOP, a);
+    rc = reserve_logprobs(ctx, d_logits, type, ld, B, V, top, fs::LP_PARTS, fs::LP_TOP, a);
     if (rc != FS_OK) return rc;
     a.params = d_params; a.tok = d_tok; a.lp = d_lp; a.rank = d_rank; a.ids = d_top_ids; a.top = d_top_lp;
     return fs::launch_logprobs(type, a, st) == hipSuccess ? FS_OK : FS_E_HIP;
@@ -1433,7 +1433,7 @@ int fs_beam_select(fs_context* ctx, const void* d_logits, int32_t type, int64_t 
     const hipStream_t st = (hipStream_t)stream;
     const Edited call(ctx, st);
     if (call.rc != FS_OK) return call.rc;
-    rc = reserve_logprobs(ctx, d_logits, type, ld, total_rows, V, n, fs::BM_LIST, a.lp);
+    rc = reserve_logprobs(ctx, d_logits, type, ld, total_rows, V, n, fs::BM_PARTS, fs::BM_LIST, a.lp);
     if (rc == FS_OK) rc = grow_buffer(ctx, ctx->bm_rows, ctx->bm_row_cap, (size_t)total_rows, 1, false);
     if (rc == FS_OK) rc = grow_buffer(ctx, ctx->bm_lists, ctx->bm_list_cap, (size_t)total_rows, fs::BM_TOP, false);
     if (rc == FS_OK) rc = grow_buffer(ctx, ctx->bm_ticket, ctx->bm_streams, (size_t)n_streams, fs::LP_LINE, true);

@@ -177,6 +177,9 @@ struct BeamRow {                           // a row: what its candidates' scores
     int unused;
 };
 constexpr int BM_LIST = 2 * BM_TOP;        // entries of a wave's list
+// Parts per row: more lists cost a row's end more than more workgroups save. 16 rows of 262144, 8 beams, with 64, 32, 16 parts
+// 16.3, 14.8, 15.9 us; 4 rows of 151936, 64 beams, with 38, 32, 16 31.0, 22.8, 24.1.
+constexpr int BM_PARTS = 32;
 struct BeamArgs {
     int S, W, n, eos;                      // streams; rows of each where row_off is NULL
     int keep_slots;
