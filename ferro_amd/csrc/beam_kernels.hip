@@ -50,16 +50,16 @@ __device__ __forceinline__ ForkRow fork_row(const ForkArgs& a, const ForkFrom& f
 
 constexpr int FK_PER = FK_ROWS / FK_T;     // rows per thread of a scan
 
-// The rows' new offsets, FK_ROWS rows at a time, FK_PER consecutive ones per thread at most: each(row, its first id, its length,
+// The rows' new offsets by NT threads, FK_PER consecutive rows per thread at most at a time: each(row, its first id, its length,
 // its parent's first id). Returns the end. Whole workgroup.
-template <class Each>
+template <int NT, class Each>
 __device__ __forceinline__ int64_t fork_scan(const ForkArgs& a, bool& bad, Each each) {
-    __shared__ int64_t wave[FK_T / WAVE];
+    __shared__ int64_t wave[NT / WAVE];
     const int tid = threadIdx.x, lane = lane_id(), w = tid / WAVE, R = a.S * a.n;
     int64_t carry = 0;
 #pragma unroll 1
-    for (int c = 0; c < R; c += FK_ROWS) {
-        const int left = R - c < FK_ROWS ? R - c : FK_ROWS, per = (left + FK_T - 1) / FK_T;
+    for (int c = 0; c < R; c += NT * FK_PER) {
+        const int left = R - c < NT * FK_PER ? R - c : NT * FK_PER, per = (left + NT - 1) / NT;
         ForkFrom from[FK_PER];
         ForkRow f[FK_PER];
         int64_t mine = 0;
@@ -80,7 +80,7 @@ __device__ __forceinline__ int64_t fork_scan(const ForkArgs& a, bool& bad, Each 
         __syncthreads();
         int64_t at = carry + sum - mine;
 #pragma unroll
-        for (int i = 0; i < FK_T / WAVE; ++i) {
+        for (int i = 0; i < NT / WAVE; ++i) {
             at += i < w ? wave[i] : 0;
             carry += wave[i];
         }
@@ -94,9 +94,10 @@ __device__ __forceinline__ int64_t fork_scan(const ForkArgs& a, bool& bad, Each 
     return carry;
 }
 
-__global__ __launch_bounds__(FK_T) void fork_offsets_kernel(ForkArgs a) {
+constexpr int FK_OFF = 1024;               // threads of the offsets' launch
+__global__ __launch_bounds__(FK_OFF) void fork_offsets_kernel(ForkArgs a) {
     bool bad = false;
-    const int64_t end = fork_scan(a, bad, [&](int o, int64_t v, int64_t, int64_t) { a.out_off[o] = v; });
+    const int64_t end = fork_scan<FK_OFF>(a, bad, [&](int o, int64_t v, int64_t, int64_t) { a.out_off[o] = v; });
     if (threadIdx.x == 0) {
         a.out_off[(int64_t)a.S * a.n] = end;
         if (end > a.out_cap) atomicOr(a.err, FS_DEVERR_HIST_APPEND);
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(FK_T) void fork_kernel(ForkArgs a) {
     bool bad = false;
     int64_t end;
     if (SELF) {
-        end = fork_scan(a, bad, [&](int o, int64_t v, int64_t, int64_t from) {
+        end = fork_scan<FK_T>(a, bad, [&](int o, int64_t v, int64_t, int64_t from) {
             s_off[o] = v;
             s_at[o] = from;
         });
@@ -196,7 +197,7 @@ hipError_t launch_hist_fork(const ForkArgs& a, int cus, hipStream_t st) {
         hipLaunchKernelGGL(fork_kernel<true>, grid, block, 0, st, a);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL(fork_offsets_kernel, dim3(1), block, 0, st, a);
+    hipLaunchKernelGGL(fork_offsets_kernel, dim3(1), dim3(FK_OFF), 0, st, a);
     hipLaunchKernelGGL(fork_kernel<false>, grid, block, 0, st, a);
     return hipGetLastError();
 }

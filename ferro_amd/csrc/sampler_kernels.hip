@@ -1450,7 +1450,7 @@ int fs_beam_select(fs_context* ctx, const void* d_logits, int32_t type, int64_t 
 int fs_hist_fork(fs_context* ctx, int32_t n_streams, const int32_t* d_hist, const int64_t* d_hist_off,
                  const int64_t* d_row_off, int32_t n, const int32_t* d_parent, const int32_t* d_tok, int32_t* d_out_hist,
                  int64_t out_cap, int64_t* d_out_hist_off, void* stream) {
-    if (!ctx || n_streams < 0 || n < 1 || out_cap < 0 || (int64_t)n_streams * n > 0x7fffffff || !d_out_hist_off ||
+    if (!ctx || n_streams < 0 || n < 1 || out_cap < 0 || (int64_t)n_streams * n > 0x3fffffff || !d_out_hist_off ||
         (out_cap > 0 && !d_out_hist))
         return FS_E_INVALID;
     if (n_streams > 0 && (!d_hist_off || !d_parent)) return FS_E_INVALID;
@@ -1475,6 +1475,10 @@ int fs_reorder_states(fs_context* ctx, int32_t n_states, const fs_state* states,
     for (int32_t i = 0; i < n_states; ++i) {
         const int rc = check_state(states[i], n_streams, n_src, n);
         if (rc != FS_OK) return rc;
+        for (int32_t j = 0; j < i; ++j)            // (interleaved states are fine; one given twice would move twice)
+            if (states[i].d_dst && (states[i].d_dst == states[j].d_dst || states[i].d_dst == states[j].d_src ||
+                                    states[i].d_src == states[j].d_dst))
+                return FS_E_INVALID;
     }
     if (n_streams == 0 || n_states == 0) return FS_OK;
     const hipStream_t st = (hipStream_t)stream;

@@ -334,7 +334,7 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
  * Token t of row r is the candidate
  *     c(r, t) = d_score[r] + log softmax((cap(l) + bias) / T)(t)      (fs_logprobs' distribution, by the stream's record)
  * in fp64; a token that is not allowed, whose logit is NaN or -inf, or whose c does not round to a fp32 above -inf is none.
- * Candidates come by c; among equal ones those of eos_id (-1: none) first, then the lower row's, in a row the larger logit's,
+ * Candidates come by c, compared to 39 bits of its mantissa (2e-12 of it); among equal ones those of eos_id (-1: none) first, then the lower row's, in a row the larger logit's,
  * then the lower token's. The n best (n <= FS_MAX_TOP) whose token is not eos_id are the new beams: d_parent [n_streams][n]
  * (the row's number in its stream, from 0), d_tok, d_out_score; places past a stream's candidates hold -1, -1 and -inf. Those
  * with eos_id that fewer than n candidates come before are ended hypotheses: their number d_done[s] and, in their order,
@@ -343,7 +343,9 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
  * flags: FS_BEAM_KEEP_SLOTS puts a parent's best child into the parent's own place (where that is below n) and the others, in
  * their order, into the free places, ascending: a state then moves for a parent's further children alone; without it the
  * beams come best first. edits: masks by row, biases by stream, may be NULL; penalties are fs_edit_batch's. d_params NULL: no
- * softcap, T = 1. Rows and types as in fs_edit_batch. No counterpart in the reference (ferro samples). */
+ * softcap, T = 1. Rows and types as in fs_edit_batch; the outputs must not overlap the inputs. The workspace is 4 KB per row
+ * and part (32 parts at most) and grows as a context's other buffers do; under graph capture a call that would have to grow it
+ * returns FS_E_NOMEM. No counterpart in the reference (ferro samples). */
 #define FS_BEAM_KEEP_SLOTS 1
 int fs_beam_select(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld, int32_t n_streams, int32_t total_rows,
                    int32_t V, const int64_t* d_row_off, const float* d_score, const fs_row_params* d_params,
@@ -376,7 +378,7 @@ typedef struct fs_state {
  * rows of a stream may change places, be copied more than once or dropped. d_from is for what a stream's beams share (the
  * prompt), which need not move. A parent below 0 leaves its row as it was. n, n_src <= FS_MAX_TOP; n_src = 1 opens the beams
  * of prompts. `states` is host memory, read before the call returns; the states' rows must not overlap one another, nor a
- * d_dst any other state of the call (in place: its own d_src alone). */
+ * d_dst any other state of the call (in place: its own d_src alone; a buffer given twice is refused). */
 int fs_reorder_states(fs_context* ctx, int32_t n_states, const fs_state* states, int32_t n_streams, int32_t n_src, int32_t n,
                       const int32_t* d_parent, const int32_t* d_from, const int32_t* d_len, void* stream);
 

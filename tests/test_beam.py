@@ -66,6 +66,9 @@ def test_state_refusals(ctx):
     bad += [state(d_src=0), state(d_dst=0), state(d_dst=(1 << 20) + 8), state(dst_row=128), state(src_row=1 << 50, dst_row=1 << 50),
             state(pos_bytes=1 << 32), state(blocks=1 << 20, positions=1 << 20), state(blocks=1 << 15, positions=1 << 15, pos_bytes=64)]
     refused(_lib.lib().fs_reorder_states, good, ctx=None, k=-1, z=[None] + bad, S=-1, n_src=[0, 65, 3], n=[0, 65, 5], parent=None)
+    twice = (_lib.FsState * 2)(state()[0], state(src_row=128, dst_row=128)[0])
+    chain = (_lib.FsState * 2)(state(d_dst=2 << 20)[0], state(d_src=2 << 20, d_dst=3 << 20)[0])
+    refused(_lib.lib().fs_reorder_states, dict(good, k=2), z=[twice, chain])
     apart = dict(good, z=state(d_dst=(1 << 20) + 512), S=0)
     assert _lib.lib().fs_reorder_states(*apart.values()) == _lib.FS_OK
     assert _lib.lib().fs_reorder_states(*dict(good, k=0, z=None).values()) == _lib.FS_OK
