@@ -29,20 +29,20 @@ __device__ __forceinline__ uint64_t bm_key(double c, uint32_t low) {
 
 struct BeamBest {                          // a stream's end
     uint64_t key[BM_T + 16];               // candidates; 0 up to a multiple of eight (few: then what ends the text)
-    uint64_t ekey[2 * BM_TOP + 8];
+    uint64_t ekey[2 * BM_TOP + 8], ebest[BM_TOP];
     uint64_t entry[BM_T];
     int crow[BM_T];
-    uint32_t hi[4][WAVE];
+    uint32_t hi[SK_NW][WAVE];
     float cvalue[BM_TOP];
-    int cnt, again;
+    int cnt, room, again;
     int from[BM_TOP], token[BM_TOP], efrom[BM_TOP], first[BM_TOP], place[BM_TOP];
     float value[BM_TOP], evalue[BM_TOP];
     int n_ends;
 };
-// (no larger than the parts' lists, whose place it takes)
+// (it takes the place of the parts' lists; four workgroups of 40 KB fit a CU)
 struct BeamShared {
     union {
-        uint64_t gather[SK_NW][512];       // a row's tokens, by the wave that ends it
+        uint64_t gather[SK_NW][1024];      // a row's tokens, by the wave that ends it
         BeamBest best;
     };
     uint16_t at[SK_NW][BM_PARTS * SK_NW];
@@ -138,147 +138,143 @@ __device__ __forceinline__ void bm_few(const BeamArgs& a, BeamShared& sh, int m,
     }
 }
 
-// Any number of rows, 64 at a time (a batch), a row per lane. Of the first four places of the rows' lists, which are in order, n
-// reach a bound (as lp_nth); places further down are read as long as one of them reaches it. The candidates so found (about 1.5 n)
-// are put in order, a thread each, with the best of earlier batches; where there is no room for them, they are before the walk
-// goes on.
+// Any number of rows, 64 at a time (a batch), a row per lane; wave w takes places w, w + 4, .. of their lists, which are in order.
+// Of the first four places n reach a bound (as lp_nth); a wave goes on down the lists as long as one of them reaches it. The
+// candidates so found (about 1.5 n) are put in order, a thread each, with the best of earlier batches; where there is no room for
+// more, they are before the walk goes on.
 constexpr uint64_t BM_MASK = ~(uint64_t)((1u << BM_LOW) - 1u);
 __device__ __forceinline__ void bm_many(const BeamArgs& a, BeamShared& sh, int64_t r0, int m, bool ends) {
     BeamBest& s = sh.best;
     const int t = threadIdx.x, lane = lane_id(), w = t / WAVE, n = a.n;
     constexpr float NONE = -__builtin_huge_valf();
-    uint32_t least = 1u;                                       // (of the keys' upper halves; the first wave's)
+    uint32_t least = 1u;                                       // (of the keys' upper halves)
     int held = 0;                                              // of s.key: the best so far, in order
     if (t < BM_TOP) {
-        s.ekey[BM_TOP + t] = 0ull;
+        s.ebest[t] = 0ull;
         s.efrom[t] = -1;
         s.evalue[t] = NONE;
     }
-    if (t == 0) s.cnt = 0;
     __syncthreads();
 #pragma unroll 1
     for (int b = 0; b < m; b += WAVE) {
         const int k = m - b < WAVE ? m - b : WAVE;             // rows of this batch
         const uint64_t* list = a.row_lists + (r0 + b + lane) * BM_TOP;
         auto fetch = [&](int p) { return lane < k && p < n ? ld_agent(list + p) : (uint64_t)0; };
-        uint64_t next[4] = {0ull, 0ull, 0ull, 0ull};           // places p .. p + 3
+        int p = w;
+        uint64_t e = fetch(p), next = fetch(p + SK_NW);
         BeamRow br = bm_dead_row();
-        int p = 0;
+        if (lane < k) br = bm_load_row(a, r0 + b + lane);
         if (w == 0) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) next[u] = fetch(u);
-            if (lane < k) br = bm_load_row(a, r0 + b + lane);
             sh.row[lane] = br;
-            if (b > 0 && lane < s.cnt) s.key[lane] = (s.key[lane] & BM_MASK) | BM_OLD | (uint32_t)(63 - lane);  // before equal ones
+            if (lane < held) s.key[lane] = (s.key[lane] & BM_MASK) | BM_OLD | (uint32_t)(63 - lane);   // before equal ones
         }
-        auto key_now = [&]() {
-            return bm_key(next[0] ? bm_score(br, val_of(comp_key(next[0]))) : (double)NONE, 4095u - (uint32_t)(lane * 64 + p));
-        };
-        auto advance = [&]() {
-            next[0] = next[1];
-            next[1] = next[2];
-            next[2] = next[3];
-            next[3] = fetch(p + 4);
-            ++p;
-        };
-        bool go = true;
+        // what ends the text: the batch's rows (wave 2) and the best of earlier ones (wave 3), which come before equal ones
+        uint64_t ek = 0ull;
+        int efrom = -1;
+        float evalue = NONE;
+        if (ends && w == 3) {
+            ek = s.ebest[lane];
+            efrom = s.efrom[lane];
+            evalue = s.evalue[lane];
+        }
+        uint64_t key = 0ull;
 #pragma unroll 1
-        for (int round = 0; go; ++round) {
-            if (w == 0) {
-                int cnt = s.cnt;
-                if (round == 0) {
-                    const uint64_t first[4] = {next[0], next[1], next[2], next[3]};
+        for (int round = 0;; ++round) {
+            bool go = true;
+            auto key_now = [&](bool end) {
+                const double c = bm_score(br, end ? br.eos : e ? val_of(comp_key(e)) : NONE);
+                if (end) evalue = (float)c;
+                return bm_key(c, 4095u - (uint32_t)(lane * 64 + (end ? 0 : p)));
+            };
+            if (round == 0) {
 #pragma unroll 1
-                    for (int u = 0; u < 4; ++u) {
-                        s.hi[u][lane] = (uint32_t)(key_now() >> 32);
-                        next[0] = next[1];
-                        next[1] = next[2];
-                        next[2] = next[3];
-                        ++p;
+                for (int end = ends && w == 2 ? 1 : 0; end >= 0; --end) {
+                    const uint64_t kk = key_now(end != 0);
+                    if (end) {
+                        ek = kk;
+                        efrom = b + lane;
+                    } else {
+                        key = kk;
                     }
-                    p = 0;
-                    bm_sync();
-                    const uint32_t hi[4] = {s.hi[0][lane], s.hi[1][lane], s.hi[2][lane], s.hi[3][lane]};
-                    // (the lists are in order: all of these reach the least of the fourth)
-                    const uint32_t reach = wave_min(lane >= k ? ~0u : hi[3] > 1u ? hi[3] : 1u);
-                    least = lp_nth(hi, 4 * k >= n && reach > least ? reach : least, n);
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) next[u] = first[u];
                 }
-#pragma unroll 1
-                while (go) {                                   // a place at a time
-                    const uint64_t key = key_now();
-                    const bool in = (uint32_t)(key >> 32) >= least;
-                    const uint64_t mm = __ballot(in);
-                    go = mm != 0ull && p < n;                  // (in order: no more below places that none reaches)
-                    if (!go || cnt + __popcll(mm) > BM_T) break;       // (no room: the next round)
-                    if (in) {
-                        const int i = cnt + (int)mbcnt(mm);
-                        s.key[i] = key;
-                        s.entry[i] = next[0];
-                        s.crow[i] = b + lane;
-                    }
-                    cnt += __popcll(mm);
-                    advance();
-                }
-                if (lane < 8) s.key[cnt + lane] = 0ull;
-                if (lane == 0) {
-                    s.cnt = cnt;
-                    s.again = go ? 1 : 0;
-                }
+                s.hi[w][lane] = (uint32_t)(key >> 32);
+                if (w >= 2) s.ekey[t - 2 * WAVE] = ek;
+                if (t < 8) s.ekey[2 * BM_TOP + t] = 0ull;
+            }
+            if (t == 0) {
+                s.cnt = held;
+                s.room = BM_T;
+                s.again = 0;
             }
             __syncthreads();
-            const int all = s.cnt;
-            go = s.again != 0;
-            const uint64_t key = t < all ? s.key[t] : 0ull, e = t < all ? s.entry[t] : 0ull;
+            if (round == 0) {
+                const uint32_t hi[4] = {s.hi[0][lane], s.hi[1][lane], s.hi[2][lane], s.hi[3][lane]};
+                // (the lists are in order: all of these reach the least of the fourth places)
+                const uint32_t reach = wave_min(lane >= k ? ~0u : hi[3] > 1u ? hi[3] : 1u);
+                least = lp_nth(hi, 4 * k >= n && reach > least ? reach : least, n);
+            }
+#pragma unroll 1
+            while (go) {
+                const bool in = (uint32_t)(key >> 32) >= least;
+                const uint64_t mm = __ballot(in);
+                go = mm != 0ull;                               // (in order: no more below places that none reaches)
+                if (!go) break;
+                int at = 0;
+                if (lane == 0) at = atomicAdd(&s.cnt, __popcll(mm));
+                at = read_lane(at, 0);
+                if (at + __popcll(mm) > BM_T) {                // no room: in the next round (what follows has none either)
+                    if (lane == 0) {
+                        atomicMin(&s.room, at);
+                        s.again = 1;
+                    }
+                    break;
+                }
+                if (in) {
+                    const int i = at + (int)mbcnt(mm);
+                    s.key[i] = key;
+                    s.entry[i] = e;
+                    s.crow[i] = b + lane;
+                }
+                p += SK_NW;
+                e = next;
+                next = fetch(p + SK_NW);
+                key = key_now(false);
+            }
+            __syncthreads();
+            const int all = s.cnt < s.room ? s.cnt : s.room;
+            const bool again = s.again != 0;
+            if (t < 8) s.key[all + t] = 0ull;
+            const uint64_t ck = t < all ? s.key[t] : 0ull, c = t < all ? s.entry[t] : 0ull;
             const int row = t < all ? s.crow[t] : -1;
             float value = t < BM_TOP ? s.cvalue[t] : NONE;     // (of the best of earlier rounds)
-            if (t < all && t >= held) value = (float)bm_score(sh.row[row - b], val_of(comp_key(e)));
-            const int at = key ? bm_above(s.key, all, key) : BM_T;
+            if (t < all && t >= held) value = (float)bm_score(sh.row[row - b], val_of(comp_key(c)));
+            __syncthreads();
+            const int at = ck ? bm_above(s.key, all, ck) : BM_T;
+            const int eat = round == 0 && ek ? bm_above(s.ekey, 2 * BM_TOP, ek) : BM_T;
             __syncthreads();
             if (at < n) {
-                s.key[at] = key;
-                s.entry[at] = e;
+                s.key[at] = ck;
+                s.entry[at] = c;
                 s.crow[at] = row;
                 s.cvalue[at] = value;
             }
+            if (round == 0 && t < BM_TOP) s.ebest[t] = 0ull;
             held = all < n ? all : n;
             if (t < 8) s.key[held + t] = 0ull;
-            if (t == 0) s.cnt = held;
             __syncthreads();
-            if (w == 0 && held == n) least = (uint32_t)(s.key[n - 1] >> 32);
-        }
-        if (!ends) continue;
-        // what ends the text: the batch's rows, and the best of earlier ones (which come before equal ones)
-        uint64_t key = 0ull;
-        int from = -1;
-        float value = NONE;
-        if (w == 0) {
-            const double c = bm_score(br, br.eos);
-            key = bm_key(c, 4095u - (uint32_t)(lane * 64));
-            from = b + lane;
-            value = (float)c;
-        } else if (w == 1) {
-            key = s.ekey[BM_TOP + lane];
-            from = s.efrom[lane];
-            value = s.evalue[lane];
-        }
-        if (w == 0) s.ekey[lane] = key;
-        __syncthreads();
-        const int at = key ? bm_above(s.ekey, 2 * BM_TOP, key) : BM_T;
-        __syncthreads();
-        if (w == 1) s.ekey[t] = 0ull;
-        __syncthreads();
-        if (at < n) {
-            s.ekey[BM_TOP + at] = (key & BM_MASK) | BM_OLD | (uint32_t)(63 - at);
-            s.efrom[at] = from;
-            s.evalue[at] = value;
+            if (eat < n) {
+                s.ebest[eat] = (ek & BM_MASK) | BM_OLD | (uint32_t)(63 - eat);
+                s.efrom[eat] = efrom;
+                s.evalue[eat] = evalue;
+            }
+            if (held == n) least = (uint32_t)(s.key[n - 1] >> 32);
+            if (!again) break;                                 // (uniform: a wave that has come to its end goes along)
         }
         __syncthreads();
     }
     if (t < BM_TOP) {
-        const bool live = t < s.cnt;
-        const uint64_t key = s.ekey[BM_TOP + t];
+        const bool live = t < held;
+        const uint64_t key = s.ebest[t];
         s.from[t] = live ? s.crow[t] : -1;
         s.token[t] = live ? (int)comp_id(s.entry[t]) : -1;
         s.value[t] = live ? s.cvalue[t] : NONE;

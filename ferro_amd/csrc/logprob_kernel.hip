@@ -239,8 +239,8 @@ __device__ __forceinline__ uint64_t beam_row_end(const LpArgs& a, BeamShared& s,
     } else {
         least = lp_nth(key, least, n);
     }
-    // lists of waves whose largest logit reaches the bound; half a wave reads 32 entries of one
-    constexpr int U = 4, ROOM = sizeof(s.gather[0]) / sizeof(uint64_t);
+    // lists of waves whose largest logit reaches the bound: half a wave reads 32 entries of one, or, of long lists, a wave 64
+    constexpr int PER = ALONE ? 32 : WAVE, LANES = WAVE / PER, U = ALONE ? 4 : 8, ROOM = sizeof(s.gather[0]) / sizeof(uint64_t);
     uint16_t* at = s.at[w];
     uint64_t* join = s.gather[w];
     int k = 0;
@@ -256,13 +256,13 @@ __device__ __forceinline__ uint64_t beam_row_end(const LpArgs& a, BeamShared& s,
     const int k0 = ALONE ? 0 : w;                              // this wave's: k0, k0 + STEP, ..
     k = (k - k0 + STEP - 1) / STEP;
     lp_wave_sync();
-    const int half = lane >> 5, pos = lane & 31;
+    const int sub = lane / PER, pos = lane % PER;
     int to[U];
     uint64_t e[U];
     auto fetch = [&](int i0, int skip) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = i0 + 2 * u + half;
+            const int i = i0 + LANES * u + sub;
             to[u] = i < k ? at[k0 + i * STEP] : 0;
             e[u] = pos + skip < (to[u] & 255) ? ld_agent(rl + (to[u] >> 8) * BM_LIST + pos + skip) : 0ull;
         }
@@ -302,11 +302,11 @@ __device__ __forceinline__ uint64_t beam_row_end(const LpArgs& a, BeamShared& s,
             const uint64_t m = __ballot(in);
             if (in) join[cnt + (int)mbcnt(m)] = e[u];
             cnt += __popcll(m);
-            more |= (to[u] & 255) > skip + 32;
+            more |= (to[u] & 255) > skip + PER;
         }
         const bool longer = __ballot(more) != 0ull;            // lists that have more entries
-        skip = longer ? skip + 32 : 0;
-        i0 = longer ? i0 : i0 + 2 * U;
+        skip = longer ? skip + PER : 0;
+        i0 = longer ? i0 : i0 + LANES * U;
         const bool last = i0 >= k;
         if (cnt > ROOM - U * WAVE || (last && (sorted || cnt > WAVE))) sort();
         if (!last) fetch(i0, skip);

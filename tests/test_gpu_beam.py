@@ -111,6 +111,21 @@ def test_select_ties(kind):
     Rows(4, [3], 2000, kind, lambda rng, R, V: np.zeros((R, V), np.float32)).run(64, eos=1999)
 
 
+@pytest.mark.parametrize("n", [5, 20, 64])
+def test_select_ties_of_many_rows(n):
+    """More equal candidates than there is room for: alike rows, of one value and of few, dead ones among them."""
+    for seed, counts, V, values in ((40, [70, 130], 200, 1), (41, [64], 90, 1), (42, [17, 65], 300, 3), (43, [20], 64, 2)):
+        r = Rows(seed, counts, V, "bf16", lambda rng, R, V: rng.integers(0, values, (1, V)).astype(np.float32).repeat(R, 0))
+        r.score[:] = -2.0
+        r.score[[0, 9]] = -np.inf
+        out = r.run(n, eos=int(r.y[0].argmax()))
+        t = [i for i in np.flatnonzero(r.y[0] == r.y[0].max()) if i != int(r.y[0].argmax())][:n]
+        assert out["parent"][0].tolist()[:len(t)] == [1] * len(t) and out["tok"][0].tolist()[:len(t)] == t
+        # scores apart by less than the rows' candidates
+        r.score = (-2.0 - 0.01 * r.rng.random(r.score.size)).astype(np.float32)
+        r.run(n, eos=0)
+
+
 def test_select_dead_rows():
     """Rows of score -inf or NaN are not read; streams of dead rows alone have no beam."""
     r = Rows(11, [4, 4, 4], 3001)
