@@ -17,7 +17,8 @@ constexpr int FK_T = 256;
 constexpr int FK_ROWS = 1024;              // rows whose offsets are kept in LDS
 constexpr int FK_STEP = FK_T * 4;          // ids a workgroup copies at a time
 constexpr int FK_U = 4;                    // of these in flight
-// Workgroups per CU. 512 histories of 2048 ids with 1, 2, 4, 8: 13.9, 10.4, 8.7, 7.5 us; 256 of 32768 32.4, 20.0, 16.7, 17.0.
+// Workgroups per CU. 512 histories of 2048 ids with 1, 2, 4, 8: 13.9, 10.4, 8.7, 7.5 us; 256 of 32768 32.4, 20.0, 16.7, 17.0
+// (then with registers for six on a CU; with registers for eight 6.7 and 13.9).
 constexpr int FK_PER_CU = 8;
 
 struct ForkRow {
@@ -108,7 +109,7 @@ __global__ __launch_bounds__(FK_OFF) void fork_offsets_kernel(ForkArgs a) {
 typedef int i32x4a __attribute__((ext_vector_type(4), aligned(4)));    // (histories begin at any id)
 
 template <bool SELF>
-__global__ __launch_bounds__(FK_T) void fork_kernel(ForkArgs a) {
+__global__ __launch_bounds__(FK_T, 8) void fork_kernel(ForkArgs a) {
     __shared__ int64_t s_off[SELF ? FK_ROWS + 1 : 1], s_at[SELF ? FK_ROWS : 1];
     __shared__ int s_row[2];
     const int tid = threadIdx.x, R = a.S * a.n;
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(FK_T) void fork_kernel(ForkArgs a) {
 #pragma unroll
         for (int u = 0; u < FK_U; ++u) {
             const int64_t i = i0 + u * FK_STEP + tid * 4;
-            if (from[u] == 4) *reinterpret_cast<i32x4a*>(a.out + i) = v[u];
+            if (from[u] == 4) __builtin_nontemporal_store(v[u], reinterpret_cast<i32x4a*>(a.out + i));
             if (from[u] == 0) {                                // a history's end, or the share's: one at a time
                 for (int64_t j = i; j < i + 4 && j < e; ++j) {
                     const int r = row_of(j, r0, r1);
@@ -305,7 +306,7 @@ __global__ __launch_bounds__(ST_T) void reorder_states_kernel(StateArgs a_) {
                         char* d = dst0 + (__ffsll((unsigned long long)m) - 1) * z.dst_row;
 #pragma unroll
                         for (int c = 0; c < K; ++c)
-                            if (on[c]) *reinterpret_cast<Vec*>(d + d_o[c]) = v[i][c];
+                            if (on[c]) __builtin_nontemporal_store(v[i][c], reinterpret_cast<Vec*>(d + d_o[c]));
                     }
             }
             turn -= total;
