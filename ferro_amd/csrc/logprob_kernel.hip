@@ -65,20 +65,35 @@ __device__ __forceinline__ float lp_max3(float a, float b, float c) {   // (fmax
     return a;
 }
 
-// BEAM: of four maxima per lane. A few tokens are found by the lanes' largest alone; for many these are too few, and the least
-// of them lets most of the logits pass (128 rows of 100003 fp16, n 64: 88 us).
-__device__ __forceinline__ uint32_t lp_nth_set(const float (&ls)[4], float reach, int n) {
-    uint32_t from;
-    auto at_least = [&](uint32_t f) { return reach > LP_LOWEST && f < key_of(reach) ? key_of(reach) : f; };
-    if (n <= 16) {
-        const uint32_t key[1] = {key_of(lp_max3(lp_max3(ls[0], ls[1], ls[2]), ls[3], ls[3]))};
-        return lp_nth(key, at_least(wave_min(key[0])), n);
-    }
-    const uint32_t key[4] = {key_of(ls[0]), key_of(ls[1]), key_of(ls[2]), key_of(ls[3])};
-    from = key[0];
+// BEAM: the key that n of the wave's maxima reach (at most that of -inf: none), of four maxima per lane. A few tokens are found
+// by the lanes' largest alone; for many these are too few, and the least of them lets most of the logits pass (128 rows of 100003
+// fp16, n 64: 88 us). Where a mask leaves few tokens, fewer than n may be above -inf and there is nothing to bisect, or from the
+// least of them on (195 rows of 151936 with a few to a few hundred allowed tokens each: 38 -> 31 us).
+template <int K>
+__device__ __forceinline__ uint32_t lp_nth_of(const float (&v)[K], float reach, int n, bool masked) {
+    uint32_t key[K], from = ~0u;
 #pragma unroll
-    for (int i = 1; i < 4; ++i) from = key[i] < from ? key[i] : from;
-    return lp_nth(key, at_least(wave_min(from)), n);
+    for (int u = 0; u < K; ++u) {
+        key[u] = key_of(v[u]);
+        from = key[u] < from ? key[u] : from;
+    }
+    if (masked) {
+        int have = 0;
+        from = ~0u;
+#pragma unroll
+        for (int u = 0; u < K; ++u) {
+            have += __popcll(__ballot(key[u] > 0x007FFFFFu));
+            from = key[u] > 0x007FFFFFu && key[u] < from ? key[u] : from;
+        }
+        if (have < n) return 0u;
+    }
+    from = wave_min(from);                                     // (every lane reaches it)
+    return lp_nth(key, reach > LP_LOWEST && from < key_of(reach) ? key_of(reach) : from, n);
+}
+__device__ __forceinline__ uint32_t lp_nth_set(const float (&ls)[4], float reach, int n, bool masked) {
+    if (n > 16) return lp_nth_of(ls, reach, n, masked);
+    const float lm[1] = {lp_max3(lp_max3(ls[0], ls[1], ls[2]), ls[3], ls[3])};
+    return lp_nth_of(lm, reach, n, masked);
 }
 
 // What the wave keeps of its list of g groups and an earlier cut: its n largest tokens at or above the bound, sorted, one
@@ -141,7 +156,7 @@ __device__ __forceinline__ void beam_publish(const LpArgs& a, LpShared& s, int r
     uint64_t* out = a.lists + ((int64_t)row * nseg * SK_NW + me) * BM_LIST;
     sum = wave_allreduce(sum, [](double u, double v) { return u + v; });
     if (n > 16) {                                              // (many tokens: a fresh bound leaves few to write and to read)
-        const uint32_t nth = lp_nth_set(ls, reach, n);
+        const uint32_t nth = lp_nth_set(ls, reach, n, true);
         reach = fmaxf(reach, nth > 0x007FFFFFu ? val_of(nth) : LP_LOWEST);
     }
     if (lane == 0) s.bound[w] = reach;
@@ -660,7 +675,7 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
             if (any && g - bound_at >= LP_GROWN) {
                 uint32_t nth;
                 if constexpr (BEAM) {
-                    nth = lp_nth_set(ls, reach, n);
+                    nth = lp_nth_set(ls, reach, n, masked);
                 } else {
                     const uint32_t key[1] = {key_of(lm)};
                     uint32_t from = wave_min(key[0]);          // (every lane reaches it)
