@@ -1,7 +1,8 @@
 // beam_device.hpp - the end of a beam search's selection: the best candidates of a stream's rows, the hypotheses that end and
 // the places of the new beams.
 // This code runs once per stream, behind everything else, from a cold instruction cache (about 40 ns per 64 bytes): loops stay
-// rolled, and few candidates are put in order by counting those before each (a sort of 64 takes 1.7 us the first time).
+// rolled, and few candidates are put in order by counting those before each (a sort of 64 takes 1.7 us the first time): 16 of
+// four rows 1.1 us, 64 and their ends of eight rows 1.8; 64 of 64 rows' 4096 (bm_many) about 7, by sorts and merges 13.7.
 #ifndef FERRO_BEAM_DEVICE_HPP
 #define FERRO_BEAM_DEVICE_HPP
 

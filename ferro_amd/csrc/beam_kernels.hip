@@ -13,8 +13,8 @@ namespace fs {
 // row, from the L2) and copies an equal share of the new ids, four per thread at a time, whose rows it finds by bisection among
 // those of its share. More rows: a launch for the offsets first, which the copying one then reads. The new ids are stored past
 // the caches (256 histories of 32768 ids: 14.2 -> 13.1 us).
-// Bound: latency for few ids (4.5 us for 4 histories of 300, 6.1 for 512 of 2048), then HBM: 256 of 32768, of which half are
-// read, 13.3 us (3.8 TB/s of 50 MB).
+// Bound: latency for few ids (4.5 us for 4 histories of 300, 6.1 for 512 of 2048), then HBM: 256 of 32768 13.3 us (4.9 TB/s of
+// 65 MB).
 constexpr int FK_T = 256;
 constexpr int FK_ROWS = 1024;              // rows whose offsets are kept in LDS
 constexpr int FK_STEP = FK_T * 4;          // ids a workgroup copies at a time
@@ -217,8 +217,8 @@ hipError_t launch_hist_fork(const ForkArgs& a, int cus, hipStream_t st) {
 // 64 MB, 209 -> 221: many states at once are not good for the memory.)
 // Stores go past the caches, loads do not (a source may be read again): 16 caches of 64 rows 87.1 -> 80.8 us with stores so; with
 // loads so, too, no more.
-// Bound: HBM: those caches 80 us (5.0 TB/s of 403 MB), 16 prompt caches of a stream opened into four beams each 224 us (5.9 TB/s,
-// four fifths of them stores), one small state 4.6.
+// Bound: HBM: those caches 79 us (4.7 TB/s of 373 MB), 16 caches of 16 prompts opened into four beams each 223 us (4.8 TB/s of
+// 1064 MB, four fifths of them stores), one small state 4.6.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 template <int VB>
