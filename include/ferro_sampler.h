@@ -339,7 +339,8 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
  * (the row's number in its stream, from 0), d_tok, d_out_score; places past a stream's candidates hold -1, -1 and -inf. Those
  * with eos_id that fewer than n candidates come before are ended hypotheses: their number d_done[s] and, in their order,
  * d_done_parent and d_done_score [n_streams][n], -1 and -inf past them (each may be NULL; min(n, the stream's rows) at most).
- * Rows whose score is -inf or NaN have no candidate and are not read: the last step's d_out_score is this step's d_score.
+ * Rows whose score is -inf or NaN have no candidate, whatever their logits (of which at most the parts' first 16 KB are read):
+ * the last step's d_out_score is this step's d_score.
  * flags: FS_BEAM_KEEP_SLOTS puts a parent's best child into the parent's own place (where that is below n) and the others, in
  * their order, into the free places, ascending: a state then moves for a parent's further children alone; without it the
  * beams come best first. edits: masks by row, biases by stream, may be NULL; penalties are fs_edit_batch's. d_params NULL: no

@@ -127,7 +127,7 @@ def test_select_ties_of_many_rows(n):
 
 
 def test_select_dead_rows():
-    """Rows of score -inf or NaN are not read; streams of dead rows alone have no beam."""
+    """Rows of score -inf or NaN do not matter, whatever they hold; streams of dead rows alone have no beam."""
     r = Rows(11, [4, 4, 4], 3001)
     r.score[[1, 4, 5, 6, 7, 9]] = -np.inf
     r.score[10] = np.nan
