@@ -804,14 +804,28 @@ def _parents(parent, dev):
     return parent
 
 
-def hist_fork(hist, hist_off, parent, tok=None, row_off=None, out_cap=None, ctx=None, stream=None):
+def _fork_ids(off, row_off, S, n):
+    """Ids that S streams' n new histories each come to at most, without new tokens: the longest of a stream's, n times. Host
+    arrays: the histories' offsets, and the streams' rows (None: n each)."""
+    lens = np.append(np.maximum(np.diff(off), 0), 0)           # (a 0 behind the last: a stream may end there)
+    ro = np.arange(0, S * n + 1, n) if row_off is None else np.clip(row_off, 0, lens.size - 1)
+    ro = np.stack([ro[:-1], ro[1:]], 1)[ro[1:] > ro[:-1]].ravel()
+    return n * int(np.maximum.reduceat(lens, ro)[::2].sum()) if ro.size else 0
+
+
+def hist_fork(hist, hist_off, parent, tok=None, row_off=None, out_cap=None, ctx=None, stream=None, max_len=None):
     """fs_hist_fork: the new beams' histories. hist, hist_off: CSR histories of the present beams, whose rows row_off gives
     (None: as many per stream as there are new ones); parent, tok [S, n] (tok None: nothing is appended), as beam_select
-    returns them. Returns (out_hist, out_off): row s * n + j the history of beam j of stream s; out_hist holds out_cap ids
-    (default: room for any parents). Nothing here waits for the GPU."""
+    returns them. Returns (out_hist, out_off): row s * n + j the history of beam j of stream s. out_hist holds out_cap ids, by
+    default room for any parents: n histories as long as a stream's longest. Nothing here waits for the GPU where the caller
+    gives out_cap, max_len (no history of hist is longer) or hist_off and row_off in host memory; else the offsets are read
+    back, except in a captured call, which takes room for n times as many ids as hist can hold."""
     dev = parent.device if isinstance(parent, torch.Tensor) and parent.is_cuda else torch.device("cuda", torch.cuda.current_device())
     parent = _parents(parent, dev)
     S, n = parent.shape
+    if n < 1:
+        raise SamplerError("streams without beams")
+    given = [hist_off, row_off]
     hist, hist_off = _dev(hist, torch.int32, dev), _dev(hist_off, torch.int64, dev)
     rows = hist_off.numel() - 1
     if row_off is not None:
@@ -825,7 +839,17 @@ def hist_fork(hist, hist_off, parent, tok=None, row_off=None, out_cap=None, ctx=
         if tok.numel() != S * n:
             raise SamplerError("one token per beam")
     if out_cap is None:
-        out_cap = hist.numel() * n + S * n
+        out_cap = hist.numel() * n
+        if max_len is not None:
+            out_cap = min(out_cap, S * n * int(max_len))
+        else:
+            host = [t is None or not (isinstance(t, torch.Tensor) and t.is_cuda) for t in given]
+            _on(stream, dev)                                   # (what the stream has before the call is read)
+            with torch.cuda.device(dev), torch.cuda.stream(stream):
+                if all(host) or not torch.cuda.is_current_stream_capturing():
+                    off, ro = (t if t is None else np.asarray(t if h else t.cpu(), np.int64) for t, h in zip(given, host))
+                    out_cap = _fork_ids(off, ro, S, n)
+        out_cap += 0 if tok is None else S * n
     out = torch.empty(max(int(out_cap), 1), dtype=torch.int32, device=dev)
     out_off = torch.empty(S * n + 1, dtype=torch.int64, device=dev)
     ctx = ctx or Context.default(dev)
