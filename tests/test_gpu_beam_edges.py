@@ -1,4 +1,6 @@
 """GPU: calls of the beam search that a long run, a captured one or an unusual program makes (tests/beam_util.py)."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -7,7 +9,9 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 import ferro_amd as F  # noqa: E402
+from ferro_amd import _lib  # noqa: E402
 from tests import beam_util as BU  # noqa: E402
+from tests.test_gpu_beam_run import Model, search  # noqa: E402
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -84,3 +88,58 @@ def test_fork_room_in_a_captured_call():
 def test_fork_refuses_streams_without_beams():
     with pytest.raises(F.SamplerError):
         F.hist_fork(cuda(np.zeros(4, np.int32)), [0, 2, 4], np.zeros((2, 0), np.int32), row_off=[0, 1, 2])
+
+
+# ------------------------------------------------------------------------------------------------ whole searches
+@pytest.mark.parametrize("S,n,V,steps", [(3, 4, 211, 8), (1, 1, 50, 5), (2, 17, 131, 5)])
+def test_steps_of_the_c_abi_on_two_buffers(S, n, V, steps):
+    """The prompts' step and those behind it by the C calls, as a C++ program makes them: scores, histories and offsets change
+    between two buffers after every step, the prompts' too; the first of them holds only the prompts' offsets."""
+    model, rng = Model(S, V), np.random.default_rng(S)
+    prompts = [rng.integers(1, V, int(rng.integers(1, 6))).tolist() for _ in range(S)]
+    want = search(model, prompts, n, steps, 0)
+    L, P, ctx = _lib.lib(), F.sampler._ptr, F.Context()
+    i32 = lambda *s: torch.full(s, -7, dtype=torch.int32, device="cuda")
+    parent, tok, done, done_parent, done_score = i32(S, n), i32(S, n), i32(S), i32(S, n), torch.zeros((S, n), device="cuda")
+    score = [torch.full((S, n), float("nan"), device="cuda") for _ in range(2)]
+    cap = S * n * (5 + steps)
+    hist, hoff = [i32(cap) for _ in range(2)], [torch.full((S * n + 1,), -1, dtype=torch.int64, device="cuda") for _ in range(2)]
+    lens = [len(p) for p in prompts]
+    hist[0][:sum(lens)] = cuda(np.concatenate(prompts).astype(np.int32))
+    hoff[0][:S + 1] = cuda(np.concatenate([[0], np.cumsum(lens)]))
+    row_off1, prompt_len = cuda(np.arange(S + 1)), cuda(np.array(lens, np.int32))
+    length = prompt_len.clone()
+    pc = torch.zeros((S, 2, 32, model.dim // 2), device="cuda")
+    for s, p in enumerate(prompts):
+        pc[s, :, :len(p)] = model.dev[1][torch.tensor(p, device="cuda")].view(len(p), 2, -1).transpose(0, 1)
+    cache = torch.full((S * n, 2, 32, model.dim // 2), float("nan"), device="cuda")
+    opening, states = F.States([pc], [cache], pos_dim=2), F.States([cache], pos_dim=2)
+    logits = model.device(torch.tensor([p[-1] for p in prompts], device="cuda"), pc, length)
+    st, cur, ended = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream), 0, [[] for _ in range(S)]
+    for step in range(steps):
+        x, ld, _, kind = F.sampler._typed_logits(logits, V)
+        first = step == 0
+        _lib.check(L.fs_beam_select(ctx.h, F.sampler._lptr(x), kind, ld, S, S if first else S * n, V,
+                                    P(row_off1) if first else None, None if first else P(score[cur]), None, None, 0, n,
+                                    F.BEAM_KEEP_SLOTS, P(parent), P(tok), P(score[cur ^ 1]), P(done), P(done_parent),
+                                    P(done_score), st), "select")
+        h, o = hist[cur].tolist(), hoff[cur].tolist()
+        for s in range(S):
+            for j in range(int(done[s])):
+                r = s * (1 if first else n) + int(done_parent[s, j])
+                ended[s].append(h[o[r]:o[r + 1]] + [0])
+        _lib.check(L.fs_hist_fork(ctx.h, S, P(hist[cur]), P(hoff[cur]), P(row_off1) if first else None, n, P(parent), P(tok),
+                                  P(hist[cur ^ 1]), cap, P(hoff[cur ^ 1]), st), "fork")
+        _lib.check(L.fs_reorder_states(ctx.h, 1, opening.c if first else states.c, S, 1 if first else n, n, P(parent),
+                                       None if first else P(prompt_len), P(length), st), "states")
+        cur ^= 1
+        rows = length.repeat_interleave(n).long()
+        cache[torch.arange(S * n, device="cuda"), :, rows] = model.dev[1][tok.view(-1).long()].view(S * n, 2, -1)
+        length += 1
+        logits = model.device(tok.view(-1), cache, length.repeat_interleave(n))
+    h, o = hist[cur].tolist(), hoff[cur].tolist()
+    for s, (beams, done) in enumerate(want):
+        got = score[cur][s].tolist()
+        order = sorted(range(n), key=lambda j: (-got[j], j))
+        assert [h[o[s * n + j]:o[s * n + j + 1]] for j in order] == [b[0] for b in beams], s
+        assert ended[s] == [e[0] for e in done], s
