@@ -347,7 +347,8 @@ __device__ __forceinline__ bool bm_last(BeamShared& s, uint32_t* ticket, uint32_
     return s.turn == of;
 }
 
-// The stream of a beam's row: the largest s with row_off[s] <= row; its first row, its rows. Rows are most often dealt evenly.
+// The stream of a beam's row: the largest s with row_off[s] <= row; its first row, its rows (of the R there are; 0: the row lies
+// behind the last stream's, and would be counted as one of them). Rows are most often dealt evenly.
 struct BeamStream {
     int s, m;
     int64_t r0;
@@ -356,7 +357,7 @@ __device__ __forceinline__ BeamStream bm_stream(const BeamArgs& b, int row, int 
     if (!b.row_off) return {row / b.W, b.W, (int64_t)(row / b.W) * b.W};
     int s = (int)((int64_t)row * b.S / R);
     int64_t r0 = ld_const(b.row_off + s), r1 = ld_const(b.row_off + s + 1);
-    if (row < r0 || row >= r1) {
+    if (__builtin_expect((uint64_t)r0 > (uint64_t)row || row >= r1 || r1 > R, 0)) {
         int s0 = 0, s1 = b.S;
         while (s1 - s0 > 1) {
             const int m = (s0 + s1) >> 1;
@@ -365,6 +366,8 @@ __device__ __forceinline__ BeamStream bm_stream(const BeamArgs& b, int row, int 
         s = s0;
         r0 = ld_const(b.row_off + s);
         r1 = ld_const(b.row_off + s + 1);
+        r0 = r0 < 0 ? 0 : r0;
+        r1 = row < r0 || row >= r1 ? r0 : r1 < R ? r1 : R;
     }
     return {s, (int)(r1 - r0), r0};
 }

@@ -380,7 +380,7 @@ __device__ __forceinline__ void beam_end(const LpBeamArgs& args, LpShared& s, Be
     uint32_t* ticket = b.ticket + (int64_t)st.s * LP_LINE;
     if (!dead) beam_publish(a, s, row, part, nseg, n, sum, mx, xv, ls, reach, g, cut);
     if (once) {
-        if (!bm_last(bm, ticket, dead ? (uint32_t)nseg : 1u, (uint32_t)(m * nseg))) return;
+        if (!bm_last(bm, ticket, !dead ? 1u : m > 0 ? (uint32_t)nseg : 0u, (uint32_t)(m * nseg))) return;
     } else if (!dead) {
         if (!bm_last(bm, a.ticket + (int64_t)row * LP_LINE, 1u, (uint32_t)nseg)) return;
     }
@@ -429,7 +429,8 @@ __device__ __forceinline__ void beam_end(const LpBeamArgs& args, LpShared& s, Be
     if (w != 0) return;
     bm_finish(b, bm.best, st.s);
     if (!b.row_off) return;
-    for (int e = st.s + 1; e < b.S && ld_const(b.row_off + e + 1) == st.r0 + m; ++e) bm_nothing(b, e);   // streams without rows
+    const int64_t end = st.r0 + m;                             // streams without rows
+    for (int e = st.s + 1; e < b.S && (end == a.B || ld_const(b.row_off + e + 1) == end); ++e) bm_nothing(b, e);
     if (st.r0 == 0)
         for (int e = 0; e < st.s; ++e) bm_nothing(b, e);
 }
@@ -479,6 +480,7 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
     BeamStream beams = {0, 0, 0};
     if constexpr (BEAM) {
         beams = bm_stream(args.b, row, B);
+        if (beams.m == 0 && ((int64_t)(row | part) | beams.r0) != 0) return;   // (row 0 ends streams without any row)
         rec = beams.s;
         score = args.b.score ? ld_const(args.b.score + row) : 0.0f;
     }
@@ -516,7 +518,8 @@ __global__ __launch_bounds__(SK_LT, 4) void logprob_kernel(const void* logits, i
     }
     const bool has = !BEAM && xv < __builtin_huge_valf();      // (none is larger than +inf)
 
-    const bool dead = BEAM && !(score > LP_NONE);              // a dead beam (NaN, too): no candidates
+    // a dead beam (NaN, too): no candidates
+    const bool dead = BEAM && (!(score > LP_NONE) || beams.m == 0);
     if (dead && part != 0) return;
     const int c_end = dead ? c0 : c1;
 

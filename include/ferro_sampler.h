@@ -330,7 +330,8 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
                 int32_t* d_rank, int32_t* d_top_ids, float* d_top_lp, void* stream);
 
 /* Beam search: a step's selection. Stream s (one request) has the beams of the logits rows d_row_off[s] .. d_row_off[s+1]-1
- * (as fs_verify's; NULL: total_rows / n_streams rows each) with the scores d_score (sums of log-probabilities; NULL: zeros).
+ * (ascending from 0; NULL: total_rows / n_streams rows each) with the scores d_score (sums of log-probabilities; NULL: zeros).
+ * Rows from d_row_off[n_streams] on are of no stream and do not matter (a padded batch); a stream ends with the last row.
  * Token t of row r is the candidate
  *     c(r, t) = d_score[r] + log softmax((cap(l) + bias) / T)(t)      (fs_logprobs' distribution, by the stream's record)
  * in fp64; a token that is not allowed, whose logit is NaN or -inf, or whose c does not round to a fp32 above -inf is none.

@@ -11,6 +11,7 @@ torch = pytest.importorskip("torch")
 import ferro_amd as F  # noqa: E402
 from ferro_amd import _lib  # noqa: E402
 from tests import beam_util as BU  # noqa: E402
+from tests.test_gpu_beam import Rows  # noqa: E402
 from tests.test_gpu_beam_run import Model, search  # noqa: E402
 
 
@@ -25,6 +26,38 @@ def gpu():
 
 def cuda(a):
     return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+# ------------------------------------------------------------------------------------------------ selection
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("counts,n,V", [([4, 4], 4, 5000), ([1, 0, 3, 0, 0], 3, 70001), ([5, 0, 9], 8, 4099), ([0, 0, 40], 64, 300),
+                                        ([70, 2], 20, 900)])
+def test_select_rows_behind_the_last_stream(counts, n, V, kind):
+    """A padded batch: offsets on the device, rows behind the last stream's (whose mask indices and scores mean nothing), in a
+    context that goes on to other calls; a stream that ends past the rows ends with them; no stream has a row."""
+    r = Rows(n, counts, V, kind)
+    R, pad = int(r.off[-1]), 7
+    x = torch.cat([r.x, torch.full((pad, V), 9.0, device="cuda", dtype=r.x.dtype)])
+    ctx, all_on = F.Context(), np.full(R + pad, -1, np.int32)
+    all_on[R:] = 99
+    ed = F.Edits(mask=F.Edits.pack(np.ones((1, V), bool)), mask_of=all_on)
+    alone = F.beam_select(r.x, cuda(r.score), n, eos_id=3, row_off=r.off, ctx=ctx)
+    BU.Step(r.y, r.score, r.off, n, 3).check(alone)
+    past, none = r.off.copy(), np.zeros_like(r.off)
+    past[-1] += 1000
+    live = torch.zeros(pad, device="cuda")
+    for i in range(3):
+        padded = F.beam_select(x, torch.cat([cuda(r.score), live + i]), n, eos_id=3, row_off=cuda(r.off), edits=ed, ctx=ctx)
+        cut = F.beam_select(r.x, cuda(r.score), n, eos_id=3, row_off=cuda(past), ctx=ctx)
+        empty = F.beam_select(x, None, n, eos_id=3, row_off=cuda(none), ctx=ctx)
+        again = F.beam_select(r.x, cuda(r.score), n, eos_id=3, row_off=r.off, ctx=ctx)
+        for k in ("parent", "tok", "done", "done_parent"):
+            assert torch.equal(padded[k], alone[k]) and torch.equal(cut[k], alone[k]) and torch.equal(again[k], alone[k]), (i, k)
+            assert torch.all(empty[k] == (0 if k == "done" else -1)), k
+        for k in ("score", "done_score"):                      # (rows split otherwise: the last bit of a sum)
+            assert torch.allclose(padded[k], alone[k], rtol=2 * BU.U, atol=2 * BU.TOL), (i, k)
+            assert torch.equal(cut[k], alone[k]) and torch.equal(again[k], alone[k]) and torch.all(empty[k] == -np.inf), (i, k)
+    assert F.device_error(ctx) == 0
 
 
 # ------------------------------------------------------------------------------------------------ histories
