@@ -3,6 +3,8 @@
 #include "sampler_device.hpp"
 #include "sampler_launch.hpp"
 
+#include <utility>
+
 namespace fs {
 
 __global__ __launch_bounds__(256) void softcap_kernel(const float* in, float* out, int64_t n, float cap) {
@@ -1430,6 +1432,17 @@ int fs_beam_select(fs_context* ctx, const void* d_logits, int32_t type, int64_t 
     rc = edit_args(edits, total_rows, V, a.lp.ed);
     if (rc != FS_OK) return rc;
     if (n_streams == 0) return FS_OK;
+    // a stream's outputs are written while parts of others' rows, and of its own dead ones, may still read theirs
+    const size_t beams = (size_t)n_streams * n * 4;
+    const std::pair<const void*, size_t> in[] = {{d_score, (size_t)total_rows * 4}, {d_row_off, ((size_t)n_streams + 1) * 8},
+                                                 {d_params, (size_t)n_streams * sizeof(fs_row_params)}};
+    const std::pair<const void*, size_t> out[] = {{d_parent, beams}, {d_tok, beams}, {d_out_score, beams},
+                                                  {d_done, (size_t)n_streams * 4}, {d_done_parent, beams}, {d_done_score, beams}};
+    for (const auto& i : in)
+        for (const auto& o : out)
+            if (i.first && o.first && (uintptr_t)i.first < (uintptr_t)o.first + o.second &&
+                (uintptr_t)o.first < (uintptr_t)i.first + i.second)
+                return FS_E_INVALID;
     const hipStream_t st = (hipStream_t)stream;
     const Edited call(ctx, st);
     if (call.rc != FS_OK) return call.rc;

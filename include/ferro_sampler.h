@@ -345,7 +345,8 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
  * flags: FS_BEAM_KEEP_SLOTS puts a parent's best child into the parent's own place (where that is below n) and the others, in
  * their order, into the free places, ascending: a state then moves for a parent's further children alone; without it the
  * beams come best first. edits: masks by row, biases by stream, may be NULL; penalties are fs_edit_batch's. d_params NULL: no
- * softcap, T = 1. Rows and types as in fs_edit_batch; the outputs must not overlap the inputs. The workspace is 4 KB per row
+ * softcap, T = 1. Rows and types as in fs_edit_batch; the outputs must not overlap the inputs (refused where they
+ * overlap the scores, offsets or records). The workspace is 4 KB per row
  * and part (32 parts at most) and grows as a context's other buffers do; under graph capture a call that would have to grow it
  * returns FS_E_NOMEM. No counterpart in the reference (ferro samples). */
 #define FS_BEAM_KEEP_SLOTS 1

@@ -1,10 +1,38 @@
 """CPU: what the beam search's Python wrappers work out on the host, and calls they refuse."""
+import ctypes
+
 import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import ferro_amd as F  # noqa: E402
+from ferro_amd import _lib  # noqa: E402
+
+P = ctypes.c_void_p
+
+
+@pytest.fixture()
+def ctx():
+    h = P()
+    assert _lib.lib().fs_create(ctypes.byref(h)) == _lib.FS_OK
+    yield h
+    _lib.lib().fs_destroy(h)
+
+
+@pytest.mark.parametrize("out", ["parent", "tok", "out", "done", "dp", "ds"])
+def test_select_refuses_outputs_over_its_inputs(ctx, out):
+    """Two streams of two rows, four beams: an output that begins or ends inside the scores, offsets or records. (Calls it
+    takes go on to the device, so those that only touch are the GPU tests'.)"""
+    MB = 1 << 20
+    good = dict(ctx=ctx, logits=P(MB), type=0, ld=8, S=2, R=4, V=8, off=P(2 * MB), score=P(3 * MB), params=P(4 * MB), edits=None,
+                eos=-1, n=4, flags=0, parent=P(5 * MB), tok=P(6 * MB), out=P(7 * MB), done=P(8 * MB), dp=P(9 * MB), ds=P(10 * MB),
+                stream=None)
+    size = 8 if out == "done" else 32
+    for name, n in (("off", 24), ("score", 16), ("params", 2 * _lib.PARAMS_DTYPE.itemsize)):
+        at = good[name].value
+        for to in (at, at + n - 4, at - size + 4):
+            assert _lib.lib().fs_beam_select(*dict(good, **{out: P(to)}).values()) == _lib.FS_E_INVALID, (name, to - at)
 
 
 @pytest.mark.parametrize("seed", range(30))

@@ -60,6 +60,25 @@ def test_select_rows_behind_the_last_stream(counts, n, V, kind):
     assert F.device_error(ctx) == 0
 
 
+def test_select_outputs_beside_inputs():
+    """Outputs in one buffer with the scores and offsets, next to them on both sides, are taken."""
+    S, n, V = 2, 4, 3000
+    r = Rows(5, [n] * S, V)
+    want = F.beam_select(r.x, cuda(r.score), n, eos_id=3, row_off=r.off)
+    buf = torch.full((64,), -7, dtype=torch.int32, device="cuda")
+    at = dict(parent=(0, 8), score_in=(8, 16), tok=(16, 24), score=(24, 32), off=(32, 38), done=(38, 40), dp=(40, 48), ds=(48, 56))
+    v = {k: buf[a:b] for k, (a, b) in at.items()}
+    v["score_in"].view(torch.float32).copy_(cuda(r.score))
+    v["off"].view(torch.int64).copy_(cuda(r.off))
+    ctx, p = F.Context.default(), F.sampler._ptr
+    _lib.check(_lib.lib().fs_beam_select(ctx.h, p(r.x), F.F32, r.x.stride(0), S, S * n, V, p(v["off"]), p(v["score_in"]), None, None,
+                                         3, n, 0, p(v["parent"]), p(v["tok"]), p(v["score"]), p(v["done"]), p(v["dp"]), p(v["ds"]),
+                                         F.sampler._stream()), "select")
+    assert torch.equal(v["parent"].view(S, n), want["parent"]) and torch.equal(v["tok"].view(S, n), want["tok"])
+    assert torch.equal(v["score"].view(torch.float32).view(S, n), want["score"]) and torch.equal(v["done"], want["done"])
+    assert v["off"].view(torch.int64).tolist() == r.off.tolist() and torch.all(buf[56:] == -7)
+
+
 # ------------------------------------------------------------------------------------------------ histories
 @pytest.mark.parametrize("how", ["default", "max_len", "stream"])
 @pytest.mark.parametrize("S,n,steps", [(3, 8, 200), (1, 64, 60), (40, 1, 60)])
