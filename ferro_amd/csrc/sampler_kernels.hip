@@ -982,6 +982,10 @@ int check_state(const fs_state& z, int64_t S, int32_t n_src, int32_t n) {
         if (stride > most) return FS_E_INVALID;
     if ((double)z.blocks * (double)pos * (double)z.pos_bytes > 2e9 * state_bytes(z, n > n_src ? n : n_src)) return FS_E_INVALID;
     if (empty) return FS_OK;
+    // places of d_dst that lie over the next ones: what is stored there last would count
+    if ((S * n > 1 && z.dst_row < z.pos_bytes) || (z.blocks > 1 && z.dst_block < z.pos_bytes) ||
+        (pos > 1 && z.dst_pos < z.pos_bytes))
+        return FS_E_INVALID;
     if (z.d_src == z.d_dst && n == n_src && z.src_row == z.dst_row && z.src_block == z.dst_block && z.src_pos == z.dst_pos)
         return FS_OK;
     auto span = [&](int64_t rows, int64_t row, int64_t block, int64_t p) {

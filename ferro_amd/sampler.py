@@ -865,7 +865,7 @@ class States:
     values, convolution and recurrent states, block tables. Tensors [rows, ...] of any type; dst: the buffers they are
     written into (default: in place). pos_dim: the dimension of a cache's positions (None: a state without any, which
     follows whole), one for all or one per tensor. The dimensions behind the positions must be packed, those before them one
-    stride apart; strides are otherwise free."""
+    stride apart; strides are otherwise free, but what is written must not overlap itself."""
 
     def __init__(self, tensors, dst=None, pos_dim=None):
         self.src = list(tensors)
@@ -914,7 +914,16 @@ class States:
             if z.blocks == 1:
                 z.src_block, z.dst_block = a.stride(i) * size, b.stride(i) * size
             z.blocks *= a.shape[i]
+        self._apart(z)
         return z
+
+    def _apart(self, z):
+        """Refuses a buffer to write whose places overlap (an expanded tensor, windows): what is stored there last would count."""
+        end, places = z.pos_bytes, [(self.dst_rows, z.dst_row), (z.blocks, z.dst_block), (z.positions, z.dst_pos)]
+        for k, stride in sorted(((k, s) for k, s in places if k > 1), key=lambda p: p[1]):
+            if stride < end and self.dst_rows > 0 and z.blocks > 0:
+                raise SamplerError("rows, blocks and positions of a state that is written must not overlap")
+            end += (k - 1) * stride
 
 
 def reorder_states(states, parent, start=None, length=None, ctx=None, stream=None):

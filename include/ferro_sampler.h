@@ -380,8 +380,9 @@ typedef struct fs_state {
  * positions [d_from[s], d_len[s]) (NULL: 0, the state's positions; cut to those), the rest of d_dst stays as it was. In place
  * rows of a stream may change places, be copied more than once or dropped. d_from is for what a stream's beams share (the
  * prompt), which need not move. A parent below 0 leaves its row as it was. n, n_src <= FS_MAX_TOP; n_src = 1 opens the beams
- * of prompts. `states` is host memory, read before the call returns; the states' rows must not overlap one another, nor a
- * d_dst any other state of the call (in place: its own d_src alone; a buffer given twice is refused). */
+ * of prompts. `states` is host memory, read before the call returns; the places that are written must not overlap one
+ * another (strides of d_dst below pos_bytes are refused), nor a d_dst any other state of the call (in place: its own d_src
+ * alone; a buffer given twice is refused). */
 int fs_reorder_states(fs_context* ctx, int32_t n_states, const fs_state* states, int32_t n_streams, int32_t n_src, int32_t n,
                       const int32_t* d_parent, const int32_t* d_from, const int32_t* d_len, void* stream);
 

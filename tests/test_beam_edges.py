@@ -46,3 +46,33 @@ def test_room_of_new_histories(seed):
     off = 4 + np.concatenate([[0], np.cumsum(lens)]).astype(np.int64)
     want = sum(n * int(max(lens[a:b], default=0)) for a, b in zip(row_off, row_off[1:]))
     assert F.sampler._fork_ids(off, None if seed % 3 == 0 else row_off, S, n) == want
+
+
+def fields(z):
+    return {n: getattr(z, n) for n, _ in z._fields_ if n not in ("d_src", "d_dst")}
+
+
+def test_states_refuse_buffers_that_overlap_themselves(ctx):
+    t = torch.zeros((6, 3, 10, 4))
+    one = torch.zeros((1, 3, 10, 4))
+    windows = torch.zeros(200).as_strided((6, 3, 10, 4), (4, 40, 4, 1))    # row r's position p is row r + 1's p - 1
+    for bad, pos in ((one.expand(6, 3, 10, 4), 2), (one.expand(6, 3, 10, 4), None), (t[:, :1].expand(6, 3, 10, 4), 2),
+                     (t[:, :, :1].expand(6, 3, 10, 4), 2), (windows, 2), (t[:, :1].expand(6, 3, 10, 4), 1)):
+        with pytest.raises(F.SamplerError, match="overlap"):
+            F.States([bad], pos_dim=pos)
+        with pytest.raises(F.SamplerError, match="overlap"):
+            F.States([t], [bad], pos_dim=pos)
+    # (read alone they are fine: one prompt's cache as every stream's; and so are sizes of one with any stride)
+    F.States([one.expand(6, 3, 10, 4)], [t], pos_dim=2)
+    F.States([one.expand(1, 3, 10, 4)], pos_dim=2)
+    F.States([torch.zeros((6, 0, 10, 4)).expand(6, 0, 10, 4)], pos_dim=2)
+    F.States([torch.zeros((13, 6, 3, 8)).transpose(0, 1)], pos_dim=1)      # rows between positions and heads
+    F.States([torch.zeros((5, 6)).t()])                        # rows innermost
+    good = dict(d_src=1 << 20, d_dst=2 << 20, src_row=64, src_block=32, src_pos=8, dst_row=64, dst_block=32, dst_pos=8, pos_bytes=8,
+                blocks=2, positions=4)
+    for bad in (dict(dst_row=0), dict(dst_row=7), dict(dst_block=0), dict(dst_block=7), dict(dst_pos=0), dict(dst_pos=7)):
+        for src in (2 << 20, 1 << 20):                         # in place, and not
+            z = dict(good, **bad)
+            z.update(d_src=src, **({f"src_{k}": z[f"dst_{k}"] for k in ("row", "block", "pos")} if src == 2 << 20 else {}))
+            rec = (_lib.FsState * 1)(_lib.FsState(**z))
+            assert _lib.lib().fs_reorder_states(ctx, 1, rec, 2, 4, 4, P(3 << 20), None, None, None) == _lib.FS_E_INVALID, (bad, src)
