@@ -900,20 +900,22 @@ class States:
             run, i = run * a.shape[i], i - 1
         if pos is not None and i > pos:
             raise SamplerError("the dimensions behind a state's positions must be packed")
-        z.pos_bytes, z.blocks = run, 1
+        z.pos_bytes, blocks, positions = run, 1, 0
         if pos is not None:
-            z.positions = min(a.shape[pos], b.shape[pos])
+            positions = min(a.shape[pos], b.shape[pos])
             z.src_pos, z.dst_pos, i = a.stride(pos) * size, b.stride(pos) * size, pos - 1
-            if z.positions == 0:
-                z.blocks = 0
+            blocks = 1 if positions > 0 else 0
         for i in range(i, 0, -1):                              # the others: blocks one stride apart
             if a.shape[i] == 1:
                 continue
-            if z.blocks > 1 and (a.stride(i) * size != z.blocks * z.src_block or b.stride(i) * size != z.blocks * z.dst_block):
+            if blocks > 1 and (a.stride(i) * size != blocks * z.src_block or b.stride(i) * size != blocks * z.dst_block):
                 raise SamplerError("the dimensions before a state's positions must be one stride apart")
-            if z.blocks == 1:
+            if blocks == 1:
                 z.src_block, z.dst_block = a.stride(i) * size, b.stride(i) * size
-            z.blocks *= a.shape[i]
+            blocks *= a.shape[i]
+        if blocks * max(positions, 1) > 0x7fffffff:            # (the records count both in 32 bits)
+            raise SamplerError("a state of more than 2^31 - 1 blocks and positions a row")
+        z.blocks, z.positions = blocks, positions
         self._apart(z)
         return z
 

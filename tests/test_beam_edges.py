@@ -76,3 +76,16 @@ def test_states_refuse_buffers_that_overlap_themselves(ctx):
             z.update(d_src=src, **({f"src_{k}": z[f"dst_{k}"] for k in ("row", "block", "pos")} if src == 2 << 20 else {}))
             rec = (_lib.FsState * 1)(_lib.FsState(**z))
             assert _lib.lib().fs_reorder_states(ctx, 1, rec, 2, 4, 4, P(3 << 20), None, None, None) == _lib.FS_E_INVALID, (bad, src)
+
+
+def test_states_past_the_records_counts():
+    """Blocks and positions that 32 bits do not hold (they were cut: no block, or a state without positions)."""
+    meta = lambda *shape: torch.empty(shape, dtype=torch.uint8, device="meta")
+    for t, pos in ((meta(2, 1 << 16, 1 << 16, 3)[..., :2], None), (meta(2, (1 << 32) + 7, 2), 1), (meta(2, 1 << 32, 2), 1),
+                   (meta(2, 1 << 20, 1 << 20, 8), 2)):
+        with pytest.raises(F.SamplerError, match="2\\^31"):
+            F.States([t], pos_dim=pos)
+    z = fields(F.States([meta(2, 3, (1 << 29) + 1, 4)], pos_dim=2).c[0])
+    assert (z["blocks"], z["positions"], z["pos_bytes"]) == (3, (1 << 29) + 1, 4)
+    z = fields(F.States([meta(2, (1 << 31) + 8)]).c[0])        # (one run of bytes: the call refuses it)
+    assert (z["blocks"], z["pos_bytes"]) == (1, (1 << 31) + 8)
