@@ -765,6 +765,10 @@ def beam_select(logits, score, n, eos_id=-1, params=None, row_off=None, streams=
     R, dev = logits.shape[0], logits.device
     if not 1 <= n <= FS_MAX_TOP:
         raise SamplerError(f"n must lie in [1, {FS_MAX_TOP}]")
+    if score is not None:
+        score = _dev(score, torch.float32, dev)
+        if score.numel() != R:
+            raise SamplerError("one score per row")
     if row_off is not None:
         row_off = _row_off(row_off, R, dev)
         S = row_off.numel() - 1
@@ -772,10 +776,6 @@ def beam_select(logits, score, n, eos_id=-1, params=None, row_off=None, streams=
         S = streams if streams is not None else score.shape[0] if score is not None and score.dim() == 2 else None
         if S is None or S < 0 or (R % S if S else R):
             raise SamplerError("the streams' rows: row_off, streams or a score [streams, rows each]")
-    if score is not None:
-        score = _dev(score, torch.float32, dev)
-        if score.numel() != R:
-            raise SamplerError("one score per row")
     p = None
     if params is not None:
         p = _dev_params(params, dev)

@@ -79,6 +79,20 @@ def test_select_outputs_beside_inputs():
     assert v["off"].view(torch.int64).tolist() == r.off.tolist() and torch.all(buf[56:] == -7)
 
 
+def test_select_scores_in_host_memory():
+    """Scores as an array or a list, [streams, rows each] or [rows], as the other arguments may be."""
+    r = Rows(6, [3, 3, 3, 3], 700)
+    want = F.beam_select(r.x, cuda(r.score), 4, streams=4)
+    two = r.score.reshape(4, 3)
+    for score, kw in ((two, {}), (two.tolist(), {}), (torch.from_numpy(two), {}), (r.score, dict(streams=4)),
+                      (two.astype(np.float64), {})):
+        out = F.beam_select(r.x, score, 4, **kw)
+        assert all(torch.equal(out[k], want[k]) for k in want)
+    for score in (r.score, r.score.tolist(), None, two[:3], 1.0):
+        with pytest.raises(F.SamplerError):
+            F.beam_select(r.x, score, 4)
+
+
 # ------------------------------------------------------------------------------------------------ histories
 @pytest.mark.parametrize("how", ["default", "max_len", "stream"])
 @pytest.mark.parametrize("S,n,steps", [(3, 8, 200), (1, 64, 60), (40, 1, 60)])
