@@ -60,6 +60,34 @@ def test_select_rows_behind_the_last_stream(counts, n, V, kind):
     assert F.device_error(ctx) == 0
 
 
+@pytest.mark.parametrize("n", [16, 17, 40, 63, 64])
+@pytest.mark.parametrize("V", [300, 20000, 262144])
+def test_select_dead_streams_of_few_rows(n, V):
+    """Streams of one to five rows, dead ones between live ones: a wave or a workgroup a row, and rows that end by themselves."""
+    r = Rows(n, [1, 1, 2, 1, 4, 3, 5, 5, 1], V, "bf16")
+    for dead in ([0], [1, 2, 3], [4, 5, 7], [8, 10, 11], [12, 13, 14, 15, 16, 17, 21], range(22), [0, 4, 22]):
+        r.score = (-r.rng.exponential(2.0, 23)).astype(np.float32)
+        r.score[list(dead)] = -np.inf
+        out = r.run(n, eos=int(r.y[3].argmax()))
+        for s in range(9):
+            if np.all(r.score[r.off[s]:r.off[s + 1]] == -np.inf):
+                assert out["parent"][s].tolist() == [-1] * n and int(out["done"][s]) == 0
+
+
+def test_select_dead_rows_after_better_ones():
+    """What an earlier call's rows left in the workspace does not come back for dead ones."""
+    for n, counts in ((4, [4]), (64, [1, 4, 5]), (8, [9, 70])):
+        r = Rows(3, counts, 5000)
+        ctx, best = F.Context(), Rows(4, counts, 5000)
+        best.score[:] = 1000.0
+        best.x[:, 7] = float("inf")
+        r.score[::2] = -np.inf
+        for _ in range(3):
+            F.beam_select(best.x, cuda(best.score), n, row_off=best.off, eos_id=5, ctx=ctx)
+            out = F.beam_select(r.x, cuda(r.score), n, row_off=r.off, eos_id=5, ctx=ctx)
+            BU.Step(r.y, r.score, r.off, n, 5).check(out)
+
+
 def test_select_outputs_beside_inputs():
     """Outputs in one buffer with the scores and offsets, next to them on both sides, are taken."""
     S, n, V = 2, 4, 3000
