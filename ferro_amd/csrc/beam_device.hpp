@@ -305,7 +305,7 @@ __device__ __forceinline__ void bm_nothing(const BeamArgs& a, int st) {
     if (a.done && lane == 0) a.done[st] = 0;
 }
 
-// The stream's outputs from what bm_few or bm_join found (one wave).
+// The stream's outputs from what bm_few or bm_many found (one wave).
 __device__ __forceinline__ void bm_finish(const BeamArgs& a, BeamBest& s, int st) {
     const int lane = lane_id(), n = a.n;
     const int64_t o = (int64_t)st * n;

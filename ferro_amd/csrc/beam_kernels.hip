@@ -13,14 +13,16 @@ namespace fs {
 // row, from the L2) and copies an equal share of the new ids, four per thread at a time, whose rows it finds by bisection among
 // those of its share. More rows: a launch for the offsets first, which the copying one then reads. The new ids are stored past
 // the caches (256 histories of 32768 ids: 14.2 -> 13.1 us).
-// Bound: latency for few ids (4.5 us for 4 histories of 300, 6.1 for 512 of 2048), then HBM: 256 of 32768 13.3 us (4.9 TB/s of
-// 65 MB).
+// Bound: latency for few ids (4.5 us for 4 histories of 300, 6.2 for 512 of 2048), then HBM: 256 of 32768 13.3 us (4.9 TB/s of
+// 65 MB). In two launches latency throughout: 4096 of 16 and of 500 ids 18.5 and 19.3 us, 16384 29.6 and 56 (its 55 MB: 11.6).
 constexpr int FK_T = 256;
-constexpr int FK_ROWS = 1024;              // rows whose offsets are kept in LDS
+// Rows whose offsets are kept in LDS. 1032 rows of 500 ids with 512, 1024, 2048: 12.8, 12.9, 7.2 us, 1024 12.3, 6.9, 7.2; but 16384
+// 60, 56, 63 (the offsets' launch takes FK_PER rows per thread).
+constexpr int FK_ROWS = 1024;
 constexpr int FK_STEP = FK_T * 4;          // ids a workgroup copies at a time
 constexpr int FK_U = 4;                    // of these in flight
-// Workgroups per CU. 512 histories of 2048 ids with 1, 2, 4, 8: 13.9, 10.4, 8.7, 7.5 us; 256 of 32768 32.4, 20.0, 16.7, 17.0
-// (then with registers for six on a CU; with registers for eight 6.7 and 13.9).
+// Workgroups per CU. 512 histories of 2048 ids with 1, 2, 4, 8, 16: 12.5, 9.1, 7.4, 6.2, 6.2 us; 256 of 32768 25.5, 17.3, 14.1,
+// 13.3, 13.7.
 constexpr int FK_PER_CU = 8;
 
 struct ForkRow {
@@ -218,7 +220,9 @@ hipError_t launch_hist_fork(const ForkArgs& a, int cus, hipStream_t st) {
 // Stores go past the caches, loads do not (a source may be read again): 16 caches of 64 rows 87.1 -> 80.8 us with stores so; with
 // loads so, too, no more.
 // Bound: HBM: those caches 79 us (4.7 TB/s of 373 MB), 16 caches of 16 prompts opened into four beams each 223 us (4.8 TB/s of
-// 1064 MB, four fifths of them stores), one small state 4.6.
+// 1064 MB, four fifths of them stores), one small state 4.6. Past 32 beams the walk over 64 rows and columns of 8 bytes: 64 rows of
+// eight caches of 0.5 MB a row in place by 4, 8, 16, 32, 64 beams 47, 44, 42, 48, 71 us (206 to 256 MB), from one prompt into 8,
+// 32, 64 beams 50, 51, 60 (273 to 302 MB).
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 template <int VB>
@@ -330,6 +334,10 @@ hipError_t launch_reorder_states(int vb, StateArgs a, int64_t cols, int cus, hip
         const dim3 grid((unsigned)n), block(ST_T);
         hipLaunchKernelGGL((reorder_states_kernel<VB, NB, K>), grid, block, 0, st, a);
     };
+    // Columns per thread: as many as keep enough loads in flight, where few rows do not. The caches above with 1, 2, 4 columns,
+    // in place by 4 beams: 54, 52, 47 us; by 8: 48, 44, 56; by 16 (1, 2): 42, 44; into other buffers by 4: 96, 100, 89; by 8:
+    // 96, 85, 99; by 16 (1, 2): 84, 86. By 64 beams with columns of 4, 8, 16 bytes: 63, 71, 48 in place, 100, 126, 93 into other
+    // buffers, 64, 60, 63 from one prompt; in place by 33: 43, 35, 36 (state_bytes in sampler_kernels.hip takes 8).
     auto by_rows = [&](auto v) {
         constexpr int VB = decltype(v)::value;
         if (rows <= 4) go(v, std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});

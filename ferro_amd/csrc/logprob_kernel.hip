@@ -34,7 +34,7 @@
 // agent scope. Streams of up to four rows are ended by their last part, a row's lists by a wave each; in wider ones a row's last
 // part ends the row (long lists by all its waves) and the last row the stream.
 // Bound as above, and by the chain behind the last read, about 8 us from a part's end to the outputs (lists 2.2, ticket 0.8, sums
-// and the bound 2, lists and ranks 1.7, the stream's candidates in order 1.1, outputs 0.5): 4 rows of 65536 11.9 us, 16 x 4 of
+// and the bound 2, lists and ranks 1.7, the stream's candidates in order 1.1, outputs 0.5): 4 rows of 65536 11.7 us, 16 x 4 of
 // 262144 22.6 (its 67 MB alone 14 at a large copy's rate), 128 x 8 of 151936 bf16 67.8 (4.6 TB/s).
 #include "beam_device.hpp"
 #include "edit_device.hpp"
@@ -136,8 +136,7 @@ __device__ __forceinline__ const LpArgs& lp_args(const LpBeamArgs& a) { return a
 struct LpRow {
     double* sum;
     float* max;
-    uint32_t* above;                       // (BEAM: of wave 0, the logit that ends the text)
-    float* bound;
+    uint32_t* above;                       // of wave 0, the logit that ends the text (as many words, then fs_logprobs' bounds)
     int* cnt;
     uint32_t* key;
 };
@@ -147,8 +146,7 @@ __device__ __forceinline__ LpRow lp_row(const LpArgs& a, int64_t row, int nseg) 
     r.sum = reinterpret_cast<double*>(a.rows + row * (int64_t)lp_row_bytes(nseg));
     r.max = reinterpret_cast<float*>(r.sum + lists);
     r.above = reinterpret_cast<uint32_t*>(r.max + lists);
-    r.bound = reinterpret_cast<float*>(r.above + lists);
-    r.cnt = reinterpret_cast<int*>(r.bound + lists);
+    r.cnt = reinterpret_cast<int*>(r.above + 2 * lists);
     r.key = reinterpret_cast<uint32_t*>(r.cnt + lists);
     return r;
 }

@@ -937,9 +937,9 @@ int edit_args(const fs_edits* edits, int32_t rows, int32_t V, fs::EdArgs& ed) {
     return FS_OK;
 }
 
-// Parts per row of fs_logprobs and fs_beam_select, at most `parts`. Four workgroups fit a CU; p parts take ceil(B p / 4 CUs) rounds of ceil(n / p) chunks of a
-// row's n and of about 4 chunks' time to begin and join, and the p with the shortest of these is taken. For few rows that
-// fills the device once (64 rows of 262144, n 20: 16 parts 25.6 us, 8 30.7, 32 31.2; 256 rows: 4 parts 57.6, 2 78.7, 8 66.3);
+// Parts per row of fs_logprobs and fs_beam_select, at most `parts`. Four workgroups fit a CU; p parts take ceil(B p / 4 CUs)
+// rounds of ceil(n / p) chunks of a row's n and of about 4 chunks' time to begin and join, and the p with the shortest of these
+// is taken. For few rows that fills the device once (64 rows of 262144, n 20: 16 parts 25.6 us, 8 30.7, 32 31.2; 256 rows: 4 parts 57.6, 2 78.7, 8 66.3);
 // past half of the slots more parts fill a last round (600 rows of 151936: 3 parts 84.1 us, 1 94.0; 1100 rows of bf16, n 1:
 // 2 parts 79.1, 1 86.1; 700 rows: 1 part 52.5, 2 56.3).
 int logprob_parts(const fs_context* c, int64_t B, int32_t V, int32_t type, int parts) {
@@ -957,7 +957,7 @@ int logprob_parts(const fs_context* c, int64_t B, int32_t V, int32_t type, int p
 
 // ---- fs_reorder_states
 // Bytes per column: what the pointers, the strides and a position's bytes are all multiples of, 16 at most (streams of more
-// than 32 rows, whose columns are all in registers: 8).
+// than 32 rows, whose columns are all in registers: 8; launch_reorder_states has the times of both).
 int state_bytes(const fs_state& z, int rows) {
     const uint64_t all = (uint64_t)(uintptr_t)z.d_src | (uint64_t)(uintptr_t)z.d_dst | (uint64_t)z.src_row |
                          (uint64_t)z.src_block | (uint64_t)z.src_pos | (uint64_t)z.dst_row | (uint64_t)z.dst_block |

@@ -26,7 +26,8 @@ from ._lib import (FS_BEAM_KEEP_SLOTS, FS_BF16, FS_F16, FS_F32, FS_MAX_TOP, PARA
                    SamplerError, check, lib)
 
 __all__ = ["SamplerParams", "Sampler", "Context", "Rng", "Edits", "params_array", "sample_batch", "argmax_batch", "verify",
-           "edit_batch", "logprobs", "beam_select", "hist_fork", "States", "reorder_states", "device_error", "PARAMS_DTYPE", "SamplerError"]
+           "edit_batch", "logprobs", "beam_select", "hist_fork", "States", "reorder_states", "device_error", "PARAMS_DTYPE",
+           "SamplerError"]
 
 F32, BF16, F16 = FS_F32, FS_BF16, FS_F16          # types of logits (edit_batch, logprobs, beam_select)
 BEAM_KEEP_SLOTS = FS_BEAM_KEEP_SLOTS
@@ -820,7 +821,8 @@ def hist_fork(hist, hist_off, parent, tok=None, row_off=None, out_cap=None, ctx=
     default room for any parents: n histories as long as a stream's longest. Nothing here waits for the GPU where the caller
     gives out_cap, max_len (no history of hist is longer) or hist_off and row_off in host memory; else the offsets are read
     back, except in a captured call, which takes room for n times as many ids as hist can hold."""
-    dev = parent.device if isinstance(parent, torch.Tensor) and parent.is_cuda else torch.device("cuda", torch.cuda.current_device())
+    on_gpu = isinstance(parent, torch.Tensor) and parent.is_cuda
+    dev = parent.device if on_gpu else torch.device("cuda", torch.cuda.current_device())
     parent = _parents(parent, dev)
     S, n = parent.shape
     if n < 1:
@@ -920,7 +922,7 @@ class States:
         return z
 
     def _apart(self, z):
-        """Refuses a buffer to write whose places overlap (an expanded tensor, windows): what is stored there last would count."""
+        """Refuses a buffer to write whose places overlap (an expanded tensor, windows): the last store there would count."""
         end, places = z.pos_bytes, [(self.dst_rows, z.dst_row), (z.blocks, z.dst_block), (z.positions, z.dst_pos)]
         for k, stride in sorted(((k, s) for k, s in places if k > 1), key=lambda p: p[1]):
             if stride < end and self.dst_rows > 0 and z.blocks > 0:

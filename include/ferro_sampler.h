@@ -44,7 +44,7 @@ extern "C" {
                                         its logits (the token is exact). The next sampling call on the context (or
                                         fs_device_error) clears the workspace; that call returns FS_W_RECOVERED (the mid-k
                                         kernel's rows leave nothing to clear) */
-#define FS_DEVERR_HIST_APPEND 4      /* fs_hist_append: the new histories exceed out_cap (ids past it are not
+#define FS_DEVERR_HIST_APPEND 4      /* fs_hist_append, fs_hist_fork: the new histories exceed out_cap (ids past it are not
                                         written), or a count lies outside [0, its stream's rows] (clamped) */
 
 #define FS_DEVERR_MASK 8             /* a row's mask index lies past the last mask: no token of the row is allowed */
@@ -335,9 +335,11 @@ int fs_logprobs(fs_context* ctx, const void* d_logits, int32_t type, int64_t ld,
  * Token t of row r is the candidate
  *     c(r, t) = d_score[r] + log softmax((cap(l) + bias) / T)(t)      (fs_logprobs' distribution, by the stream's record)
  * in fp64; a token that is not allowed, whose logit is NaN or -inf, or whose c does not round to a fp32 above -inf is none.
- * Candidates come by c, compared to 39 bits of its mantissa (2e-12 of it); among equal ones those of eos_id (-1: none) first, then the lower row's, in a row the larger logit's,
- * then the lower token's. The n best (n <= FS_MAX_TOP) whose token is not eos_id are the new beams: d_parent [n_streams][n]
- * (the row's number in its stream, from 0), d_tok, d_out_score; places past a stream's candidates hold -1, -1 and -inf. Those
+ * Candidates come by c, compared to 39 bits of its mantissa (2e-12 of it); among equal ones those of eos_id (-1: none)
+ * first, then the lower row's, in a row the larger logit's, then the lower token's. The n best (n <= FS_MAX_TOP) whose token
+ * is not eos_id are the new beams: d_parent [n_streams][n] (the row's number in its stream, from 0), d_tok, d_out_score;
+ * places past a stream's candidates hold -1, -1 and -inf (a token that a model must not be fed). Of several tokens that end a
+ * text one can be eos_id; another is a token like any, whose beam the program ends (score -inf in the next call). Those
  * with eos_id that fewer than n candidates come before are ended hypotheses: their number d_done[s] and, in their order,
  * d_done_parent and d_done_score [n_streams][n], -1 and -inf past them (each may be NULL; min(n, the stream's rows) at most).
  * Rows whose score is -inf or NaN have no candidate, whatever their logits (of which at most the parts' first 16 KB are read):
@@ -365,7 +367,9 @@ int fs_hist_fork(fs_context* ctx, int32_t n_streams, const int32_t* d_hist, cons
                  int64_t out_cap, int64_t* d_out_hist_off, void* stream);
 
 /* A model's state by rows: caches of keys and values, convolution and recurrent states, block tables, of any type. A row
- * holds `blocks` blocks of `positions` positions of pos_bytes bytes each; strides in bytes, none negative. */
+ * holds `blocks` blocks of `positions` positions of pos_bytes bytes each; strides in bytes, none negative. In a row pos_bytes
+ * and blocks * positions are below 2^31, and there are at most 2e9 columns: 16 bytes (8 for more than 32 rows per stream), or
+ * as many as divide the pointers, strides and pos_bytes. */
 typedef struct fs_state {
     const void* d_src;
     void* d_dst;                /* d_src: in place (equal strides, as many rows per stream) */
@@ -380,9 +384,9 @@ typedef struct fs_state {
  * positions [d_from[s], d_len[s]) (NULL: 0, the state's positions; cut to those), the rest of d_dst stays as it was. In place
  * rows of a stream may change places, be copied more than once or dropped. d_from is for what a stream's beams share (the
  * prompt), which need not move. A parent below 0 leaves its row as it was. n, n_src <= FS_MAX_TOP; n_src = 1 opens the beams
- * of prompts. `states` is host memory, read before the call returns; the places that are written must not overlap one
- * another (strides of d_dst below pos_bytes are refused), nor a d_dst any other state of the call (in place: its own d_src
- * alone; a buffer given twice is refused). */
+ * of prompts. A launch takes up to 32 states whose columns are alike. `states` is host memory, read before the call
+ * returns; the places that are written must not overlap one another (strides of d_dst below pos_bytes are refused), nor a
+ * d_dst any other state of the call (in place: its own d_src alone; a buffer given twice is refused). */
 int fs_reorder_states(fs_context* ctx, int32_t n_states, const fs_state* states, int32_t n_streams, int32_t n_src, int32_t n,
                       const int32_t* d_parent, const int32_t* d_from, const int32_t* d_len, void* stream);
 
