@@ -849,7 +849,8 @@ def hist_fork(hist, hist_off, parent, tok=None, row_off=None, out_cap=None, ctx=
             _on(stream, dev)                                   # (what the stream has before the call is read)
             with torch.cuda.device(dev), torch.cuda.stream(stream):
                 if all(host) or not torch.cuda.is_current_stream_capturing():
-                    off, ro = (t if t is None else np.asarray(t if h else t.cpu(), np.int64) for t, h in zip(given, host))
+                    off, ro = (t if t is None else np.asarray(t if h else t.cpu(), np.int64).reshape(-1)
+                               for t, h in zip(given, host))
                     out_cap = _fork_ids(off, ro, S, n)
         out_cap += 0 if tok is None else S * n
     out = torch.empty(max(int(out_cap), 1), dtype=torch.int32, device=dev)
@@ -925,7 +926,7 @@ class States:
         """Refuses a buffer to write whose places overlap (an expanded tensor, windows): the last store there would count."""
         end, places = z.pos_bytes, [(self.dst_rows, z.dst_row), (z.blocks, z.dst_block), (z.positions, z.dst_pos)]
         for k, stride in sorted(((k, s) for k, s in places if k > 1), key=lambda p: p[1]):
-            if stride < end and self.dst_rows > 0 and z.blocks > 0:
+            if stride < end and self.dst_rows > 0 and z.blocks > 0 and z.pos_bytes > 0:
                 raise SamplerError("rows, blocks and positions of a state that is written must not overlap")
             end += (k - 1) * stride
 

@@ -66,6 +66,7 @@ def test_states_refuse_buffers_that_overlap_themselves(ctx):
     F.States([one.expand(6, 3, 10, 4)], [t], pos_dim=2)
     F.States([one.expand(1, 3, 10, 4)], pos_dim=2)
     F.States([torch.zeros((6, 0, 10, 4)).expand(6, 0, 10, 4)], pos_dim=2)
+    F.States([torch.zeros((1, 3, 10, 0)).expand(6, 3, 10, 0)], pos_dim=2)
     F.States([torch.zeros((13, 6, 3, 8)).transpose(0, 1)], pos_dim=1)      # rows between positions and heads
     F.States([torch.zeros((5, 6)).t()])                        # rows innermost
     good = dict(d_src=1 << 20, d_dst=2 << 20, src_row=64, src_block=32, src_pos=8, dst_row=64, dst_block=32, dst_pos=8, pos_bytes=8,

@@ -107,6 +107,24 @@ def test_select_outputs_beside_inputs():
     assert v["off"].view(torch.int64).tolist() == r.off.tolist() and torch.all(buf[56:] == -7)
 
 
+def test_captured_select_of_smaller_batches():
+    """A recorded call of nine rows, replayed for batches of fewer rows and streams: what changes is in the offsets' tensor."""
+    n, V = 3, 6000
+    ctx, r = F.Context(), Rows(8, [9], V)
+    score, off = cuda(r.score), cuda(np.array([0, 3, 6, 9]))
+    F.beam_select(r.x, score, n, eos_id=4, row_off=off, ctx=ctx)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = F.beam_select(r.x, score, n, eos_id=4, row_off=off, ctx=ctx)
+    for cut in ([0, 3, 6, 9], [0, 3, 3, 3], [0, 0, 0, 0], [0, 1, 2, 3], [0, 0, 4, 8], [0, 0, 0, 1], [0, 9, 9, 9], [0, 0, 0, 0],
+                [0, 3, 6, 9]):
+        off.copy_(torch.tensor(cut))
+        graph.replay()
+        m = cut[-1]
+        BU.Step(r.y[:m], r.score[:m], np.array(cut), n, 4).check(out)
+    assert F.device_error(ctx) == 0
+
+
 def test_select_scores_in_host_memory():
     """Scores as an array or a list, [streams, rows each] or [rows], as the other arguments may be."""
     r = Rows(6, [3, 3, 3, 3], 700)
@@ -155,6 +173,8 @@ def test_fork_room_of_offsets_on_the_host():
     parent, tok = np.array([[-1, -1], [2, 2], [0, 0]], np.int32), np.arange(6, dtype=np.int32).reshape(3, 2)
     for t in (tok, None):
         out, o = F.hist_fork(hist, off, parent, t, row_off=ro)
+        again, _ = F.hist_fork(hist, cuda(off.astype(np.int32))[None], parent, t, row_off=cuda(np.array(ro, np.int32))[None])
+        assert again.numel() == out.numel() and torch.equal(again[:int(o[-1])], out[:int(o[-1])])
         assert out.numel() == 2 * (0 + 9 + 1) + (6 if t is not None else 0)
         want = BU.fork([np.arange(a, b) for a, b in zip(off, off[1:])], ro, parent, t)
         assert out[:int(o[-1])].tolist() == [x for h in want for x in h]
